@@ -71,7 +71,7 @@ def draw(rng):
     dtype = rng.choice(("bf16", "bf16", "fp16", "fp32"))
     if kind.startswith("relative"):
         clipped = rng.random() < 0.6
-        reach = _spread(rng, 8, 128) if clipped else rng.choice((64, 128, 500))
+        reach = _spread(rng, 8, 127) if clipped else rng.choice((64, 128, 500))
         buckets = 0 if clipped else rng.choice((16, 32, 64))
         chains = rng.choice((0, 0, 2, 5))
         if kind == "relative-row":
