@@ -198,15 +198,15 @@ def run(state):
     if not own:
         with torch.no_grad():
             return _relative_plain(s) if s["kind"] == "relative" else _projection_plain(s)
-    from evoformer_triton_amd import Fp8Weight, fp8_linear, relative_position_bias
+    import evoformer_triton_amd as evo
     if s["kind"] == "relative":
-        out = relative_position_bias(s["table"], s["lut"], s["positions"], s["key_positions"], chains=s["chain"], key_chains=s["key_chain"], pair_bias=s["pair"])
+        out = evo.relative_position_bias(s["table"], s["lut"], s["positions"], s["key_positions"], chains=s["chain"], key_chains=s["key_chain"], pair_bias=s["pair"])
         leaves, d = [s["table"]] + ([s["pair"]] if s["pair"] is not None else []), s.get("dout")
     elif s["grad"]:
-        out = fp8_linear(s["x"], s["weight"], s["bias"])
+        out = evo.fp8_linear(s["x"], s["weight"], s["bias"])
         leaves, d = [s["x"], s["weight"]] + ([s["bias"]] if s["bias"] is not None else []), s["dy"]
     else:
-        out = fp8_linear(s["x"], Fp8Weight(s["values"], s["scales"], s["k"]), s["bias"])
+        out = evo.fp8_linear(s["x"], evo.Fp8Weight(s["values"], s["scales"], s["k"]), s["bias"])
     return [out, *torch.autograd.grad(out, leaves, d)] if s["grad"] else [out]
 
 
