@@ -2,5 +2,7 @@
 hand-written gfx950 kernels.  Same call surface as lvhoaa/evoformer_triton's
 `evoformer.EvoformerAttention`."""
 from .evoformer import EvoformerAttention, DS4Sci_EvoformerAttention, evoformer_attention, slot_attention  # noqa: F401
+from .relative import RelativePositionBias, relative_buckets, relative_position_bias  # noqa: F401
 
-__all__ = ["EvoformerAttention", "DS4Sci_EvoformerAttention", "evoformer_attention", "slot_attention"]
+__all__ = ["EvoformerAttention", "DS4Sci_EvoformerAttention", "evoformer_attention", "slot_attention",
+           "RelativePositionBias", "relative_buckets", "relative_position_bias"]

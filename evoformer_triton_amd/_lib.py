@@ -35,7 +35,8 @@ EXPORTS = ("evoattn_version", "evoattn_strerror", "evoattn_check", "evoattn_prep
            "evoattn_layernorm_fwd", "evoattn_layernorm_bwd_workspace_bytes", "evoattn_layernorm_bwd",
            "evoattn_colsum_workspace_bytes", "evoattn_colsum",
            "evoattn_pair_bias_workspace_bytes", "evoattn_pair_bias_fwd", "evoattn_pair_bias_bwd",
-           "evoattn_keep_mask", "evoattn_linear_fwd", "evoattn_linear_dx", "evoattn_linear_dw_workspace_bytes", "evoattn_linear_dw")
+           "evoattn_keep_mask", "evoattn_linear_fwd", "evoattn_linear_dx", "evoattn_linear_dw_workspace_bytes", "evoattn_linear_dw",
+           "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd")
 EVOATTN_STATIC_PREP_BYTES = 16 << 20
 
 
@@ -58,6 +59,22 @@ class EvoAttnParams(ctypes.Structure):
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
         ("prep", ctypes.c_void_p), ("prep_bytes", ctypes.c_size_t),
         ("gate", ctypes.c_void_p), ("o_gated", ctypes.c_void_p), ("dgate", ctypes.c_void_p),
+    ]
+
+
+class EvoRelativeBias(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("H", ctypes.c_int32), ("Nq", ctypes.c_int32), ("Nk", ctypes.c_int32),
+        ("rows", ctypes.c_int32), ("reach", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("table_dtype", ctypes.c_int32),
+        ("pos_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("pos_q_stride_b", ctypes.c_int64), ("pos_k_stride_b", ctypes.c_int64),
+        ("pair_stride_b", ctypes.c_int64), ("pair_stride_h", ctypes.c_int64), ("pair_stride_row", ctypes.c_int64),
+        ("table", ctypes.c_void_p), ("lut", ctypes.c_void_p),
+        ("pos_q", ctypes.c_void_p), ("pos_k", ctypes.c_void_p), ("chain_q", ctypes.c_void_p), ("chain_k", ctypes.c_void_p),
+        ("pair", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dout", ctypes.c_void_p),
+        ("dtable", ctypes.c_void_p), ("dpair", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -125,6 +142,12 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_pair_bias_fwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, i64, i64, i32, i32, i32, ctypes.c_float, vp]
     lib.evoattn_pair_bias_bwd.restype = ctypes.c_int
     lib.evoattn_pair_bias_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i64, i64, i32, i32, i32, vp]
+    RB = ctypes.POINTER(EvoRelativeBias)
+    for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd"):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [RB, vp]
+    lib.evoattn_relative_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
+    lib.evoattn_relative_bias_bwd_workspace_bytes.argtypes = [RB]
     lib.evoattn_path.restype = ctypes.c_char_p
     lib.evoattn_kernels.restype = ctypes.c_char_p
     lib.evoattn_path.argtypes = [P, ctypes.c_int]

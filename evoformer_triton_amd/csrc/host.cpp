@@ -1094,6 +1094,8 @@ OptTensor block(const std::vector<OptTensor> &in, const OptTensor &keep, int64_t
     return y;
 }
 
+#include "host_relative.h"
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -1108,4 +1110,8 @@ PYBIND11_MODULE(_host, m) {
     m.def("pair_bias", &pair_bias, no_gil, py::arg("z"), py::arg("ln_weight"), py::arg("ln_bias"), py::arg("eps"), py::arg("weight"));
     m.def("block", &block, no_gil, py::arg("inputs"), py::arg("keep"), py::arg("heads"), py::arg("eps_m"), py::arg("eps_z"), py::arg("inf"),
           py::arg("flags"));
+    m.def("relative_bias", &relative_bias, no_gil);
+    m.def("relative_bias_forward", &relative_bias_forward, no_gil);
+    m.def("relative_bias_backward", &relative_bias_backward, no_gil);
+    m.def("relative_bias_wrong", &relative_bias_wrong, no_gil);
 }

@@ -287,6 +287,38 @@ int evoattn_pair_bias_bwd(const void *dbias, const void *z, const void *gamma, c
                           const float *rstd, void *dz, void *dparams, void *workspace, size_t workspace_bytes, int64_t batches,
                           int64_t pairs, int32_t cols, int32_t heads, int32_t dtype, void *hip_stream);
 
+/* The learned relative position bias (no counterpart in the reference, which takes a pair bias as given):
+ *   out[b][h][i][j] = table[bucket][h] (+ pair[b][h][i][j]),  rounded once to dtype,
+ *   bucket = lut[clamp(pos_q[b][i] - pos_k[b][j], -reach, reach) + reach], or rows - 1 where chain_q[b][i] != chain_k[b][j];
+ *   an entry of lut of `rows` or more stands for no bias (0) and takes no gradient.
+ *   bwd  dtable[r][h] = sum of dout over the pairs of bucket r, in table_dtype, in a fixed order (bit-reproducible), through `workspace`
+ *        (none needed where evoattn_relative_bias_bwd_workspace_bytes() is that of one sum, rows * H * 4);
+ *        dpair[h][i][j] = sum of dout over b: the gradient of a pair bias that the batches share (pair_stride_b 0).  Either may be NULL.
+ * table [rows][H] and lut [2 reach + 1] dense; out, dout [B][H][Nq][Nk] dense, dpair [H][Nq][Nk].  pos_*, chain_* [B][N*], rows
+ * pos_*_stride_b apart (0: shared by the batches), signed integers of pos_bytes (4 or 8) each, any values.  pair: key contiguous, any
+ * strides.  chain_q and chain_k may both be NULL.  dtype (out, pair, dout, dpair) and table_dtype (table, dtable): EVO_BF16 / _F16 /
+ * _F32.  Pointers on their elements' boundaries.  reach at most 4096, rows at most 256 (EVO_EUNSUPPORTED beyond).
+ * Nothing is allocated or synchronised. */
+typedef struct EvoRelativeBias {
+    int32_t B, H, Nq, Nk;
+    int32_t rows, reach;
+    int32_t dtype, table_dtype;
+    int32_t pos_bytes, reserved;
+    int64_t pos_q_stride_b, pos_k_stride_b;
+    int64_t pair_stride_b, pair_stride_h, pair_stride_row;
+    const void *table, *lut;
+    const void *pos_q, *pos_k, *chain_q, *chain_k;
+    const void *pair;
+    void       *out;
+    const void *dout;
+    void       *dtable, *dpair;
+    void       *workspace;
+    size_t      workspace_bytes;
+} EvoRelativeBias;
+int evoattn_relative_bias_fwd(const EvoRelativeBias *p, void *hip_stream);
+size_t evoattn_relative_bias_bwd_workspace_bytes(const EvoRelativeBias *p);
+int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif
