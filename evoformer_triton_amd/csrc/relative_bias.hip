@@ -27,17 +27,12 @@ struct RbVec {
     __device__ __forceinline__ void store(T *p) const { __builtin_memcpy(p, this, 16); }
 };
 
-// What a lane holds of its V keys for all rows, and of a query; positions and chains of 4 or 8 bytes.
-template <typename P, bool CHAIN>
-struct RbSide {
-    const P *pos, *chain;
-    __device__ __forceinline__ int64_t at(int64_t i) const { return (int64_t)pos[i]; }
-    __device__ __forceinline__ int64_t chain_at(int64_t i) const { return CHAIN ? (int64_t)chain[i] : 0; }
-};
-
-struct RbShape {
-    int lanes;    // that a row's strip takes, a power of two up to 64
-    int strips;   // of 64 lanes' elements, of a row
+// Positions or chains of one side, of 4 or 8 bytes each.
+struct RbIndex {
+    const void *p;
+    int64_t b;
+    bool wide;
+    __device__ __forceinline__ int64_t operator[](int64_t i) const { return wide ? ((const int64_t *)p)[b + i] : (int64_t)((const int32_t *)p)[b + i]; }
 };
 
 struct RbArgs {
@@ -47,11 +42,22 @@ struct RbArgs {
     int64_t pos_q_b, pos_k_b;     // from one batch to the next (0: the same)
     int64_t pair_b, pair_h, pair_row;
     int B, H, Nq, Nk, rows, reach, table_dtype;
-    int lanes, strips, chunk, chunks;   // chunk: rows of a workgroup
+    int lanes;            // forward: that a row takes, a power of two up to 64
+    int strips, heads;    // pieces of a row (backward: and of the heads) that a workgroup each takes
+    int chunk, chunks;    // rows of a workgroup
+    bool wide;            // positions and chains of 8 bytes
+    __device__ __forceinline__ RbIndex queries(const void *t, int b) const { return {t, b * pos_q_b, wide}; }
+    __device__ __forceinline__ RbIndex keys(const void *t, int b) const { return {t, b * pos_k_b, wide}; }
 };
 
 __device__ __forceinline__ float rb_entry(const void *t, int64_t i, int dtype) {
     return dtype == EVO_F32 ? ((const float *)t)[i] : dtype == EVO_BF16 ? (float)((const bf16_t *)t)[i] : (float)((const f16_t *)t)[i];
+}
+
+__device__ __forceinline__ void rb_store(void *t, int64_t i, float v, int dtype) {
+    if (dtype == EVO_F32) ((float *)t)[i] = v;
+    else if (dtype == EVO_BF16) ((bf16_t *)t)[i] = (bf16_t)v;
+    else ((f16_t *)t)[i] = (f16_t)v;
 }
 
 __device__ __forceinline__ bool rb_near(int64_t p) { return p > -kRbNear && p < kRbNear; }
@@ -64,7 +70,7 @@ __device__ __forceinline__ int rb_offset(int64_t q, int64_t k, int reach) {
 }
 
 // Forward.
-template <typename T, typename P, bool PAIR, bool CHAIN>
+template <typename T, bool PAIR, bool CHAIN>
 __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, const T *pair, T *out) {
     constexpr int V = RbVec<T>::V, U = 4;
     extern __shared__ float val[];   // [2 R + 1]: this head's number for each clipped distance
@@ -80,8 +86,7 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
         val[o] = r < a.rows ? rb_entry(a.table, (int64_t)r * a.H + h, a.table_dtype) : 0.0f;
     }
     const float other = CHAIN ? rb_entry(a.table, (int64_t)(a.rows - 1) * a.H + h, a.table_dtype) : 0.0f;
-    const RbSide<P, CHAIN> qs{(const P *)a.pos_q + b * a.pos_q_b, CHAIN ? (const P *)a.chain_q + b * a.pos_q_b : nullptr};
-    const RbSide<P, CHAIN> ks{(const P *)a.pos_k + b * a.pos_k_b, CHAIN ? (const P *)a.chain_k + b * a.pos_k_b : nullptr};
+    const RbIndex qs = a.queries(a.pos_q, b), ks = a.keys(a.pos_k, b), qc = a.queries(a.chain_q, b), kc = a.keys(a.chain_k, b);
     // The last lane of a row that is no whole number of pieces steps back: two lanes write the same values there.
     const int col = (strip * 64 + lane % a.lanes) * V, first = min(col, max(a.Nk - V, 0)), sub = lane / a.lanes, per = 64 / a.lanes;
     const bool mine = col < a.Nk;
@@ -90,8 +95,8 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 #pragma unroll
     for (int e = 0; e < V; ++e) {
         const int64_t j = min(first + e, a.Nk - 1);
-        pk[e] = ks.at(j);
-        ck[e] = ks.chain_at(j);
+        pk[e] = ks[j];
+        ck[e] = CHAIN ? kc[j] : 0;
         near = near && rb_near(pk[e]);
     }
     near = __all(near);
@@ -105,8 +110,8 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = min(base + u * per + sub, r1 - 1);
-            pq[u] = qs.at(i);
-            cq[u] = qs.chain_at(i);
+            pq[u] = qs[i];
+            cq[u] = CHAIN ? qc[i] : 0;
             if (PAIR && mine) {
                 const T *p = pair + b * a.pair_b + h * a.pair_h + i * a.pair_row;
                 if (whole) {
@@ -149,123 +154,237 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
     }
 }
 
-// Sums over 64 lanes, the same in all.
-__device__ __forceinline__ float rb_wave_sum(float s) {
+// Backward: the sums of dout over the pairs of each bucket, as products: buckets x pairs (one where a pair is of the bucket, else zero) times
+// pairs x heads, on v_mfma_f32_16x16x32 (lane l, q = l / 16: operands' row or column l % 16, contraction 8q .. 8q + 7; accumulator column l % 16, rows
+// 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones as three bf16 parts, which hold all of their 24 bits.  A
+// product with one is exact, and sums are fp32 in a fixed order.  Zero times an infinity is no number: a workgroup that ends with a
+// sum that is not finite forms its sums again one by one, and so does one whose positions or chains lie 2^30 or more apart.
+constexpr int kRbKeys = 64, kRbHeads = 16;   // a workgroup's keys and heads
+
+typedef float f32x4r __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4r rb_mma(bf16x8 a, bf16x8 b, f32x4r c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4r rb_mma(f16x8 a, f16x8 b, f32x4r c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+typedef uint32_t u32x4r __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2r __attribute__((ext_vector_type(2)));
+
+// Eight gradients of a head, and their products.
+template <typename T>
+struct RbRow {
+    typedef typename std::conditional<sizeof(T) == 4, bf16_t, T>::type O;   // operands' type
+    typedef typename Mfma<O>::v8 v8;
+    static constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+    static constexpr uint32_t ONE = std::is_same<O, f16_t>::value ? 0x3c00 : 0x3f80;
+    T e[8];
+    __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(e, p, sizeof e); }
+    __device__ __forceinline__ void parts(v8 (&out)[PARTS]) const {
+        if constexpr (PARTS == 1) {
+            out[0] = __builtin_bit_cast(v8, e);
+        } else {
+            uint32_t x[8];
 #pragma unroll
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o);
-    return s;
+            for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(e[i]);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {   // the upper halves, then what they leave
+                u32x4r h;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) h[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302);
+                out[k] = __builtin_bit_cast(v8, h);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (k < 2) x[i] = __float_as_uint(__uint_as_float(x[i]) - __uint_as_float(x[i] & 0xffff0000u));
+            }
+        }
+    }
+};
+
+// min(x, 1) in both halves; not as the compiler would have it, two comparisons and two selections
+__device__ __forceinline__ u16x2r rb_any_bits(u16x2r x) {
+    u16x2r r;
+    asm("v_pk_min_u16 %0, %1, %2" : "=v"(r) : "v"(x), "s"(0x00010001));
+    return r;
 }
 
-// Backward: sums of dout over the pairs of each bucket, of a workgroup's rows.  A wave keeps COPIES sums of each bucket in LDS, lane l
-// adding to copy l % COPIES; where there are fewer copies than lanes, the lanes take turns.  The LDS takes a wave's additions in their
-// order, and lanes that add at once add to different copies: the order of a sum is fixed.
-template <typename T, typename P, int COPIES, bool CHAIN>
+// A position or chain less the workgroup's first, in 32 bits; false where that is not within 2^30.
+__device__ __forceinline__ bool rb_from(int64_t p, int64_t base, int &d) {
+    int64_t w;
+    const bool over = __builtin_sub_overflow(p, base, &w);
+    d = (int)w;
+    return !over && rb_near(w);
+}
+
+// Lanes of a workgroup's keys: group g of 32, a lane's eight from `first` on, of which the first `skip` are another lane's (or none).
+template <int TILES, typename T, bool CHAIN>
 __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, const T *dout, float *part, void *dtable) {
-    constexpr int V = RbVec<T>::V, U = 4;
-    extern __shared__ float sums[];   // [waves][rows + 1][COPIES], the last row for distances without a bucket; then uint16 [2 R + 1]
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int held = (a.rows + 1) * COPIES;
-    uint16_t *at = reinterpret_cast<uint16_t *>(sums + kRbWaves * held);
+    typedef RbRow<T> Row;
+    typedef typename Row::v8 v8;
+    constexpr int G = kRbKeys / 32, U = 2;
+    extern __shared__ float lds[];   // [waves - 1][TILES * 4][64] sums; uint16 [2 R + 2] buckets, the last one of pairs in different chains
+    uint16_t *lut = reinterpret_cast<uint16_t *>(lds + (kRbWaves - 1) * TILES * 4 * 64);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), q = lane >> 4, li = lane & 15;
     unsigned id = blockIdx.x;
     const int strip = id % a.strips;
     id /= a.strips;
     const int chunk = id % a.chunks;
     id /= a.chunks;
-    const int b = id % a.B, h = id / a.B;
-    for (int i = threadIdx.x; i < kRbWaves * held; i += kRbWaves * 64) sums[i] = 0.0f;
-    for (int o = threadIdx.x; o <= 2 * a.reach; o += kRbWaves * 64) at[o] = (uint16_t)(min((int)a.lut[o], a.rows) * COPIES);
-    const RbSide<P, CHAIN> qs{(const P *)a.pos_q + b * a.pos_q_b, CHAIN ? (const P *)a.chain_q + b * a.pos_q_b : nullptr};
-    const RbSide<P, CHAIN> ks{(const P *)a.pos_k + b * a.pos_k_b, CHAIN ? (const P *)a.chain_k + b * a.pos_k_b : nullptr};
-    const int col = (strip * 64 + lane % a.lanes) * V, first = min(col, max(a.Nk - V, 0)), sub = lane / a.lanes, per = 64 / a.lanes;
-    const bool mine = col < a.Nk;
-    int64_t pk[V], ck[V];
+    const int b = id % a.B, h0 = id / a.B * kRbHeads, j0 = strip * kRbKeys;
+    const RbIndex qs = a.queries(a.pos_q, b), ks = a.keys(a.pos_k, b), qc = a.queries(a.chain_q, b), kc = a.keys(a.chain_k, b);
+    const int r0 = chunk * a.chunk, r1 = min(r0 + a.chunk, a.Nq);
+    const bool whole = a.Nk >= 8, ragged = j0 + kRbKeys > a.Nk;
+    const T *rows = dout + (((int64_t)b * a.H + min(h0 + li, a.H - 1)) * a.Nq) * a.Nk;
+
+    const int64_t p0 = qs[r0], c0 = CHAIN ? qc[r0] : 0;
+    int first[G], skip[G], pk[G][8], ck[CHAIN ? G : 1][8];
     bool near = true;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int64_t j = min(first + e, a.Nk - 1);
-        pk[e] = ks.at(j);
-        ck[e] = ks.chain_at(j);
-        near = near && rb_near(pk[e]);
-    }
-    near = __all(near);
-    __syncthreads();
-    float *own = sums + wave * held + lane % COPIES;
-    const int r0 = chunk * a.chunk, r1 = min(r0 + a.chunk, a.Nq);
-    const int64_t plane = ((int64_t)b * a.H + h) * a.Nq;
-    const bool whole = a.Nk >= V;
-    for (int base = r0 + wave * per * U; base < r1; base += kRbWaves * per * U) {
-        RbVec<T> in[U];
-        int64_t pq[U], cq[U];
+    for (int g = 0; g < G; ++g) {
+        const int col = j0 + 32 * g + 8 * q;
+        first[g] = min(col, max(a.Nk - 8, 0));
+        skip[g] = min(col - first[g], 8);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = min(base + u * per + sub, r1 - 1);
-            pq[u] = qs.at(i);
-            cq[u] = qs.chain_at(i);
-            const T *p = dout + (plane + i) * a.Nk;
-            if (whole) {
-                in[u] = RbVec<T>::load(p + first);
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) in[u].e[e] = p[min(e, a.Nk - 1)];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool on = mine && base + u * per + sub < r1;
-            int o[V];
-            if (near && __all(rb_near(pq[u]))) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = rb_offset((int)pq[u], (int)pk[e], a.reach);
-            } else {
-#pragma unroll
-                for (int e = 0; e < V; ++e) o[e] = rb_offset(pq[u], pk[e], a.reach);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                int r = at[o[e]];
-                if (CHAIN) r = ck[e] == cq[u] ? r : (a.rows - 1) * COPIES;
-                // (of a lane that stepped back, what the lane before it has; of a row shorter than a piece, what lies behind it)
-                const bool counts = on && first + e >= col && first + e < a.Nk;
-#pragma unroll
-                for (int turn = 0; turn < 64 / COPIES; ++turn)
-                    if (counts && lane / COPIES == turn) __builtin_amdgcn_ds_atomic_fadd_f32((__attribute__((address_space(3))) float *)(own + r), (float)in[u].e[e]);
-            }
+        for (int e = 0; e < 8; ++e) {
+            const int j = min(first[g] + e, a.Nk - 1);
+            near = rb_from(ks[j], p0, pk[g][e]) && near;
+            pk[g][e] -= a.reach;
+            if (CHAIN) near = rb_from(kc[j], c0, ck[g][e]) && near;
         }
     }
+    for (int o = threadIdx.x; o <= 2 * a.reach + 1; o += kRbWaves * 64) lut[o] = o <= 2 * a.reach ? a.lut[o] : a.rows - 1;
+
+    f32x4r acc[TILES];
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) acc[t] = f32x4r{0.0f, 0.0f, 0.0f, 0.0f};
+    Row next[U][G];
+    int pq[U], cq[U];
+    auto fetch = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = min(base + u * kRbWaves, r1 - 1);
+            near = rb_from(qs[i], p0, pq[u]) && near;
+            if (CHAIN) near = rb_from(qc[i], c0, cq[u]) && near;
+            const T *p = rows + (int64_t)i * a.Nk;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                if (whole) {
+                    next[u][g].load(p + first[g]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) next[u][g].e[e] = p[min(e, a.Nk - 1)];
+                }
+            }
+        }
+    };
+    fetch(r0 + wave);
     __syncthreads();
-    for (int r = wave; r < a.rows; r += kRbWaves) {
+    for (int base = r0 + wave; base < r1; base += U * kRbWaves) {
+        Row now[U][G];
+        int pn[U], cn[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            pn[u] = pq[u];
+            cn[u] = CHAIN ? cq[u] : 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g) now[u][g] = next[u][g];
+        }
+        if (base + U * kRbWaves < r1) fetch(base + U * kRbWaves);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (base + u * kRbWaves >= r1) break;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                int o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    o[e] = min(max(pn[u] - pk[g][e], 0), 2 * a.reach);
+                    if (CHAIN) o[e] = ck[g][e] == cn[u] ? o[e] : 2 * a.reach + 1;
+                }
+                u16x2r bucket[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) bucket[i] = u16x2r{lut[o[2 * i]], lut[o[2 * i + 1]]};
+                if (ragged) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (e < skip[g] || first[g] + e >= a.Nk) bucket[e / 2][e % 2] = 0xffff;
+                }
+                v8 d[Row::PARTS];
+                now[u][g].parts(d);
+#pragma unroll
+                for (int t = 0; t < TILES; ++t) {
+                    const uint16_t r = (uint16_t)(16 * t + li);
+                    u32x4r hot;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {   // ONE where equal: ONE - min(different bits, 1) * ONE
+                        const u16x2r off = rb_any_bits(bucket[i] ^ u16x2r{r, r});
+                        hot[i] = __builtin_bit_cast(uint32_t, u16x2r{(uint16_t)Row::ONE, (uint16_t)Row::ONE} - off * u16x2r{(uint16_t)Row::ONE, (uint16_t)Row::ONE});
+                    }
+#pragma unroll
+                    for (int k = 0; k < Row::PARTS; ++k) acc[t] = rb_mma(__builtin_bit_cast(v8, hot), d[k], acc[t]);
+                }
+            }
+        }
+    }
+    bool fine = near;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) fine = fine && __builtin_fabsf(acc[t][r]) < __builtin_inff();
+    if (wave > 0) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds[((wave - 1) * TILES * 4 + 4 * t + r) * 64 + lane] = acc[t][r];
+    }
+    const bool again = __syncthreads_or(!fine);
+    const int64_t at = ((int64_t)b * a.chunks + chunk) * a.strips + strip;
+    auto write = [&](int row, int h, float s) {
+        if (part) part[(at * a.rows + row) * a.H + h] = s;
+        else rb_store(dtable, (int64_t)row * a.H + h, s, a.table_dtype);
+    };
+    if (!again) {
+        if (wave > 0 || h0 + li >= a.H) return;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float s = acc[t][r];
+#pragma unroll
+                for (int w = 0; w < kRbWaves - 1; ++w) s += lds[(w * TILES * 4 + 4 * t + r) * 64 + lane];
+                const int row = 16 * t + 4 * q + r;
+                if (row < a.rows) write(row, h0 + li, s);
+            }
+        return;
+    }
+    // one entry of the table per thread, pair by pair
+    const int h = h0 + threadIdx.x % kRbHeads;
+    if (h >= a.H) return;
+    const T *mine = dout + ((int64_t)b * a.H + h) * a.Nq * a.Nk;
+    for (int row = threadIdx.x / kRbHeads; row < a.rows; row += kRbWaves * 64 / kRbHeads) {
         float s = 0.0f;
-        if (lane < COPIES) {
-#pragma unroll
-            for (int w = 0; w < kRbWaves; ++w) s += sums[w * held + r * COPIES + lane];
-        }
-        s = rb_wave_sum(s);
-        if (lane == 0) {
-            if (part) {
-                part[((int64_t)r * a.H + h) * ((int64_t)a.B * a.chunks * a.strips) + ((int64_t)b * a.chunks + chunk) * a.strips + strip] = s;
-            } else if (a.table_dtype == EVO_F32) {
-                ((float *)dtable)[(int64_t)r * a.H + h] = s;
-            } else if (a.table_dtype == EVO_BF16) {
-                ((bf16_t *)dtable)[(int64_t)r * a.H + h] = (bf16_t)s;
-            } else {
-                ((f16_t *)dtable)[(int64_t)r * a.H + h] = (f16_t)s;
+        for (int i = r0; i < r1; ++i)
+            for (int j = j0; j < min(j0 + kRbKeys, a.Nk); ++j) {
+                const int o = CHAIN && kc[j] != qc[i] ? 2 * a.reach + 1 : rb_offset(qs[i], ks[j], a.reach);
+                if (lut[o] == row) s += (float)mine[(int64_t)i * a.Nk + j];
             }
-        }
+        write(row, h, s);
     }
 }
 
-// The workgroups' sums, a wave for each entry of the table.
-__global__ void __launch_bounds__(256) relative_bias_sum(const float *part, void *dtable, int entries, int parts, int dtype) {
-    const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (e >= entries) return;
+// The workgroups' sums: 32 entries of the table by 32 slices of the parts.
+__global__ void __launch_bounds__(1024) relative_bias_sum(const float *part, void *dtable, int entries, int parts, int dtype) {
+    __shared__ float sums[32][33];
+    const int e = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
     float s = 0.0f;
-#pragma unroll 4
-    for (int i = lane; i < parts; i += 64) s += part[(int64_t)e * parts + i];
-    s = rb_wave_sum(s);
-    if (lane) return;
-    if (dtype == EVO_F32) ((float *)dtable)[e] = s;
-    else if (dtype == EVO_BF16) ((bf16_t *)dtable)[e] = (bf16_t)s;
-    else ((f16_t *)dtable)[e] = (f16_t)s;
+    if (e < entries) {
+#pragma unroll 8
+        for (int i = slice; i < parts; i += 32) s += part[(int64_t)i * entries + e];
+    }
+    sums[slice][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (slice || e >= entries) return;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sums[i][threadIdx.x];
+    rb_store(dtable, e, s, dtype);
 }
 
 // The gradient of a pair bias that all batches share: the sum of the output's over them.
@@ -304,20 +423,13 @@ static int rb_rc() {
 
 static bool rb_dtype(int d) { return d == EVO_BF16 || d == EVO_F16 || d == EVO_F32; }
 
-// How a row is dealt to lanes, and how many rows a workgroup takes so that `want` of them cover the call.
-static void rb_shape(RbArgs &a, const EvoRelativeBias &p, int want) {
-    const int v = p.dtype == EVO_F32 ? 4 : 8;
-    const int64_t pieces = ((int64_t)p.Nk + v - 1) / v;
-    a.lanes = 1;
-    while (a.lanes < 64 && a.lanes < pieces) a.lanes *= 2;
-    a.strips = (int)((pieces + 63) / 64);
-    const int step = kRbWaves * 64 / a.lanes;   // rows that a workgroup's waves take at once
-    const int64_t rows = (int64_t)p.B * p.H * p.Nq * a.strips;
-    int64_t chunk = (rows + want - 1) / want;
+// Rows of a workgroup, a multiple of `step`, so that `want` workgroups cover a call of `each` strips of rows.
+static void rb_chunks(RbArgs &a, int64_t each, int step, int want) {
+    int64_t chunk = (each * a.Nq + want - 1) / want;
     chunk = (chunk + step - 1) / step * step;
-    if (chunk > p.Nq) chunk = p.Nq;
+    if (chunk > a.Nq) chunk = a.Nq;
     a.chunk = (int)chunk;
-    a.chunks = (p.Nq + a.chunk - 1) / a.chunk;
+    a.chunks = (a.Nq + a.chunk - 1) / a.chunk;
 }
 
 static int rb_check(const EvoRelativeBias *p) {
@@ -352,6 +464,7 @@ static RbArgs rb_args(const EvoRelativeBias &p) {
     a.rows = p.rows;
     a.reach = p.reach;
     a.table_dtype = p.table_dtype;
+    a.wide = p.pos_bytes == 8;
     return a;
 }
 
@@ -359,25 +472,45 @@ template <typename F>
 static int rb_by_dtype(int dtype, F &&f) {
     return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
 }
-// positions' type and whether there are chains
-template <typename F>
-static int rb_by_side(const EvoRelativeBias &p, F &&f) {
-    if (p.pos_bytes == 4) return p.chain_q ? f(int32_t(), std::true_type()) : f(int32_t(), std::false_type());
-    return p.chain_q ? f(int64_t(), std::true_type()) : f(int64_t(), std::false_type());
-}
-
 constexpr int kRbFwdGroups = 2048, kRbBwdGroups = 1024;
 
-static int rb_copies(int rows) { return rows <= 72 ? 64 : rows <= 144 ? 32 : 16; }
-constexpr int kRbMaxLds = 96 << 10;
-static_assert(kRbWaves * 73 * 64 * 4 + (2 * kRbMaxReach + 1) * 2 <= kRbMaxLds && 145 * 32 <= 73 * 64 && (kRbMaxRows + 1) * 16 <= 73 * 64, "what a workgroup keeps");
+static RbArgs rb_fwd_args(const EvoRelativeBias &p) {
+    RbArgs a = rb_args(p);
+    const int v = p.dtype == EVO_F32 ? 4 : 8;
+    const int64_t pieces = ((int64_t)p.Nk + v - 1) / v;
+    a.lanes = 1;
+    while (a.lanes < 64 && a.lanes < pieces) a.lanes *= 2;
+    a.strips = (int)((pieces + 63) / 64);
+    rb_chunks(a, (int64_t)p.B * p.H * a.strips, kRbWaves * 64 / a.lanes, kRbFwdGroups);
+    return a;
+}
 
 static RbArgs rb_bwd_args(const EvoRelativeBias &p) {
     RbArgs a = rb_args(p);
-    rb_shape(a, p, kRbBwdGroups);
+    a.strips = (p.Nk + kRbKeys - 1) / kRbKeys;
+    a.heads = (p.H + kRbHeads - 1) / kRbHeads;
+    rb_chunks(a, (int64_t)p.B * a.strips * a.heads, kRbWaves, kRbBwdGroups);
     return a;
 }
 static int64_t rb_parts(const RbArgs &a) { return (int64_t)a.B * a.chunks * a.strips; }
+
+template <typename T, bool CHAIN>
+static int rb_launch_bwd(const RbArgs &a, unsigned grid, const T *dout, float *part, void *dtable, hipStream_t st) {
+    auto go = [&](auto n) {
+        constexpr int TILES = decltype(n)::value;
+        constexpr int sums = (kRbWaves - 1) * TILES * 4 * 64 * sizeof(float), most = sums + (2 * kRbMaxReach + 2) * sizeof(uint16_t);
+        constexpr auto kernel = relative_bias_bwd<TILES, T, CHAIN>;
+        static PerDevice done;
+        if (const int rc = ensure_dynamic_lds((const void *)kernel, most, done, nullptr)) return rc;
+        kernel<<<grid, kRbWaves * 64, sums + (2 * a.reach + 2) * sizeof(uint16_t), st>>>(a, dout, part, dtable);
+        return rb_rc();
+    };
+    if (a.rows <= 32) return go(std::integral_constant<int, 2>());
+    if (a.rows <= 48) return go(std::integral_constant<int, 3>());
+    if (a.rows <= 80) return go(std::integral_constant<int, 5>());
+    if (a.rows <= 144) return go(std::integral_constant<int, 9>());
+    return go(std::integral_constant<int, 16>());
+}
 
 }  // namespace evo
 
@@ -388,20 +521,19 @@ int evoattn_relative_bias_fwd(const EvoRelativeBias *p, void *hip_stream) {
     if (const int rc = rb_check(p)) return rc;
     if (!p->table || !p->out) return EVO_EINVAL;
     if (p->pair && (p->pair_stride_row < 0 || p->pair_stride_h < 0 || p->pair_stride_b < 0)) return EVO_EINVAL;
-    RbArgs a = rb_args(*p);
-    rb_shape(a, *p, kRbFwdGroups);
+    const RbArgs a = rb_fwd_args(*p);
     const int64_t grid = (int64_t)a.strips * a.chunks * a.H * a.B;
     if (grid > INT32_MAX) return EVO_EOVERFLOW;
     const size_t lds = (2 * (size_t)p->reach + 1) * sizeof(float);
     return rb_by_dtype(p->dtype, [&](auto t) {
         typedef decltype(t) T;
-        return rb_by_side(*p, [&](auto pos, auto chain) {
-            typedef decltype(pos) P;
-            constexpr bool C = decltype(chain)::value;
-            if (p->pair) relative_bias_fwd<T, P, true, C><<<(unsigned)grid, kRbWaves * 64, lds, (hipStream_t)hip_stream>>>(a, (const T *)p->pair, (T *)p->out);
-            else relative_bias_fwd<T, P, false, C><<<(unsigned)grid, kRbWaves * 64, lds, (hipStream_t)hip_stream>>>(a, nullptr, (T *)p->out);
+        auto go = [&](auto pair, auto chain) {
+            relative_bias_fwd<T, decltype(pair)::value, decltype(chain)::value><<<(unsigned)grid, kRbWaves * 64, lds, (hipStream_t)hip_stream>>>(a, (const T *)p->pair, (T *)p->out);
             return rb_rc();
-        });
+        };
+        const std::true_type yes;
+        const std::false_type no;
+        return p->pair ? p->chain_q ? go(yes, yes) : go(yes, no) : p->chain_q ? go(no, yes) : go(no, no);
     });
 }
 
@@ -419,30 +551,18 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream) {
     hipStream_t st = (hipStream_t)hip_stream;
     if (p->dtable) {
         const RbArgs a = rb_bwd_args(*p);
-        const int64_t parts = rb_parts(a), grid = parts * a.H, entries = (int64_t)a.rows * a.H;
-        if (grid > INT32_MAX || entries > INT32_MAX || parts > INT32_MAX) return EVO_EOVERFLOW;
+        const int64_t parts = rb_parts(a), grid = parts * a.heads, entries = (int64_t)a.rows * a.H;
+        if (grid > INT32_MAX || entries > INT32_MAX) return EVO_EOVERFLOW;
         float *part = parts > 1 ? (float *)p->workspace : nullptr;
         if (parts > 1 && (!p->workspace || p->workspace_bytes < evoattn_relative_bias_bwd_workspace_bytes(p))) return EVO_EWORKSPACE;
-        const int copies = rb_copies(a.rows);
-        const size_t lds = (size_t)kRbWaves * (a.rows + 1) * copies * sizeof(float) + (2 * (size_t)a.reach + 1) * sizeof(uint16_t);
         const int rc = rb_by_dtype(p->dtype, [&](auto t) {
             typedef decltype(t) T;
-            return rb_by_side(*p, [&](auto pos, auto chain) {
-                typedef decltype(pos) P;
-                constexpr bool C = decltype(chain)::value;
-                auto go = [&](auto n) {
-                    constexpr auto kernel = relative_bias_bwd<T, P, decltype(n)::value, C>;
-                    static PerDevice done;
-                    if (const int rc = ensure_dynamic_lds((const void *)kernel, kRbMaxLds, done, nullptr)) return rc;
-                    kernel<<<(unsigned)grid, kRbWaves * 64, lds, st>>>(a, (const T *)p->dout, part, p->dtable);
-                    return rb_rc();
-                };
-                return copies == 64 ? go(std::integral_constant<int, 64>()) : copies == 32 ? go(std::integral_constant<int, 32>()) : go(std::integral_constant<int, 16>());
-            });
+            return p->chain_q ? rb_launch_bwd<T, true>(a, (unsigned)grid, (const T *)p->dout, part, p->dtable, st)
+                              : rb_launch_bwd<T, false>(a, (unsigned)grid, (const T *)p->dout, part, p->dtable, st);
         });
         if (rc) return rc;
         if (part) {
-            relative_bias_sum<<<(unsigned)((entries + 3) / 4), 256, 0, st>>>(part, p->dtable, (int)entries, (int)parts, p->table_dtype);
+            relative_bias_sum<<<(unsigned)((entries + 31) / 32), 1024, 0, st>>>(part, p->dtable, (int)entries, (int)parts, p->table_dtype);
             if (const int rc2 = rb_rc()) return rc2;
         }
     }
