@@ -36,7 +36,8 @@ EXPORTS = ("evoattn_version", "evoattn_strerror", "evoattn_check", "evoattn_prep
            "evoattn_colsum_workspace_bytes", "evoattn_colsum",
            "evoattn_pair_bias_workspace_bytes", "evoattn_pair_bias_fwd", "evoattn_pair_bias_bwd",
            "evoattn_keep_mask", "evoattn_linear_fwd", "evoattn_linear_dx", "evoattn_linear_dw_workspace_bytes", "evoattn_linear_dw",
-           "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd")
+           "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd",
+           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul")
 EVOATTN_STATIC_PREP_BYTES = 16 << 20
 
 
@@ -74,6 +75,16 @@ class EvoRelativeBias(ctypes.Structure):
         ("pos_q", ctypes.c_void_p), ("pos_k", ctypes.c_void_p), ("chain_q", ctypes.c_void_p), ("chain_k", ctypes.c_void_p),
         ("pair", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dout", ctypes.c_void_p),
         ("dtable", ctypes.c_void_p), ("dpair", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvoFp8Matmul(ctypes.Structure):
+    _fields_ = [
+        ("m", ctypes.c_int64), ("n", ctypes.c_int64), ("k", ctypes.c_int64), ("ldo", ctypes.c_int64),
+        ("dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+        ("a", ctypes.c_void_p), ("scales_a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scales_b", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
@@ -143,11 +154,20 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_pair_bias_bwd.restype = ctypes.c_int
     lib.evoattn_pair_bias_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i64, i64, i32, i32, i32, vp]
     RB = ctypes.POINTER(EvoRelativeBias)
-    for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd"):
+    for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd",
+           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [RB, vp]
     lib.evoattn_relative_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
     lib.evoattn_relative_bias_bwd_workspace_bytes.argtypes = [RB]
+    lib.evoattn_fp8_quantize.restype = ctypes.c_int
+    lib.evoattn_fp8_quantize.argtypes = [vp, i64, vp, vp, vp, vp, vp, i64, i64, i32, vp]
+    lib.evoattn_fp8_column_sums.restype = ctypes.c_int
+    lib.evoattn_fp8_column_sums.argtypes = [vp, vp, i64, i64, i32, vp]
+    lib.evoattn_fp8_matmul_workspace_bytes.restype = ctypes.c_size_t
+    lib.evoattn_fp8_matmul_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
+    lib.evoattn_fp8_matmul.restype = ctypes.c_int
+    lib.evoattn_fp8_matmul.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp]
     lib.evoattn_path.restype = ctypes.c_char_p
     lib.evoattn_kernels.restype = ctypes.c_char_p
     lib.evoattn_path.argtypes = [P, ctypes.c_int]

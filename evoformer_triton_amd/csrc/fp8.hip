@@ -1,0 +1,569 @@
+// Linear layers in 8 bits: e4m3 operands with a power-of-two scale (E8M0, the exponent + 127) for each block of 128 along the
+// contraction, y = Q(x) Q(w)^T + b.  Two kernels: the rounding of a matrix, along its rows, its columns or both in one pass, and the product of two
+// rounded matrices that both lie with the contraction along their rows.  A training step's products are all of that form:
+//   y = Qk(x) Qk(w)^T,  dx = Qn(dy) Qn(w^T)^T,  dw = Qm(dy^T) Qm(x^T)^T
+// each operand rounded along the axis that its product contracts.
+#include <type_traits>
+
+#include "common.h"
+#include "bwd_common.h"
+#include "kernels.h"
+
+namespace evo {
+
+constexpr int kF8Block = 128;   // elements that share a scale
+
+typedef int i32x8f __attribute__((ext_vector_type(8)));
+typedef int i32x4f __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2f __attribute__((ext_vector_type(2)));
+
+static int64_t f8_pitch(int64_t k) { return (k + kF8Block - 1) / kF8Block * kF8Block; }             // bytes of a rounded row
+static int64_t f8_scale_pitch(int64_t k) { return (k + 4 * kF8Block - 1) / (4 * kF8Block) * 4; }   // bytes of its scales
+
+// ---- rounding ----
+
+// The exponent e of a block whose largest finite magnitude has these bits: the least with magnitude <= 448 2^e, at least -127 (0 for a block of zeros).
+__device__ __forceinline__ int f8_exponent(unsigned amax) {
+    const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);   // 448 = 1.75 * 2^8
+    return amax ? max(e, -127) : 0;
+}
+__device__ __forceinline__ float f8_inverse(int e) { return __uint_as_float((unsigned)(127 - e) << 23); }
+// |x| of a finite x, else 0
+__device__ __forceinline__ unsigned f8_magnitude(float x) {
+    const unsigned a = __float_as_uint(x) & 0x7fffffffu;
+    return a < 0x7f800000u ? a : 0u;
+}
+// Four values times `inv` as e4m3, to nearest, ties to even; infinities and NaN as NaN (what the conversion makes of them).
+__device__ __forceinline__ int f8_pack(float a, float b, float c, float d, float inv) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+    return __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, lo, true);
+}
+template <int N>
+__device__ __forceinline__ unsigned f8_max_ror(unsigned v) {   // with the value N lanes further within 16
+    return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 | N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ unsigned f8_max16(unsigned v) { return f8_max_ror<1>(f8_max_ror<2>(f8_max_ror<4>(f8_max_ror<8>(v)))); }
+
+struct F8Quantize {
+    const void *x;
+    int64_t ldx, rows;
+    int cols, sp, tiles_k;        // sp: bytes of a row's scales
+    int64_t spt, tiles_r;         // of a column's
+    int64_t kp, rp;               // bytes of a rounded row, of a rounded column
+    uint8_t *q, *s, *qt, *st;
+    float *sums;
+};
+
+constexpr int kF8Threads = 256;
+
+// A workgroup rounds 128 rows x 128 columns: thread t eight rows (8 (t / 16) ..) of eight columns (8 (t % 16) ..).
+template <typename T, bool ROWS, bool COLS>
+__global__ void __launch_bounds__(kF8Threads) fp8_quantize(F8Quantize p) {
+    constexpr int V = 8;
+    __shared__ __attribute__((aligned(16))) unsigned char tile[COLS ? 128 * 128 : 16];
+    __shared__ unsigned amaxs[COLS ? 4 : 1][128];
+    __shared__ float sums[COLS ? 4 : 1][128];
+    const int t = threadIdx.x, cg = t % 16, rg = t / 16, wave = t / 64;
+    const int kt = blockIdx.x % p.tiles_k;
+    const int64_t rt = blockIdx.x / p.tiles_k;
+    const int c0 = kt * 128 + cg * 8;
+    const int64_t r0 = rt * 128 + rg * 8;
+    float v[V][8];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const T *x = (const T *)p.x + (r0 + i) * p.ldx + c0;
+        T e[8];
+        if (r0 + i < p.rows && c0 + 8 <= p.cols) {
+            __builtin_memcpy(e, x, sizeof e);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) e[c] = r0 + i < p.rows && c0 + c < p.cols ? x[c] : (T)0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) v[i][c] = (float)e[c];
+    }
+    if (ROWS) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            unsigned a = 0;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) a = max(a, f8_magnitude(v[i][c]));
+            const int e = f8_exponent(f8_max16(a));
+            const float inv = f8_inverse(e);
+            if (r0 + i < p.rows) {
+                *reinterpret_cast<u32x2f *>(p.q + (r0 + i) * p.kp + c0) =
+                    u32x2f{(unsigned)f8_pack(v[i][0], v[i][1], v[i][2], v[i][3], inv), (unsigned)f8_pack(v[i][4], v[i][5], v[i][6], v[i][7], inv)};
+                if (cg == 0) {
+                    uint8_t *s = p.s + (r0 + i) * p.sp;
+                    s[kt] = (uint8_t)(e + 127);
+                    if (kt == p.tiles_k - 1)
+                        for (int k = kt + 1; k < p.sp; ++k) s[k] = 127;
+                }
+            }
+        }
+    }
+    if (COLS) {
+        unsigned a[8];
+        float s[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            a[c] = 0;
+            s[c] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                a[c] = max(a[c], f8_magnitude(v[i][c]));
+                s[c] += v[i][c];
+            }
+            a[c] = max(a[c], (unsigned)__shfl_xor((int)a[c], 16));
+            a[c] = max(a[c], (unsigned)__shfl_xor((int)a[c], 32));
+            s[c] += __shfl_xor(s[c], 16);
+            s[c] += __shfl_xor(s[c], 32);
+        }
+        if (rg % 4 == 0) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                amaxs[wave][cg * 8 + c] = a[c];
+                sums[wave][cg * 8 + c] = s[c];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            const int col = cg * 8 + c;
+            const int e = f8_exponent(max(max(amaxs[0][col], amaxs[1][col]), max(amaxs[2][col], amaxs[3][col])));
+            const float inv = f8_inverse(e);
+            *reinterpret_cast<u32x2f *>(tile + col * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + (rg & 1) * 8) =
+                u32x2f{(unsigned)f8_pack(v[0][c], v[1][c], v[2][c], v[3][c], inv), (unsigned)f8_pack(v[4][c], v[5][c], v[6][c], v[7][c], inv)};
+            if (rg == 0 && c0 + c < p.cols) {
+                uint8_t *st = p.st + (c0 + c) * p.spt;
+                st[rt] = (uint8_t)(e + 127);
+                if (rt == p.tiles_r - 1)
+                    for (int64_t k = rt + 1; k < p.spt; ++k) st[k] = 127;
+            }
+        }
+        __syncthreads();
+        if (p.sums && t < 128 && kt * 128 + t < p.cols)
+            p.sums[rt * p.cols + kt * 128 + t] = (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int col = t / 8 + 32 * k, slot = t % 8;
+            if (kt * 128 + col < p.cols)
+                *reinterpret_cast<i32x4f *>(p.qt + (int64_t)(kt * 128 + col) * p.rp + rt * 128 + slot * 16) =
+                    *reinterpret_cast<const i32x4f *>(tile + col * 128 + ((slot ^ ((col >> 3) & 7)) << 4));
+        }
+    }
+}
+
+__device__ __forceinline__ void f8_store_as(void *out, int64_t i, float v, int dtype) {
+    if (dtype == EVO_F32) ((float *)out)[i] = v;
+    else if (dtype == EVO_BF16) ((bf16_t *)out)[i] = (bf16_t)v;
+    else ((f16_t *)out)[i] = (f16_t)v;
+}
+
+// Column sums from those of 128 rows each: 32 columns by 32 slices of the parts.
+__global__ void __launch_bounds__(1024) fp8_sums(const float *part, void *out, int cols, int64_t parts, int dtype) {
+    __shared__ float sums[32][33];
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+    float s = 0.0f;
+    if (c < cols) {
+#pragma unroll 8
+        for (int64_t i = slice; i < parts; i += 32) s += part[i * cols + c];
+    }
+    sums[slice][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (slice || c >= cols) return;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sums[i][threadIdx.x];
+    f8_store_as(out, c, s, dtype);
+}
+
+// ---- product ----
+
+struct F8Matmul {
+    const uint8_t *a, *b;        // [M][kp], [N][kp]
+    const uint32_t *sa, *sb;     // [M][sd], [N][sd]: four blocks' scales each
+    const void *bias;
+    void *out;
+    int64_t ldo, kp;
+    int M, N, blocks, sd;        // blocks of the contraction
+    int mt, nt, slice;           // tiles; blocks of a slice, a multiple of four (or all)
+    int bias_dtype;
+};
+
+// 16-byte chunk c of row r of a staged tile (rows of 128 bytes): any chunk of 16 rows touches all banks once
+__device__ __forceinline__ int f8_swz(int r) { return ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1); }
+__device__ __forceinline__ int f8_at(int r, int c) { return r * 128 + ((c ^ f8_swz(r)) << 4); }
+// output that row r of a 32-row accumulator tile holds: lane group g ends up with outputs 16 g .. 16 g + 15 in register order
+__device__ __forceinline__ int f8_deal(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
+
+// 16 bytes per lane from base + offset to dst (uniform) + 16 * lane, as an instruction that the compiler does not count
+__device__ __forceinline__ void f8_dma(const uint8_t *base, int offset, unsigned char *dst) {
+    const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "m0", "memory");
+}
+// this wave's loads have landed, everybody's have, and everybody is done with the stage before
+__device__ __forceinline__ void f8_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int J>
+__device__ __forceinline__ f32x16 f8_mma(i32x8f a, i32x8f b, f32x16 c, int sa, int sb) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, J, sa, J, sb);
+}
+
+// Eight e4m3 values (two registers) with their scale as bf16.
+__device__ __forceinline__ bf16x8 f8_widen(int lo, int hi, float scale) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int w = i ? hi : lo;
+        const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+        r[4 * i] = x[0];
+        r[4 * i + 1] = x[1];
+        r[4 * i + 2] = y[0];
+        r[4 * i + 3] = y[1];
+    }
+    return r;
+}
+__device__ __forceinline__ float f8_scale(uint32_t four, int j) {
+    const unsigned byte = (four >> (8 * j)) & 0xff;
+    return __uint_as_float(byte ? byte << 23 : 0x400000u);
+}
+
+__device__ __forceinline__ float f8_bias(const void *b, int i, int dtype) {
+    return dtype == EVO_F32 ? ((const float *)b)[i] : dtype == EVO_BF16 ? (float)((const bf16_t *)b)[i] : (float)((const f16_t *)b)[i];
+}
+
+// Eight results of a row, of which the last may lie beyond it.
+template <typename T>
+__device__ __forceinline__ void f8_store8(T *p, const T (&e)[8], int left) {
+    if (left >= 8) {
+        __builtin_memcpy(p, e, sizeof e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) p[i] = e[i];
+    }
+}
+
+// out[m][n] (+ slice M N) = sum over the slice's blocks of a[m] . b[n], times the scales, + bias[n].  WM x WN waves of TM x TN tiles
+// of 32 x 32; outputs (rows of b) are the accumulators' rows, rows of a their columns.
+template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
+__global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
+    constexpr int W = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128, PIECES = (BM + BN) / 8 / W;
+    static_assert(BM / 8 % PIECES == 0, "a wave brings rows of one side");
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
+    const unsigned lid = xcd_remap(blockIdx.x, gridDim.x), tiles = p.mt * p.nt;
+    const int slice = lid / tiles;
+    // tiles of a band of eight rows of tiles one below the other: what runs at once on an XCD shares rows of both sides
+    constexpr int BAND = 8;
+    const int tile = lid % tiles, band = tile / (BAND * p.nt), high = min(BAND, p.mt - band * BAND);
+    const int m0 = (band * BAND + tile % (BAND * p.nt) % high) * BM, n0 = tile % (BAND * p.nt) / high * BN;
+    const int wm = wave % WM * TM * 32, wn = wave / WM * TN * 32;
+    const int first = slice * p.slice, nb = min(p.slice, p.blocks - first);
+
+    // this wave's pieces of a stage: eight rows of 128 bytes each
+    const bool tokens = wave * PIECES * 8 < BM;
+    const int at = wave * PIECES * 8 - (tokens ? 0 : BM), last = (tokens ? p.M - m0 : p.N - n0) - 1;
+    const uint8_t *base = (tokens ? p.a + (int64_t)m0 * p.kp : p.b + (int64_t)n0 * p.kp) + (int64_t)first * kF8Block;
+    int off[PIECES];
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int r = at + i * 8 + lane / 8, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
+        off[i] = min(row, last) * (int)p.kp + (((lane % 8) ^ f8_swz(r)) << 4);
+    }
+    auto fetch = [&](int s) {
+        unsigned char *to = lds8 + (s & 1) * STAGE + wave * PIECES * 1024;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) f8_dma(base + s * kF8Block, off[i], to + i * 1024);
+    };
+    const uint32_t *sa[TM], *sb[TN];
+#pragma unroll
+    for (int u = 0; u < TM; ++u) sa[u] = p.sa + (int64_t)min(m0 + wm + 32 * u + li, p.M - 1) * p.sd + first / 4;
+#pragma unroll
+    for (int t = 0; t < TN; ++t) sb[t] = p.sb + (int64_t)min(n0 + wn + 32 * t + f8_deal(li), p.N - 1) * p.sd + first / 4;
+    int xs[TM], ws[TN], xn[TM], wn4[TN];
+    auto scales = [&](int s4) {
+#pragma unroll
+        for (int u = 0; u < TM; ++u) xn[u] = (int)sa[u][s4];
+#pragma unroll
+        for (int t = 0; t < TN; ++t) wn4[t] = (int)sb[t][s4];
+    };
+
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int u = 0; u < TM; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][u][r] = 0.0f;
+
+    scales(0);
+    fetch(0);
+    for (int s4 = 0; s4 < nb; s4 += 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (s4 + j >= nb) break;
+            f8_sync();
+            if (j == 0) {   // asked for four stages ago: here, before the next loads are, and not where they are used
+#pragma unroll
+                for (int u = 0; u < TM; ++u) {
+                    asm volatile("" : "+v"(xn[u]));
+                    xs[u] = xn[u];
+                }
+#pragma unroll
+                for (int t = 0; t < TN; ++t) {
+                    asm volatile("" : "+v"(wn4[t]));
+                    ws[t] = wn4[t];
+                }
+                if (s4 + 4 < nb) scales(s4 / 4 + 1);
+            }
+            if (s4 + j + 1 < nb) fetch(s4 + j + 1);
+            const unsigned char *buf = lds8 + (j & 1) * STAGE;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                i32x8f b[TN], a[TM];
+                auto operand = [&](int row) {
+                    const i32x4f lo = *reinterpret_cast<const i32x4f *>(buf + f8_at(row, 4 * ks + 2 * g)),
+                                 hi = *reinterpret_cast<const i32x4f *>(buf + f8_at(row, 4 * ks + 2 * g + 1));
+                    return i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                };
+#pragma unroll
+                for (int t = 0; t < TN; ++t) b[t] = operand(BM + wn + 32 * t + li);
+#pragma unroll
+                for (int u = 0; u < TM; ++u) a[u] = operand(wm + 32 * u + li);
+                if constexpr (WIDE) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        bf16x8 bw[TN], aw[TM];
+#pragma unroll
+                        for (int t = 0; t < TN; ++t) bw[t] = f8_widen(b[t][2 * i], b[t][2 * i + 1], f8_scale(ws[t], j));
+#pragma unroll
+                        for (int u = 0; u < TM; ++u) aw[u] = f8_widen(a[u][2 * i], a[u][2 * i + 1], f8_scale(xs[u], j));
+#pragma unroll
+                        for (int t = 0; t < TN; ++t)
+#pragma unroll
+                            for (int u = 0; u < TM; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bw[t], aw[u], acc[t][u], 0, 0, 0);
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < TN; ++t)
+#pragma unroll
+                        for (int u = 0; u < TM; ++u)
+                            acc[t][u] = j == 0 ? f8_mma<0>(b[t], a[u], acc[t][u], ws[t], xs[u]) : j == 1 ? f8_mma<1>(b[t], a[u], acc[t][u], ws[t], xs[u])
+                                      : j == 2 ? f8_mma<2>(b[t], a[u], acc[t][u], ws[t], xs[u]) : f8_mma<3>(b[t], a[u], acc[t][u], ws[t], xs[u]);
+                }
+            }
+        }
+    }
+    // Through LDS, 32 rows of the wave's outputs at a time, so that neighbouring lanes store a row's pieces.
+    __syncthreads();
+    constexpr int ROW = TN * 32 * sizeof(T), CHUNKS = TN * 4;   // bytes of a row, chunks of eight results
+    static_assert(W * 32 * ROW <= 2 * STAGE, "what the waves hold at a time");
+    unsigned char *mine = lds8 + wave * 32 * ROW;
+    auto place = [](int r, int c) { return r * ROW + ((c ^ (r & (CHUNKS - 1))) * (int)(8 * sizeof(T))); };
+    T *out = (T *)p.out + (int64_t)slice * p.M * p.N;
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int o = n0 + wn + 32 * t + 16 * g + 8 * h;
+                T e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float b = p.bias && o + i < p.N ? f8_bias(p.bias, o + i, p.bias_dtype) : 0.0f;
+                    e[i] = (T)(acc[t][u][8 * h + i] + b);
+                }
+                __builtin_memcpy(__builtin_assume_aligned(mine + place(li, 4 * t + 2 * g + h), 16), e, sizeof e);
+            }
+        }
+        constexpr int RPI = 64 / CHUNKS;   // rows that the wave's lanes store at once
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = i * RPI + lane / CHUNKS, c = lane % CHUNKS, m = m0 + wm + 32 * u + r, o = n0 + wn + 8 * c;
+            T e[8];
+            __builtin_memcpy(e, __builtin_assume_aligned(mine + place(r, c), 16), sizeof e);
+            if (m < p.M && o < p.N) f8_store8(out + (int64_t)m * p.ldo + o, e, p.N - o);
+        }
+    }
+}
+
+// The slices' sums, eight columns per thread.
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, const void *bias, int bias_dtype, int64_t M, int N, int64_t ldo, int slices) {
+    const int pieces = (N + 7) / 8;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / pieces;
+    const int o = (int)(id % pieces) * 8;
+    if (m >= M) return;
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = 0.0f;
+    const float *x = part + m * N + o;
+    if (o + 8 <= N) {
+#pragma unroll 4
+        for (int k = 0; k < slices; ++k) {
+            float v[8];
+            __builtin_memcpy(v, x + (int64_t)k * M * N, sizeof v);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] += v[i];
+        }
+    } else {
+        for (int k = 0; k < slices; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (o + i < N) s[i] += x[(int64_t)k * M * N + i];
+    }
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (T)(bias && o + i < N ? s[i] + f8_bias(bias, o + i, bias_dtype) : s[i]);
+    f8_store8(out + m * ldo + o, e, N - o);
+}
+
+static int f8_rc() {
+    const hipError_t err = hipGetLastError();
+    return err == hipSuccess ? EVO_OK : EVO_EHIP - (int)err;
+}
+static bool f8_dtype(int d) { return d == EVO_BF16 || d == EVO_F16 || d == EVO_F32; }
+static bool f8_off(const void *p, int n) { return ((uintptr_t)p & (n - 1)) != 0; }
+template <typename F>
+static int f8_by_dtype(int dtype, F &&f) {
+    return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
+}
+
+constexpr int64_t kF8MaxK = 1 << 22;   // of the contraction: a tile's rows stay within 32-bit offsets
+
+// How a product is cut: into slices of the contraction where there are too few tiles for the chip.
+struct F8Plan {
+    int mt, nt, slice, slices;
+};
+static F8Plan f8_plan(int64_t m, int64_t n, int64_t k) {
+    F8Plan q{};
+    q.mt = (int)((m + 127) / 128);
+    q.nt = (int)((n + 127) / 128);
+    const int blocks = (int)((k + kF8Block - 1) / kF8Block);
+    const int64_t tiles = (int64_t)q.mt * q.nt;
+    int64_t want = tiles >= 256 ? 1 : 512 / tiles;
+    if (want > blocks / 8) want = blocks / 8;
+    if (want < 1) want = 1;
+    q.slice = (int)((blocks + want - 1) / want + 3) / 4 * 4;
+    q.slices = (blocks + q.slice - 1) / q.slice;
+    if (q.slices == 1) q.slice = blocks;
+    return q;
+}
+
+static int f8_check(const EvoFp8Matmul *p) {
+    if (!p || p->m <= 0 || p->n <= 0 || p->k <= 0 || !f8_dtype(p->dtype)) return EVO_EINVAL;
+    if (p->m > INT32_MAX - 512 || p->n > INT32_MAX - 512) return EVO_EOVERFLOW;
+    if (p->k > kF8MaxK) return EVO_EUNSUPPORTED;
+    const F8Plan q = f8_plan(p->m, p->n, p->k);
+    if ((int64_t)q.mt * q.nt > INT32_MAX || (int64_t)q.mt * q.nt * q.slices > INT32_MAX) return EVO_EOVERFLOW;
+    return EVO_OK;
+}
+
+template <typename T, bool WIDE>
+static int f8_launch(const F8Matmul &a, unsigned grid, hipStream_t st) {
+    constexpr int lds = 2 * 256 * 128;
+    constexpr auto kernel = fp8_matmul<2, 2, 2, 2, T, WIDE>;
+    static PerDevice done;
+    if (const int rc = ensure_dynamic_lds((const void *)kernel, lds, done, nullptr)) return rc;
+    kernel<<<grid, 256, lds, st>>>(a);
+    return f8_rc();
+}
+
+}  // namespace evo
+
+extern "C" {
+
+int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void *qt, void *scales_t, float *sums, int64_t rows, int64_t cols, int32_t dtype,
+                         void *hip_stream) {
+    using namespace evo;
+    if (!x || rows <= 0 || cols <= 0 || ldx < cols || !f8_dtype(dtype) || !q != !scales || !qt != !scales_t || (!q && !qt) || (sums && !qt)) return EVO_EINVAL;
+    if (cols > kF8MaxK || (qt && rows > ((int64_t)1 << 40))) return EVO_EUNSUPPORTED;
+    if (f8_off(q, 16) || f8_off(qt, 16)) return EVO_EALIGN;
+    F8Quantize p{};
+    p.x = x;
+    p.ldx = ldx;
+    p.rows = rows;
+    p.cols = (int)cols;
+    p.kp = f8_pitch(cols);
+    p.sp = (int)f8_scale_pitch(cols);
+    p.tiles_k = (int)(p.kp / kF8Block);
+    p.rp = f8_pitch(rows);
+    p.spt = f8_scale_pitch(rows);
+    p.tiles_r = p.rp / kF8Block;
+    p.q = (uint8_t *)q;
+    p.s = (uint8_t *)scales;
+    p.qt = (uint8_t *)qt;
+    p.st = (uint8_t *)scales_t;
+    p.sums = sums;
+    if (p.tiles_r > INT32_MAX / p.tiles_k) return EVO_EOVERFLOW;
+    const unsigned grid = (unsigned)(p.tiles_r * p.tiles_k);
+    hipStream_t st = (hipStream_t)hip_stream;
+    return f8_by_dtype(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (q && qt) fp8_quantize<T, true, true><<<grid, kF8Threads, 0, st>>>(p);
+        else if (q) fp8_quantize<T, true, false><<<grid, kF8Threads, 0, st>>>(p);
+        else fp8_quantize<T, false, true><<<grid, kF8Threads, 0, st>>>(p);
+        return f8_rc();
+    });
+}
+
+int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t cols, int32_t dtype, void *hip_stream) {
+    using namespace evo;
+    if (!sums || !out || rows <= 0 || cols <= 0 || !f8_dtype(dtype)) return EVO_EINVAL;
+    if (cols > kF8MaxK) return EVO_EUNSUPPORTED;
+    fp8_sums<<<(unsigned)((cols + 31) / 32), 1024, 0, (hipStream_t)hip_stream>>>(sums, out, (int)cols, (rows + kF8Block - 1) / kF8Block, dtype);
+    return f8_rc();
+}
+
+size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p) {
+    using namespace evo;
+    if (f8_check(p)) return 0;
+    const F8Plan q = f8_plan(p->m, p->n, p->k);
+    return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
+}
+
+int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
+    using namespace evo;
+    if (const int rc = f8_check(p)) return rc;
+    if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
+    if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
+    const F8Plan q = f8_plan(p->m, p->n, p->k);
+    if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
+    F8Matmul a{};
+    a.a = (const uint8_t *)p->a;
+    a.b = (const uint8_t *)p->b;
+    a.sa = (const uint32_t *)p->scales_a;
+    a.sb = (const uint32_t *)p->scales_b;
+    a.bias = q.slices > 1 ? nullptr : p->bias;
+    a.out = q.slices > 1 ? p->workspace : p->out;
+    a.ldo = q.slices > 1 ? p->n : p->ldo;
+    a.kp = f8_pitch(p->k);
+    a.M = (int)p->m;
+    a.N = (int)p->n;
+    a.blocks = (int)(a.kp / kF8Block);
+    a.sd = (int)(f8_scale_pitch(p->k) / 4);
+    a.mt = q.mt;
+    a.nt = q.nt;
+    a.slice = q.slice;
+    a.bias_dtype = p->bias_dtype;
+    const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
+    hipStream_t st = (hipStream_t)hip_stream;
+    const bool wide = p->dtype == EVO_F32;
+    if (q.slices == 1) {
+        return p->dtype == EVO_F32 ? f8_launch<float, true>(a, grid, st) : p->dtype == EVO_BF16 ? f8_launch<bf16_t, false>(a, grid, st) : f8_launch<f16_t, false>(a, grid, st);
+    }
+    if (const int rc = wide ? f8_launch<float, true>(a, grid, st) : f8_launch<float, false>(a, grid, st)) return rc;
+    return f8_by_dtype(p->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        const int64_t pieces = p->m * ((p->n + 7) / 8), groups = (pieces + 255) / 256;
+        if (groups > INT32_MAX) return (int)EVO_EOVERFLOW;
+        fp8_slices<T><<<(unsigned)groups, 256, 0, st>>>((const float *)p->workspace, (T *)p->out, p->bias, p->bias_dtype, p->m, (int)p->n, p->ldo, q.slices);
+        return f8_rc();
+    });
+}
+
+}  // extern "C"

@@ -1095,6 +1095,7 @@ OptTensor block(const std::vector<OptTensor> &in, const OptTensor &keep, int64_t
 }
 
 #include "host_relative.h"
+#include "host_fp8.h"
 
 }  // namespace
 
@@ -1114,4 +1115,12 @@ PYBIND11_MODULE(_host, m) {
     m.def("relative_bias_forward", &relative_bias_forward, no_gil);
     m.def("relative_bias_backward", &relative_bias_backward, no_gil);
     m.def("relative_bias_wrong", &relative_bias_wrong, no_gil);
+    m.def("fp8_linear", &fp8_linear, no_gil);
+    m.def("fp8_linear_held", &fp8_linear_held, no_gil);
+    m.def("fp8_linear_forward", &fp8_linear_forward, no_gil);
+    m.def("fp8_linear_backward", &fp8_linear_backward, no_gil);
+    m.def("fp8_linear_held_forward", &fp8_linear_held_forward, no_gil);
+    m.def("fp8_linear_wrong", &fp8_linear_wrong, no_gil);
+    m.def("fp8_linear_held_wrong", &fp8_linear_held_wrong, no_gil);
+    m.def("fp8_round", &fp8_round, no_gil);
 }

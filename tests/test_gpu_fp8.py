@@ -1,0 +1,135 @@
+"""Linear layers in 8 bits on the GPU against their definition in 64 bits.
+
+The rounding is exact: bytes and scales are compared as such.  A product is held to the rounding of its result (half a step), and to
+that of its sums: in fp32, where every addition may lose a step of what it has added up to, K 2^-23 of the sum of magnitudes; with a
+16-bit result the 8-bit matrix instruction's, of which neighbouring products are cut off 13 bits below the largest of
+them: each loses up to 2^-13 of a product that is in the sum as well, eight neighbours 2^-10 of the largest."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _rounded(x):
+    """Q along the last axis: (values in units of the scale, exponents), 64 bits, on the CPU."""
+    k = x.shape[-1]
+    v = torch.zeros((*x.shape[:-1], -(-k // 128) * 128), dtype=torch.float64)
+    v[..., :k] = x.double().cpu()
+    v = v.unflatten(-1, (-1, 128))
+    a = torch.where(v.isfinite(), v.abs(), 0).amax(-1, keepdim=True)
+    m, e = torch.frexp(a)
+    e = torch.where(a == 0, 0, torch.where(m > 0.875, e - 8, e - 9).clamp(-127, 127))
+    u = torch.ldexp(v, -e)
+    u = torch.where(u.isfinite(), u, float("nan"))
+    step = torch.exp2(torch.floor(torch.log2(torch.where((u == 0) | u.isnan(), 1.0, u.abs()))).clamp(-6, 8) - 3)
+    return torch.round(u / step) * step, e.squeeze(-1)
+
+
+def _q(x):
+    u, e = _rounded(x)
+    return torch.ldexp(u, e.unsqueeze(-1)).flatten(-2)[..., :x.shape[-1]]
+
+
+def _near(got, want, magnitudes, K):
+    """Whether `got` is within its own and its sums' rounding of `want`."""
+    f = torch.finfo(got.dtype)
+    sums = magnitudes * (K * 2 ** -23 if got.dtype == F32 else 2 ** -10 + K * 2 ** -23)
+    bound = sums + (want.abs() + sums) * (f.eps / 2) + f.tiny * f.eps
+    d = (got.detach().cpu().double() - want).abs()
+    assert (d <= bound).all(), ((d / bound).max().item(), (d > bound).sum().item())
+
+
+def _data(shape, dt, g, spread=1.0):
+    return (torch.randn(shape, generator=g) * torch.exp(spread * torch.randn(shape[-1:], generator=g))).to(dt)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16, F32])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 128), (5, 129), (127, 40), (128, 512), (130, 641), (300, 200)])
+def test_rounding_is_the_definitions(gpu_device, dt, shape):
+    from evoformer_triton_amd import Fp8Weight
+    g = torch.Generator().manual_seed(1)
+    x = _data(shape, dt, g)
+    x[0, 0] = 0
+    x.view(-1)[-1] = -0.0
+    if shape[1] >= 128:
+        x[1, :128] = 0                                                       # a block of zeros
+        x[2, :4] = torch.tensor([448., 232., 248., 1.0625]).to(dt)            # ties, up and down
+        x[2, 4:128] = 0
+    w = Fp8Weight.of(x.to(gpu_device))
+    u, e = _rounded(x)
+    assert w.values.dtype == torch.float8_e4m3fn and w.values.shape == (shape[0], u.shape[1] * 128) and w.scales.shape == (shape[0], -(-u.shape[1] // 4) * 4)
+    assert torch.equal(w.values.cpu().double(), u.flatten(-2))
+    assert torch.equal(w.scales.cpu()[:, :u.shape[1]].int() - 127, e.int()) and (w.scales[:, u.shape[1]:] == 127).all()
+    assert torch.equal(w.dequantize().cpu().double(), _q(x).float().double())
+
+
+def test_rounding_at_the_ends_of_fp32(gpu_device):
+    from evoformer_triton_amd import Fp8Weight
+    inf, nan, big, tiny = float("inf"), float("nan"), torch.finfo(F32).max, 2.0 ** -149
+    x = torch.zeros(8, 128)
+    x[0, :5] = torch.tensor([inf, 3.0, -inf, nan, -448.0])        # found by the finite ones
+    x[1, :2] = torch.tensor([inf, nan])                            # nothing finite but zeros
+    x[2, :3] = torch.tensor([big, -big, 1.0])
+    x[3, :3] = torch.tensor([tiny, -tiny, 3 * tiny])
+    x[4, :2] = torch.tensor([448 * 2.0 ** -127, 2.0 ** -136])
+    x[5, :2] = torch.tensor([1.75, 1.75 * 2.0 ** -20])
+    x[6, :2] = torch.tensor([1.7500001, -1.0])
+    w = Fp8Weight.of(x.to(gpu_device))
+    u, e = _rounded(x)
+    got = w.values.cpu().double()
+    assert torch.equal(got.isnan(), u.flatten(-2).isnan()) and torch.equal(got.nan_to_num(), u.flatten(-2).nan_to_num())
+    assert torch.equal(w.scales.cpu()[:, :1].int() - 127, e.int())
+
+
+# rows, k, n, bias, x, weight, bias dtypes
+CASES = [
+    (1, 1, 1, True, BF16, BF16, BF16),
+    (1, 256, 1024, False, BF16, BF16, None),
+    (5, 128, 3, True, F32, F32, F32),
+    (17, 200, 130, True, F16, F32, F16),
+    (64, 640, 257, False, F32, BF16, None),
+    (129, 129, 127, True, BF16, BF16, F32),           # a tile and a row; a block and a value
+    (300, 1100, 96, True, F16, F16, F16),             # three groups of four blocks
+    (2500, 96, 40, True, BF16, F32, BF16),            # the weight's gradient in slices of the rows
+    (2500, 640, 200, False, F32, F32, None),
+    (128, 4224, 64, True, BF16, BF16, BF16),          # the forward in slices of the contraction
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(str(x).replace("torch.", "") for x in c))
+def test_products_and_gradients(gpu_device, case):
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    rows, k, n, with_bias, dt, wdt, bdt = case
+    g = torch.Generator().manual_seed(17)
+    x, w = _data((rows, k), dt, g), (_data((n, k), F32, g, 0.5) * k ** -0.5).to(wdt)
+    b = torch.randn((n,), generator=g).to(bdt) if with_bias else None
+    dy = (torch.randn((rows, n), generator=g) * torch.exp(torch.randn((rows, 1), generator=g) - 4)).to(dt)
+    if rows > 4:
+        x[3], dy[3] = 0, 0
+    leaves = [t.to(gpu_device).requires_grad_() for t in (x, w) + ((b,) if with_bias else ())]
+    y = fp8_linear(leaves[0], leaves[1], leaves[2] if with_bias else None)
+    assert y.grad_fn.name() == "Fp8LinearBackward" and y.dtype == dt
+    got = torch.autograd.grad(y, leaves, dy.to(gpu_device), retain_graph=True)
+    assert [t.dtype for t in got] == [t.dtype for t in leaves]
+
+    def product(a, bt):
+        return a @ bt.t(), a.abs() @ bt.abs().t()
+
+    want, size = product(_q(x), _q(w))
+    if with_bias:
+        want, size = want + b.double(), size + b.double().abs()
+    _near(y, want, size, k)
+    _near(got[0], *product(_q(dy), _q(w.t())), n)
+    _near(got[1], *product(_q(dy.t()), _q(x.t())), rows)
+    if with_bias:
+        _near(got[2].float() if bdt == F32 else got[2], dy.double().sum(0), dy.double().abs().sum(0), rows)
+    again = torch.autograd.grad(y, leaves, dy.to(gpu_device))
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
+    for i, t in enumerate(leaves):      # one gradient at a time
+        y1 = fp8_linear(*(u if j == i else u.detach() for j, u in enumerate(leaves)))
+        assert torch.equal(y1, y) and torch.equal(torch.autograd.grad(y1, t, dy.to(gpu_device))[0], got[i])
+    with torch.no_grad():
+        held = fp8_linear(leaves[0], Fp8Weight.of(leaves[1]), leaves[2] if with_bias else None)
+    assert torch.equal(held, y)
