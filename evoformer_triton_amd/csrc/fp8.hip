@@ -69,18 +69,20 @@ __global__ void __launch_bounds__(kF8Threads) fp8_quantize(F8Quantize p) {
     const int c0 = kt * 128 + cg * 8;
     const int64_t r0 = rt * 128 + rg * 8;
     float v[V][8];
+    const T *x = (const T *)p.x + r0 * p.ldx + c0;
+    if ((rt + 1) * 128 <= p.rows && (kt + 1) * 128 <= p.cols) {   // uniform: all loads under way together
+        T e[V][8];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        const T *x = (const T *)p.x + (r0 + i) * p.ldx + c0;
-        T e[8];
-        if (r0 + i < p.rows && c0 + 8 <= p.cols) {
-            __builtin_memcpy(e, x, sizeof e);
-        } else {
+        for (int i = 0; i < V; ++i) __builtin_memcpy(e[i], x + i * p.ldx, sizeof e[i]);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) e[c] = r0 + i < p.rows && c0 + c < p.cols ? x[c] : (T)0.0f;
-        }
+        for (int i = 0; i < V; ++i)
 #pragma unroll
-        for (int c = 0; c < 8; ++c) v[i][c] = (float)e[c];
+            for (int c = 0; c < 8; ++c) v[i][c] = (float)e[i][c];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) v[i][c] = r0 + i < p.rows && c0 + c < p.cols ? (float)x[i * p.ldx + c] : 0.0f;
     }
     if (ROWS) {
 #pragma unroll
@@ -301,6 +303,8 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
 
     scales(0);
     fetch(0);
+    float *bias = reinterpret_cast<float *>(lds8 + 2 * STAGE);
+    for (int i = threadIdx.x; i < BN; i += W * 64) bias[i] = p.bias && n0 + i < p.N ? f8_bias(p.bias, n0 + i, p.bias_dtype) : 0.0f;
     for (int s4 = 0; s4 < nb; s4 += 4) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -370,13 +374,10 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
         for (int t = 0; t < TN; ++t) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int o = n0 + wn + 32 * t + 16 * g + 8 * h;
+                const f32x4 *b = reinterpret_cast<const f32x4 *>(bias + wn + 32 * t + 16 * g + 8 * h);
                 T e[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float b = p.bias && o + i < p.N ? f8_bias(p.bias, o + i, p.bias_dtype) : 0.0f;
-                    e[i] = (T)(acc[t][u][8 * h + i] + b);
-                }
+                for (int i = 0; i < 8; ++i) e[i] = (T)(acc[t][u][8 * h + i] + b[i / 4][i % 4]);
                 __builtin_memcpy(__builtin_assume_aligned(mine + place(li, 4 * t + 2 * g + h), 16), e, sizeof e);
             }
         }
@@ -435,15 +436,18 @@ static int f8_by_dtype(int dtype, F &&f) {
 
 constexpr int64_t kF8MaxK = 1 << 22;   // of the contraction: a tile's rows stay within 32-bit offsets
 
-// How a product is cut: into slices of the contraction where there are too few tiles for the chip.
+// How a product is cut: tiles of 256 x 256 or 128 x 128, and into slices of the contraction where there are too few for the chip.
 struct F8Plan {
     int mt, nt, slice, slices;
+    bool big;
 };
-static F8Plan f8_plan(int64_t m, int64_t n, int64_t k) {
+static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
     F8Plan q{};
-    q.mt = (int)((m + 127) / 128);
-    q.nt = (int)((n + 127) / 128);
     const int blocks = (int)((k + kF8Block - 1) / kF8Block);
+    q.big = dtype != EVO_F32 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
+    const int side = q.big ? 256 : 128;
+    q.mt = (int)((m + side - 1) / side);
+    q.nt = (int)((n + side - 1) / side);
     const int64_t tiles = (int64_t)q.mt * q.nt;
     int64_t want = tiles >= 256 ? 1 : 512 / tiles;
     if (want > blocks / 8) want = blocks / 8;
@@ -458,19 +462,27 @@ static int f8_check(const EvoFp8Matmul *p) {
     if (!p || p->m <= 0 || p->n <= 0 || p->k <= 0 || !f8_dtype(p->dtype)) return EVO_EINVAL;
     if (p->m > INT32_MAX - 512 || p->n > INT32_MAX - 512) return EVO_EOVERFLOW;
     if (p->k > kF8MaxK) return EVO_EUNSUPPORTED;
-    const F8Plan q = f8_plan(p->m, p->n, p->k);
+    const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     if ((int64_t)q.mt * q.nt > INT32_MAX || (int64_t)q.mt * q.nt * q.slices > INT32_MAX) return EVO_EOVERFLOW;
     return EVO_OK;
 }
 
-template <typename T, bool WIDE>
-static int f8_launch(const F8Matmul &a, unsigned grid, hipStream_t st) {
-    constexpr int lds = 2 * 256 * 128;
-    constexpr auto kernel = fp8_matmul<2, 2, 2, 2, T, WIDE>;
+template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
+static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
+    constexpr int lds = 2 * 32 * (WM * TM + WN * TN) * 128 + 32 * WN * TN * 4;
+    constexpr auto kernel = fp8_matmul<WM, WN, TM, TN, T, WIDE>;
     static PerDevice done;
     if (const int rc = ensure_dynamic_lds((const void *)kernel, lds, done, nullptr)) return rc;
-    kernel<<<grid, 256, lds, st>>>(a);
+    kernel<<<grid, WM * WN * 64, lds, st>>>(a);
     return f8_rc();
+}
+template <typename T, bool WIDE>
+static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
+    const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
+    if constexpr (!WIDE) {
+        if (q.big) return f8_launch_tiles<2, 4, 4, 2, T, WIDE>(a, grid, st);
+    }
+    return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
 }
 
 }  // namespace evo
@@ -522,7 +534,7 @@ int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t 
 size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p) {
     using namespace evo;
     if (f8_check(p)) return 0;
-    const F8Plan q = f8_plan(p->m, p->n, p->k);
+    const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
 
@@ -531,7 +543,7 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     if (const int rc = f8_check(p)) return rc;
     if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
-    const F8Plan q = f8_plan(p->m, p->n, p->k);
+    const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
     F8Matmul a{};
     a.a = (const uint8_t *)p->a;
@@ -550,13 +562,12 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     a.nt = q.nt;
     a.slice = q.slice;
     a.bias_dtype = p->bias_dtype;
-    const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
     hipStream_t st = (hipStream_t)hip_stream;
     const bool wide = p->dtype == EVO_F32;
     if (q.slices == 1) {
-        return p->dtype == EVO_F32 ? f8_launch<float, true>(a, grid, st) : p->dtype == EVO_BF16 ? f8_launch<bf16_t, false>(a, grid, st) : f8_launch<f16_t, false>(a, grid, st);
+        return p->dtype == EVO_F32 ? f8_launch<float, true>(a, q, st) : p->dtype == EVO_BF16 ? f8_launch<bf16_t, false>(a, q, st) : f8_launch<f16_t, false>(a, q, st);
     }
-    if (const int rc = wide ? f8_launch<float, true>(a, grid, st) : f8_launch<float, false>(a, grid, st)) return rc;
+    if (const int rc = wide ? f8_launch<float, true>(a, q, st) : f8_launch<float, false>(a, q, st)) return rc;
     return f8_by_dtype(p->dtype, [&](auto t) {
         typedef decltype(t) T;
         const int64_t pieces = p->m * ((p->n + 7) / 8), groups = (pieces + 255) / 256;
