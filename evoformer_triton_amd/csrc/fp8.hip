@@ -5,9 +5,17 @@
 // each operand rounded along the axis that its product contracts.
 #include <type_traits>
 
-#include "fp8_common.h"
+#include "common.h"
+#include "bwd_common.h"
+#include "kernels.h"
 
 namespace evo {
+
+constexpr int kF8Block = 128;   // elements that share a scale
+
+typedef int i32x8f __attribute__((ext_vector_type(8)));
+typedef int i32x4f __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2f __attribute__((ext_vector_type(2)));
 
 static int64_t f8_pitch(int64_t k) { return (k + kF8Block - 1) / kF8Block * kF8Block; }             // bytes of a rounded row
 static int64_t f8_scale_pitch(int64_t k) { return (k + 4 * kF8Block - 1) / (4 * kF8Block) * 4; }   // bytes of its scales
@@ -174,6 +182,120 @@ __global__ void __launch_bounds__(1024) fp8_sums(const float *part, void *out, i
 
 // ---- product ----
 
+struct F8Matmul {
+    const uint8_t *a, *b;        // [M][kp], [N][kp]
+    const uint32_t *sa, *sb;     // [M][sd], [N][sd]: four blocks' scales each
+    const void *bias;
+    void *out;
+    int64_t ldo, kp;
+    int M, N, blocks, sd;        // blocks of the contraction
+    int mt, nt, slice;           // tiles; blocks of a slice, a multiple of four (or all)
+    int bias_dtype;
+};
+
+// 16-byte chunk c of row r of a staged tile (rows of 128 bytes): any chunk of 16 rows touches all banks once
+__device__ __forceinline__ int f8_swz(int r) { return ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1); }
+__device__ __forceinline__ int f8_at(int r, int c) { return r * 128 + ((c ^ f8_swz(r)) << 4); }
+// output that row r of a 32-row accumulator tile holds: lane group g ends up with outputs 16 g .. 16 g + 15 in register order
+__device__ __forceinline__ int f8_deal(int r) { return 16 * ((r >> 2) & 1) + 4 * (r >> 3) + (r & 3); }
+
+// 16 bytes per lane from base + offset to dst (uniform) + 16 * lane, as an instruction that the compiler does not count
+__device__ __forceinline__ void f8_dma(const uint8_t *base, int offset, unsigned char *dst) {
+    const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(offset), "s"(base) : "m0", "memory");
+}
+// 4 bytes per lane
+__device__ __forceinline__ void f8_dma4(const uint32_t *base, int offset, unsigned char *dst) {
+    const unsigned to = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dword %1, %2" : : "s"(to), "v"(offset), "s"(base) : "m0", "memory");
+}
+// this wave's loads have landed, everybody's have, and everybody is done with the stage before
+__device__ __forceinline__ void f8_sync() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <int J>
+__device__ __forceinline__ f32x16 f8_mma(i32x8f a, i32x8f b, f32x16 c, int sa, int sb) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, J, sa, J, sb);
+}
+
+// Eight e4m3 values (two registers) with their scale as bf16.
+__device__ __forceinline__ bf16x8 f8_widen(int lo, int hi, float scale) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x8 r;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int w = i ? hi : lo;
+        const bf16x2 x = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false), y = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true);
+        r[4 * i] = x[0];
+        r[4 * i + 1] = x[1];
+        r[4 * i + 2] = y[0];
+        r[4 * i + 3] = y[1];
+    }
+    return r;
+}
+__device__ __forceinline__ float f8_scale(uint32_t four, int j) {
+    const unsigned byte = (four >> (8 * j)) & 0xff;
+    return __uint_as_float(byte ? byte << 23 : 0x400000u);
+}
+
+__device__ __forceinline__ float f8_bias(const void *b, int i, int dtype) {
+    return dtype == EVO_F32 ? ((const float *)b)[i] : dtype == EVO_BF16 ? (float)((const bf16_t *)b)[i] : (float)((const f16_t *)b)[i];
+}
+
+// Eight results of a row, of which the last may lie beyond it.
+template <typename T>
+__device__ __forceinline__ void f8_store8(T *p, const T (&e)[8], int left) {
+    if (left >= 8) {
+        __builtin_memcpy(p, e, sizeof e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < left) p[i] = e[i];
+    }
+}
+
+// A workgroup's slice and tile.  Tiles of a band of eight rows of tiles come one below the other: what runs at once on an XCD shares rows of both sides.
+__device__ __forceinline__ void f8_tile(const F8Matmul &p, int &slice, int &mt, int &nt) {
+    constexpr unsigned BAND = 8;
+    const unsigned lid = xcd_remap(blockIdx.x, gridDim.x), tiles = p.mt * p.nt, tile = lid % tiles, band = tile / (BAND * p.nt), in = tile % (BAND * p.nt);
+    const unsigned high = min(BAND, p.mt - band * BAND);
+    slice = lid / tiles;
+    mt = band * BAND + in % high;
+    nt = in / high;
+}
+
+// A wave's results, TM x TN tiles of 32 x 32, to memory: through LDS, 32 rows at a time, so that neighbouring lanes store a row's pieces.
+template <int W, int TM, int TN, typename T>
+__device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const F8Matmul &p, unsigned char *lds, const float *bias, int wave, int lane, int m0,
+                                              int n0, int wm, int wn, int slice) {
+    constexpr int ROW = TN * 32 * sizeof(T), CHUNKS = TN * 4;   // bytes of a row, chunks of eight results
+    const int li = lane & 31, g = lane >> 5;
+    unsigned char *mine = lds + wave * 32 * ROW;
+    auto place = [](int r, int c) { return r * ROW + ((c ^ (r & (CHUNKS - 1))) * (int)(8 * sizeof(T))); };
+    T *out = (T *)p.out + (int64_t)slice * p.M * p.N;
+#pragma unroll
+    for (int u = 0; u < TM; ++u) {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 *b = reinterpret_cast<const f32x4 *>(bias + wn + 32 * t + 16 * g + 8 * h);
+                T e[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = (T)(acc[t][u][8 * h + i] + b[i / 4][i % 4]);
+                __builtin_memcpy(__builtin_assume_aligned(mine + place(li, 4 * t + 2 * g + h), 16), e, sizeof e);
+            }
+        }
+        constexpr int RPI = 64 / CHUNKS;   // rows that the wave's lanes store at once
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+            const int r = i * RPI + lane / CHUNKS, c = lane % CHUNKS, m = m0 + wm + 32 * u + r, o = n0 + wn + 8 * c;
+            T e[8];
+            __builtin_memcpy(e, __builtin_assume_aligned(mine + place(r, c), 16), sizeof e);
+            if (m < p.M && o < p.N) f8_store8(out + (int64_t)m * p.ldo + o, e, p.N - o);
+        }
+    }
+}
+
 // out[m][n] (+ slice M N) = sum over the slice's blocks of a[m] . b[n], times the scales, + bias[n].  WM x WN waves of TM x TN tiles
 // of 32 x 32; outputs (rows of b) are the accumulators' rows, rows of a their columns.
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
@@ -184,7 +306,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
     int slice, m0, n0;
-    f8_tile(p, xcd_remap(blockIdx.x, gridDim.x), slice, m0, n0);
+    f8_tile(p, slice, m0, n0);
     m0 *= BM;
     n0 *= BN;
     const int wm = wave % WM * TM * 32, wn = wave / WM * TN * 32;
@@ -290,6 +412,131 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     f8_store_tile<W, TM, TN, T>(acc, p, lds8, bias, wave, lane, m0, n0, wm, wn, slice);
 }
 
+// The same for large products: tiles of 256 x 256, eight waves of 128 x 64, 64 of the contraction at a time in a ring of four stages of 32 KB.
+// The two waves of a SIMD take turns: between two barriers one of them reads its operands (and asks for a stage) while the other
+// multiplies.  Waves 4 to 7 run one barrier behind waves 0 to 3.
+//
+// Step s: a wave reads stage s, asks for stage s + 3 into the place of stage s - 1, which the other half has read before the last barrier;
+// barrier; eight products; barrier.  Stage s + 1 is first read by waves 0 to 3 after their step s: before that barrier every wave's loads of it
+// have landed.  That is the end of step s for waves 0 to 3 and the middle of it for waves 4 to 7, when stages s + 2 and s + 3 are still under way.
+template <typename T>
+__global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
+    constexpr int W = 8, TM = 4, TN = 2, BM = 256, BN = 256, STAGE = (BM + BN) * 64, RING = 4, PIECES = 4;
+    constexpr int SCALES = RING * STAGE, BIAS = SCALES + 2 * (BM + BN) * 4;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
+    int slice, m0, n0;
+    f8_tile(p, slice, m0, n0);
+    m0 *= BM;
+    n0 *= BN;
+    const bool late = wave >= 4;
+    const int wm = (wave & 1) * 128, wn = (wave >> 1) * 64;
+    const int first = slice * p.slice, nb = min(p.slice, p.blocks - first), ns = 2 * nb;
+
+    // this wave's pieces of a stage, 16 rows of 64 bytes each: rows of a from waves 0, 2, 4, 6, of b from the others
+    const bool tokens = (wave & 1) == 0;
+    const int at = (wave >> 1) * 64, last = (tokens ? p.M - m0 : p.N - n0) - 1;
+    const uint8_t *base = (tokens ? p.a + (int64_t)m0 * p.kp : p.b + (int64_t)n0 * p.kp) + (int64_t)first * kF8Block;
+    const uint32_t *sbase = (tokens ? p.sa + (int64_t)m0 * p.sd : p.sb + (int64_t)n0 * p.sd) + first / 4;
+    int off[PIECES], soff;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+        const int r = at + i * 16 + lane / 4, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
+        off[i] = min(row, last) * (int)p.kp + (((lane % 4) ^ ((r >> 2) & 3)) << 4);
+    }
+    {
+        const int r = at + lane, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
+        soff = min(row, last) * p.sd * 4;
+    }
+    unsigned char *to = lds8 + (tokens ? 0 : BM * 64) + at * 64;
+    auto fetch = [&](int s) {
+        unsigned char *dst = to + (s & 3) * STAGE;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) f8_dma(base + s * 64, off[i], dst + i * 1024);
+    };
+    auto fetch_scales = [&](int s8) {   // of steps 8 s8 .. 8 s8 + 7
+        f8_dma4(sbase + s8, soff, lds8 + SCALES + (s8 & 1) * (BM + BN) * 4 + ((tokens ? 0 : BM) + at) * 4);
+    };
+
+    f32x16 acc[TN][TM];
+#pragma unroll
+    for (int t = 0; t < TN; ++t)
+#pragma unroll
+        for (int u = 0; u < TM; ++u)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][u][r] = 0.0f;
+
+    float *bias = reinterpret_cast<float *>(lds8 + BIAS);
+    if (threadIdx.x < BN) bias[threadIdx.x] = p.bias && n0 + (int)threadIdx.x < p.N ? f8_bias(p.bias, n0 + threadIdx.x, p.bias_dtype) : 0.0f;
+    fetch_scales(0);
+    fetch(0);
+    fetch(1);                          // (two steps at least)
+    if (ns > 2) fetch(2);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (late) asm volatile("s_barrier" ::: "memory");
+
+    const int rs = (li >> 2) & 3;
+    const unsigned char *ap = lds8 + (wm + li) * 64, *bp = lds8 + BM * 64 + (wn + li) * 64;
+    const int c0 = ((2 * g) ^ rs) << 4, c1 = ((2 * g + 1) ^ rs) << 4;
+    int xs[TM], ws[TN];
+    auto steps = [&](auto half) {
+        constexpr bool LATE = decltype(half)::value;
+        for (int s8 = 0; s8 < ns; s8 += 8) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int s = s8 + j;
+                if (j % 2 == 0 && s >= ns) break;
+                if (j == 0) {
+                    const int *x = reinterpret_cast<const int *>(lds8 + SCALES + ((s8 >> 3) & 1) * (BM + BN) * 4);
+#pragma unroll
+                    for (int u = 0; u < TM; ++u) xs[u] = x[wm + 32 * u + li];
+#pragma unroll
+                    for (int t = 0; t < TN; ++t) ws[t] = x[BM + wn + 32 * t + li];
+                    if (s8 + 8 < ns) fetch_scales(s8 / 8 + 1);
+                }
+                const int slot = (j & 3) * STAGE;
+                i32x8f b[TN], a[TM];
+                auto operand = [&](const unsigned char *row) {
+                    const i32x4f lo = *reinterpret_cast<const i32x4f *>(row + slot + c0), hi = *reinterpret_cast<const i32x4f *>(row + slot + c1);
+                    return i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                };
+#pragma unroll
+                for (int t = 0; t < TN; ++t) b[t] = operand(bp + t * 2048);
+#pragma unroll
+                for (int u = 0; u < TM; ++u) a[u] = operand(ap + u * 2048);
+                // stage s + 1 has landed where stages s + 2 and s + 3, four loads each, may be under way; the last stages are waited for altogether
+                if (s + 3 < ns) {
+                    fetch(s + 3);
+                    if (LATE) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                } else if (LATE) {
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                }
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier\n\ts_setprio 1" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < TN; ++t)
+#pragma unroll
+                    for (int u = 0; u < TM; ++u)
+                        acc[t][u] = j / 2 == 0 ? f8_mma<0>(b[t], a[u], acc[t][u], ws[t], xs[u]) : j / 2 == 1 ? f8_mma<1>(b[t], a[u], acc[t][u], ws[t], xs[u])
+                                  : j / 2 == 2 ? f8_mma<2>(b[t], a[u], acc[t][u], ws[t], xs[u]) : f8_mma<3>(b[t], a[u], acc[t][u], ws[t], xs[u]);
+#pragma unroll
+                for (int t = 0; t < TN; ++t)   // the products stay between the barriers
+#pragma unroll
+                    for (int u = 0; u < TM; ++u) asm volatile("" : "+v"(acc[t][u]));
+                __builtin_amdgcn_sched_barrier(0);
+                if (LATE) asm volatile("s_setprio 0\n\ts_barrier" ::: "memory");
+                else if (s + 3 < ns) asm volatile("s_setprio 0\n\ts_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+                else asm volatile("s_setprio 0\n\ts_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            }
+        }
+    };
+    if (late) steps(std::true_type());
+    else steps(std::false_type());
+    if (!late) asm volatile("s_barrier" ::: "memory");
+    __syncthreads();
+    f8_store_tile<W, TM, TN, T>(acc, p, lds8, bias, wave, lane, m0, n0, wm, wn, slice);
+}
+
 // The slices' sums, eight columns per thread.
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, const void *bias, int bias_dtype, int64_t M, int N, int64_t ldo, int slices) {
@@ -342,7 +589,7 @@ struct F8Plan {
 static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
     F8Plan q{};
     const int blocks = (int)((k + kF8Block - 1) / kF8Block);
-    q.big = dtype != EVO_F32 && blocks >= 2 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
+    q.big = dtype != EVO_F32 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
     const int side = q.big ? 256 : 128;
     q.mt = (int)((m + side - 1) / side);
     q.nt = (int)((n + side - 1) / side);
@@ -378,7 +625,13 @@ template <typename T, bool WIDE>
 static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
     const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
     if constexpr (!WIDE) {
-        if (q.big) return launch_fp8_large(a, q.slices, std::is_same<T, float>::value ? EVO_F32 : std::is_same<T, f16_t>::value ? EVO_F16 : EVO_BF16, st);
+        if (q.big) {
+            constexpr int lds = 4 * 512 * 64 + 2 * 512 * 4 + 256 * 4;
+            static PerDevice done;
+            if (const int rc = ensure_dynamic_lds((const void *)fp8_matmul_big<T>, lds, done, nullptr)) return rc;
+            fp8_matmul_big<T><<<grid, 512, lds, st>>>(a);
+            return f8_rc();
+        }
     }
     return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
 }
@@ -440,7 +693,7 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
     if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
-    if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4) || f8_off(p->bias, 4)) return EVO_EALIGN;
+    if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
     const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
     F8Matmul a{};

@@ -32,12 +32,6 @@ void f8_quantize(const Tensor &x, Rounded *along_rows, Rounded *along_cols, Tens
                                sums ? (float *)sums->data_ptr() : nullptr, rows, cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
 }
 
-// A bias as the kernels read it: dense, on a 4-byte boundary.
-Tensor f8_ready(const Tensor &bias) {
-    Tensor b = bias.defined() ? bias.contiguous() : bias;
-    return b.defined() && (uintptr_t)b.data_ptr() % 4 ? b.clone() : b;
-}
-
 // a b^T (+ bias), [a.rows, b.rows]
 Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype) {
     Tensor out = at::empty({a.rows, b.rows}, a.q.options().dtype(dtype)), ws;
@@ -105,7 +99,7 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
         Tensor y = at::zeros(shape, x.options());
         return k == 0 && bias.defined() ? y.add_(bias) : y;
     }
-    const Tensor x2 = f8_rows(x), w2 = f8_rows(w), b = f8_ready(bias);
+    const Tensor x2 = f8_rows(x), w2 = f8_rows(w), b = bias.defined() ? bias.contiguous() : bias;
     Rounded xr, wr;
     f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
     f8_quantize(w2, &wr, need_x ? &saved->wt : nullptr, nullptr);
@@ -203,7 +197,7 @@ Tensor f8_held_forward(const Tensor &x, const Tensor &q, const Tensor &s, int64_
     }
     Rounded xr;
     f8_quantize(f8_rows(x), &xr, nullptr, nullptr);
-    return f8_matmul(xr, Rounded(q, s, k), f8_ready(bias), x.scalar_type()).view(shape);
+    return f8_matmul(xr, Rounded(q, s, k), bias.defined() ? bias.contiguous() : bias, x.scalar_type()).view(shape);
 }
 OptTensor fp8_linear_held(const Tensor &x, const Tensor &values, const Tensor &scales, int64_t k, const OptTensor &bias) {
     if (!plain_modes() || !plain(x) || !plain(values) || !plain(scales) || (bias && bias->defined() && !plain(*bias)) || !x.is_cuda()) return std::nullopt;

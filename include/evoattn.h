@@ -338,7 +338,7 @@ int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t 
 /* out [m][n] = a [m][k] b [n][k]^T (+ bias [n]): rounded matrices as above, fp32 sums, rounded once to dtype (EVO_BF16 / _F16 / _F32); out's
  * rows ldo elements apart.  With a 16-bit result the 8-bit matrix instructions form the sums, which add neighbouring products with what lies
  * some 13 bits below the largest of them cut off (1.4e-5 of a result, measured); with an fp32 result the values are widened to bf16 first and
- * every sum is fp32.  bias in bias_dtype, may be NULL.  a, b on 16-byte, scales and bias on 4-byte boundaries.  k at most 2^22.  `workspace` of
+ * every sum is fp32.  bias in bias_dtype, may be NULL.  a, b on 16-byte, scales on 4-byte boundaries.  k at most 2^22.  `workspace` of
  * evoattn_fp8_matmul_workspace_bytes() (0: none needed; also for what evoattn_fp8_matmul refuses).  Nothing is allocated or synchronised;
  * two calls give the same bits. */
 typedef struct EvoFp8Matmul {
