@@ -241,6 +241,10 @@ __device__ __forceinline__ float f8_bias(const void *b, int i, int dtype) {
     return dtype == EVO_F32 ? ((const float *)b)[i] : dtype == EVO_BF16 ? (float)((const bf16_t *)b)[i] : (float)((const f16_t *)b)[i];
 }
 
+// What the lanes of a wave have written to LDS before and read after, or the other way round: LDS takes a wave's accesses in their order, and the compiler, which
+// sees that no lane reads what it has written itself, keeps that order only if it is told to.
+__device__ __forceinline__ void f8_wave_sync() { asm volatile("" ::: "memory"); }
+
 // Eight results of a row, of which the last may lie beyond it.
 template <typename T>
 __device__ __forceinline__ void f8_store8(T *p, const T (&e)[8], int left) {
@@ -285,6 +289,7 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
                 __builtin_memcpy(__builtin_assume_aligned(mine + place(li, 4 * t + 2 * g + h), 16), e, sizeof e);
             }
         }
+        f8_wave_sync();
         constexpr int RPI = 64 / CHUNKS;   // rows that the wave's lanes store at once
 #pragma unroll
         for (int i = 0; i < 32 / RPI; ++i) {
@@ -293,6 +298,7 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
             __builtin_memcpy(e, __builtin_assume_aligned(mine + place(r, c), 16), sizeof e);
             if (m < p.M && o < p.N) f8_store8(out + (int64_t)m * p.ldo + o, e, p.N - o);
         }
+        f8_wave_sync();
     }
 }
 
