@@ -245,17 +245,24 @@ __device__ __forceinline__ float f8_bias(const void *b, int i, int dtype) {
 // sees that no lane reads what it has written itself, keeps that order only if it is told to.
 __device__ __forceinline__ void f8_wave_sync() { asm volatile("" ::: "memory"); }
 
-// Eight results of a row, of which the last may lie beyond it.
+// Eight results, at any element's address: global memory takes 16 bytes at any alignment.  (As a vector type: copied element by element, the whole and the partial
+// store of a row's end became one sequence of two-byte stores, and the results of 256 x 256 took longer than 8 blocks of their products.)
 template <typename T>
-__device__ __forceinline__ void f8_store8(T *p, const T (&e)[8], int left) {
-    if (left >= 8) {
-        __builtin_memcpy(p, e, sizeof e);
-    } else {
+struct F8Eight {
+    typedef T V __attribute__((ext_vector_type(8)));
+    typedef V U __attribute__((aligned(sizeof(T))));
+    V v;
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<U *>(p) = v; }
+    __device__ __forceinline__ void store_some(T *p, int left) const {   // the first `left`
+        if (left >= 8) {
+            store(p);
+            return;
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < left) p[i] = e[i];
+        for (int i = 0; i < 7; ++i)
+            if (i < left) p[i] = v[i];
     }
-}
+};
 
 // A workgroup's slice and tile.  Tiles of a band of eight rows of tiles come one below the other: what runs at once on an XCD shares rows of both sides.
 __device__ __forceinline__ void f8_tile(const F8Matmul &p, int &slice, int &mt, int &nt) {
@@ -276,6 +283,7 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
     unsigned char *mine = lds + wave * 32 * ROW;
     auto place = [](int r, int c) { return r * ROW + ((c ^ (r & (CHUNKS - 1))) * (int)(8 * sizeof(T))); };
     T *out = (T *)p.out + (int64_t)slice * p.M * p.N;
+    const bool inside = m0 + wm + 32 * TM <= p.M && n0 + wn + 32 * TN <= p.N;   // uniform
 #pragma unroll
     for (int u = 0; u < TM; ++u) {
 #pragma unroll
@@ -283,20 +291,23 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const f32x4 *b = reinterpret_cast<const f32x4 *>(bias + wn + 32 * t + 16 * g + 8 * h);
-                T e[8];
+                F8Eight<T> e;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = (T)(acc[t][u][8 * h + i] + b[i / 4][i % 4]);
-                __builtin_memcpy(__builtin_assume_aligned(mine + place(li, 4 * t + 2 * g + h), 16), e, sizeof e);
+                for (int i = 0; i < 8; ++i) e.v[i] = (T)(acc[t][u][8 * h + i] + b[i / 4][i % 4]);
+                *reinterpret_cast<typename F8Eight<T>::V *>(mine + place(li, 4 * t + 2 * g + h)) = e.v;
             }
         }
         f8_wave_sync();
         constexpr int RPI = 64 / CHUNKS;   // rows that the wave's lanes store at once
+        const int c = lane % CHUNKS, o = n0 + wn + 8 * c;
 #pragma unroll
         for (int i = 0; i < 32 / RPI; ++i) {
-            const int r = i * RPI + lane / CHUNKS, c = lane % CHUNKS, m = m0 + wm + 32 * u + r, o = n0 + wn + 8 * c;
-            T e[8];
-            __builtin_memcpy(e, __builtin_assume_aligned(mine + place(r, c), 16), sizeof e);
-            if (m < p.M && o < p.N) f8_store8(out + (int64_t)m * p.ldo + o, e, p.N - o);
+            const int r = i * RPI + lane / CHUNKS, m = m0 + wm + 32 * u + r;
+            F8Eight<T> e;
+            e.v = *reinterpret_cast<const typename F8Eight<T>::V *>(mine + place(r, c));
+            T *to = out + (int64_t)m * p.ldo + o;
+            if (inside) e.store(to);
+            else if (m < p.M && o < p.N) e.store_some(to, p.N - o);
         }
         f8_wave_sync();
     }
@@ -568,10 +579,10 @@ __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, con
             for (int i = 0; i < 8; ++i)
                 if (o + i < N) s[i] += x[(int64_t)k * M * N + i];
     }
-    T e[8];
+    F8Eight<T> e;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = (T)(bias && o + i < N ? s[i] + f8_bias(bias, o + i, bias_dtype) : s[i]);
-    f8_store8(out + m * ldo + o, e, N - o);
+    for (int i = 0; i < 8; ++i) e.v[i] = (T)(bias && o + i < N ? s[i] + f8_bias(bias, o + i, bias_dtype) : s[i]);
+    e.store_some(out + m * ldo + o, N - o);
 }
 
 static int f8_rc() {
