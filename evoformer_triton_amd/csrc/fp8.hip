@@ -252,6 +252,7 @@ struct F8Eight {
     typedef T V __attribute__((ext_vector_type(8)));
     typedef V U __attribute__((aligned(sizeof(T))));
     V v;
+    __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const U *>(p); }
     __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<U *>(p) = v; }
     __device__ __forceinline__ void store_some(T *p, int left) const {   // the first `left`
         if (left >= 8) {
@@ -585,6 +586,133 @@ __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, con
     e.store_some(out + m * ldo + o, N - o);
 }
 
+// ---- few rows ----
+
+// Up to 64 rows of a: the rows of b are read once, straight into operands, and what there is to multiply is hidden behind that.  A workgroup takes 16 rows of b (outputs)
+// and all rows of a; its waves take turns at the blocks of the contraction and add up through LDS.  v_mfma_scale_f32_16x16x128: one product per block and 16 rows of
+// a (lane l, q = l / 16: row l % 16, contraction 32 q .. 32 q + 31; results of row l % 16 of a, outputs 4 q .. 4 q + 3).
+// ROUND: up to 16 rows that are rounded on the way, a lane's 32 values and its three neighbours' at a time, by every workgroup again: one launch
+// instead of two.
+struct F8Few {
+    const void *x;               // ROUND: [M][k], rows ldx apart; else
+    const uint8_t *a, *b;
+    const uint32_t *sa, *sb;
+    const void *bias;
+    void *out;
+    int64_t ldx, ldo, kp;
+    int M, N, k, blocks, sd, bias_dtype;
+};
+constexpr int kF8FewRows = 64, kF8RoundRows = 16, kF8FewWaves = 8;
+
+template <typename T, int MT, bool ROUND>
+__global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    constexpr int U = 4;
+    __shared__ f32x4 sums[kF8FewWaves][MT][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, li = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * 16, row = min(n0 + li, p.N - 1);
+    const uint8_t *b = p.b + row * p.kp + q * 32;
+    const uint32_t *sb = p.sb + (int64_t)row * p.sd;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int u = 0; u < MT; ++u) acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    auto load = [](const uint8_t *from) {
+        const i32x4f lo = *reinterpret_cast<const i32x4f *>(from), hi = *reinterpret_cast<const i32x4f *>(from + 16);
+        return i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    };
+    auto multiply = [&](const i32x8f &bo, const i32x8f &ao, int bs, int as, int u) {   // scales in the lowest byte
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_widen(bo[2 * i], bo[2 * i + 1], f8_scale(bs, 0)), f8_widen(ao[2 * i], ao[2 * i + 1], f8_scale(as, 0)), acc[u], 0, 0, 0);
+        } else {
+            acc[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bo, ao, acc[u], 0, 0, 0, bs, 0, as);
+        }
+    };
+    for (int first = wave; first < p.blocks; first += waves * U) {
+        i32x8f bo[U];
+        int bs[U];
+#pragma unroll
+        for (int j = 0; j < U; ++j) {   // (blocks beyond the last repeat it; they are not multiplied)
+            const int k = min(first + j * waves, p.blocks - 1);
+            bo[j] = load(b + (int64_t)k * kF8Block);
+            bs[j] = (int)(sb[k >> 2] >> (8 * (k & 3)));
+        }
+        if constexpr (ROUND) {
+            const T *x = (const T *)p.x + (int64_t)min(li, p.M - 1) * p.ldx + q * 32;
+            F8Eight<T> e[U][4];
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int k = min(first + j * waves, p.blocks - 1), c = k * kF8Block + q * 32;
+                if ((k + 1) * kF8Block <= p.k) {   // uniform
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[j][i].load(x + k * kF8Block + 8 * i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) e[j][i / 8].v[i % 8] = c + i < p.k ? x[k * kF8Block + i] : (T)0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                if (first + j * waves >= p.blocks) break;
+                unsigned most = 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) most = max(most, f8_magnitude((float)e[j][i / 8].v[i % 8]));
+                {
+                    const auto w = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+                    most = max(w[0], w[1]);
+                }
+                {
+                    const auto w = __builtin_amdgcn_permlane16_swap(most, most, false, false);
+                    most = max(w[0], w[1]);
+                }
+                const int ex = f8_exponent(most);
+                const float inv = f8_inverse(ex);
+                i32x8f ao;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const auto &v = e[j][i / 2].v;
+                    const int c = i % 2 * 4;
+                    ao[i] = f8_pack((float)v[c], (float)v[c + 1], (float)v[c + 2], (float)v[c + 3], inv);
+                }
+                multiply(bo[j], ao, bs[j], ex + 127, 0);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                const int m = min(16 * u + li, p.M - 1);
+                const uint8_t *a = p.a + m * p.kp + q * 32;
+                i32x8f ao[U];
+                int as[U];
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    const int k = min(first + j * waves, p.blocks - 1);
+                    ao[j] = load(a + (int64_t)k * kF8Block);
+                    as[j] = (int)(p.sa[(int64_t)m * p.sd + (k >> 2)] >> (8 * (k & 3)));
+                }
+#pragma unroll
+                for (int j = 0; j < U; ++j)
+                    if (first + j * waves < p.blocks) multiply(bo[j], ao[j], bs[j], as[j], u);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < MT; ++u) sums[wave][u][lane] = acc[u];
+    __syncthreads();
+    for (int u = wave; u < MT; u += waves) {
+        f32x4 s = sums[0][u][lane];
+        for (int w = 1; w < waves; ++w) s += sums[w][u][lane];
+        const int m = 16 * u + li, o = n0 + 4 * q;
+        if (m < p.M) {
+            T *out = (T *)p.out + (int64_t)m * p.ldo + o;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (o + i < p.N) out[i] = (T)(s[i] + (p.bias ? f8_bias(p.bias, o + i, p.bias_dtype) : 0.0f));
+        }
+    }
+}
+
 static int f8_rc() {
     const hipError_t err = hipGetLastError();
     return err == hipSuccess ? EVO_OK : EVO_EHIP - (int)err;
@@ -606,7 +734,7 @@ struct F8Plan {
 static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
     F8Plan q{};
     const int blocks = (int)((k + kF8Block - 1) / kF8Block);
-    q.big = dtype != EVO_F32 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
+    q.big = dtype != EVO_F32 && blocks >= 4 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
     const int side = q.big ? 256 : 128;
     q.mt = (int)((m + side - 1) / side);
     q.nt = (int)((n + side - 1) / side);
@@ -651,6 +779,42 @@ static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
         }
     }
     return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
+}
+
+// Few rows: which kernel, and with how many waves.
+static bool f8_few(const EvoFp8Matmul &p) { return p.m <= kF8FewRows; }
+static F8Few f8_few_args(const EvoFp8Matmul &p) {
+    F8Few a{};
+    a.a = (const uint8_t *)p.a;
+    a.b = (const uint8_t *)p.b;
+    a.sa = (const uint32_t *)p.scales_a;
+    a.sb = (const uint32_t *)p.scales_b;
+    a.bias = p.bias;
+    a.out = p.out;
+    a.ldo = p.ldo;
+    a.kp = f8_pitch(p.k);
+    a.M = (int)p.m;
+    a.N = (int)p.n;
+    a.k = (int)p.k;
+    a.blocks = (int)(a.kp / kF8Block);
+    a.sd = (int)(f8_scale_pitch(p.k) / 4);
+    a.bias_dtype = p.bias_dtype;
+    return a;
+}
+template <typename T, bool ROUND>
+static int f8_launch_few(const F8Few &a, hipStream_t st) {
+    const unsigned grid = (unsigned)((a.N + 15) / 16), threads = 64 * (a.blocks < kF8FewWaves ? a.blocks : kF8FewWaves);
+    if constexpr (ROUND) {
+        fp8_few<T, 1, true><<<grid, threads, 0, st>>>(a);
+    } else {
+        switch ((a.M + 15) / 16) {
+            case 1: fp8_few<T, 1, false><<<grid, threads, 0, st>>>(a); break;
+            case 2: fp8_few<T, 2, false><<<grid, threads, 0, st>>>(a); break;
+            case 3: fp8_few<T, 3, false><<<grid, threads, 0, st>>>(a); break;
+            default: fp8_few<T, 4, false><<<grid, threads, 0, st>>>(a);
+        }
+    }
+    return f8_rc();
 }
 
 }  // namespace evo
@@ -702,6 +866,7 @@ int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t 
 size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p) {
     using namespace evo;
     if (f8_check(p)) return 0;
+    if (f8_few(*p)) return 0;
     const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
@@ -711,6 +876,10 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     if (const int rc = f8_check(p)) return rc;
     if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
+    if (f8_few(*p)) {
+        const F8Few few = f8_few_args(*p);
+        return f8_by_dtype(p->dtype, [&](auto t) { return f8_launch_few<decltype(t), false>(few, (hipStream_t)hip_stream); });
+    }
     const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
     F8Matmul a{};
@@ -743,6 +912,18 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
         fp8_slices<T><<<(unsigned)groups, 256, 0, st>>>((const float *)p->workspace, (T *)p->out, p->bias, p->bias_dtype, p->m, (int)p->n, p->ldo, q.slices);
         return f8_rc();
     });
+}
+
+int evoattn_fp8_matmul_few(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream) {
+    using namespace evo;
+    if (const int rc = f8_check(p)) return rc;
+    if (p->m > kF8RoundRows) return EVO_EUNSUPPORTED;
+    if (!x || ldx < p->k || !p->b || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
+    if (f8_off(p->b, 16) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
+    F8Few few = f8_few_args(*p);
+    few.x = x;
+    few.ldx = ldx;
+    return f8_by_dtype(p->dtype, [&](auto t) { return f8_launch_few<decltype(t), true>(few, (hipStream_t)hip_stream); });
 }
 
 }  // extern "C"

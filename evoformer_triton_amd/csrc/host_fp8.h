@@ -32,17 +32,13 @@ void f8_quantize(const Tensor &x, Rounded *along_rows, Rounded *along_cols, Tens
                                sums ? (float *)sums->data_ptr() : nullptr, rows, cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
 }
 
-// a b^T (+ bias), [a.rows, b.rows]
-Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype) {
-    Tensor out = at::empty({a.rows, b.rows}, a.q.options().dtype(dtype)), ws;
+EvoFp8Matmul f8_product(int64_t rows, const Rounded &b, const Tensor &bias, const Tensor &out) {
     EvoFp8Matmul p{};
-    p.m = a.rows;
+    p.m = rows;
     p.n = b.rows;
-    p.k = a.k;
+    p.k = b.k;
     p.ldo = b.rows;
-    p.dtype = evo_dtype(dtype);
-    p.a = a.q.data_ptr();
-    p.scales_a = a.s.data_ptr();
+    p.dtype = evo_dtype(out.scalar_type());
     p.b = b.q.data_ptr();
     p.scales_b = b.s.data_ptr();
     if (bias.defined()) {
@@ -50,6 +46,14 @@ Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::Sca
         p.bias_dtype = evo_dtype(bias.scalar_type());
     }
     p.out = out.data_ptr();
+    return p;
+}
+// a b^T (+ bias), [a.rows, b.rows]
+Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype) {
+    Tensor out = at::empty({a.rows, b.rows}, a.q.options().dtype(dtype)), ws;
+    EvoFp8Matmul p = f8_product(a.rows, b, bias, out);
+    p.a = a.q.data_ptr();
+    p.scales_a = a.s.data_ptr();
     if (const size_t bytes = evoattn_fp8_matmul_workspace_bytes(&p)) {
         ws = scratch(bytes, a.q);
         p.workspace = ws.data_ptr();
@@ -57,6 +61,20 @@ Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::Sca
     }
     check(evoattn_fp8_matmul(&p, stream_of(a.q)), "evoattn_fp8_matmul");
     return out;
+}
+
+// x b^T (+ bias) with x rounded on the way
+Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
+    const int64_t rows = x.size(0);
+    if (rows <= 16) {
+        Tensor out = at::empty({rows, b.rows}, x.options());
+        const EvoFp8Matmul p = f8_product(rows, b, bias, out);
+        check(evoattn_fp8_matmul_few(&p, x.data_ptr(), x.stride(0), stream_of(x)), "evoattn_fp8_matmul_few");
+        return out;
+    }
+    Rounded a;
+    f8_quantize(x, &a, nullptr, nullptr);
+    return f8_matmul(a, b, bias, x.scalar_type());
 }
 
 const char *f8_wrong(const Tensor &x, int64_t n, int64_t k, const c10::Device &device, const OptTensor &bias) {
@@ -101,8 +119,9 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
     }
     const Tensor x2 = f8_rows(x), w2 = f8_rows(w), b = bias.defined() ? bias.contiguous() : bias;
     Rounded xr, wr;
-    f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
     f8_quantize(w2, &wr, need_x ? &saved->wt : nullptr, nullptr);
+    if (!need_w) return f8_times(x2, wr, b).view(shape);
+    f8_quantize(x2, &xr, &saved->xt, nullptr);
     return f8_matmul(xr, wr, b, x.scalar_type()).view(shape);
 }
 // dx, dw, db from dy [rows, n]
@@ -195,9 +214,7 @@ Tensor f8_held_forward(const Tensor &x, const Tensor &q, const Tensor &s, int64_
         Tensor y = at::zeros(shape, x.options());
         return k == 0 && bias.defined() ? y.add_(bias) : y;
     }
-    Rounded xr;
-    f8_quantize(f8_rows(x), &xr, nullptr, nullptr);
-    return f8_matmul(xr, Rounded(q, s, k), bias.defined() ? bias.contiguous() : bias, x.scalar_type()).view(shape);
+    return f8_times(f8_rows(x), Rounded(q, s, k), bias.defined() ? bias.contiguous() : bias).view(shape);
 }
 OptTensor fp8_linear_held(const Tensor &x, const Tensor &values, const Tensor &scales, int64_t k, const OptTensor &bias) {
     if (!plain_modes() || !plain(x) || !plain(values) || !plain(scales) || (bias && bias->defined() && !plain(*bias)) || !x.is_cuda()) return std::nullopt;
