@@ -20,6 +20,26 @@ typedef unsigned u32x2f __attribute__((ext_vector_type(2)));
 static int64_t f8_pitch(int64_t k) { return (k + kF8Block - 1) / kF8Block * kF8Block; }             // bytes of a rounded row
 static int64_t f8_scale_pitch(int64_t k) { return (k + 4 * kF8Block - 1) / (4 * kF8Block) * 4; }   // bytes of its scales
 
+// Eight elements, at any element's address: global memory takes 16 bytes at any alignment.  (As a vector type: copied element by element, the whole and the partial
+// store of a row's end became one sequence of two-byte stores, and the results of 256 x 256 took longer than 8 blocks of their products.)
+template <typename T>
+struct F8Eight {
+    typedef T V __attribute__((ext_vector_type(8)));
+    typedef V U __attribute__((aligned(sizeof(T))));
+    V v;
+    __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const U *>(p); }
+    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<U *>(p) = v; }
+    __device__ __forceinline__ void store_some(T *p, int left) const {   // the first `left`
+        if (left >= 8) {
+            store(p);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+            if (i < left) p[i] = v[i];
+    }
+};
+
 // ---- rounding ----
 
 // The exponent e of a block whose largest finite magnitude has these bits: the least with magnitude <= 448 2^e, at least -127 (0 for a block of zeros).
@@ -44,6 +64,20 @@ __device__ __forceinline__ unsigned f8_max_ror(unsigned v) {   // with the value
 }
 __device__ __forceinline__ unsigned f8_max16(unsigned v) { return f8_max_ror<1>(f8_max_ror<2>(f8_max_ror<4>(f8_max_ror<8>(v)))); }
 
+// over the four groups of 16 lanes
+__device__ __forceinline__ unsigned f8_max_rows(unsigned v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(b[0], b[1]);
+}
+__device__ __forceinline__ float f8_sum_rows(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 struct F8Quantize {
     const void *x;
     int64_t ldx, rows;
@@ -54,35 +88,65 @@ struct F8Quantize {
     float *sums;
 };
 
-constexpr int kF8Threads = 256;
+// The scale of block k of a row (or column) of `blocks`; with the last one, the places up to the next multiple of four.
+__device__ __forceinline__ void f8_store_scale(uint8_t *s, int64_t k, int64_t blocks, int64_t pitch, uint8_t scale) {
+    s[k] = scale;
+    if (k == blocks - 1) {
+        if (k + 1 < pitch) s[k + 1] = 127;
+        if (k + 2 < pitch) s[k + 2] = 127;
+        if (k + 3 < pitch) s[k + 3] = 127;
+    }
+}
 
-// A workgroup rounds 128 rows x 128 columns: thread t eight rows (8 (t / 16) ..) of eight columns (8 (t % 16) ..).
-template <typename T, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(kF8Threads) fp8_quantize(F8Quantize p) {
-    constexpr int V = 8;
+// A workgroup rounds R rows x 128 columns, 128 rows where it rounds columns, too: thread t V rows (V (t / 16) ..) of eight columns (8 (t % 16) ..).
+template <typename T, int R, int V, bool ROWS, bool COLS>
+__global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
+    static_assert(R == 128 || !COLS, "a column's block is 128 rows");
+    constexpr int WAVES = R / V / 4, THREADS = R / V * 16;
     __shared__ __attribute__((aligned(16))) unsigned char tile[COLS ? 128 * 128 : 16];
-    __shared__ unsigned amaxs[COLS ? 4 : 1][128];
-    __shared__ float sums[COLS ? 4 : 1][128];
+    __shared__ unsigned amaxs[COLS ? WAVES : 1][128];
+    __shared__ float sums[COLS ? WAVES : 1][128];
+    __shared__ __attribute__((aligned(16))) float col_inverse[COLS ? 128 : 4];
+    __shared__ uint8_t row_scale[R];
     const int t = threadIdx.x, cg = t % 16, rg = t / 16, wave = t / 64;
     const int kt = blockIdx.x % p.tiles_k;
     const int64_t rt = blockIdx.x / p.tiles_k;
     const int c0 = kt * 128 + cg * 8;
-    const int64_t r0 = rt * 128 + rg * 8;
+    const int64_t r0 = rt * R + rg * V;
     float v[V][8];
-    const T *x = (const T *)p.x + r0 * p.ldx + c0;
-    if ((rt + 1) * 128 <= p.rows && (kt + 1) * 128 <= p.cols) {   // uniform: all loads under way together
-        T e[V][8];
+    const T *x = (const T *)p.x;
+    const bool last_rows = (rt + 1) * R >= p.rows, ragged = (kt + 1) * 128 > p.cols;   // uniform
+    const bool corner = ragged && last_rows;
+    if (p.cols >= 8 && (!corner || p.rows >= 2)) {
+        // All loads under way together: rows beyond the last repeat it, and what lies behind a row's end is the next row's; the last row of all, which may not be read
+        // beyond, element by element.
+        F8Eight<T> e[V];
+        T l[8];
 #pragma unroll
-        for (int i = 0; i < V; ++i) __builtin_memcpy(e[i], x + i * p.ldx, sizeof e[i]);
+        for (int i = 0; i < V; ++i) e[i].load(x + min(r0 + i, p.rows - (corner ? 2 : 1)) * p.ldx + (c0 < p.cols ? c0 : 0));
+        if (corner) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c) l[c] = x[(p.rows - 1) * p.ldx + min(c0 + c, p.cols - 1)];
+        }
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v[i][c] = (float)e[i][c];
+            for (int c = 0; c < 8; ++c) v[i][c] = (float)(corner && r0 + i == p.rows - 1 ? l[c] : e[i].v[c]);
+        if (last_rows || ragged) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    if (r0 + i >= p.rows || c0 + c >= p.cols) v[i][c] = 0.0f;
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v[i][c] = r0 + i < p.rows && c0 + c < p.cols ? (float)x[i * p.ldx + c] : 0.0f;
+            for (int c = 0; c < 8; ++c) {
+                const float e = (float)x[min(r0 + i, p.rows - 1) * p.ldx + min(c0 + c, p.cols - 1)];
+                v[i][c] = r0 + i < p.rows && c0 + c < p.cols ? e : 0.0f;
+            }
     }
     if (ROWS) {
 #pragma unroll
@@ -95,16 +159,11 @@ __global__ void __launch_bounds__(kF8Threads) fp8_quantize(F8Quantize p) {
             if (r0 + i < p.rows) {
                 *reinterpret_cast<u32x2f *>(p.q + (r0 + i) * p.kp + c0) =
                     u32x2f{(unsigned)f8_pack(v[i][0], v[i][1], v[i][2], v[i][3], inv), (unsigned)f8_pack(v[i][4], v[i][5], v[i][6], v[i][7], inv)};
-                if (cg == 0) {
-                    uint8_t *s = p.s + (r0 + i) * p.sp;
-                    s[kt] = (uint8_t)(e + 127);
-                    if (kt == p.tiles_k - 1)
-                        for (int k = kt + 1; k < p.sp; ++k) s[k] = 127;
-                }
             }
+            if (cg == 0) row_scale[rg * V + i] = (uint8_t)(e + 127);
         }
     }
-    if (COLS) {
+    if constexpr (COLS) {
         unsigned a[8];
         float s[8];
 #pragma unroll
@@ -116,10 +175,8 @@ __global__ void __launch_bounds__(kF8Threads) fp8_quantize(F8Quantize p) {
                 a[c] = max(a[c], f8_magnitude(v[i][c]));
                 s[c] += v[i][c];
             }
-            a[c] = max(a[c], (unsigned)__shfl_xor((int)a[c], 16));
-            a[c] = max(a[c], (unsigned)__shfl_xor((int)a[c], 32));
-            s[c] += __shfl_xor(s[c], 16);
-            s[c] += __shfl_xor(s[c], 32);
+            a[c] = f8_max_rows(a[c]);
+            s[c] = f8_sum_rows(s[c]);
         }
         if (rg % 4 == 0) {
 #pragma unroll
@@ -129,30 +186,49 @@ __global__ void __launch_bounds__(kF8Threads) fp8_quantize(F8Quantize p) {
             }
         }
         __syncthreads();
+        if (t < 128) {
+            unsigned most = 0;
+            float s = 0.0f;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const int col = cg * 8 + c;
-            const int e = f8_exponent(max(max(amaxs[0][col], amaxs[1][col]), max(amaxs[2][col], amaxs[3][col])));
-            const float inv = f8_inverse(e);
-            *reinterpret_cast<u32x2f *>(tile + col * 128 + (((rg >> 1) ^ (cg & 7)) << 4) + (rg & 1) * 8) =
-                u32x2f{(unsigned)f8_pack(v[0][c], v[1][c], v[2][c], v[3][c], inv), (unsigned)f8_pack(v[4][c], v[5][c], v[6][c], v[7][c], inv)};
-            if (rg == 0 && c0 + c < p.cols) {
-                uint8_t *st = p.st + (c0 + c) * p.spt;
-                st[rt] = (uint8_t)(e + 127);
-                if (rt == p.tiles_r - 1)
-                    for (int64_t k = rt + 1; k < p.spt; ++k) st[k] = 127;
+            for (int w = 0; w < WAVES; ++w) {
+                most = max(most, amaxs[w][t]);
+                s += sums[w][t];
+            }
+            const int e = f8_exponent(most);
+            col_inverse[t] = f8_inverse(e);
+            if (kt * 128 + t < p.cols) {
+                f8_store_scale(p.st + (kt * 128 + t) * p.spt, rt, p.tiles_r, p.spt, (uint8_t)(e + 127));
+                if (p.sums) p.sums[rt * p.cols + kt * 128 + t] = s;
             }
         }
         __syncthreads();
-        if (p.sums && t < 128 && kt * 128 + t < p.cols)
-            p.sums[rt * p.cols + kt * 128 + t] = (sums[0][t] + sums[1][t]) + (sums[2][t] + sums[3][t]);
+        // byte of row r of column col: 16-byte chunks of a column's 128 rows, moved about so that neighbouring columns' lie in different banks
+        auto at = [](int col, int r) { return col * 128 + (((r >> 4) ^ ((col >> 3) & 7)) << 4) + (r & 15); };
+        float invs[8];
+        __builtin_memcpy(invs, __builtin_assume_aligned(col_inverse + cg * 8, 16), sizeof invs);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int col = t / 8 + 32 * k, slot = t % 8;
-            if (kt * 128 + col < p.cols)
-                *reinterpret_cast<i32x4f *>(p.qt + (int64_t)(kt * 128 + col) * p.rp + rt * 128 + slot * 16) =
-                    *reinterpret_cast<const i32x4f *>(tile + col * 128 + ((slot ^ ((col >> 3) & 7)) << 4));
+        for (int c = 0; c < 8; ++c) {
+            const int col = cg * 8 + c;
+            const float inv = invs[c];
+            if constexpr (V == 8) {
+                *reinterpret_cast<u32x2f *>(tile + at(col, rg * 8)) =
+                    u32x2f{(unsigned)f8_pack(v[0][c], v[1][c], v[2][c], v[3][c], inv), (unsigned)f8_pack(v[4][c], v[5][c], v[6][c], v[7][c], inv)};
+            } else {
+                static_assert(V == 2, "");
+                *reinterpret_cast<uint16_t *>(tile + at(col, rg * 2)) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0][c] * inv, v[1][c] * inv, 0, false);
+            }
         }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 1024 / THREADS; ++k) {
+            const int col = t / 8 + THREADS / 8 * k, slot = t % 8;
+            if (kt * 128 + col < p.cols)
+                *reinterpret_cast<i32x4f *>(p.qt + (int64_t)(kt * 128 + col) * p.rp + rt * 128 + slot * 16) = *reinterpret_cast<const i32x4f *>(tile + at(col, slot * 16));
+        }
+    }
+    if constexpr (ROWS) {
+        if (!COLS) __syncthreads();
+        if (t < R && rt * R + t < p.rows) f8_store_scale(p.s + (rt * R + t) * p.sp, kt, p.tiles_k, p.sp, row_scale[t]);
     }
 }
 
@@ -244,26 +320,6 @@ __device__ __forceinline__ float f8_bias(const void *b, int i, int dtype) {
 // What the lanes of a wave have written to LDS before and read after, or the other way round: LDS takes a wave's accesses in their order, and the compiler, which
 // sees that no lane reads what it has written itself, keeps that order only if it is told to.
 __device__ __forceinline__ void f8_wave_sync() { asm volatile("" ::: "memory"); }
-
-// Eight results, at any element's address: global memory takes 16 bytes at any alignment.  (As a vector type: copied element by element, the whole and the partial
-// store of a row's end became one sequence of two-byte stores, and the results of 256 x 256 took longer than 8 blocks of their products.)
-template <typename T>
-struct F8Eight {
-    typedef T V __attribute__((ext_vector_type(8)));
-    typedef V U __attribute__((aligned(sizeof(T))));
-    V v;
-    __device__ __forceinline__ void load(const T *p) { v = *reinterpret_cast<const U *>(p); }
-    __device__ __forceinline__ void store(T *p) const { *reinterpret_cast<U *>(p) = v; }
-    __device__ __forceinline__ void store_some(T *p, int left) const {   // the first `left`
-        if (left >= 8) {
-            store(p);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 7; ++i)
-            if (i < left) p[i] = v[i];
-    }
-};
 
 // A workgroup's slice and tile.  Tiles of a band of eight rows of tiles come one below the other: what runs at once on an XCD shares rows of both sides.
 __device__ __forceinline__ void f8_tile(const F8Matmul &p, int &slice, int &mt, int &nt) {
@@ -590,7 +646,7 @@ __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, con
 
 // Up to 64 rows of a: the rows of b are read once, straight into operands, and what there is to multiply is hidden behind that.  A workgroup takes 16 rows of b (outputs)
 // and all rows of a; its waves take turns at the blocks of the contraction and add up through LDS.  v_mfma_scale_f32_16x16x128: one product per block and 16 rows of
-// a (lane l, q = l / 16: row l % 16, contraction 32 q .. 32 q + 31; results of row l % 16 of a, outputs 4 q .. 4 q + 3).
+// a (lane l, q = l / 16: row l % 16, of a block's 128 values 16 q .. 16 q + 15 and 64 + 16 q ..; results of row l % 16 of a, outputs 4 q .. 4 q + 3).
 // ROUND: up to 16 rows that are rounded on the way, a lane's 32 values and its three neighbours' at a time, by every workgroup again: one launch
 // instead of two.
 struct F8Few {
@@ -611,14 +667,14 @@ __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
     __shared__ f32x4 sums[kF8FewWaves][MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, li = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * 16, row = min(n0 + li, p.N - 1);
-    const uint8_t *b = p.b + row * p.kp + q * 32;
+    const uint8_t *b = p.b + row * p.kp + q * 16;
     const uint32_t *sb = p.sb + (int64_t)row * p.sd;
     f32x4 acc[MT];
 #pragma unroll
     for (int u = 0; u < MT; ++u) acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
     auto load = [](const uint8_t *from) {
-        const i32x4f lo = *reinterpret_cast<const i32x4f *>(from), hi = *reinterpret_cast<const i32x4f *>(from + 16);
+        const i32x4f lo = *reinterpret_cast<const i32x4f *>(from), hi = *reinterpret_cast<const i32x4f *>(from + 64);
         return i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
     auto multiply = [&](const i32x8f &bo, const i32x8f &ao, int bs, int as, int u) {   // scales in the lowest byte
@@ -640,17 +696,20 @@ __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
             bs[j] = (int)(sb[k >> 2] >> (8 * (k & 3)));
         }
         if constexpr (ROUND) {
-            const T *x = (const T *)p.x + (int64_t)min(li, p.M - 1) * p.ldx + q * 32;
+            const T *x = (const T *)p.x + (int64_t)min(li, p.M - 1) * p.ldx + q * 16;
             F8Eight<T> e[U][4];
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                const int k = min(first + j * waves, p.blocks - 1), c = k * kF8Block + q * 32;
+                const int k = min(first + j * waves, p.blocks - 1), c = k * kF8Block + q * 16;
                 if ((k + 1) * kF8Block <= p.k) {   // uniform
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[j][i].load(x + k * kF8Block + 8 * i);
+                    for (int i = 0; i < 4; ++i) e[j][i].load(x + k * kF8Block + 64 * (i / 2) + 8 * (i % 2));
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) e[j][i / 8].v[i % 8] = c + i < p.k ? x[k * kF8Block + i] : (T)0.0f;
+                    for (int i = 0; i < 32; ++i) {
+                        const int w = 64 * (i / 16) + i % 16;
+                        e[j][i / 8].v[i % 8] = c + w < p.k ? x[k * kF8Block + w] : (T)0.0f;
+                    }
                 }
             }
 #pragma unroll
@@ -659,15 +718,7 @@ __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
                 unsigned most = 0;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) most = max(most, f8_magnitude((float)e[j][i / 8].v[i % 8]));
-                {
-                    const auto w = __builtin_amdgcn_permlane32_swap(most, most, false, false);
-                    most = max(w[0], w[1]);
-                }
-                {
-                    const auto w = __builtin_amdgcn_permlane16_swap(most, most, false, false);
-                    most = max(w[0], w[1]);
-                }
-                const int ex = f8_exponent(most);
+                const int ex = f8_exponent(f8_max_rows(most));
                 const float inv = f8_inverse(ex);
                 i32x8f ao;
 #pragma unroll
@@ -679,22 +730,25 @@ __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
                 multiply(bo[j], ao, bs[j], ex + 127, 0);
             }
         } else {
+            i32x8f ao[MT][U];
+            int as[MT][U];
 #pragma unroll
             for (int u = 0; u < MT; ++u) {
                 const int m = min(16 * u + li, p.M - 1);
-                const uint8_t *a = p.a + m * p.kp + q * 32;
-                i32x8f ao[U];
-                int as[U];
+                const uint8_t *a = p.a + m * p.kp + q * 16;
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
                     const int k = min(first + j * waves, p.blocks - 1);
-                    ao[j] = load(a + (int64_t)k * kF8Block);
-                    as[j] = (int)(p.sa[(int64_t)m * p.sd + (k >> 2)] >> (8 * (k & 3)));
+                    ao[u][j] = load(a + (int64_t)k * kF8Block);
+                    as[u][j] = (int)(p.sa[(int64_t)m * p.sd + (k >> 2)] >> (8 * (k & 3)));
                 }
-#pragma unroll
-                for (int j = 0; j < U; ++j)
-                    if (first + j * waves < p.blocks) multiply(bo[j], ao[j], bs[j], as[j], u);
             }
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+                if (first + j * waves < p.blocks) {
+#pragma unroll
+                    for (int u = 0; u < MT; ++u) multiply(bo[j], ao[u][j], bs[j], as[u][j], u);
+                }
         }
     }
 #pragma unroll
@@ -848,9 +902,11 @@ int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void
     hipStream_t st = (hipStream_t)hip_stream;
     return f8_by_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
-        if (q && qt) fp8_quantize<T, true, true><<<grid, kF8Threads, 0, st>>>(p);
-        else if (q) fp8_quantize<T, true, false><<<grid, kF8Threads, 0, st>>>(p);
-        else fp8_quantize<T, false, true><<<grid, kF8Threads, 0, st>>>(p);
+        const bool few = p.tiles_r * p.tiles_k < 512;   // tiles: more threads for each
+        if (q && qt) few ? fp8_quantize<T, 128, 2, true, true><<<grid, 1024, 0, st>>>(p) : fp8_quantize<T, 128, 8, true, true><<<grid, 256, 0, st>>>(p);
+        else if (!q) few ? fp8_quantize<T, 128, 2, false, true><<<grid, 1024, 0, st>>>(p) : fp8_quantize<T, 128, 8, false, true><<<grid, 256, 0, st>>>(p);
+        else if (few) fp8_quantize<T, 16, 1, true, false><<<(unsigned)((rows + 15) / 16 * p.tiles_k), 256, 0, st>>>(p);
+        else fp8_quantize<T, 128, 8, true, false><<<grid, 256, 0, st>>>(p);
         return f8_rc();
     });
 }
