@@ -644,125 +644,133 @@ __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, con
 
 // ---- few rows ----
 
-// Up to 64 rows of a: the rows of b are read once, straight into operands, and what there is to multiply is hidden behind that.  A workgroup takes 16 rows of b (outputs)
-// and all rows of a; its waves take turns at the blocks of the contraction and add up through LDS.  v_mfma_scale_f32_16x16x128: one product per block and 16 rows of
-// a (lane l, q = l / 16: row l % 16, of a block's 128 values 16 q .. 16 q + 15 and 64 + 16 q ..; results of row l % 16 of a, outputs 4 q .. 4 q + 3).
-// ROUND: up to 16 rows that are rounded on the way, a lane's 32 values and its three neighbours' at a time, by every workgroup again: one launch
-// instead of two.
+// Up to 64 rows, rounded on the way: the weight's rows are read once, straight into operands, and what there is to multiply is hidden behind that; one launch where a
+// rounding pass and a product of tiles take two or three.  A workgroup takes 16 NT rows of b (outputs) and all rows of x, for a slice of the contraction; its
+// waves take turns at the slice's blocks and add up through LDS.  v_mfma_scale_f32_16x16x128: one product per block and 16 rows of either side (lane l, q = l / 16: row
+// l % 16, of a block's 128 values 16 q .. 16 q + 15 and 64 + 16 q ..; results of row l % 16 of x, outputs 4 q .. 4 q + 3).  The rows of x are rounded by every
+// workgroup again, a block's 32 values of a lane and its three neighbours' at a time.
 struct F8Few {
-    const void *x;               // ROUND: [M][k], rows ldx apart; else
-    const uint8_t *a, *b;
-    const uint32_t *sa, *sb;
+    const void *x;               // [M][k], rows ldx apart
+    const uint8_t *b;
+    const uint32_t *sb;
     const void *bias;
-    void *out;
+    void *out;                   // [slices][M][N] where there are several slices
     int64_t ldx, ldo, kp;
-    int M, N, k, blocks, sd, bias_dtype;
+    int M, N, k, blocks, slice, sd, bias_dtype;
 };
-constexpr int kF8FewRows = 64, kF8RoundRows = 16, kF8FewWaves = 8;
+constexpr int kF8FewRows = 64, kF8FewWaves = 8;
 
-template <typename T, int MT, bool ROUND>
+template <typename T, typename O, int MT, int NT, int U>   // U: blocks under way at a time
 __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
     constexpr bool WIDE = sizeof(T) == 4;
-    constexpr int U = 4;
-    __shared__ f32x4 sums[kF8FewWaves][MT][64];
+    __shared__ f32x4 sums[kF8FewWaves / 2][NT * MT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, li = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16, row = min(n0 + li, p.N - 1);
-    const uint8_t *b = p.b + row * p.kp + q * 16;
-    const uint32_t *sb = p.sb + (int64_t)row * p.sd;
-    f32x4 acc[MT];
+    const int tiles = (p.N + 16 * NT - 1) / (16 * NT), slice = blockIdx.x / tiles, n0 = blockIdx.x % tiles * (16 * NT);
+    const int begin = slice * p.slice, end = min(begin + p.slice, p.blocks);
+    const uint8_t *b[NT];
+    const uint32_t *sb[NT];
 #pragma unroll
-    for (int u = 0; u < MT; ++u) acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int t = 0; t < NT; ++t) {
+        const int64_t row = min(n0 + 16 * t + li, p.N - 1);
+        b[t] = p.b + row * p.kp + q * 16;
+        sb[t] = p.sb + row * p.sd;
+    }
+    f32x4 acc[NT][MT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < MT; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto load = [](const uint8_t *from) {
-        const i32x4f lo = *reinterpret_cast<const i32x4f *>(from), hi = *reinterpret_cast<const i32x4f *>(from + 64);
-        return i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    };
-    auto multiply = [&](const i32x8f &bo, const i32x8f &ao, int bs, int as, int u) {   // scales in the lowest byte
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_widen(bo[2 * i], bo[2 * i + 1], f8_scale(bs, 0)), f8_widen(ao[2 * i], ao[2 * i + 1], f8_scale(as, 0)), acc[u], 0, 0, 0);
-        } else {
-            acc[u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bo, ao, acc[u], 0, 0, 0, bs, 0, as);
-        }
-    };
-    for (int first = wave; first < p.blocks; first += waves * U) {
-        i32x8f bo[U];
-        int bs[U];
+    for (int first = begin + wave; first < end; first += waves * U) {
+        i32x8f bo[U][NT];
+        int bs[U][NT];
+        F8Eight<T> e[U][MT][4];
 #pragma unroll
         for (int j = 0; j < U; ++j) {   // (blocks beyond the last repeat it; they are not multiplied)
-            const int k = min(first + j * waves, p.blocks - 1);
-            bo[j] = load(b + (int64_t)k * kF8Block);
-            bs[j] = (int)(sb[k >> 2] >> (8 * (k & 3)));
-        }
-        if constexpr (ROUND) {
-            const T *x = (const T *)p.x + (int64_t)min(li, p.M - 1) * p.ldx + q * 16;
-            F8Eight<T> e[U][4];
+            const int k = min(first + j * waves, end - 1);
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int k = min(first + j * waves, p.blocks - 1), c = k * kF8Block + q * 16;
+            for (int t = 0; t < NT; ++t) {
+                const uint8_t *from = b[t] + (int64_t)k * kF8Block;
+                const i32x4f lo = *reinterpret_cast<const i32x4f *>(from), hi = *reinterpret_cast<const i32x4f *>(from + 64);
+                bo[j][t] = i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                bs[j][t] = (int)(sb[t][k >> 2] >> (8 * (k & 3)));
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            const int k = min(first + j * waves, end - 1), c = k * kF8Block + q * 16;
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
+                const T *x = (const T *)p.x + min(16 * u + li, p.M - 1) * p.ldx + c;
                 if ((k + 1) * kF8Block <= p.k) {   // uniform
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) e[j][i].load(x + k * kF8Block + 64 * (i / 2) + 8 * (i % 2));
+                    for (int i = 0; i < 4; ++i) e[j][u][i].load(x + 64 * (i / 2) + 8 * (i % 2));
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const int w = 64 * (i / 16) + i % 16;
-                        e[j][i / 8].v[i % 8] = c + w < p.k ? x[k * kF8Block + w] : (T)0.0f;
+                        e[j][u][i / 8].v[i % 8] = c + w < p.k ? x[w] : (T)0.0f;
                     }
                 }
             }
+        }
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                if (first + j * waves >= p.blocks) break;
+        for (int j = 0; j < U; ++j) {
+            if (first + j * waves >= end) break;
+#pragma unroll
+            for (int u = 0; u < MT; ++u) {
                 unsigned most = 0;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) most = max(most, f8_magnitude((float)e[j][i / 8].v[i % 8]));
+                for (int i = 0; i < 32; ++i) most = max(most, f8_magnitude((float)e[j][u][i / 8].v[i % 8]));
                 const int ex = f8_exponent(f8_max_rows(most));
                 const float inv = f8_inverse(ex);
                 i32x8f ao;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const auto &v = e[j][i / 2].v;
+                    const auto &v = e[j][u][i / 2].v;
                     const int c = i % 2 * 4;
                     ao[i] = f8_pack((float)v[c], (float)v[c + 1], (float)v[c + 2], (float)v[c + 3], inv);
                 }
-                multiply(bo[j], ao, bs[j], ex + 127, 0);
-            }
-        } else {
-            i32x8f ao[MT][U];
-            int as[MT][U];
 #pragma unroll
-            for (int u = 0; u < MT; ++u) {
-                const int m = min(16 * u + li, p.M - 1);
-                const uint8_t *a = p.a + m * p.kp + q * 16;
+                for (int t = 0; t < NT; ++t) {
+                    if constexpr (WIDE) {
+                        const float as = f8_scale(ex + 127, 0), ws = f8_scale(bs[j][t], 0);
 #pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    const int k = min(first + j * waves, p.blocks - 1);
-                    ao[u][j] = load(a + (int64_t)k * kF8Block);
-                    as[u][j] = (int)(p.sa[(int64_t)m * p.sd + (k >> 2)] >> (8 * (k & 3)));
+                        for (int i = 0; i < 4; ++i)
+                            acc[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f8_widen(bo[j][t][2 * i], bo[j][t][2 * i + 1], ws), f8_widen(ao[2 * i], ao[2 * i + 1], as),
+                                                                                acc[t][u], 0, 0, 0);
+                    } else {
+                        acc[t][u] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bo[j][t], ao, acc[t][u], 0, 0, 0, bs[j][t], 0, ex + 127);
+                    }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < U; ++j)
-                if (first + j * waves < p.blocks) {
-#pragma unroll
-                    for (int u = 0; u < MT; ++u) multiply(bo[j], ao[u][j], bs[j], as[u][j], u);
-                }
         }
     }
+    // the upper half of the waves to the lower, then all four
+    constexpr int HALF = kF8FewWaves / 2;
+    if (wave >= HALF) {
 #pragma unroll
-    for (int u = 0; u < MT; ++u) sums[wave][u][lane] = acc[u];
+        for (int i = 0; i < NT * MT; ++i) sums[wave - HALF][i][lane] = acc[i / MT][i % MT];
+    }
     __syncthreads();
-    for (int u = wave; u < MT; u += waves) {
-        f32x4 s = sums[0][u][lane];
-        for (int w = 1; w < waves; ++w) s += sums[w][u][lane];
-        const int m = 16 * u + li, o = n0 + 4 * q;
-        if (m < p.M) {
-            T *out = (T *)p.out + (int64_t)m * p.ldo + o;
+    if (wave < HALF) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (o + i < p.N) out[i] = (T)(s[i] + (p.bias ? f8_bias(p.bias, o + i, p.bias_dtype) : 0.0f));
+        for (int i = 0; i < NT * MT; ++i) {
+            f32x4 s = acc[i / MT][i % MT];
+            if (wave + HALF < waves) s += sums[wave][i][lane];
+            sums[wave][i][lane] = s;
+        }
+    }
+    __syncthreads();
+    O *out = (O *)p.out + (int64_t)slice * p.M * p.N;
+    for (int i = wave; i < NT * MT; i += waves) {
+        f32x4 s = sums[0][i][lane];
+        for (int w = 1; w < min(waves, HALF); ++w) s += sums[w][i][lane];
+        const int m = 16 * (i % MT) + li, o = n0 + 16 * (i / MT) + 4 * q;
+        if (m < p.M) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (o + r < p.N) out[m * p.ldo + o + r] = (O)(s[r] + (p.bias ? f8_bias(p.bias, o + r, p.bias_dtype) : 0.0f));
         }
     }
 }
@@ -835,39 +843,41 @@ static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
     return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
 }
 
-// Few rows: which kernel, and with how many waves.
-static bool f8_few(const EvoFp8Matmul &p) { return p.m <= kF8FewRows; }
-static F8Few f8_few_args(const EvoFp8Matmul &p) {
-    F8Few a{};
-    a.a = (const uint8_t *)p.a;
-    a.b = (const uint8_t *)p.b;
-    a.sa = (const uint32_t *)p.scales_a;
-    a.sb = (const uint32_t *)p.scales_b;
-    a.bias = p.bias;
-    a.out = p.out;
-    a.ldo = p.ldo;
-    a.kp = f8_pitch(p.k);
-    a.M = (int)p.m;
-    a.N = (int)p.n;
-    a.k = (int)p.k;
-    a.blocks = (int)(a.kp / kF8Block);
-    a.sd = (int)(f8_scale_pitch(p.k) / 4);
-    a.bias_dtype = p.bias_dtype;
-    return a;
+// Few rows: 64 outputs to a workgroup where there are then enough of them for the chip, else 16, and slices of the contraction of a block at least for each wave.
+struct F8FewPlan {
+    int nt, slice, slices;
+};
+static F8FewPlan f8_few_plan(int64_t n, int64_t k) {
+    const int blocks = (int)((k + kF8Block - 1) / kF8Block), most = blocks < kF8FewWaves ? 1 : blocks / kF8FewWaves;
+    F8FewPlan q{};
+    q.nt = n >= 256 && (most >= 4 || (n + 63) / 64 * most >= 256) ? 4 : 1;
+    const int64_t groups = (n + 16 * q.nt - 1) / (16 * q.nt);
+    int64_t want = (256 + groups - 1) / groups;
+    if (want > most) want = most;
+    q.slice = (int)((blocks + want - 1) / want);
+    q.slices = (blocks + q.slice - 1) / q.slice;
+    return q;
 }
-template <typename T, bool ROUND>
-static int f8_launch_few(const F8Few &a, hipStream_t st) {
-    const unsigned grid = (unsigned)((a.N + 15) / 16), threads = 64 * (a.blocks < kF8FewWaves ? a.blocks : kF8FewWaves);
-    if constexpr (ROUND) {
-        fp8_few<T, 1, true><<<grid, threads, 0, st>>>(a);
-    } else {
-        switch ((a.M + 15) / 16) {
-            case 1: fp8_few<T, 1, false><<<grid, threads, 0, st>>>(a); break;
-            case 2: fp8_few<T, 2, false><<<grid, threads, 0, st>>>(a); break;
-            case 3: fp8_few<T, 3, false><<<grid, threads, 0, st>>>(a); break;
-            default: fp8_few<T, 4, false><<<grid, threads, 0, st>>>(a);
-        }
-    }
+template <typename T, typename O>
+static int f8_launch_few(const F8Few &a, const F8FewPlan &q, hipStream_t st) {
+    const unsigned grid = (unsigned)((a.N + 16 * q.nt - 1) / (16 * q.nt) * q.slices), threads = 64 * (q.slice < kF8FewWaves ? q.slice : kF8FewWaves);
+    auto go = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        constexpr int MANY = sizeof(T) == 4 ? 1 : MT > 2 ? 2 : 4;
+        if (q.nt == 4) fp8_few<T, O, MT, 4, 1><<<grid, threads, 0, st>>>(a);
+        else if (q.slice <= kF8FewWaves) fp8_few<T, O, MT, 1, 1><<<grid, threads, 0, st>>>(a);
+        else fp8_few<T, O, MT, 1, MANY><<<grid, threads, 0, st>>>(a);
+        return f8_rc();
+    };
+    const int mt = (a.M + 15) / 16;
+    return mt == 1 ? go(std::integral_constant<int, 1>()) : mt == 2 ? go(std::integral_constant<int, 2>()) : mt == 3 ? go(std::integral_constant<int, 3>())
+                                                                                                          : go(std::integral_constant<int, 4>());
+}
+template <typename T>
+static int f8_add_slices(const EvoFp8Matmul &p, int slices, hipStream_t st) {
+    const int64_t pieces = p.m * ((p.n + 7) / 8), groups = (pieces + 255) / 256;
+    if (groups > INT32_MAX) return EVO_EOVERFLOW;
+    fp8_slices<T><<<(unsigned)groups, 256, 0, st>>>((const float *)p.workspace, (T *)p.out, p.bias, p.bias_dtype, p.m, (int)p.n, p.ldo, slices);
     return f8_rc();
 }
 
@@ -922,7 +932,6 @@ int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t 
 size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p) {
     using namespace evo;
     if (f8_check(p)) return 0;
-    if (f8_few(*p)) return 0;
     const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
@@ -932,10 +941,6 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     if (const int rc = f8_check(p)) return rc;
     if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
-    if (f8_few(*p)) {
-        const F8Few few = f8_few_args(*p);
-        return f8_by_dtype(p->dtype, [&](auto t) { return f8_launch_few<decltype(t), false>(few, (hipStream_t)hip_stream); });
-    }
     const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
     F8Matmul a{};
@@ -961,25 +966,48 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
         return p->dtype == EVO_F32 ? f8_launch<float, true>(a, q, st) : p->dtype == EVO_BF16 ? f8_launch<bf16_t, false>(a, q, st) : f8_launch<f16_t, false>(a, q, st);
     }
     if (const int rc = wide ? f8_launch<float, true>(a, q, st) : f8_launch<float, false>(a, q, st)) return rc;
-    return f8_by_dtype(p->dtype, [&](auto t) {
-        typedef decltype(t) T;
-        const int64_t pieces = p->m * ((p->n + 7) / 8), groups = (pieces + 255) / 256;
-        if (groups > INT32_MAX) return (int)EVO_EOVERFLOW;
-        fp8_slices<T><<<(unsigned)groups, 256, 0, st>>>((const float *)p->workspace, (T *)p->out, p->bias, p->bias_dtype, p->m, (int)p->n, p->ldo, q.slices);
-        return f8_rc();
-    });
+    return f8_by_dtype(p->dtype, [&](auto t) { return f8_add_slices<decltype(t)>(*p, q.slices, st); });
+}
+
+size_t evoattn_fp8_matmul_few_workspace_bytes(const EvoFp8Matmul *p) {
+    using namespace evo;
+    if (f8_check(p) || p->m > kF8FewRows) return 0;
+    const F8FewPlan q = f8_few_plan(p->n, p->k);
+    return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
 
 int evoattn_fp8_matmul_few(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream) {
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
-    if (p->m > kF8RoundRows) return EVO_EUNSUPPORTED;
+    if (p->m > kF8FewRows) return EVO_EUNSUPPORTED;
     if (!x || ldx < p->k || !p->b || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->b, 16) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
-    F8Few few = f8_few_args(*p);
-    few.x = x;
-    few.ldx = ldx;
-    return f8_by_dtype(p->dtype, [&](auto t) { return f8_launch_few<decltype(t), true>(few, (hipStream_t)hip_stream); });
+    const F8FewPlan q = f8_few_plan(p->n, p->k);
+    const bool cut = q.slices > 1;
+    if (cut && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_few_workspace_bytes(p))) return EVO_EWORKSPACE;
+    F8Few a{};
+    a.x = x;
+    a.ldx = ldx;
+    a.b = (const uint8_t *)p->b;
+    a.sb = (const uint32_t *)p->scales_b;
+    a.bias = cut ? nullptr : p->bias;
+    a.out = cut ? p->workspace : p->out;
+    a.ldo = cut ? p->n : p->ldo;
+    a.kp = f8_pitch(p->k);
+    a.M = (int)p->m;
+    a.N = (int)p->n;
+    a.k = (int)p->k;
+    a.blocks = (int)(a.kp / kF8Block);
+    a.slice = q.slice;
+    a.sd = (int)(f8_scale_pitch(p->k) / 4);
+    a.bias_dtype = p->bias_dtype;
+    hipStream_t st = (hipStream_t)hip_stream;
+    return f8_by_dtype(p->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (!cut) return f8_launch_few<T, T>(a, q, st);
+        if (const int rc = f8_launch_few<T, float>(a, q, st)) return rc;
+        return f8_add_slices<T>(*p, q.slices, st);
+    });
 }
 
 }  // extern "C"

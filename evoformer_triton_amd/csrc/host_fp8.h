@@ -64,11 +64,17 @@ Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::Sca
 }
 
 // x b^T (+ bias) with x rounded on the way
+constexpr int64_t kF8FewRows = 64;   // that evoattn_fp8_matmul_few takes
 Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
     const int64_t rows = x.size(0);
-    if (rows <= 16) {
-        Tensor out = at::empty({rows, b.rows}, x.options());
-        const EvoFp8Matmul p = f8_product(rows, b, bias, out);
+    if (rows <= kF8FewRows) {
+        Tensor out = at::empty({rows, b.rows}, x.options()), ws;
+        EvoFp8Matmul p = f8_product(rows, b, bias, out);
+        if (const size_t bytes = evoattn_fp8_matmul_few_workspace_bytes(&p)) {
+            ws = scratch(bytes, x);
+            p.workspace = ws.data_ptr();
+            p.workspace_bytes = (size_t)ws.numel();
+        }
         check(evoattn_fp8_matmul_few(&p, x.data_ptr(), x.stride(0), stream_of(x)), "evoattn_fp8_matmul_few");
         return out;
     }
@@ -120,8 +126,12 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
     const Tensor x2 = f8_rows(x), w2 = f8_rows(w), b = bias.defined() ? bias.contiguous() : bias;
     Rounded xr, wr;
     f8_quantize(w2, &wr, need_x ? &saved->wt : nullptr, nullptr);
-    if (!need_w) return f8_times(x2, wr, b).view(shape);
-    f8_quantize(x2, &xr, &saved->xt, nullptr);
+    // (the same kernels whether or not gradients are wanted)
+    if (x2.size(0) <= kF8FewRows) {
+        if (need_w) f8_quantize(x2, nullptr, &saved->xt, nullptr);
+        return f8_times(x2, wr, b).view(shape);
+    }
+    f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
     return f8_matmul(xr, wr, b, x.scalar_type()).view(shape);
 }
 // dx, dw, db from dy [rows, n]

@@ -88,9 +88,12 @@ CASES = [
     (1, 1, 1, True, BF16, BF16, BF16),
     (1, 256, 1024, False, BF16, BF16, None),
     (5, 128, 3, True, F32, F32, F32),
-    (16, 1200, 33, True, BF16, BF16, F32),            # the most rows that are rounded on the way; ten blocks over eight waves
-    (33, 5000, 50, False, F16, BF16, None),           # three tiles of few rows, forty blocks
+    (16, 1200, 33, True, BF16, BF16, F32),            # few rows, rounded on the way: one tile, ten blocks over eight waves
+    (33, 5000, 50, False, F16, BF16, None),           # three tiles, five slices of eight blocks
     (50, 513, 200, True, F32, F32, F32),
+    (64, 1920, 8200, True, BF16, BF16, BF16),         # the most; 64 outputs to a workgroup, two slices
+    (20, 2048, 8192, True, F32, BF16, F32),
+    (65, 300, 70, True, BF16, BF16, BF16),            # one more
     (17, 200, 130, True, F16, F32, F16),
     (64, 640, 257, False, F32, BF16, None),
     (129, 129, 127, True, BF16, BF16, F32),           # a tile and a row; a block and a value
