@@ -486,6 +486,10 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     f8_store_tile<W, TM, TN, T>(acc, p, lds8, bias, wave, lane, m0, n0, wm, wn, slice);
 }
 
+struct F8Wide {   // 16 of a lane's values of a row as operands of two products
+    bf16x8 k[2];
+};
+
 // The same for large products: tiles of 256 x 256, eight waves of 128 x 64, 64 of the contraction at a time in a ring of four stages of 32 KB.
 // The two waves of a SIMD take turns: between two barriers one of them reads its operands (and asks for a stage) while the other
 // multiplies.  Waves 4 to 7 run one barrier behind waves 0 to 3.
@@ -493,7 +497,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
 // Step s: a wave reads stage s, asks for stage s + 3 into the place of stage s - 1, which the other half has read before the last barrier;
 // barrier; eight products; barrier.  Stage s + 1 is first read by waves 0 to 3 after their step s: before that barrier every wave's loads of it
 // have landed.  That is the end of step s for waves 0 to 3 and the middle of it for waves 4 to 7, when stages s + 2 and s + 3 are still under way.
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
     constexpr int W = 8, TM = 4, TN = 2, BM = 256, BN = 256, STAGE = (BM + BN) * 64, RING = 4, PIECES = 4;
     constexpr int SCALES = RING * STAGE, BIAS = SCALES + 2 * (BM + BN) * 4;
@@ -569,38 +573,64 @@ __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
                     if (s8 + 8 < ns) fetch_scales(s8 / 8 + 1);
                 }
                 const int slot = (j & 3) * STAGE;
-                i32x8f b[TN], a[TM];
-                auto operand = [&](const unsigned char *row) {
-                    const i32x4f lo = *reinterpret_cast<const i32x4f *>(row + slot + c0), hi = *reinterpret_cast<const i32x4f *>(row + slot + c1);
-                    return i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                };
+                // WIDE: half a stage at a time, widened before the barrier, while the other wave of the SIMD multiplies
+                constexpr int PARTS = WIDE ? 2 : 1;
 #pragma unroll
-                for (int t = 0; t < TN; ++t) b[t] = operand(bp + t * 2048);
+                for (int part = 0; part < PARTS; ++part) {
+                    constexpr bool ONCE = PARTS == 1;
+                    const bool ends = part == PARTS - 1;
+                    typename std::conditional<WIDE, F8Wide, i32x8f>::type b[TN], a[TM];
+                    i32x4f lo[TN + TM], hi[TN + TM];
 #pragma unroll
-                for (int u = 0; u < TM; ++u) a[u] = operand(ap + u * 2048);
-                // stage s + 1 has landed where stages s + 2 and s + 3, four loads each, may be under way; the last stages are waited for altogether
-                if (s + 3 < ns) {
-                    fetch(s + 3);
-                    if (LATE) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-                } else if (LATE) {
-                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    for (int i = 0; i < TN + TM; ++i) {
+                        const unsigned char *row = (i < TN ? bp + i * 2048 : ap + (i - TN) * 2048) + slot;
+                        lo[i] = *reinterpret_cast<const i32x4f *>(row + (part == 0 ? c0 : c1));
+                        if (ONCE) hi[i] = *reinterpret_cast<const i32x4f *>(row + c1);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TN + TM; ++i) {
+                        auto &to_ = i < TN ? b[i] : a[i - TN];
+                        if constexpr (ONCE) {
+                            to_ = i32x8f{lo[i][0], lo[i][1], lo[i][2], lo[i][3], hi[i][0], hi[i][1], hi[i][2], hi[i][3]};
+                        } else {
+                            const float f = f8_scale(i < TN ? ws[i] : xs[i - TN], j / 2);
+                            to_.k[0] = f8_widen(lo[i][0], lo[i][1], f);
+                            to_.k[1] = f8_widen(lo[i][2], lo[i][3], f);
+                            asm volatile("" : "+v"(to_.k[0]), "+v"(to_.k[1]));   // here, not where they are wanted
+                        }
+                    }
+                    // stage s + 1 has landed where stages s + 2 and s + 3, four loads each, may be under way; the last stages are waited for altogether
+                    if (part == 0 && s + 3 < ns) fetch(s + 3);
+                    if (LATE && ends) {
+                        if (s + 3 < ns) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+                        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier\n\ts_setprio 1" ::: "memory");
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (WIDE) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int t = 0; t < TN; ++t)
+#pragma unroll
+                                for (int u = 0; u < TM; ++u) acc[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[t].k[i], a[u].k[i], acc[t][u], 0, 0, 0);
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < TN; ++t)
+#pragma unroll
+                            for (int u = 0; u < TM; ++u)
+                                acc[t][u] = j / 2 == 0 ? f8_mma<0>(b[t], a[u], acc[t][u], ws[t], xs[u]) : j / 2 == 1 ? f8_mma<1>(b[t], a[u], acc[t][u], ws[t], xs[u])
+                                          : j / 2 == 2 ? f8_mma<2>(b[t], a[u], acc[t][u], ws[t], xs[u]) : f8_mma<3>(b[t], a[u], acc[t][u], ws[t], xs[u]);
+                    }
+#pragma unroll
+                    for (int t = 0; t < TN; ++t)   // the products stay between the barriers
+#pragma unroll
+                        for (int u = 0; u < TM; ++u) asm volatile("" : "+v"(acc[t][u]));
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (LATE || !ends) asm volatile("s_setprio 0\n\ts_barrier" ::: "memory");
+                    else if (s + 3 < ns) asm volatile("s_setprio 0\n\ts_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+                    else asm volatile("s_setprio 0\n\ts_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
                 }
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier\n\ts_setprio 1" ::: "memory");
-                __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-                for (int t = 0; t < TN; ++t)
-#pragma unroll
-                    for (int u = 0; u < TM; ++u)
-                        acc[t][u] = j / 2 == 0 ? f8_mma<0>(b[t], a[u], acc[t][u], ws[t], xs[u]) : j / 2 == 1 ? f8_mma<1>(b[t], a[u], acc[t][u], ws[t], xs[u])
-                                  : j / 2 == 2 ? f8_mma<2>(b[t], a[u], acc[t][u], ws[t], xs[u]) : f8_mma<3>(b[t], a[u], acc[t][u], ws[t], xs[u]);
-#pragma unroll
-                for (int t = 0; t < TN; ++t)   // the products stay between the barriers
-#pragma unroll
-                    for (int u = 0; u < TM; ++u) asm volatile("" : "+v"(acc[t][u]));
-                __builtin_amdgcn_sched_barrier(0);
-                if (LATE) asm volatile("s_setprio 0\n\ts_barrier" ::: "memory");
-                else if (s + 3 < ns) asm volatile("s_setprio 0\n\ts_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
-                else asm volatile("s_setprio 0\n\ts_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
             }
         }
     };
@@ -796,7 +826,7 @@ struct F8Plan {
 static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
     F8Plan q{};
     const int blocks = (int)((k + kF8Block - 1) / kF8Block);
-    q.big = dtype != EVO_F32 && blocks >= 4 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
+    q.big = blocks >= 4 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
     const int side = q.big ? 256 : 128;
     q.mt = (int)((m + side - 1) / side);
     q.nt = (int)((n + side - 1) / side);
@@ -831,14 +861,12 @@ static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
 template <typename T, bool WIDE>
 static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
     const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
-    if constexpr (!WIDE) {
-        if (q.big) {
-            constexpr int lds = 4 * 512 * 64 + 2 * 512 * 4 + 256 * 4;
-            static PerDevice done;
-            if (const int rc = ensure_dynamic_lds((const void *)fp8_matmul_big<T>, lds, done, nullptr)) return rc;
-            fp8_matmul_big<T><<<grid, 512, lds, st>>>(a);
-            return f8_rc();
-        }
+    if (q.big) {
+        constexpr int lds = 4 * 512 * 64 + 2 * 512 * 4 + 256 * 4;
+        static PerDevice done;
+        if (const int rc = ensure_dynamic_lds((const void *)fp8_matmul_big<T, WIDE>, lds, done, nullptr)) return rc;
+        fp8_matmul_big<T, WIDE><<<grid, 512, lds, st>>>(a);
+        return f8_rc();
     }
     return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
 }

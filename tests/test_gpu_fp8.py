@@ -103,6 +103,7 @@ CASES = [
     (128, 4224, 64, True, BF16, BF16, BF16),          # the forward in slices of the contraction
     (65537, 130, 200, True, BF16, BF16, BF16),        # tiles of 256 x 256, the last of one row; two blocks, of which one has two values
     (33000, 700, 300, False, F16, F16, None),         # two and three of them side by side; more than one group of scales
+    (33000, 600, 520, True, F32, F32, F32),           # the same in fp32
 ]
 
 
