@@ -831,7 +831,7 @@ static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
     q.mt = (int)((m + side - 1) / side);
     q.nt = (int)((n + side - 1) / side);
     const int64_t tiles = (int64_t)q.mt * q.nt;
-    int64_t want = tiles >= 256 ? 1 : 512 / tiles;
+    int64_t want = tiles >= 256 ? 1 : 256 / tiles;
     if (want > blocks / 8) want = blocks / 8;
     if (want < 1) want = 1;
     q.slice = (int)((blocks + want - 1) / want + 3) / 4 * 4;

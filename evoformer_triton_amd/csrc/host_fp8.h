@@ -1,16 +1,15 @@
 // Linear layers in 8 bits (csrc/fp8.hip): part of host.cpp.
 
-// A matrix [rows, k] rounded along its rows: values [rows, k up to the next 128], scales [rows, blocks up to the next 4].
+// A matrix [rows, k] rounded along its rows: values [rows, k up to the next 128], scales [rows, blocks up to the next 4], in one piece of memory (an
+// allocation costs the host a microsecond) or a caller's two.
 struct Rounded {
-    Tensor q, s;
+    Tensor hold;
+    void *q = nullptr, *s = nullptr;
     int64_t rows = 0, k = 0;
     Rounded() = default;
-    Rounded(const Tensor &q_, const Tensor &s_, int64_t k_) : q(q_), s(s_), rows(q_.size(0)), k(k_) {}
-    Rounded(int64_t rows_, int64_t k_, const Tensor &like) : rows(rows_), k(k_) {
-        const auto o = like.options().dtype(at::kByte);
-        q = at::empty({rows, pitch(k)}, o);
-        s = at::empty({rows, scale_pitch(k)}, o);
-    }
+    Rounded(const Tensor &values, const Tensor &scales, int64_t k_) : q(values.data_ptr()), s(scales.data_ptr()), rows(values.size(0)), k(k_) {}
+    Rounded(const Tensor &hold_, int64_t rows_, int64_t k_) : hold(hold_), q(hold_.data_ptr()), s((char *)hold_.data_ptr() + rows_ * pitch(k_)), rows(rows_), k(k_) {}
+    Rounded(int64_t rows_, int64_t k_, const Tensor &like) : Rounded(at::empty({rows_ * (pitch(k_) + scale_pitch(k_))}, like.options().dtype(at::kByte)), rows_, k_) {}
     static int64_t pitch(int64_t k) { return (k + 127) / 128 * 128; }
     static int64_t scale_pitch(int64_t k) { return (k + 511) / 512 * 4; }
 };
@@ -27,9 +26,9 @@ void f8_quantize(const Tensor &x, Rounded *along_rows, Rounded *along_cols, Tens
     if (along_rows) *along_rows = Rounded(rows, cols, x);
     if (along_cols) *along_cols = Rounded(cols, rows, x);
     if (sums) *sums = at::empty({(rows + 127) / 128, cols}, x.options().dtype(at::kFloat));
-    check(evoattn_fp8_quantize(x.data_ptr(), x.stride(0), along_rows ? along_rows->q.data_ptr() : nullptr, along_rows ? along_rows->s.data_ptr() : nullptr,
-                               along_cols ? along_cols->q.data_ptr() : nullptr, along_cols ? along_cols->s.data_ptr() : nullptr,
-                               sums ? (float *)sums->data_ptr() : nullptr, rows, cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
+    check(evoattn_fp8_quantize(x.data_ptr(), x.stride(0), along_rows ? along_rows->q : nullptr, along_rows ? along_rows->s : nullptr,
+                               along_cols ? along_cols->q : nullptr, along_cols ? along_cols->s : nullptr, sums ? (float *)sums->data_ptr() : nullptr, rows,
+                               cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
 }
 
 EvoFp8Matmul f8_product(int64_t rows, const Rounded &b, const Tensor &bias, const Tensor &out) {
@@ -39,8 +38,8 @@ EvoFp8Matmul f8_product(int64_t rows, const Rounded &b, const Tensor &bias, cons
     p.k = b.k;
     p.ldo = b.rows;
     p.dtype = evo_dtype(out.scalar_type());
-    p.b = b.q.data_ptr();
-    p.scales_b = b.s.data_ptr();
+    p.b = b.q;
+    p.scales_b = b.s;
     if (bias.defined()) {
         p.bias = bias.data_ptr();
         p.bias_dtype = evo_dtype(bias.scalar_type());
@@ -48,18 +47,18 @@ EvoFp8Matmul f8_product(int64_t rows, const Rounded &b, const Tensor &bias, cons
     p.out = out.data_ptr();
     return p;
 }
-// a b^T (+ bias), [a.rows, b.rows]
-Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype) {
-    Tensor out = at::empty({a.rows, b.rows}, a.q.options().dtype(dtype)), ws;
+// a b^T (+ bias), [a.rows, b.rows], on `like`'s device
+Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype, const Tensor &like) {
+    Tensor out = at::empty({a.rows, b.rows}, like.options().dtype(dtype)), ws;
     EvoFp8Matmul p = f8_product(a.rows, b, bias, out);
-    p.a = a.q.data_ptr();
-    p.scales_a = a.s.data_ptr();
+    p.a = a.q;
+    p.scales_a = a.s;
     if (const size_t bytes = evoattn_fp8_matmul_workspace_bytes(&p)) {
-        ws = scratch(bytes, a.q);
+        ws = scratch(bytes, like);
         p.workspace = ws.data_ptr();
         p.workspace_bytes = (size_t)ws.numel();
     }
-    check(evoattn_fp8_matmul(&p, stream_of(a.q)), "evoattn_fp8_matmul");
+    check(evoattn_fp8_matmul(&p, stream_of(like)), "evoattn_fp8_matmul");
     return out;
 }
 
@@ -80,7 +79,7 @@ Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
     }
     Rounded a;
     f8_quantize(x, &a, nullptr, nullptr);
-    return f8_matmul(a, b, bias, x.scalar_type());
+    return f8_matmul(a, b, bias, x.scalar_type(), x);
 }
 
 const char *f8_wrong(const Tensor &x, int64_t n, int64_t k, const c10::Device &device, const OptTensor &bias) {
@@ -132,7 +131,7 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
         return f8_times(x2, wr, b).view(shape);
     }
     f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
-    return f8_matmul(xr, wr, b, x.scalar_type()).view(shape);
+    return f8_matmul(xr, wr, b, x.scalar_type(), x2).view(shape);
 }
 // dx, dw, db from dy [rows, n]
 void f8_backward(const Tensor &dy, const F8Saved &saved, bool need_x, bool need_w, bool need_b, at::ScalarType wtype, at::ScalarType btype, Tensor &dx, Tensor &dw,
@@ -142,8 +141,8 @@ void f8_backward(const Tensor &dy, const F8Saved &saved, bool need_x, bool need_
     Tensor sums;
     const bool cols = need_w || need_b;
     f8_quantize(dy, need_x ? &along_rows : nullptr, cols ? &along_cols : nullptr, need_b ? &sums : nullptr);
-    if (need_x) dx = f8_matmul(along_rows, saved.wt, Tensor(), dy.scalar_type());
-    if (need_w) dw = f8_matmul(along_cols, saved.xt, Tensor(), wtype);
+    if (need_x) dx = f8_matmul(along_rows, saved.wt, Tensor(), dy.scalar_type(), dy);
+    if (need_w) dw = f8_matmul(along_cols, saved.xt, Tensor(), wtype, dy);
     if (need_b) {
         db = at::empty({dy.size(1)}, dy.options().dtype(btype));
         check(evoattn_fp8_column_sums((const float *)sums.data_ptr(), db.data_ptr(), dy.size(0), dy.size(1), evo_dtype(btype), stream_of(dy)),
@@ -157,7 +156,7 @@ struct Fp8LinearNode : SavingNode {
     at::ScalarType x_type = at::kFloat, w_type = at::kFloat, b_type = at::kFloat;
     bool has_bias = false;
     std::string name() const override { return "Fp8LinearBackward"; }
-    // saved: x^T and w^T rounded, values and scales; results: x, weight, bias
+    // saved: x^T and w^T rounded; results: x, weight, bias
     variable_list apply(variable_list &&grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         const bool rec = at::GradMode::is_enabled();
@@ -166,11 +165,7 @@ struct Fp8LinearNode : SavingNode {
         {
             at::AutoDispatchBelowADInplaceOrView guard;
             const Tensor d = grads[0].scalar_type() == x_type ? grads[0] : grads[0].to(x_type);
-            Tensor t[4];
-            for (int i = 0; i < 4; ++i) {
-                t[i] = saved[i].unpack();
-                if (t[i].defined()) t[i] = t[i].contiguous();
-            }
+            const Tensor xt = saved[0].unpack(), wt = saved[1].unpack();
             const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = has_bias && task_should_compute_output(2);
             if (d.numel() == 0 || k == 0) {
                 if (need_x) out[0] = at::zeros(x_shape, d.options());
@@ -178,8 +173,8 @@ struct Fp8LinearNode : SavingNode {
                 if (need_b) out[2] = d.numel() ? as_rows(d).sum(0).to(b_type) : at::zeros({n}, d.options().dtype(b_type));
             } else if (need_x || need_w || need_b) {
                 F8Saved s;
-                if (need_w) s.xt = Rounded(t[0], t[1], d.numel() / n);
-                if (need_x) s.wt = Rounded(t[2], t[3], n);
+                if (need_w) s.xt = Rounded(xt.contiguous(), k, d.numel() / n);
+                if (need_x) s.wt = Rounded(wt.contiguous(), k, n);
                 f8_backward(f8_rows(d), s, need_x, need_w, need_b, w_type, b_type, out[0], out[1], out[2]);
                 if (need_x) out[0] = out[0].view(x_shape);
             }
@@ -210,7 +205,8 @@ OptTensor fp8_linear(const Tensor &x, const Tensor &weight, const OptTensor &bia
         node->has_bias = b.defined();
         if (b.defined()) node->b_type = b.scalar_type();
         torch::autograd::set_history(y, node);
-        for (const Tensor *t : {&s.xt.q, &s.xt.s, &s.wt.q, &s.wt.s}) node->save(*t);
+        node->save(s.xt.hold);
+        node->save(s.wt.hold);
     }
     return y;
 }
@@ -279,9 +275,14 @@ std::pair<Tensor, Tensor> fp8_round(const Tensor &w) {
     TORCH_CHECK_VALUE(w.size(1) <= 1 << 22, "the weight has more than 2^22 columns");
     TORCH_CHECK(w.is_cuda(), "rounding to 8 bits runs on the GPU only");
     c10::DeviceGuard on(w.device());
-    Rounded r(w.size(0), w.size(1), w);
-    if (w.numel()) f8_quantize(f8_rows(w), &r, nullptr, nullptr);
-    return {r.q, r.s};
+    const auto o = w.options().dtype(at::kByte);
+    const Tensor values = at::empty({w.size(0), Rounded::pitch(w.size(1))}, o), scales = at::empty({w.size(0), Rounded::scale_pitch(w.size(1))}, o);
+    if (w.numel()) {
+        const Tensor r = f8_rows(w);
+        check(evoattn_fp8_quantize(r.data_ptr(), r.stride(0), values.data_ptr(), scales.data_ptr(), nullptr, nullptr, nullptr, r.size(0), r.size(1),
+                                   evo_dtype(r.scalar_type()), stream_of(r)), "evoattn_fp8_quantize");
+    }
+    return {values, scales};
 }
 std::optional<std::string> fp8_linear_wrong(const Tensor &x, const Tensor &weight, const OptTensor &bias) {
     const char *wrong = f8_linear_wrong(x, weight, bias);
