@@ -20,11 +20,13 @@ idle), and lays the results out so that the attention kernels read them as they 
     of its own;
   * the gated output [B,S,N,H,D] viewed as [B,S,N,H*D] is the input of the output projection;
   * the pair bias Linear(LayerNorm(z)) comes from one kernel as [B,1,H,N,N] in the dtype of Q, so the attention kernels
-    take it from 16-bit tiles; for shapes that kernel does not take, from the separate steps and a permute.
+    take it from 16-bit tiles; for shapes that kernel does not take, from the separate steps and a permute;
+  * a learned relative position bias (`relative.py`) is added to the pair bias, or stands for it, if the block has one;
+  * the projections run in 8 bits (`fp8.py`) if the block is made so.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch import nn
@@ -32,6 +34,8 @@ from torch import nn
 from . import _lib
 from . import evoformer as _evoformer
 from .evoformer import _DTYPES, _HEAD_DIMS, _SlotAttention, _alloc_bytes, _on_device, _ptr, _stream, evoformer_attention
+from .fp8 import Fp8Weight, fp8_linear
+from .relative import RelativePositionBias
 
 
 def _row_slices(rows: int, n_out: int, n_in: int) -> int:
@@ -182,6 +186,13 @@ _NO_PARAMETERS = {"weight": None, "bias": None}
 _UNBIASED = ("linear_q", "linear_k", "linear_v", "linear_z")
 
 
+class Fp8BlockWeights(NamedTuple):
+    """A block's projections in 8 bits, for inference: `GatedAttentionBlock.fp8_weights`."""
+    projections: Fp8Weight               # Q, K, V (and the gate), stacked
+    bias: Optional[torch.Tensor]         # theirs: zeros but for the gate's
+    output: Fp8Weight
+
+
 class GatedAttentionBlock(nn.Module):
     """Row-wise gated self-attention with pair bias (the MSA row attention of an Evoformer
     block).
@@ -189,12 +200,22 @@ class GatedAttentionBlock(nn.Module):
     m    [B,S,N,c_m]   the representation attended over (S rows of N residues)
     z    [B,N,N,c_z]   optional pair representation; its projection to H channels is the bias
     mask [B,S,N]       optional, 1 = keep, 0 = drop the key (bool or float)
+    positions [B,N] or [N], chains alike (optional): the residues' numbers and chains, for a block with a relative position bias
+    weights            Fp8BlockWeights of `fp8_weights()`, for inference with a block in 8 bits; else the weights are rounded with each call
     ->   [B,S,N,c_m]
+
+    fp8                       the projections in 8 bits (fp8_linear): operands rounded to e4m3 with a scale for each block of 128, forward and backward
+    relative_distance, relative_buckets, other_chain   a learned relative position bias, as RelativePositionBias takes them
     """
 
+    fp8 = False
+
     def __init__(self, c_m: int, c_hidden: int, no_heads: int, c_z: Optional[int] = None, gating: bool = True,
-                 inf: float = 1e9):
+                 inf: float = 1e9, fp8: bool = False, relative_distance: Optional[int] = None, relative_buckets: Optional[int] = None,
+                 other_chain: bool = False):
         super().__init__()
+        if fp8:
+            self.fp8 = True
         self.c_hidden, self.no_heads, self.inf = c_hidden, no_heads, inf
         hd = c_hidden * no_heads
         self.layer_norm_m = nn.LayerNorm(c_m)
@@ -208,8 +229,28 @@ class GatedAttentionBlock(nn.Module):
             self.linear_z = nn.Linear(c_z, no_heads, bias=False)
         else:
             self.layer_norm_z = self.linear_z = None
+        if relative_distance is not None:
+            self.relative = RelativePositionBias(no_heads, relative_distance, relative_buckets, other_chain)
+        elif relative_buckets is not None or other_chain:
+            raise ValueError("relative_buckets and other_chain need relative_distance")
+        else:
+            self.register_module("relative", None)
 
-    def operands(self, m: torch.Tensor, z: Optional[torch.Tensor], mask: Optional[torch.Tensor], plain: bool = False):
+    def _stacked_weights(self):
+        layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
+        weight, bias = torch.cat([l.weight for l in layers], 0), None
+        if self.linear_g is not None:
+            bias = torch.nn.functional.pad(self.linear_g.bias, (weight.shape[0] - self.linear_g.bias.shape[0], 0))
+        return weight, bias
+
+    @torch.no_grad()
+    def fp8_weights(self) -> Fp8BlockWeights:
+        """The projections rounded once, to be given to inference calls (and made anew after the parameters have changed)."""
+        weight, bias = self._stacked_weights()
+        return Fp8BlockWeights(Fp8Weight.of(weight), bias, Fp8Weight.of(self.linear_o.weight))
+
+    def operands(self, m: torch.Tensor, z: Optional[torch.Tensor], mask: Optional[torch.Tensor], plain: bool = False,
+                 positions: Optional[torch.Tensor] = None, chains: Optional[torch.Tensor] = None, weights: Optional[Fp8BlockWeights] = None):
         """Q, K, V, gate [B,S,N,H,D] (views of the projections), additive mask [B,S,1,1,N],
         bias [B,1,H,N,N].  `plain`: the framework's LayerNorm and Linear throughout (what
         `forward_eager` uses), else the library's LayerNorm kernels and the projections with
@@ -222,23 +263,47 @@ class GatedAttentionBlock(nn.Module):
         layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
         if plain:
             outs = [layer(x) for layer in layers]
+        elif self.fp8:
+            outs = self._project(x, weights).unflatten(-1, (len(layers), H * D)).unbind(-2)
         else:
             outs = _Projections.apply(x, *(t for layer in layers for t in (layer.weight, layer.bias)))
         q, k, v = (t.view(B, S, N, H, D) for t in outs[:3])
         g = outs[3].view(B, S, N, H, D) if self.linear_g is not None else None
-        bias, add_mask = self._bias_and_mask(z, mask, q.dtype, (B, S, N), norm, lin)
+        bias, add_mask = self._bias_and_mask(z, mask, q.dtype, (B, S, N), norm, lin, positions, chains, plain)
         return q, k, v, g, add_mask, bias
 
-    def _bias_and_mask(self, z, mask, dtype, shape, norm, lin):
+    def _project(self, x: torch.Tensor, weights: Optional[Fp8BlockWeights]) -> torch.Tensor:
+        """Q, K, V (and the gate) side by side, in 8 bits."""
+        if weights is not None:
+            return fp8_linear(x, weights.projections, weights.bias)
+        return fp8_linear(x, *self._stacked_weights())
+
+    def _output(self, o: torch.Tensor, weights: Optional[Fp8BlockWeights], place: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if self.fp8:
+            return fp8_linear(o, self.linear_o.weight if weights is None else weights.output, self.linear_o.bias)
+        return _linear(self.linear_o, o, place)
+
+    def _bias_and_mask(self, z, mask, dtype, shape, norm, lin, positions=None, chains=None, plain=False):
         B, S, N = shape
         bias = add_mask = None
         if z is not None and self.linear_z is not None and norm is _layer_norm and lin is _linear and z.dtype == dtype:
             bias = _pair_bias(self.layer_norm_z, self.linear_z, z)
         if bias is None and z is not None and self.linear_z is not None:
             bias = lin(self.linear_z, norm(self.layer_norm_z, z)).permute(0, 3, 1, 2).unsqueeze(1).contiguous().to(dtype)
+        if self.relative is not None:
+            bias = (self.relative.plain if plain else self.relative)(positions, chains=chains, pair_bias=bias, dtype=dtype)
         if mask is not None:
             add_mask = (self.inf * (mask.to(torch.float32) - 1.0)).view(B, S, 1, 1, N)
         return bias, add_mask
+
+    def _check(self, positions, chains, weights):
+        if (positions is None) != (self.relative is None):
+            raise ValueError("a block with a relative position bias needs the residues' positions" if positions is None else
+                             "positions are for a block with a relative position bias (relative_distance)")
+        if chains is not None and (self.relative is None or not self.relative.other_chain):
+            raise ValueError("chains are for a block with a bucket for pairs of different chains (other_chain=True)")
+        if weights is not None and not self.fp8:
+            raise ValueError("weights in 8 bits are for a block made with fp8=True")
 
     def _slots_ok(self, m: torch.Tensor) -> bool:
         """Whether Q, K, V and the gate can come from one GEMM and reach the kernels as slots of its result."""
@@ -268,29 +333,38 @@ class GatedAttentionBlock(nn.Module):
         return _lib.host().block(inputs, mask, self.no_heads, mods["layer_norm_m"].eps, mods["layer_norm_z"].eps if with_z else 0.0, self.inf,
                                  _evoformer.FLAGS)
 
-    def forward(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
+    def forward(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                positions: Optional[torch.Tensor] = None, chains: Optional[torch.Tensor] = None, weights: Optional[Fp8BlockWeights] = None):
         B, S, N, _ = m.shape
+        simple = not self.fp8 and self.relative is None and positions is None and chains is None and weights is None
+        if not simple:
+            self._check(positions, chains, weights)
         if self._slots_ok(m):
-            out = self._native(m, z, mask)
+            out = self._native(m, z, mask) if simple else None
             if out is not None:
                 return out
             H, D = self.no_heads, self.c_hidden
             gated = self.linear_g is not None
             x = _layer_norm(self.layer_norm_m, m)
-            weights = [self.linear_q.weight, self.linear_k.weight, self.linear_v.weight] + ([self.linear_g.weight] if gated else [])
-            P = _StackedProjection.apply(x, self.linear_g.bias if gated else None, *weights).view(B, S, N, len(weights), H, D)
-            bias, add_mask = self._bias_and_mask(z, mask, m.dtype, (B, S, N), _layer_norm, _linear)
+            if self.fp8:
+                P = self._project(x, weights).view(B, S, N, 4 if gated else 3, H, D)
+            else:
+                projections = [self.linear_q.weight, self.linear_k.weight, self.linear_v.weight] + ([self.linear_g.weight] if gated else [])
+                P = _StackedProjection.apply(x, self.linear_g.bias if gated else None, *projections).view(B, S, N, len(projections), H, D)
+            bias, add_mask = self._bias_and_mask(z, mask, m.dtype, (B, S, N), _layer_norm, _linear, positions, chains)
             o, grad_slot = _SlotAttention.apply(P, add_mask, bias, gated)
-            return _linear(self.linear_o, o.reshape(B, S, N, H * D), grad_slot.view(B, S, N, H * D))
-        q, k, v, g, add_mask, bias = self.operands(m, z, mask)
+            return self._output(o.reshape(B, S, N, H * D), weights, grad_slot.view(B, S, N, H * D))
+        q, k, v, g, add_mask, bias = self.operands(m, z, mask, positions=positions, chains=chains, weights=weights)
         o = evoformer_attention(q, k, v, add_mask, bias, layout="ds4sci", gate=g)
-        return _linear(self.linear_o, o.reshape(B, S, N, self.no_heads * self.c_hidden))
+        return self._output(o.reshape(B, S, N, self.no_heads * self.c_hidden), weights)
 
-    def forward_eager(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None):
+    def forward_eager(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
+                      positions: Optional[torch.Tensor] = None, chains: Optional[torch.Tensor] = None):
         """The same block with plain torch operations (the formula of the reference's oracle,
-        test.py:47-57, with the per-head view): what `forward` is tested against."""
+        test.py:47-57, with the per-head view), nothing rounded to 8 bits: what `forward` is tested against."""
         B, S, N, _ = m.shape
-        q, k, v, g, add_mask, bias = self.operands(m, z, mask, plain=True)
+        self._check(positions, chains, None)
+        q, k, v, g, add_mask, bias = self.operands(m, z, mask, plain=True, positions=positions, chains=chains)
         qh, kh, vh = (t.permute(0, 1, 3, 2, 4) for t in (q, k, v))              # [B,S,H,N,D]
         s = torch.matmul(qh * self.c_hidden ** -0.5, kh.transpose(-1, -2)).float()
         if bias is not None:

@@ -158,3 +158,16 @@ class RelativePositionBias(nn.Module):
         if chains is not None and not self.other_chain:
             raise ValueError("chains need a table with a row for pairs of different chains (other_chain=True)")
         return relative_position_bias(self.weight, self.buckets, positions, key_positions, chains=chains, key_chains=key_chains, pair_bias=pair_bias, dtype=dtype)
+
+    def plain(self, positions: torch.Tensor, *, chains: Optional[torch.Tensor] = None, pair_bias: Optional[torch.Tensor] = None,
+              dtype: Optional[torch.dtype] = None):
+        """The bias of residues among themselves in plain torch operations, on any device: what the kernel is tested against."""
+        at, reach = positions if positions.dim() == 2 else positions[None], self.buckets.numel() // 2
+        bucket = self.buckets.long()[(at[:, :, None] - at[:, None, :]).clamp(-reach, reach) + reach]
+        if chains is not None:
+            c = chains if chains.dim() == 2 else chains[None]
+            bucket = torch.where(c[:, :, None] == c[:, None, :], bucket, self.weight.shape[0] - 1)
+        out = self.weight.float()[bucket].permute(0, 3, 1, 2).unsqueeze(1)
+        if pair_bias is not None:
+            out = out + pair_bias.float()
+        return out.to(dtype or (self.weight if pair_bias is None else pair_bias).dtype)

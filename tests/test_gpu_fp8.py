@@ -142,3 +142,135 @@ def test_products_and_gradients(gpu_device, case):
     with torch.no_grad():
         held = fp8_linear(leaves[0], Fp8Weight.of(leaves[1]), leaves[2] if with_bias else None)
     assert torch.equal(held, y)
+
+
+def test_rows_with_infinities_and_nan_are_theirs_alone(gpu_device):
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    g = torch.Generator().manual_seed(4)
+    w = Fp8Weight.of(torch.randn((70, 300), generator=g).to(gpu_device))
+    for rows in (5, 200):
+        x = torch.randn((rows, 300), generator=g).to(BF16)
+        with torch.no_grad():
+            want = fp8_linear(x.to(gpu_device), w)
+            x[2, 7], x[4, 299] = float("inf"), float("nan")
+            got = fp8_linear(x.to(gpu_device), w)
+        bad = torch.tensor([2, 4], device=gpu_device)
+        assert got[bad].isnan().all()
+        keep = torch.ones(rows, dtype=torch.bool, device=gpu_device)
+        keep[bad] = False
+        assert torch.equal(got[keep], want[keep])
+
+
+def test_strides_shapes_and_streams(gpu_device):
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    g = torch.Generator().manual_seed(6)
+    wide = torch.randn((4, 40, 901), generator=g).to(F16).to(gpu_device)
+    wt = torch.randn((333, 300), generator=g).to(gpu_device)                         # the weight as the transpose of a tensor
+    bias = torch.randn((601,), generator=g).to(F16).to(gpu_device)[1::2][:300]
+    cases = (wide[..., 3:336], wide[:, ::2, 3:336], wide[0, :, 1:334], wide[0, 0, :333], wide.transpose(0, 1)[..., :333], wide[..., ::2][..., 100:433])
+    for x in cases:
+        def step():
+            leaves = [x.detach().requires_grad_(), wt.detach().t().requires_grad_(), bias.detach().requires_grad_()]
+            y = fp8_linear(*leaves)
+            return [y.detach(), *torch.autograd.grad(y.sum(), leaves)]
+
+        leaves = [x.detach().contiguous().requires_grad_(), wt.detach().t().contiguous().requires_grad_(), bias.detach().contiguous().requires_grad_()]
+        y = fp8_linear(*leaves)
+        want = [y.detach(), *torch.autograd.grad(y, leaves, torch.ones_like(y))]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = step()
+        torch.cuda.current_stream().wait_stream(side)
+        with torch.autograd.graph.save_on_cpu():
+            hooked = step()
+        for a, b, c in zip(got, want, hooked):
+            assert a.shape == b.shape and torch.equal(a, b) and torch.equal(c, b)
+        with torch.no_grad():
+            assert torch.equal(fp8_linear(x, Fp8Weight.of(wt.t()), bias), want[0])
+
+
+def test_empty_calls(gpu_device):
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    for rows, k, n in ((0, 5, 3), (4, 0, 3), (4, 5, 0), (0, 0, 0)):
+        x, w, b = (torch.randn(s, device=gpu_device).requires_grad_() for s in ((rows, k), (n, k), (n,)))
+        y = fp8_linear(x, w, b)
+        assert y.shape == (rows, n)
+        if k == 0:
+            assert torch.equal(y, b.detach().expand(rows, n))
+        dx, dw, db = torch.autograd.grad(y.sum() + 0 * (x.sum() + w.sum() + b.sum()), [x, w, b])
+        assert not dx.any() and not dw.any() and dx.shape == x.shape and dw.shape == w.shape and torch.equal(db, torch.full_like(b, float(rows)))
+        with torch.no_grad():
+            assert torch.equal(fp8_linear(x, Fp8Weight.of(w), b), y)
+
+
+def test_an_8_bit_weight_takes_no_gradients(gpu_device):
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    w = Fp8Weight.of(torch.randn(8, 16, device=gpu_device))
+    x, b = torch.randn(3, 16, device=gpu_device), torch.randn(8, device=gpu_device)
+    for args in ((x.clone().requires_grad_(), w), (x, w, b.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            fp8_linear(*args)
+        with torch.no_grad():
+            assert fp8_linear(*args).shape == (3, 8)
+
+
+@pytest.mark.parametrize("rows", [20, 300])
+def test_a_captured_step_replays(gpu_device, rows):
+    from evoformer_triton_amd import fp8_linear
+    x, w, b = (torch.randn(s, device=gpu_device).to(BF16).requires_grad_() for s in ((rows, 1200), (90, 1200), (90,)))
+    dy = torch.randn(rows, 90, device=gpu_device).to(BF16)
+
+    def step():
+        y = fp8_linear(x, w, b)
+        return [y.detach(), *torch.autograd.grad(y, [x, w, b], dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in range(4):
+        g = torch.Generator().manual_seed(seed)
+        for t in (x, w, dy):
+            t.data.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, c in zip(held, step()):
+            assert torch.equal(a, c)
+
+
+def test_compiled_and_watched_calls_and_transforms(gpu_device):
+    from torch.autograd import forward_ad
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    leaves = [torch.randn(s, device=gpu_device).requires_grad_() for s in ((70, 140), (30, 140), (30,))]
+    want = fp8_linear(*leaves)
+    want_g = torch.autograd.grad(want, leaves, torch.ones_like(want))
+    seen = []
+
+    class Recorder(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    with Recorder():
+        watched = fp8_linear(*leaves)
+    compiled = torch.compile(fp8_linear, fullgraph=True, backend="aot_eager")(*leaves)
+    assert any("fp8_linear" in s for s in seen)
+    for y in (watched, compiled):
+        assert torch.equal(y, want) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, torch.ones_like(y)), want_g))
+    held = Fp8Weight.of(leaves[1])
+    with torch.no_grad():
+        assert torch.equal(torch.compile(lambda t: fp8_linear(t, held, leaves[2]), fullgraph=True, backend="aot_eager")(leaves[0]), want)
+    x, w = leaves[0].detach(), leaves[1].detach()
+    pair = torch.stack((x, 2 * x))
+    assert torch.equal(torch.func.vmap(lambda t: fp8_linear(t, w))(pair), torch.stack((fp8_linear(x, w), fp8_linear(2 * x, w))))
+    with forward_ad.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+        fp8_linear(forward_ad.make_dual(x, torch.ones_like(x)).requires_grad_(), w)
+    dx, = torch.autograd.grad(fp8_linear(*leaves).square().sum(), leaves[0], create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        dx.sum().backward()
