@@ -37,7 +37,7 @@ EXPORTS = ("evoattn_version", "evoattn_strerror", "evoattn_check", "evoattn_prep
            "evoattn_pair_bias_workspace_bytes", "evoattn_pair_bias_fwd", "evoattn_pair_bias_bwd",
            "evoattn_keep_mask", "evoattn_linear_fwd", "evoattn_linear_dx", "evoattn_linear_dw_workspace_bytes", "evoattn_linear_dw",
            "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd",
-           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_few_workspace_bytes", "evoattn_fp8_matmul_few")
+           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding")
 EVOATTN_STATIC_PREP_BYTES = 16 << 20
 
 
@@ -155,7 +155,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_pair_bias_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i64, i64, i32, i32, i32, vp]
     RB = ctypes.POINTER(EvoRelativeBias)
     for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd",
-           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_few_workspace_bytes", "evoattn_fp8_matmul_few"):
+           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [RB, vp]
     lib.evoattn_relative_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
@@ -168,10 +168,10 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_fp8_matmul_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
     lib.evoattn_fp8_matmul.restype = ctypes.c_int
     lib.evoattn_fp8_matmul.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp]
-    lib.evoattn_fp8_matmul_few_workspace_bytes.restype = ctypes.c_size_t
-    lib.evoattn_fp8_matmul_few_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
-    lib.evoattn_fp8_matmul_few.restype = ctypes.c_int
-    lib.evoattn_fp8_matmul_few.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp, i64, vp]
+    lib.evoattn_fp8_matmul_rounding_workspace_bytes.restype = ctypes.c_size_t
+    lib.evoattn_fp8_matmul_rounding_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
+    lib.evoattn_fp8_matmul_rounding.restype = ctypes.c_int
+    lib.evoattn_fp8_matmul_rounding.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp, i64, vp]
     lib.evoattn_path.restype = ctypes.c_char_p
     lib.evoattn_kernels.restype = ctypes.c_char_p
     lib.evoattn_path.argtypes = [P, ctypes.c_int]

@@ -3,6 +3,7 @@
 // rounded matrices that both lie with the contraction along their rows.  A training step's products are all of that form:
 //   y = Qk(x) Qk(w)^T,  dx = Qn(dy) Qn(w^T)^T,  dw = Qm(dy^T) Qm(x^T)^T
 // each operand rounded along the axis that its product contracts.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -47,16 +48,81 @@ __device__ __forceinline__ int f8_exponent(unsigned amax) {
     const int e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);   // 448 = 1.75 * 2^8
     return amax ? max(e, -127) : 0;
 }
-__device__ __forceinline__ float f8_inverse(int e) { return __uint_as_float((unsigned)(127 - e) << 23); }
-// |x| of a finite x, else 0
-__device__ __forceinline__ unsigned f8_magnitude(float x) {
-    const unsigned a = __float_as_uint(x) & 0x7fffffffu;
-    return a < 0x7f800000u ? a : 0u;
+__device__ __forceinline__ float f8_power(int e) { return __uint_as_float(e == -127 ? 0x400000u : (unsigned)(e + 127) << 23); }   // 2^e
+
+// Magnitudes of 16-bit types are compared as whole numbers, two at a time; infinities and NaN, which count for nothing, come out the largest and are looked for only then.
+template <typename T>
+struct F8Bits {
+    static constexpr bool HALF = sizeof(T) == 2;
+    typedef typename std::conditional<HALF, uint16_t, uint32_t>::type U;
+    typedef U V __attribute__((ext_vector_type(8)));
+    static constexpr U INF = !HALF ? 0x7f800000u : std::is_same<T, bf16_t>::value ? 0x7f80 : 0x7c00;
+    __device__ __forceinline__ static V of(const F8Eight<T> &e) { return __builtin_bit_cast(V, e.v) & (U)(HALF ? 0x7fff : 0x7fffffff); }
+    __device__ __forceinline__ static V finite(V v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] < INF ? v[i] : (U)0;
+        return v;
+    }
+    __device__ __forceinline__ static unsigned most(V v) {
+        const auto a = __builtin_elementwise_max(v.lo, v.hi);
+        const auto b = __builtin_elementwise_max(a.lo, a.hi);
+        return max((unsigned)b[0], (unsigned)b[1]);
+    }
+    // a magnitude as that of a float
+    __device__ __forceinline__ static unsigned wide(unsigned m) {
+        if constexpr (!HALF) return m;
+        else if constexpr (std::is_same<T, bf16_t>::value) return m << 16;
+        else return __float_as_uint((float)__builtin_bit_cast(f16_t, (uint16_t)m));
+    }
+};
+// The largest finite magnitude of each of the eight places, of N times eight values.
+template <int N, typename T>
+__device__ __forceinline__ typename F8Bits<T>::V f8_magnitudes(const F8Eight<T> (&e)[N]) {
+    typename F8Bits<T>::V all = F8Bits<T>::of(e[0]);
+#pragma unroll
+    for (int i = 1; i < N; ++i) all = __builtin_elementwise_max(all, F8Bits<T>::of(e[i]));
+    if (F8Bits<T>::most(all) >= F8Bits<T>::INF) {
+        all = F8Bits<T>::finite(F8Bits<T>::of(e[0]));
+#pragma unroll
+        for (int i = 1; i < N; ++i) all = __builtin_elementwise_max(all, F8Bits<T>::finite(F8Bits<T>::of(e[i])));
+    }
+    return all;
 }
-// Four values times `inv` as e4m3, to nearest, ties to even; infinities and NaN as NaN (what the conversion makes of them).
-__device__ __forceinline__ int f8_pack(float a, float b, float c, float d, float inv) {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
-    return __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, lo, true);
+
+// The largest of all, as that of a float.
+template <int N, typename T>
+__device__ __forceinline__ unsigned f8_largest(const F8Eight<T> (&e)[N]) {
+    typedef F8Bits<T> B;
+    if constexpr (B::HALF) return B::wide(B::most(f8_magnitudes(e)));
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) m = max(m, (unsigned)B::of(e[i])[c]);
+    if (m >= B::INF) {
+        m = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) m = max(m, (unsigned)B::finite(B::of(e[i]))[c]);
+    }
+    return m;
+}
+
+// Two values over `scale`, a power of two, as e4m3, to nearest, ties to even; infinities and NaN as NaN.
+template <bool HI, typename T>
+__device__ __forceinline__ int f8_pair(int old, T a, T b, float scale) {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    typedef T V __attribute__((ext_vector_type(2)));
+    s16x2 o = __builtin_bit_cast(s16x2, old);
+    if constexpr (sizeof(T) == 4) o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(o, a, b, scale, HI);
+    else if constexpr (std::is_same<T, bf16_t>::value) o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, V{a, b}, scale, HI);
+    else o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, V{a, b}, scale, HI);
+    return __builtin_bit_cast(int, o);
+}
+template <typename T>
+__device__ __forceinline__ int f8_pack(T a, T b, T c, T d, float scale) {
+    return f8_pair<true>(f8_pair<false>(0, a, b, scale), c, d, scale);
 }
 template <int N>
 __device__ __forceinline__ unsigned f8_max_ror(unsigned v) {   // with the value N lanes further within 16
@@ -70,6 +136,26 @@ __device__ __forceinline__ unsigned f8_max_rows(unsigned v) {
     v = max(a[0], a[1]);
     const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     return max(b[0], b[1]);
+}
+template <typename V>   // eight values each, of 16 or 32 bits
+__device__ __forceinline__ V f8_max_rows(V v) {
+    typedef unsigned W __attribute__((ext_vector_type(sizeof(V) / 4)));
+    W w = __builtin_bit_cast(W, v), x, y;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(V) / 4; ++i) {
+        const auto a = __builtin_amdgcn_permlane32_swap(w[i], w[i], false, false);
+        x[i] = a[0];
+        y[i] = a[1];
+    }
+    v = __builtin_elementwise_max(__builtin_bit_cast(V, x), __builtin_bit_cast(V, y));
+    w = __builtin_bit_cast(W, v);
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(V) / 4; ++i) {
+        const auto a = __builtin_amdgcn_permlane16_swap(w[i], w[i], false, false);
+        x[i] = a[0];
+        y[i] = a[1];
+    }
+    return __builtin_elementwise_max(__builtin_bit_cast(V, x), __builtin_bit_cast(V, y));
 }
 __device__ __forceinline__ float f8_sum_rows(float v) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -102,25 +188,25 @@ __device__ __forceinline__ void f8_store_scale(uint8_t *s, int64_t k, int64_t bl
 template <typename T, int R, int V, bool ROWS, bool COLS>
 __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
     static_assert(R == 128 || !COLS, "a column's block is 128 rows");
+    typedef F8Bits<T> B;
     constexpr int WAVES = R / V / 4, THREADS = R / V * 16;
     __shared__ __attribute__((aligned(16))) unsigned char tile[COLS ? 128 * 128 : 16];
     __shared__ unsigned amaxs[COLS ? WAVES : 1][128];
     __shared__ float sums[COLS ? WAVES : 1][128];
-    __shared__ __attribute__((aligned(16))) float col_inverse[COLS ? 128 : 4];
+    __shared__ __attribute__((aligned(16))) float col_scale[COLS ? 128 : 4];
     __shared__ uint8_t row_scale[R];
     const int t = threadIdx.x, cg = t % 16, rg = t / 16, wave = t / 64;
     const int kt = blockIdx.x % p.tiles_k;
     const int64_t rt = blockIdx.x / p.tiles_k;
     const int c0 = kt * 128 + cg * 8;
     const int64_t r0 = rt * R + rg * V;
-    float v[V][8];
+    F8Eight<T> e[V];
     const T *x = (const T *)p.x;
     const bool last_rows = (rt + 1) * R >= p.rows, ragged = (kt + 1) * 128 > p.cols;   // uniform
     const bool corner = ragged && last_rows;
     if (p.cols >= 8 && (!corner || p.rows >= 2)) {
         // All loads under way together: rows beyond the last repeat it, and what lies behind a row's end is the next row's; the last row of all, which may not be read
         // beyond, element by element.
-        F8Eight<T> e[V];
         T l[8];
 #pragma unroll
         for (int i = 0; i < V; ++i) e[i].load(x + min(r0 + i, p.rows - (corner ? 2 : 1)) * p.ldx + (c0 < p.cols ? c0 : 0));
@@ -128,54 +214,50 @@ __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
 #pragma unroll
             for (int c = 0; c < 8; ++c) l[c] = x[(p.rows - 1) * p.ldx + min(c0 + c, p.cols - 1)];
         }
+        if (corner) {
 #pragma unroll
-        for (int i = 0; i < V; ++i)
+            for (int i = 0; i < V; ++i)
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v[i][c] = (float)(corner && r0 + i == p.rows - 1 ? l[c] : e[i].v[c]);
+                for (int c = 0; c < 8; ++c) e[i].v[c] = r0 + i == p.rows - 1 ? l[c] : e[i].v[c];
+        }
         if (last_rows || ragged) {
 #pragma unroll
             for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
-                    if (r0 + i >= p.rows || c0 + c >= p.cols) v[i][c] = 0.0f;
+                    if (r0 + i >= p.rows || c0 + c >= p.cols) e[i].v[c] = (T)0.0f;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                const float e = (float)x[min(r0 + i, p.rows - 1) * p.ldx + min(c0 + c, p.cols - 1)];
-                v[i][c] = r0 + i < p.rows && c0 + c < p.cols ? e : 0.0f;
+                const T one = x[min(r0 + i, p.rows - 1) * p.ldx + min(c0 + c, p.cols - 1)];
+                e[i].v[c] = r0 + i < p.rows && c0 + c < p.cols ? one : (T)0.0f;
             }
     }
     if (ROWS) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            unsigned a = 0;
-#pragma unroll
-            for (int c = 0; c < 8; ++c) a = max(a, f8_magnitude(v[i][c]));
-            const int e = f8_exponent(f8_max16(a));
-            const float inv = f8_inverse(e);
+            const F8Eight<T> one[1] = {e[i]};
+            const auto &v = e[i].v;
+            const int ex = f8_exponent(f8_max16(f8_largest(one)));
+            const float scale = f8_power(ex);
             if (r0 + i < p.rows) {
                 *reinterpret_cast<u32x2f *>(p.q + (r0 + i) * p.kp + c0) =
-                    u32x2f{(unsigned)f8_pack(v[i][0], v[i][1], v[i][2], v[i][3], inv), (unsigned)f8_pack(v[i][4], v[i][5], v[i][6], v[i][7], inv)};
+                    u32x2f{(unsigned)f8_pack(v[0], v[1], v[2], v[3], scale), (unsigned)f8_pack(v[4], v[5], v[6], v[7], scale)};
             }
-            if (cg == 0) row_scale[rg * V + i] = (uint8_t)(e + 127);
+            if (cg == 0) row_scale[rg * V + i] = (uint8_t)(ex + 127);
         }
     }
     if constexpr (COLS) {
-        unsigned a[8];
+        const typename B::V a = f8_max_rows(f8_magnitudes(e));
         float s[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            a[c] = 0;
             s[c] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                a[c] = max(a[c], f8_magnitude(v[i][c]));
-                s[c] += v[i][c];
-            }
-            a[c] = f8_max_rows(a[c]);
+            for (int i = 0; i < V; ++i) s[c] += (float)e[i].v[c];
             s[c] = f8_sum_rows(s[c]);
         }
         if (rg % 4 == 0) {
@@ -194,28 +276,28 @@ __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
                 most = max(most, amaxs[w][t]);
                 s += sums[w][t];
             }
-            const int e = f8_exponent(most);
-            col_inverse[t] = f8_inverse(e);
+            const int ex = f8_exponent(B::wide(most));
+            col_scale[t] = f8_power(ex);
             if (kt * 128 + t < p.cols) {
-                f8_store_scale(p.st + (kt * 128 + t) * p.spt, rt, p.tiles_r, p.spt, (uint8_t)(e + 127));
+                f8_store_scale(p.st + (kt * 128 + t) * p.spt, rt, p.tiles_r, p.spt, (uint8_t)(ex + 127));
                 if (p.sums) p.sums[rt * p.cols + kt * 128 + t] = s;
             }
         }
         __syncthreads();
         // byte of row r of column col: 16-byte chunks of a column's 128 rows, moved about so that neighbouring columns' lie in different banks
         auto at = [](int col, int r) { return col * 128 + (((r >> 4) ^ ((col >> 3) & 7)) << 4) + (r & 15); };
-        float invs[8];
-        __builtin_memcpy(invs, __builtin_assume_aligned(col_inverse + cg * 8, 16), sizeof invs);
+        float scales[8];
+        __builtin_memcpy(scales, __builtin_assume_aligned(col_scale + cg * 8, 16), sizeof scales);
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
             const int col = cg * 8 + c;
-            const float inv = invs[c];
+            const float scale = scales[c];
             if constexpr (V == 8) {
                 *reinterpret_cast<u32x2f *>(tile + at(col, rg * 8)) =
-                    u32x2f{(unsigned)f8_pack(v[0][c], v[1][c], v[2][c], v[3][c], inv), (unsigned)f8_pack(v[4][c], v[5][c], v[6][c], v[7][c], inv)};
+                    u32x2f{(unsigned)f8_pack<T>(e[0].v[c], e[1].v[c], e[2].v[c], e[3].v[c], scale), (unsigned)f8_pack<T>(e[4].v[c], e[5].v[c], e[6].v[c], e[7].v[c], scale)};
             } else {
                 static_assert(V == 2, "");
-                *reinterpret_cast<uint16_t *>(tile + at(col, rg * 2)) = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[0][c] * inv, v[1][c] * inv, 0, false);
+                *reinterpret_cast<uint16_t *>(tile + at(col, rg * 2)) = (uint16_t)f8_pair<false, T>(0, e[0].v[c], e[1].v[c], scale);
             }
         }
         __syncthreads();
@@ -267,6 +349,9 @@ struct F8Matmul {
     int M, N, blocks, sd;        // blocks of the contraction
     int mt, nt, slice;           // tiles; blocks of a slice, a multiple of four (or all)
     int bias_dtype;
+    const void *x;               // strips, rounded on the way: [M][k], rows ldx apart
+    int64_t ldx;
+    int k, pieces, tiles;        // strips: workgroups that share one's columns, tiles of a workgroup
 };
 
 // 16-byte chunk c of row r of a staged tile (rows of 128 bytes): any chunk of 16 rows touches all banks once
@@ -332,12 +417,13 @@ __device__ __forceinline__ void f8_tile(const F8Matmul &p, int &slice, int &mt, 
 }
 
 // A wave's results, TM x TN tiles of 32 x 32, to memory: through LDS, 32 rows at a time, so that neighbouring lanes store a row's pieces.
-template <int W, int TM, int TN, typename T>
-__device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const F8Matmul &p, unsigned char *lds, const float *bias, int wave, int lane, int m0,
-                                              int n0, int wm, int wn, int slice) {
+template <int TN, typename T>
+constexpr int kF8TileLds = 32 * TN * 32 * sizeof(T);   // bytes that a wave needs for that
+template <int TM, int TN, typename T>
+__device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const F8Matmul &p, unsigned char *mine, const float *bias, int lane, int m0, int n0, int wm,
+                                              int wn, int slice) {
     constexpr int ROW = TN * 32 * sizeof(T), CHUNKS = TN * 4;   // bytes of a row, chunks of eight results
     const int li = lane & 31, g = lane >> 5;
-    unsigned char *mine = lds + wave * 32 * ROW;
     auto place = [](int r, int c) { return r * ROW + ((c ^ (r & (CHUNKS - 1))) * (int)(8 * sizeof(T))); };
     T *out = (T *)p.out + (int64_t)slice * p.M * p.N;
     const bool inside = m0 + wm + 32 * TM <= p.M && n0 + wn + 32 * TN <= p.N;   // uniform
@@ -376,7 +462,7 @@ template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     constexpr int W = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128, PIECES = (BM + BN) / 8 / W;
     static_assert(BM / 8 % PIECES == 0, "a wave brings rows of one side");
-    static_assert(W * 32 * TN * 32 * sizeof(T) <= 2 * STAGE, "what the waves hold of their results at a time");
+    static_assert(W * kF8TileLds<TN, T> <= 2 * STAGE, "what the waves hold of their results at a time");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
     int slice, m0, n0;
@@ -483,7 +569,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
         }
     }
     __syncthreads();
-    f8_store_tile<W, TM, TN, T>(acc, p, lds8, bias, wave, lane, m0, n0, wm, wn, slice);
+    f8_store_tile<TM, TN, T>(acc, p, lds8 + wave * kF8TileLds<TN, T>, bias, lane, m0, n0, wm, wn, slice);
 }
 
 struct F8Wide {   // 16 of a lane's values of a row as operands of two products
@@ -638,7 +724,167 @@ __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
     else steps(std::false_type());
     if (!late) asm volatile("s_barrier" ::: "memory");
     __syncthreads();
-    f8_store_tile<W, TM, TN, T>(acc, p, lds8, bias, wave, lane, m0, n0, wm, wn, slice);
+    f8_store_tile<TM, TN, T>(acc, p, lds8 + wave * kF8TileLds<TN, T>, bias, lane, m0, n0, wm, wn, slice);
+}
+
+// ---- a contraction of up to four blocks ----
+
+// What such products cost is their results, and how soon one tile's are on their way after the last one's.  A workgroup stays on a strip of 128 rows of a, 32 in the
+// registers of each wave, as operands, and takes a piece of b's rows in tiles of 64: the next tile is on its way to LDS while this one is multiplied and stored.  ROUND: the
+// strip comes as it is and is rounded on the way, once for all tiles.  The sums are those of the other kernels, product for product.
+template <typename T, int NB, bool ROUND>
+__global__ void __launch_bounds__(256, 2) fp8_strip(F8Matmul p) {
+    constexpr bool WIDE = sizeof(T) == 4;
+    constexpr int TN = 2, BM = 128, BN = 64;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
+    __shared__ float bias[4][BN];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
+    const unsigned lid = xcd_remap(blockIdx.x, gridDim.x);   // pieces of a strip side by side
+    const int m0 = (int)(lid / p.pieces) * BM, first = (int)(lid % p.pieces) * p.tiles, end = min(first + p.tiles, p.nt);
+    // A tile of b in LDS: four parts of 16 rows, [block][row]; each wave fetches one, and takes its place, when all have read it, for its results' way out.
+    const int part = max(p.blocks * 2048, kF8TileLds<TN, T>);
+
+    // this wave's rows: two pieces of eight for each block
+    int row[2], at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = wave * 16 + i * 8 + lane / 8;
+        row[i] = (r & ~31) + f8_deal(r & 31);
+        at[i] = ((lane % 8) ^ f8_swz(r)) << 4;
+    }
+    auto fetch = [&](int tile) {
+        const uint8_t *base = p.b + (int64_t)tile * BN * p.kp;
+        unsigned char *to = lds8 + ((tile & 1) * 4 + wave) * part;
+        const int last = p.N - tile * BN - 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int off = min(row[i], last) * (int)p.kp + at[i];
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (b < p.blocks) f8_dma(base + b * kF8Block, off, to + b * 2048 + i * 1024);
+        }
+    };
+    int ws[TN], wn[TN];
+    float next = 0.0f;
+    auto ask = [&](int tile) {   // its scales and this thread's number of its bias
+#pragma unroll
+        for (int t = 0; t < TN; ++t) wn[t] = (int)p.sb[(int64_t)min(tile * BN + 32 * t + f8_deal(li), p.N - 1) * p.sd];
+        const int n = tile * BN + (int)threadIdx.x;
+        if (threadIdx.x < BN && p.bias) next = n < p.N ? f8_bias(p.bias, n, p.bias_dtype) : 0.0f;
+    };
+    auto take = [&](int tile) {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            asm volatile("" : "+v"(wn[t]));
+            ws[t] = wn[t];
+        }
+        if (threadIdx.x < BN) bias[tile & 3][threadIdx.x] = next;
+    };
+
+    ask(first);
+    fetch(first);
+    const int mw = m0 + wave * 32;
+    i32x8f a[2 * NB];
+    int xs = 0;
+    if constexpr (ROUND) {
+        const T *x = (const T *)p.x + (int64_t)min(mw + li, p.M - 1) * p.ldx + 32 * g;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (b >= p.blocks) break;
+            F8Eight<T> e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = b * kF8Block + 64 * (i / 4) + 8 * (i % 4), left = p.k - c - 32 * g;
+                if (left >= 8) {
+                    e[i].load(x + c);
+                } else {
+#pragma unroll
+                    for (int w = 0; w < 8; ++w) e[i].v[w] = w < left ? x[c + w] : (T)0.0f;
+                }
+            }
+            const unsigned most = f8_largest(e);
+            const auto both = __builtin_amdgcn_permlane32_swap(most, most, false, false);
+            const int ex = f8_exponent(max(both[0], both[1]));
+            const float scale = f8_power(ex);
+            xs |= (ex + 127) << (8 * b);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const auto &v = e[i / 2].v;
+                const int c = i % 2 * 4;
+                a[2 * b + i / 8][i % 8] = f8_pack<T>(v[c], v[c + 1], v[c + 2], v[c + 3], scale);
+            }
+        }
+    } else {
+        // The wave's rows come by neighbouring lanes, and a block at a time through its part of the other tile's place.
+        unsigned char *mine = lds8 + (((first + 1) & 1) * 4 + wave) * part;
+        xs = (int)p.sa[(int64_t)min(mw + li, p.M - 1) * p.sd];
+        i32x4f e[NB][4];
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (b < p.blocks) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[b][i] = *reinterpret_cast<const i32x4f *>(p.a + (int64_t)min(mw + 8 * i + lane / 8, p.M - 1) * p.kp + b * kF8Block + lane % 8 * 16);
+            }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (b >= p.blocks) break;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *reinterpret_cast<i32x4f *>(mine + f8_at(8 * i + lane / 8, lane % 8)) = e[b][i];
+            f8_wave_sync();
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+                const i32x4f lo = *reinterpret_cast<const i32x4f *>(mine + f8_at(li, 4 * ks + 2 * g)),
+                             hi = *reinterpret_cast<const i32x4f *>(mine + f8_at(li, 4 * ks + 2 * g + 1));
+                a[2 * b + ks] = i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            }
+            f8_wave_sync();
+        }
+    }
+    take(first);
+    f8_sync();
+
+    for (int tile = first; tile < end; ++tile) {
+        const bool more = tile + 1 < end;
+        if (more) {
+            ask(tile + 1);
+            fetch(tile + 1);
+        }
+        f32x16 acc[TN][1];
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[t][0][r] = 0.0f;
+        unsigned char *buf = lds8 + (tile & 1) * 4 * part;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if (b >= p.blocks) break;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+                for (int t = 0; t < TN; ++t) {
+                    const unsigned char *from = buf + (2 * t + li / 16) * part + b * 2048;
+                    const i32x4f lo = *reinterpret_cast<const i32x4f *>(from + f8_at(li % 16, 4 * ks + 2 * g)),
+                                 hi = *reinterpret_cast<const i32x4f *>(from + f8_at(li % 16, 4 * ks + 2 * g + 1));
+                    const i32x8f w = i32x8f{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+                    const i32x8f &v = a[2 * b + ks];
+                    if constexpr (WIDE) {
+                        const float wf = f8_scale(ws[t], b), xf = f8_scale(xs, b);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[t][0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f8_widen(w[2 * i], w[2 * i + 1], wf), f8_widen(v[2 * i], v[2 * i + 1], xf), acc[t][0], 0, 0, 0);
+                    } else {
+                        acc[t][0] = b == 0 ? f8_mma<0>(w, v, acc[t][0], ws[t], xs) : b == 1 ? f8_mma<1>(w, v, acc[t][0], ws[t], xs)
+                                  : b == 2 ? f8_mma<2>(w, v, acc[t][0], ws[t], xs) : f8_mma<3>(w, v, acc[t][0], ws[t], xs);
+                    }
+                }
+            }
+        }
+        // the next tile has landed, the results of the one before are out, and everybody has read this one
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (more) take(tile + 1);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        f8_store_tile<1, TN, T>(acc, p, buf + wave * part, bias[tile & 3], lane, m0, tile * BN, wave * 32, 0, 0);
+    }
 }
 
 // The slices' sums, eight columns per thread.
@@ -749,17 +995,14 @@ __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
             if (first + j * waves >= end) break;
 #pragma unroll
             for (int u = 0; u < MT; ++u) {
-                unsigned most = 0;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) most = max(most, f8_magnitude((float)e[j][u][i / 8].v[i % 8]));
-                const int ex = f8_exponent(f8_max_rows(most));
-                const float inv = f8_inverse(ex);
+                const int ex = f8_exponent(f8_max_rows(f8_largest(e[j][u])));
+                const float scale = f8_power(ex);
                 i32x8f ao;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const auto &v = e[j][u][i / 2].v;
                     const int c = i % 2 * 4;
-                    ao[i] = f8_pack((float)v[c], (float)v[c + 1], (float)v[c + 2], (float)v[c + 3], inv);
+                    ao[i] = f8_pack<T>(v[c], v[c + 1], v[c + 2], v[c + 3], scale);
                 }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
@@ -816,17 +1059,19 @@ static int f8_by_dtype(int dtype, F &&f) {
     return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
 }
 
+constexpr int kF8StripBlocks = 4;
 constexpr int64_t kF8MaxK = 1 << 22;   // of the contraction: a tile's rows stay within 32-bit offsets
 
 // How a product is cut: tiles of 256 x 256 or 128 x 128, and into slices of the contraction where there are too few for the chip.
 struct F8Plan {
     int mt, nt, slice, slices;
-    bool big;
+    bool big, strip;
 };
 static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
     F8Plan q{};
     const int blocks = (int)((k + kF8Block - 1) / kF8Block);
-    q.big = blocks >= 4 && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
+    q.strip = blocks <= kF8StripBlocks;
+    q.big = !q.strip && ((m + 255) / 256) * ((n + 255) / 256) >= 256;
     const int side = q.big ? 256 : 128;
     q.mt = (int)((m + side - 1) / side);
     q.nt = (int)((n + side - 1) / side);
@@ -849,6 +1094,25 @@ static int f8_check(const EvoFp8Matmul *p) {
     return EVO_OK;
 }
 
+static F8Matmul f8_operands(const EvoFp8Matmul &p) {
+    F8Matmul a{};
+    a.a = (const uint8_t *)p.a;
+    a.b = (const uint8_t *)p.b;
+    a.sa = (const uint32_t *)p.scales_a;
+    a.sb = (const uint32_t *)p.scales_b;
+    a.bias = p.bias;
+    a.out = p.out;
+    a.ldo = p.ldo;
+    a.k = (int)p.k;
+    a.kp = f8_pitch(p.k);
+    a.M = (int)p.m;
+    a.N = (int)p.n;
+    a.blocks = (int)(a.kp / kF8Block);
+    a.sd = (int)(f8_scale_pitch(p.k) / 4);
+    a.bias_dtype = p.bias_dtype;
+    return a;
+}
+
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
     constexpr int lds = 2 * 32 * (WM * TM + WN * TN) * 128 + 32 * WN * TN * 4;
@@ -860,6 +1124,7 @@ static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
 }
 template <typename T, bool WIDE>
 static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
+    if (q.strip) return f8_launch_strip<T, false>(a, st);
     const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
     if (q.big) {
         constexpr int lds = 4 * 512 * 64 + 2 * 512 * 4 + 256 * 4;
@@ -869,6 +1134,43 @@ static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
         return f8_rc();
     }
     return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
+}
+
+// Strips of 128 rows, their columns in pieces for two workgroups on each unit.
+struct F8StripPlan {
+    int strips, tiles, pieces;
+};
+static F8StripPlan f8_strip_plan(int64_t m, int64_t n) {
+    F8StripPlan q{};
+    q.strips = (int)((m + 127) / 128);
+    const int nt = (int)((n + 63) / 64), want = std::min((512 + q.strips - 1) / q.strips, nt);
+    q.tiles = (nt + want - 1) / want;
+    q.pieces = (nt + q.tiles - 1) / q.tiles;
+    return q;
+}
+// Whether a strip is rounded by its workgroups: where there are few of them to do that again, or little of it.
+static bool f8_strip_rounds(int64_t m, int64_t n, int64_t k, int dtype) {
+    return k <= 2 * kF8Block || (k <= kF8StripBlocks * kF8Block && dtype != EVO_F32 && f8_strip_plan(m, n).pieces <= 6);
+}
+template <typename T, bool ROUND>
+static int f8_launch_strip(F8Matmul a, hipStream_t st) {
+    const F8StripPlan q = f8_strip_plan(a.M, a.N);
+    a.nt = (a.N + 63) / 64;
+    a.tiles = q.tiles;
+    a.pieces = q.pieces;
+    auto go = [&](auto nb) {
+        constexpr int NB = decltype(nb)::value;
+        auto lds = [](int blocks) { return 8 * std::max(blocks * 2048, kF8TileLds<2, T>); };
+        constexpr auto kernel = fp8_strip<T, NB, ROUND>;
+        static PerDevice done;
+        if (const int rc = ensure_dynamic_lds((const void *)kernel, lds(NB), done, nullptr)) return rc;
+        kernel<<<(unsigned)(q.strips * q.pieces), 256, lds(a.blocks), st>>>(a);
+        return f8_rc();
+    };
+    if (a.blocks == 1) return go(std::integral_constant<int, 1>());
+    if (a.blocks == 2) return go(std::integral_constant<int, 2>());
+    if constexpr (ROUND && sizeof(T) == 4) return EVO_EUNSUPPORTED;
+    else return go(std::integral_constant<int, kF8StripBlocks>());
 }
 
 // Few rows: 64 outputs to a workgroup where there are then enough of them for the chip, else 16, and slices of the contraction of a block at least for each wave.
@@ -971,23 +1273,15 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
     const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
     if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
-    F8Matmul a{};
-    a.a = (const uint8_t *)p->a;
-    a.b = (const uint8_t *)p->b;
-    a.sa = (const uint32_t *)p->scales_a;
-    a.sb = (const uint32_t *)p->scales_b;
-    a.bias = q.slices > 1 ? nullptr : p->bias;
-    a.out = q.slices > 1 ? p->workspace : p->out;
-    a.ldo = q.slices > 1 ? p->n : p->ldo;
-    a.kp = f8_pitch(p->k);
-    a.M = (int)p->m;
-    a.N = (int)p->n;
-    a.blocks = (int)(a.kp / kF8Block);
-    a.sd = (int)(f8_scale_pitch(p->k) / 4);
+    F8Matmul a = f8_operands(*p);
+    if (q.slices > 1) {
+        a.bias = nullptr;
+        a.out = p->workspace;
+        a.ldo = p->n;
+    }
     a.mt = q.mt;
     a.nt = q.nt;
     a.slice = q.slice;
-    a.bias_dtype = p->bias_dtype;
     hipStream_t st = (hipStream_t)hip_stream;
     const bool wide = p->dtype == EVO_F32;
     if (q.slices == 1) {
@@ -997,22 +1291,30 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     return f8_by_dtype(p->dtype, [&](auto t) { return f8_add_slices<decltype(t)>(*p, q.slices, st); });
 }
 
-size_t evoattn_fp8_matmul_few_workspace_bytes(const EvoFp8Matmul *p) {
+size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p) {
     using namespace evo;
-    if (f8_check(p) || p->m > kF8FewRows) return 0;
+    if (f8_check(p) || p->m > kF8FewRows) return 0;   // (strips need none)
     const F8FewPlan q = f8_few_plan(p->n, p->k);
     return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
 
-int evoattn_fp8_matmul_few(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream) {
+int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream) {
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
-    if (p->m > kF8FewRows) return EVO_EUNSUPPORTED;
+    const bool few = p->m <= kF8FewRows;
+    if (!few && !f8_strip_rounds(p->m, p->n, p->k, p->dtype)) return EVO_EUNSUPPORTED;
     if (!x || ldx < p->k || !p->b || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->b, 16) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
+    hipStream_t st = (hipStream_t)hip_stream;
+    if (!few) {
+        F8Matmul a = f8_operands(*p);
+        a.x = x;
+        a.ldx = ldx;
+        return f8_by_dtype(p->dtype, [&](auto t) { return f8_launch_strip<decltype(t), true>(a, st); });
+    }
     const F8FewPlan q = f8_few_plan(p->n, p->k);
     const bool cut = q.slices > 1;
-    if (cut && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_few_workspace_bytes(p))) return EVO_EWORKSPACE;
+    if (cut && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_rounding_workspace_bytes(p))) return EVO_EWORKSPACE;
     F8Few a{};
     a.x = x;
     a.ldx = ldx;
@@ -1029,7 +1331,6 @@ int evoattn_fp8_matmul_few(const EvoFp8Matmul *p, const void *x, int64_t ldx, vo
     a.slice = q.slice;
     a.sd = (int)(f8_scale_pitch(p->k) / 4);
     a.bias_dtype = p->bias_dtype;
-    hipStream_t st = (hipStream_t)hip_stream;
     return f8_by_dtype(p->dtype, [&](auto t) {
         typedef decltype(t) T;
         if (!cut) return f8_launch_few<T, T>(a, q, st);

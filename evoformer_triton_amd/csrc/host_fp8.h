@@ -62,21 +62,28 @@ Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::Sca
     return out;
 }
 
-// x b^T (+ bias) with x rounded on the way
-constexpr int64_t kF8FewRows = 64;   // that evoattn_fp8_matmul_few takes
-Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
-    const int64_t rows = x.size(0);
-    if (rows <= kF8FewRows) {
-        Tensor out = at::empty({rows, b.rows}, x.options()), ws;
-        EvoFp8Matmul p = f8_product(rows, b, bias, out);
-        if (const size_t bytes = evoattn_fp8_matmul_few_workspace_bytes(&p)) {
+// x b^T (+ bias), x rounded on the way where that is how it is done; not defined for other sizes
+constexpr int64_t kF8FewRows = 64, kF8StripColumns = 512;   // up to so many rows, or so long a contraction
+Tensor f8_rounding(const Tensor &x, const Rounded &b, const Tensor &bias) {
+    Tensor out;
+    if (x.size(0) <= kF8FewRows || x.size(1) <= kF8StripColumns) {
+        Tensor ws;
+        out = at::empty({x.size(0), b.rows}, x.options());
+        EvoFp8Matmul p = f8_product(x.size(0), b, bias, out);
+        if (const size_t bytes = evoattn_fp8_matmul_rounding_workspace_bytes(&p)) {
             ws = scratch(bytes, x);
             p.workspace = ws.data_ptr();
             p.workspace_bytes = (size_t)ws.numel();
         }
-        check(evoattn_fp8_matmul_few(&p, x.data_ptr(), x.stride(0), stream_of(x)), "evoattn_fp8_matmul_few");
-        return out;
+        const int rc = evoattn_fp8_matmul_rounding(&p, x.data_ptr(), x.stride(0), stream_of(x));
+        if (rc == EVO_EUNSUPPORTED) return Tensor();
+        check(rc, "evoattn_fp8_matmul_rounding");
     }
+    return out;
+}
+Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
+    Tensor out = f8_rounding(x, b, bias);
+    if (out.defined()) return out;
     Rounded a;
     f8_quantize(x, &a, nullptr, nullptr);
     return f8_matmul(a, b, bias, x.scalar_type(), x);
@@ -126,7 +133,7 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
     Rounded xr, wr;
     f8_quantize(w2, &wr, need_x ? &saved->wt : nullptr, nullptr);
     // (the same kernels whether or not gradients are wanted)
-    if (x2.size(0) <= kF8FewRows) {
+    if (x2.size(0) <= kF8FewRows || !need_w) {
         if (need_w) f8_quantize(x2, nullptr, &saved->xt, nullptr);
         return f8_times(x2, wr, b).view(shape);
     }

@@ -354,9 +354,9 @@ size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream);
 
 /* The same with at most 64 rows x [m][k], ldx elements apart, in the result's dtype, that are rounded on the way (p's a and scales_a are not
- * read): the products of evoattn_fp8_quantize's rows.  `workspace` of evoattn_fp8_matmul_few_workspace_bytes(). */
-size_t evoattn_fp8_matmul_few_workspace_bytes(const EvoFp8Matmul *p);
-int evoattn_fp8_matmul_few(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream);
+ * read): the products of evoattn_fp8_quantize's rows.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
+size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p);
+int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream);
 
 #ifdef __cplusplus
 }

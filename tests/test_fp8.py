@@ -92,7 +92,7 @@ def test_products_that_the_c_abi_rejects_before_any_launch(change, code):
     (dict(), 0x10000, 5000, _lib.EVO_EUNSUPPORTED), (dict(m=64), None, 5000, _lib.EVO_EINVAL), (dict(m=64), 0x10000, 4999, _lib.EVO_EINVAL), (dict(m=64, b=0x10001), 0x10000, 5000, _lib.EVO_EALIGN),
     (dict(m=64, workspace=None), 0x10000, 5000, _lib.EVO_EWORKSPACE), (dict(m=0), 0x10000, 5000, _lib.EVO_EINVAL)])
 def test_few_rows_that_the_c_abi_rejects_before_any_launch(change, x, ldx, code):
-    assert _lib.load().evoattn_fp8_matmul_few(ctypes.byref(_product(**change)), x, ldx, None) == code
+    assert _lib.load().evoattn_fp8_matmul_rounding(ctypes.byref(_product(**change)), x, ldx, None) == code
 
 
 def test_the_c_abis_workspaces():
@@ -100,8 +100,8 @@ def test_the_c_abis_workspaces():
     need = lib.evoattn_fp8_matmul_workspace_bytes(ctypes.byref(_product()))
     assert need > 0 and need % (300 * 200 * 4) == 0
     assert lib.evoattn_fp8_matmul_workspace_bytes(ctypes.byref(_product(m=8192, n=8192))) == 0 and lib.evoattn_fp8_matmul_workspace_bytes(ctypes.byref(_product(k=0))) == 0
-    assert lib.evoattn_fp8_matmul_few_workspace_bytes(ctypes.byref(_product(m=65))) == 0 and lib.evoattn_fp8_matmul_few_workspace_bytes(ctypes.byref(_product(m=3, k=256))) == 0
-    assert lib.evoattn_fp8_matmul_few_workspace_bytes(ctypes.byref(_product(m=3))) % (3 * 200 * 4) == 0
+    assert lib.evoattn_fp8_matmul_rounding_workspace_bytes(ctypes.byref(_product(m=65))) == 0 and lib.evoattn_fp8_matmul_rounding_workspace_bytes(ctypes.byref(_product(m=3, k=256))) == 0
+    assert lib.evoattn_fp8_matmul_rounding_workspace_bytes(ctypes.byref(_product(m=3))) % (3 * 200 * 4) == 0
 
 
 @pytest.mark.parametrize("args,code", [

@@ -101,7 +101,12 @@ CASES = [
     (2500, 96, 40, True, BF16, F32, BF16),            # the weight's gradient in slices of the rows
     (2500, 640, 200, False, F32, F32, None),
     (128, 4224, 64, True, BF16, BF16, BF16),          # the forward in slices of the contraction
-    (65537, 130, 200, True, BF16, BF16, BF16),        # tiles of 256 x 256, the last of one row; two blocks, of which one has two values
+    (65537, 130, 200, True, BF16, BF16, BF16),        # strips of 128 rows, the last of one row; two blocks, of which one has two values
+    (700, 250, 130, True, F32, F32, F32),             # strips in fp32, three tiles, the last of two columns
+    (40000, 400, 100, True, F16, F16, BF16),          # four blocks to a strip
+    (200, 512, 1000, False, BF16, BF16, None),        # the same, rounded before: eight pieces to a strip
+    (300, 380, 200, True, F32, F32, F32),             # three in fp32
+    (66000, 520, 260, True, BF16, BF16, BF16),        # tiles of 256 x 256, the last ones of a few rows and columns
     (33000, 700, 300, False, F16, F16, None),         # two and three of them side by side; more than one group of scales
     (33000, 600, 520, True, F32, F32, F32),           # the same in fp32
 ]
