@@ -132,13 +132,14 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
     const Tensor x2 = f8_rows(x), w2 = f8_rows(w), b = bias.defined() ? bias.contiguous() : bias;
     Rounded xr, wr;
     f8_quantize(w2, &wr, need_x ? &saved->wt : nullptr, nullptr);
-    // (the same kernels whether or not gradients are wanted)
-    if (x2.size(0) <= kF8FewRows || !need_w) {
+    Tensor y = f8_rounding(x2, wr, b);
+    if (y.defined()) {
         if (need_w) f8_quantize(x2, nullptr, &saved->xt, nullptr);
-        return f8_times(x2, wr, b).view(shape);
+    } else {
+        f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
+        y = f8_matmul(xr, wr, b, x.scalar_type(), x2);
     }
-    f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
-    return f8_matmul(xr, wr, b, x.scalar_type(), x2).view(shape);
+    return y.view(shape);
 }
 // dx, dw, db from dy [rows, n]
 void f8_backward(const Tensor &dy, const F8Saved &saved, bool need_x, bool need_w, bool need_b, at::ScalarType wtype, at::ScalarType btype, Tensor &dx, Tensor &dw,
