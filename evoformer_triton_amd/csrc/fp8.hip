@@ -461,7 +461,7 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     constexpr int W = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128, PIECES = (BM + BN) / 8 / W;
-    static_assert(BM / 8 % PIECES == 0, "a wave brings rows of one side");
+    static_assert(BM / 8 % PIECES == 0 && PIECES % 4 == 0, "a wave brings rows of one side, 32 at least");
     static_assert(W * kF8TileLds<TN, T> <= 2 * STAGE, "what the waves hold of their results at a time");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
@@ -475,17 +475,18 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     // this wave's pieces of a stage: eight rows of 128 bytes each
     const bool tokens = wave * PIECES * 8 < BM;
     const int at = wave * PIECES * 8 - (tokens ? 0 : BM), last = (tokens ? p.M - m0 : p.N - n0) - 1;
-    const uint8_t *base = (tokens ? p.a + (int64_t)m0 * p.kp : p.b + (int64_t)n0 * p.kp) + (int64_t)first * kF8Block;
+    const uint8_t *base[PIECES / 4];   // of 32 rows each: what a lane adds to it stays within 32 bits
     int off[PIECES];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        const int r = at + i * 8 + lane / 8, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
-        off[i] = min(row, last) * (int)p.kp + (((lane % 8) ^ f8_swz(r)) << 4);
+        const int from = min(at + i / 4 * 32, last), r = at + i * 8 + lane / 8, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
+        if (i % 4 == 0) base[i / 4] = (tokens ? p.a + (int64_t)(m0 + from) * p.kp : p.b + (int64_t)(n0 + from) * p.kp) + (int64_t)first * kF8Block;
+        off[i] = (min(row, last) - from) * (int)p.kp + (((lane % 8) ^ f8_swz(r)) << 4);
     }
     auto fetch = [&](int s) {
         unsigned char *to = lds8 + (s & 1) * STAGE + wave * PIECES * 1024;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) f8_dma(base + s * kF8Block, off[i], to + i * 1024);
+        for (int i = 0; i < PIECES; ++i) f8_dma(base[i / 4] + s * kF8Block, off[i], to + i * 1024);
     };
     const uint32_t *sa[TM], *sb[TN];
 #pragma unroll
@@ -600,13 +601,14 @@ __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
     // this wave's pieces of a stage, 16 rows of 64 bytes each: rows of a from waves 0, 2, 4, 6, of b from the others
     const bool tokens = (wave & 1) == 0;
     const int at = (wave >> 1) * 64, last = (tokens ? p.M - m0 : p.N - n0) - 1;
-    const uint8_t *base = (tokens ? p.a + (int64_t)m0 * p.kp : p.b + (int64_t)n0 * p.kp) + (int64_t)first * kF8Block;
+    const uint8_t *base[PIECES / 2];   // of 32 rows each, as above
     const uint32_t *sbase = (tokens ? p.sa + (int64_t)m0 * p.sd : p.sb + (int64_t)n0 * p.sd) + first / 4;
     int off[PIECES], soff;
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-        const int r = at + i * 16 + lane / 4, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
-        off[i] = min(row, last) * (int)p.kp + (((lane % 4) ^ ((r >> 2) & 3)) << 4);
+        const int from = min(at + i / 2 * 32, last), r = at + i * 16 + lane / 4, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
+        if (i % 2 == 0) base[i / 2] = (tokens ? p.a + (int64_t)(m0 + from) * p.kp : p.b + (int64_t)(n0 + from) * p.kp) + (int64_t)first * kF8Block;
+        off[i] = (min(row, last) - from) * (int)p.kp + (((lane % 4) ^ ((r >> 2) & 3)) << 4);
     }
     {
         const int r = at + lane, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
@@ -616,7 +618,7 @@ __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
     auto fetch = [&](int s) {
         unsigned char *dst = to + (s & 3) * STAGE;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) f8_dma(base + s * 64, off[i], dst + i * 1024);
+        for (int i = 0; i < PIECES; ++i) f8_dma(base[i / 2] + s * 64, off[i], dst + i * 1024);
     };
     auto fetch_scales = [&](int s8) {   // of steps 8 s8 .. 8 s8 + 7
         f8_dma4(sbase + s8, soff, lds8 + SCALES + (s8 & 1) * (BM + BN) * 4 + ((tokens ? 0 : BM) + at) * 4);
@@ -1060,7 +1062,7 @@ static int f8_by_dtype(int dtype, F &&f) {
 }
 
 constexpr int kF8StripBlocks = 4;
-constexpr int64_t kF8MaxK = 1 << 22;   // of the contraction: a tile's rows stay within 32-bit offsets
+constexpr int64_t kF8MaxK = 1 << 26;   // of the contraction: 32 rows stay within 32-bit offsets
 
 // How a product is cut: tiles of 256 x 256 or 128 x 128, and into slices of the contraction where there are too few for the chip.
 struct F8Plan {

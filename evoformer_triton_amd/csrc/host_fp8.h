@@ -20,13 +20,15 @@ Tensor f8_rows(const Tensor &x) {
     return r.stride(1) == 1 && r.stride(0) >= r.size(1) ? r : r.contiguous();
 }
 
+int64_t f8_apart(const Tensor &x) { return x.size(0) == 1 ? std::max(x.stride(0), x.size(1)) : x.stride(0); }   // (one row's stride may be anything)
+
 // x rounded along its rows and its columns, as far as asked for, and the column sums of its blocks of rows.
 void f8_quantize(const Tensor &x, Rounded *along_rows, Rounded *along_cols, Tensor *sums) {
     const int64_t rows = x.size(0), cols = x.size(1);
     if (along_rows) *along_rows = Rounded(rows, cols, x);
     if (along_cols) *along_cols = Rounded(cols, rows, x);
     if (sums) *sums = at::empty({(rows + 127) / 128, cols}, x.options().dtype(at::kFloat));
-    check(evoattn_fp8_quantize(x.data_ptr(), x.stride(0), along_rows ? along_rows->q : nullptr, along_rows ? along_rows->s : nullptr,
+    check(evoattn_fp8_quantize(x.data_ptr(), f8_apart(x), along_rows ? along_rows->q : nullptr, along_rows ? along_rows->s : nullptr,
                                along_cols ? along_cols->q : nullptr, along_cols ? along_cols->s : nullptr, sums ? (float *)sums->data_ptr() : nullptr, rows,
                                cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
 }
@@ -75,7 +77,7 @@ Tensor f8_rounding(const Tensor &x, const Rounded &b, const Tensor &bias) {
             p.workspace = ws.data_ptr();
             p.workspace_bytes = (size_t)ws.numel();
         }
-        const int rc = evoattn_fp8_matmul_rounding(&p, x.data_ptr(), x.stride(0), stream_of(x));
+        const int rc = evoattn_fp8_matmul_rounding(&p, x.data_ptr(), f8_apart(x), stream_of(x));
         if (rc == EVO_EUNSUPPORTED) return Tensor();
         check(rc, "evoattn_fp8_matmul_rounding");
     }
@@ -89,14 +91,16 @@ Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
     return f8_matmul(a, b, bias, x.scalar_type(), x);
 }
 
+constexpr int64_t kF8Most = 1 << 26;
 const char *f8_wrong(const Tensor &x, int64_t n, int64_t k, const c10::Device &device, const OptTensor &bias) {
     if (evo_dtype(x.scalar_type()) == EVO_NONE || x.dim() < 1) return "the input must be [..., k] in bf16, fp16 or fp32";
     if (x.size(-1) != k) return "the input's last dimension must be the weight's columns";
     if (x.device() != device || (bias && bias->defined() && bias->device() != device)) return "all tensors must live on one device";
     if (bias && bias->defined() && (bias->dim() != 1 || bias->size(0) != n || evo_dtype(bias->scalar_type()) == EVO_NONE))
         return "the bias must be [n] in bf16, fp16 or fp32";
-    if (n > INT32_MAX - 512 || k > (1 << 22)) return "the weight has more than 2^31 rows or 2^22 columns";
-    if (k > 0 && x.numel() / k > INT32_MAX - 512) return "the input has more than 2^31 rows";
+    // (each of them is contracted in one of the three products)
+    if (n > kF8Most || k > kF8Most) return "the weight has more than 2^26 rows or columns";
+    if (k > 0 && x.numel() / k > kF8Most) return "the input has more than 2^26 rows";
     return nullptr;
 }
 const char *f8_linear_wrong(const Tensor &x, const Tensor &w, const OptTensor &bias) {
@@ -280,14 +284,14 @@ Tensor fp8_linear_held_forward(const Tensor &x, const Tensor &values, const Tens
 // values and scales of a matrix rounded along its rows
 std::pair<Tensor, Tensor> fp8_round(const Tensor &w) {
     TORCH_CHECK_VALUE(w.dim() == 2 && evo_dtype(w.scalar_type()) != EVO_NONE, "the weight must be [n, k] in bf16, fp16 or fp32");
-    TORCH_CHECK_VALUE(w.size(1) <= 1 << 22, "the weight has more than 2^22 columns");
+    TORCH_CHECK_VALUE(w.size(0) <= kF8Most && w.size(1) <= kF8Most, "the weight has more than 2^26 rows or columns");
     TORCH_CHECK(w.is_cuda(), "rounding to 8 bits runs on the GPU only");
     c10::DeviceGuard on(w.device());
     const auto o = w.options().dtype(at::kByte);
     const Tensor values = at::empty({w.size(0), Rounded::pitch(w.size(1))}, o), scales = at::empty({w.size(0), Rounded::scale_pitch(w.size(1))}, o);
     if (w.numel()) {
         const Tensor r = f8_rows(w);
-        check(evoattn_fp8_quantize(r.data_ptr(), r.stride(0), values.data_ptr(), scales.data_ptr(), nullptr, nullptr, nullptr, r.size(0), r.size(1),
+        check(evoattn_fp8_quantize(r.data_ptr(), f8_apart(r), values.data_ptr(), scales.data_ptr(), nullptr, nullptr, nullptr, r.size(0), r.size(1),
                                    evo_dtype(r.scalar_type()), stream_of(r)), "evoattn_fp8_quantize");
     }
     return {values, scales};

@@ -54,7 +54,7 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
     bias     [n], bf16, fp16 or fp32, added in fp32
 
     Gradients come in the dtype of what they belong to.  A result or weight gradient in fp32 is summed in fp32 throughout; towards
-    16 bits the 8-bit matrix instructions form the sums, to about 1.4e-5 of the result.  n up to 2^31, k up to 2^22.  Runs on the current
+    16 bits the 8-bit matrix instructions form the sums, to about 1.4e-5 of the result.  Rows, n and k up to 2^26.  Runs on the current
     stream of the tensors' device; GPU only."""
     held = isinstance(weight, Fp8Weight)
     for name, t in (("x", x), ("bias", bias)) + ((("weight.values", weight.values), ("weight.scales", weight.scales)) if held else (("weight", weight),)):

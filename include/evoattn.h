@@ -330,7 +330,7 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream);
  *   qt, scales_t   its transpose [cols][rows] rounded along x's columns, or both NULL
  *   sums           [ceil(rows / 128)][cols] fp32 column sums of x's blocks of rows (with qt; may be NULL)
  * evoattn_fp8_column_sums: those added up, out [cols] in dtype, in a fixed order.
- * q and qt on 16-byte boundaries.  cols at most 2^22. */
+ * q and qt on 16-byte boundaries.  cols at most 2^26. */
 int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void *qt, void *scales_t, float *sums, int64_t rows, int64_t cols,
                          int32_t dtype, void *hip_stream);
 int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t cols, int32_t dtype, void *hip_stream);
@@ -338,7 +338,7 @@ int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t 
 /* out [m][n] = a [m][k] b [n][k]^T (+ bias [n]): rounded matrices as above, fp32 sums, rounded once to dtype (EVO_BF16 / _F16 / _F32); out's
  * rows ldo elements apart.  With a 16-bit result the 8-bit matrix instructions form the sums, which add neighbouring products with what lies
  * some 13 bits below the largest of them cut off (1.4e-5 of a result, measured); with an fp32 result the values are widened to bf16 first and
- * every sum is fp32.  bias in bias_dtype, may be NULL.  a, b on 16-byte, scales on 4-byte boundaries.  k at most 2^22.  `workspace` of
+ * every sum is fp32.  bias in bias_dtype, may be NULL.  a, b on 16-byte, scales on 4-byte boundaries.  k at most 2^26.  `workspace` of
  * evoattn_fp8_matmul_workspace_bytes() (0: none needed; also for what evoattn_fp8_matmul refuses).  Nothing is allocated or synchronised;
  * two calls give the same bits. */
 typedef struct EvoFp8Matmul {
@@ -353,8 +353,9 @@ typedef struct EvoFp8Matmul {
 size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream);
 
-/* The same with at most 64 rows x [m][k], ldx elements apart, in the result's dtype, that are rounded on the way (p's a and scales_a are not
- * read): the products of evoattn_fp8_quantize's rows.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
+/* The same with x [m][k], rows ldx elements apart, in the result's dtype, that is rounded on the way (p's a and scales_a are not read): the products
+ * of evoattn_fp8_quantize's rows, bit for bit.  m at most 64; or k at most 512 where that takes less time than the two calls do, which is whenever k is at
+ * most 256: EVO_EUNSUPPORTED for all others, and they go through the two calls.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
 size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream);
 

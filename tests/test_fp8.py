@@ -13,7 +13,8 @@ from evoformer_triton_amd.block import Fp8BlockWeights, GatedAttentionBlock
     (torch.zeros(3, 5), torch.zeros(4, 6), None, "last dimension"), (torch.zeros(3, 5), torch.zeros(4, 5, 1), None, "weight must be"),
     (torch.zeros(3, 5), torch.zeros(4, 5, dtype=torch.int8), None, "weight must be"), (torch.zeros(3, 5), torch.zeros(4, 5), torch.zeros(5), "bias must be"),
     (torch.zeros(3, 5), torch.zeros(4, 5), torch.zeros(4, dtype=torch.float64), "bias must be"), (torch.zeros(3, 5), torch.zeros(4, 5), torch.zeros(4, device="meta"), "one device"),
-    (torch.zeros(3, 5), torch.zeros(4, 5), None, "GPU only")])
+    (torch.zeros(1, 1).expand(2 ** 26 + 1, 1), torch.zeros(4, 1), None, "2.26 rows"), (torch.zeros(1, 1), torch.zeros(1, 1).expand(2 ** 26 + 1, 1), None, "2.26 rows or columns"),
+    (torch.zeros(1, 1).expand(1, 2 ** 26 + 1), torch.zeros(1, 1).expand(1, 2 ** 26 + 1), None, "2.26 rows or columns"), (torch.zeros(3, 5), torch.zeros(4, 5), None, "GPU only")])
 def test_calls_that_are_refused(x, w, b, match):
     with pytest.raises((ValueError, RuntimeError), match=match):
         fp8_linear(x, w, b)
@@ -82,7 +83,7 @@ def _product(**change):
 @pytest.mark.parametrize("change,code", [
     (dict(m=0), _lib.EVO_EINVAL), (dict(n=-1), _lib.EVO_EINVAL), (dict(k=0), _lib.EVO_EINVAL), (dict(dtype=5), _lib.EVO_EINVAL), (dict(a=None), _lib.EVO_EINVAL),
     (dict(scales_b=None), _lib.EVO_EINVAL), (dict(out=None), _lib.EVO_EINVAL), (dict(ldo=199), _lib.EVO_EINVAL), (dict(bias=0x10000, bias_dtype=-1), _lib.EVO_EINVAL),
-    (dict(a=0x10008), _lib.EVO_EALIGN), (dict(scales_a=0x10002), _lib.EVO_EALIGN), (dict(k=(1 << 22) + 1), _lib.EVO_EUNSUPPORTED), (dict(m=1 << 31), _lib.EVO_EOVERFLOW),
+    (dict(a=0x10008), _lib.EVO_EALIGN), (dict(scales_a=0x10002), _lib.EVO_EALIGN), (dict(k=(1 << 26) + 1), _lib.EVO_EUNSUPPORTED), (dict(m=1 << 31), _lib.EVO_EOVERFLOW),
     (dict(workspace=None), _lib.EVO_EWORKSPACE), (dict(workspace_bytes=100), _lib.EVO_EWORKSPACE)])
 def test_products_that_the_c_abi_rejects_before_any_launch(change, code):
     assert _lib.load().evoattn_fp8_matmul(ctypes.byref(_product(**change)), None) == code
@@ -109,7 +110,7 @@ def test_the_c_abis_workspaces():
     ((0x10000, 40, 0x10000, None, None, None, None, 3, 40, 0), _lib.EVO_EINVAL), ((0x10000, 40, None, None, None, None, None, 3, 40, 0), _lib.EVO_EINVAL),
     ((0x10000, 40, 0x10000, 0x10000, None, None, 0x10000, 3, 40, 0), _lib.EVO_EINVAL), ((0x10000, 40, 0x10000, 0x10000, None, None, None, 0, 40, 0), _lib.EVO_EINVAL),
     ((0x10000, 40, 0x10000, 0x10000, None, None, None, 3, 40, 3), _lib.EVO_EINVAL), ((0x10000, 40, 0x10008, 0x10000, None, None, None, 3, 40, 0), _lib.EVO_EALIGN),
-    ((0x10000, 1 << 23, 0x10000, 0x10000, None, None, None, 3, (1 << 22) + 1, 0), _lib.EVO_EUNSUPPORTED)])
+    ((0x10000, 1 << 27, 0x10000, 0x10000, None, None, None, 3, (1 << 26) + 1, 0), _lib.EVO_EUNSUPPORTED)])
 def test_rounding_that_the_c_abi_rejects_before_any_launch(args, code):
     assert _lib.load().evoattn_fp8_quantize(*args, None) == code
 

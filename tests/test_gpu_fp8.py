@@ -195,6 +195,47 @@ def test_strides_shapes_and_streams(gpu_device):
             assert torch.equal(fp8_linear(x, Fp8Weight.of(wt.t()), bias), want[0])
 
 
+def test_a_single_row_of_any_stride(gpu_device):
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    for k in (1, 5, 200):
+        x, w = torch.randn(k, 1, device=gpu_device).t(), torch.randn(k, 1, device=gpu_device).t()      # [1, k], strides (1, 1)
+        y, want = (fp8_linear(a.detach().requires_grad_(), b, None) for a, b in ((x, w), (x.clone(memory_format=torch.contiguous_format), w.reshape(-1).view(1, k))))
+        dy = torch.randn(1, device=gpu_device).expand(1, 1)
+        assert torch.equal(y, want) and torch.equal(Fp8Weight.of(w).dequantize(), Fp8Weight.of(w.reshape(-1).view(1, k)).dequantize())
+        y.backward(dy)
+        z = fp8_linear(torch.randn(300, k, device=gpu_device), w)
+        assert z.shape == (300, 1) and torch.isfinite(z).all()
+
+
+def test_more_rows_than_fit_32_bits(gpu_device):
+    """The weight's gradient contracts them; their rounded columns lie 4 MB apart, and a group of 512 of them spans 2^31 bytes."""
+    from evoformer_triton_amd import fp8_linear
+    g = torch.Generator().manual_seed(3)
+    rows, k, n = 2 ** 22 + 133, 5, 600
+    x, w = torch.randn((rows, k), generator=g).to(BF16), torch.randn((n, k), generator=g)
+    xg, wg = x.to(gpu_device), w.to(gpu_device).requires_grad_()
+    y = fp8_linear(xg, wg)
+    for part in (slice(0, 300), slice(rows - 300, rows)):
+        want = _q(x[part]) @ _q(w).t()
+        _near(y[part], want, _q(x[part]).abs() @ _q(w).abs().t(), k)
+    dy = torch.zeros((rows, n), dtype=BF16, device=gpu_device)
+    at = torch.tensor([0, 127, 5000, 2 ** 22 - 1, 2 ** 22, rows - 1])
+    values = torch.randn((len(at), n), generator=g).to(BF16)
+    dy[at.to(gpu_device)] = values.to(gpu_device)
+    dw, = torch.autograd.grad(y, wg, dy)
+    want, size = torch.zeros(n, k, dtype=torch.float64), torch.zeros(n, k, dtype=torch.float64)
+    for i, r in enumerate(at.tolist()):        # each alone in its block of 128 rows, but for the two around 2^22
+        block = slice(r // 128 * 128, min(r // 128 * 128 + 128, rows))
+        one = torch.zeros(block.stop - block.start, n, dtype=torch.float64)
+        for j, other in enumerate(at.tolist()):
+            if block.start <= other < block.stop:
+                one[other - block.start] = values[j].double()
+        a, b = _q(one.t())[:, r - block.start], _q(x[block].t())[:, r - block.start]
+        want += torch.outer(a, b)
+        size += torch.outer(a, b).abs()
+    _near(dw, want, size, 8)
+
+
 def test_empty_calls(gpu_device):
     from evoformer_triton_amd import Fp8Weight, fp8_linear
     for rows, k, n in ((0, 5, 3), (4, 0, 3), (4, 5, 0), (0, 0, 0)):
