@@ -2,6 +2,7 @@
 //   out[b,h,i,j] = table[bucket(b,i,j), h] (+ pair[b,h,i,j]),  bucket = lut[clamp(pos_q[b,i] - pos_k[b,j], -R, R) + R],
 // or the table's last row where i and j lie in different chains; and the table's gradient, the sum of the output's over the pairs of
 // each bucket.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -472,7 +473,11 @@ template <typename F>
 static int rb_by_dtype(int dtype, F &&f) {
     return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
 }
-constexpr int kRbFwdGroups = 2048, kRbBwdGroups = 1024;
+// Workgroups.  Forward: one for every 64 KB, since each looks its table and positions up first, two for each unit at least and eight at most, that enough is under
+// way.  Of 512 / 1024 / 2048 / 4096, us: 2 x 64 x 256^2 with a bias in bf16 12.1 / 12.7 / 17.6 / 24.5, 1 x 32 x 1024^2 in fp32 81 / 58 / 47 / 47.
+// Backward: two for each unit, whose parts are few to add up.  Of 256 / 384 / 512 / 1024 / 2048: 4 x 32 x 1024^2 in fp32 140 / 131 / 107 / 116 / 121,
+// 2 x 64 x 256^2 in bf16 14.2 / 15.4 / 14.3 / 15.2 / 21.5.
+constexpr int kRbBytes = 1 << 16, kRbFwdLeast = 512, kRbFwdMost = 2048, kRbBwdGroups = 512;
 
 static RbArgs rb_fwd_args(const EvoRelativeBias &p) {
     RbArgs a = rb_args(p);
@@ -481,7 +486,9 @@ static RbArgs rb_fwd_args(const EvoRelativeBias &p) {
     a.lanes = 1;
     while (a.lanes < 64 && a.lanes < pieces) a.lanes *= 2;
     a.strips = (int)((pieces + 63) / 64);
-    rb_chunks(a, (int64_t)p.B * p.H * a.strips, kRbWaves * 64 / a.lanes, kRbFwdGroups);
+    const int64_t bytes = (int64_t)p.B * p.H * p.Nq * p.Nk * (p.dtype == EVO_F32 ? 4 : 2) * (p.pair ? 2 : 1);
+    const int want = (int)std::min<int64_t>(std::max<int64_t>(bytes / kRbBytes, kRbFwdLeast), kRbFwdMost);
+    rb_chunks(a, (int64_t)p.B * p.H * a.strips, kRbWaves * 64 / a.lanes, want);
     return a;
 }
 
