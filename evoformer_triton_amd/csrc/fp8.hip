@@ -467,12 +467,16 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
 
 // out[m][n] (+ slice M N) = sum over the slice's blocks of a[m] . b[n], times the scales, + bias[n].  WM x WN waves of TM x TN tiles
 // of 32 x 32; outputs (rows of b) are the accumulators' rows, rows of a their columns: a lane then holds 16 outputs side by side.  128 x 128 with two stages of a block each:
-// 64 KB, two workgroups to a unit, one of which multiplies while the other waits for its loads or stores.  Bound by those: 32 768 x 256 x 1024 in 14.4 us (1190 TFLOP/s; 50 MB,
+// 64 KB, two workgroups to a unit, one of which multiplies while the other waits for its loads or stores; eight waves of 32 x 64, two of a SIMD in turn (us, instead of four of
+// 64 x 64: 2048^3 13.0 / 14.4, 1024 x 4096 x 1024 9.0 / 9.8, 32 768 x 256 x 1024 15.1 / 15.0; four stages for the one workgroup that then fits: 14.8, 9.8, 14.7).  Bound by those: 32 768 x 256 x 1024 in 14.4 us (1190 TFLOP/s; 50 MB,
 // 3.5 TB/s); results written two bytes at a time instead of 16 made 32 768 x 1024 x 256 30 us instead of 23.
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
-    constexpr int W = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128, PIECES = (BM + BN) / 8 / W;
+    constexpr int W = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128, PIECES = (BM + BN) / 8 / W, SCALES = 2 * STAGE,
+                  BIAS = SCALES + 2 * (BM + BN) * 4;
     static_assert(BM / 8 % PIECES == 0 && PIECES % 4 == 0, "a wave brings rows of one side, 32 at least");
+    constexpr int ROWS = (BM + BN) / W;
+    static_assert(ROWS <= 64, "a lane brings a row's scales");
     static_assert(W * kF8TileLds<TN, T> <= 2 * STAGE, "what the waves hold of their results at a time");
     extern __shared__ __attribute__((aligned(1024))) unsigned char lds8[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
@@ -499,18 +503,16 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) f8_dma(base[i / 4] + s * kF8Block, off[i], to + i * 1024);
     };
-    const uint32_t *sa[TM], *sb[TN];
-#pragma unroll
-    for (int u = 0; u < TM; ++u) sa[u] = p.sa + (int64_t)min(m0 + wm + 32 * u + li, p.M - 1) * p.sd + first / 4;
-#pragma unroll
-    for (int t = 0; t < TN; ++t) sb[t] = p.sb + (int64_t)min(n0 + wn + 32 * t + f8_deal(li), p.N - 1) * p.sd + first / 4;
-    int xs[TM], ws[TN], xn[TM], wn4[TN];
-    auto scales = [&](int s4) {
-#pragma unroll
-        for (int u = 0; u < TM; ++u) xn[u] = (int)sa[u][s4];
-#pragma unroll
-        for (int t = 0; t < TN; ++t) wn4[t] = (int)sb[t][s4];
+    const uint32_t *sbase = (tokens ? p.sa + (int64_t)m0 * p.sd : p.sb + (int64_t)n0 * p.sd) + first / 4;
+    int soff;
+    {
+        const int r = at + lane % ROWS, row = tokens ? r : (r & ~31) + f8_deal(r & 31);
+        soff = min(row, last) * p.sd * 4;
+    }
+    auto fetch_scales = [&](int s4) {   // of four stages
+        if (lane < ROWS) f8_dma4(sbase + s4, soff, lds8 + SCALES + (s4 & 1) * (BM + BN) * 4 + ((tokens ? 0 : BM) + at) * 4);
     };
+    int xs[TM], ws[TN];
 
     f32x16 acc[TN][TM];
 #pragma unroll
@@ -520,27 +522,22 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[t][u][r] = 0.0f;
 
-    scales(0);
-    fetch(0);
-    float *bias = reinterpret_cast<float *>(lds8 + 2 * STAGE);
+    float *bias = reinterpret_cast<float *>(lds8 + BIAS);
     for (int i = threadIdx.x; i < BN; i += W * 64) bias[i] = p.bias && n0 + i < p.N ? f8_bias(p.bias, n0 + i, p.bias_dtype) : 0.0f;
+    fetch_scales(0);
+    fetch(0);
     for (int s4 = 0; s4 < nb; s4 += 4) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (s4 + j >= nb) break;
             f8_sync();
-            if (j == 0) {   // asked for four stages ago: here, before the next loads are, and not where they are used
+            if (j == 0) {
+                const int *x = reinterpret_cast<const int *>(lds8 + SCALES + ((s4 >> 2) & 1) * (BM + BN) * 4);
 #pragma unroll
-                for (int u = 0; u < TM; ++u) {
-                    asm volatile("" : "+v"(xn[u]));
-                    xs[u] = xn[u];
-                }
+                for (int u = 0; u < TM; ++u) xs[u] = x[wm + 32 * u + li];
 #pragma unroll
-                for (int t = 0; t < TN; ++t) {
-                    asm volatile("" : "+v"(wn4[t]));
-                    ws[t] = wn4[t];
-                }
-                if (s4 + 4 < nb) scales(s4 / 4 + 1);
+                for (int t = 0; t < TN; ++t) ws[t] = x[BM + wn + 32 * t + li];
+                if (s4 + 4 < nb) fetch_scales(s4 / 4 + 1);
             }
             if (s4 + j + 1 < nb) fetch(s4 + j + 1);
             const unsigned char *buf = lds8 + (j & 1) * STAGE;
@@ -1141,7 +1138,7 @@ static F8Matmul f8_operands(const EvoFp8Matmul &p) {
 
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
-    constexpr int lds = 2 * 32 * (WM * TM + WN * TN) * 128 + 32 * WN * TN * 4;
+    constexpr int side = 32 * (WM * TM + WN * TN), lds = 2 * side * 128 + 2 * side * 4 + 32 * WN * TN * 4;
     constexpr auto kernel = fp8_matmul<WM, WN, TM, TN, T, WIDE>;
     static PerDevice done;
     if (const int rc = ensure_dynamic_lds((const void *)kernel, lds, done, nullptr)) return rc;
@@ -1159,7 +1156,7 @@ static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
         fp8_matmul_big<T, WIDE><<<grid, 512, lds, st>>>(a);
         return f8_rc();
     }
-    return f8_launch_tiles<2, 2, 2, 2, T, WIDE>(a, grid, st);
+    return f8_launch_tiles<4, 2, 1, 2, T, WIDE>(a, grid, st);
 }
 
 // Strips of 128 rows, their columns in pieces for two workgroups on each unit (one: 32 768 x 1024 x 256 27.3 us instead of 20.1, 8192 x 4096 x 256 26.1 instead of 20.8).
