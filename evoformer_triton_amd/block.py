@@ -234,7 +234,7 @@ class GatedAttentionBlock(nn.Module):
         elif relative_buckets is not None or other_chain:
             raise ValueError("relative_buckets and other_chain need relative_distance")
         else:
-            self.register_module("relative", None)
+            self.relative = None
 
     def _stacked_weights(self):
         layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
@@ -290,17 +290,19 @@ class GatedAttentionBlock(nn.Module):
             bias = _pair_bias(self.layer_norm_z, self.linear_z, z)
         if bias is None and z is not None and self.linear_z is not None:
             bias = lin(self.linear_z, norm(self.layer_norm_z, z)).permute(0, 3, 1, 2).unsqueeze(1).contiguous().to(dtype)
-        if self.relative is not None:
-            bias = (self.relative.plain if plain else self.relative)(positions, chains=chains, pair_bias=bias, dtype=dtype)
+        relative = self._modules.get("relative")
+        if relative is not None:
+            bias = (relative.plain if plain else relative)(positions, chains=chains, pair_bias=bias, dtype=dtype)
         if mask is not None:
             add_mask = (self.inf * (mask.to(torch.float32) - 1.0)).view(B, S, 1, 1, N)
         return bias, add_mask
 
     def _check(self, positions, chains, weights):
-        if (positions is None) != (self.relative is None):
+        relative = self._modules.get("relative")      # (a block that was saved before it could have one has none)
+        if (positions is None) != (relative is None):
             raise ValueError("a block with a relative position bias needs the residues' positions" if positions is None else
                              "positions are for a block with a relative position bias (relative_distance)")
-        if chains is not None and (self.relative is None or not self.relative.other_chain):
+        if chains is not None and (relative is None or not relative.other_chain):
             raise ValueError("chains are for a block with a bucket for pairs of different chains (other_chain=True)")
         if weights is not None and not self.fp8:
             raise ValueError("weights in 8 bits are for a block made with fp8=True")
@@ -336,7 +338,7 @@ class GatedAttentionBlock(nn.Module):
     def forward(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None, chains: Optional[torch.Tensor] = None, weights: Optional[Fp8BlockWeights] = None):
         B, S, N, _ = m.shape
-        simple = not self.fp8 and self.relative is None and positions is None and chains is None and weights is None
+        simple = not self.fp8 and self._modules.get("relative") is None and positions is None and chains is None and weights is None
         if not simple:
             self._check(positions, chains, weights)
         if self._slots_ok(m):

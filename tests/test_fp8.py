@@ -129,6 +129,19 @@ def test_the_blocks_options():
         GatedAttentionBlock(64, 32, 4, other_chain=True)
 
 
+def test_a_block_that_was_saved_without_the_options():
+    import copy
+    torch.manual_seed(2)
+    block = GatedAttentionBlock(16, 8, 2, c_z=8)
+    old = copy.copy(block)
+    old.__dict__ = {k: v for k, v in block.__dict__.items() if k not in ("relative", "fp8")}
+    old._modules = {k: v for k, v in block._modules.items() if k != "relative"}
+    m, z = torch.randn(1, 3, 7, 16), torch.randn(1, 7, 7, 8)
+    assert torch.equal(old.forward_eager(m, z), block.forward_eager(m, z))
+    with pytest.raises(ValueError, match="relative_distance"):
+        old(m, z, None, torch.arange(7))
+
+
 def test_the_relative_bias_in_plain_operations_moves_the_blocks_result():
     torch.manual_seed(3)
     block = GatedAttentionBlock(16, 8, 2, c_z=8, relative_distance=4, other_chain=True)

@@ -149,6 +149,30 @@ def test_products_and_gradients(gpu_device, case):
     assert torch.equal(held, y)
 
 
+@pytest.mark.parametrize("rows,k,n", [(9, 150, 11), (140, 150, 70), (140, 700, 33)])
+def test_gradients_are_the_differences(gpu_device, rows, k, n):
+    """Whole numbers of up to 4 bits are what they are in 8 bits, whatever their block's scale, and so are the steps between them: differences are exact."""
+    from evoformer_triton_amd import fp8_linear
+    g = torch.Generator().manual_seed(8)
+    leaves = [torch.randint(-7, 8, s, generator=g).float().to(gpu_device).requires_grad_() for s in ((rows, k), (n, k), (n,))]
+    c = torch.randint(-7, 8, (rows, n), generator=g).float().to(gpu_device)
+
+    def loss():
+        return (fp8_linear(*leaves).double() * c).sum()
+
+    grads = torch.autograd.grad(loss(), leaves)
+    for t, got in zip(leaves, grads):
+        for at in torch.randint(0, t.numel(), (6,), generator=g).tolist() + [0, t.numel() - 1]:
+            with torch.no_grad():
+                flat, was = t.view(-1), t.view(-1)[at].clone()
+                flat[at] = was + 2
+                up = loss()
+                flat[at] = was - 3
+                down = loss()
+                flat[at] = was
+            assert (up - down) / 5 == got.view(-1)[at]
+
+
 def test_rows_with_infinities_and_nan_are_theirs_alone(gpu_device):
     from evoformer_triton_amd import Fp8Weight, fp8_linear
     g = torch.Generator().manual_seed(4)
