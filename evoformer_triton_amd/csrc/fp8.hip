@@ -1199,7 +1199,8 @@ static int f8_launch_strip(F8Matmul a, hipStream_t st) {
 }
 
 // Few rows: 64 outputs to a workgroup where there are then enough of them for the chip, or slices of the contraction to make up for it, else 16; of a block at least for each
-// wave.  us, 16 / 64 outputs: 24 x 4096 x 4096 16.5 / 12.9, 24 x 8192 x 8192 48.8 / 25.5, 48 x 500 x 8000 25.4 / 20.0; 24 x 1024 x 256 4.7 / 6.6, 8 x 8192 x 1024 5.9 / 6.5.
+// wave.  us, 16 / 64 outputs: 24 x 4096 x 4096 14.4 / 12.1 (1 row 8.9 / 9.8), 24 x 8192 x 8192 49 / 25, 48 x 500 x 8000 24.4 / 19.1; 24 x 1024 x 256 4.7 / 6.6,
+// 8 x 8192 x 1024 5.9 / 6.5.
 struct F8FewPlan {
     int nt, slice, slices;
 };
