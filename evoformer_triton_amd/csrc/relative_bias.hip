@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 // 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones as three bf16 parts, which hold all of their 24 bits.  A
 // product with one is exact, and sums are fp32 in a fixed order.  Zero times an infinity is no number: a workgroup that ends with a
 // sum that is not finite forms its sums again one by one, and so does one whose positions or chains lie 2^30 or more apart.
-// Bound by memory: 4 x 32 x 1024^2 in fp32 107 us (537 MB, 5.0 TB/s; with the loads alone 113 where this took 117), after the forward's results have been written
+// Bound by memory: 4 x 32 x 1024^2 in fp32 110 us (537 MB, 4.9 TB/s; with the loads alone 113 where this took 117), after the forward's results have been written
 // 141.  As many additions to sums in LDS: 681 us.  32 heads to a workgroup, whose buckets are then looked up once: 151 instead of 116.
 constexpr int kRbKeys = 64, kRbHeads = 16;   // a workgroup's keys and heads
 
