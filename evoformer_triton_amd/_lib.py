@@ -37,7 +37,7 @@ EXPORTS = ("evoattn_version", "evoattn_strerror", "evoattn_check", "evoattn_prep
            "evoattn_pair_bias_workspace_bytes", "evoattn_pair_bias_fwd", "evoattn_pair_bias_bwd",
            "evoattn_keep_mask", "evoattn_linear_fwd", "evoattn_linear_dx", "evoattn_linear_dw_workspace_bytes", "evoattn_linear_dw",
            "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd",
-           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding")
+           "evoattn_fp8_quantize", "evoattn_fp8_quantize_two", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_sums", "evoattn_fp8_matmul_rounds", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding")
 EVOATTN_STATIC_PREP_BYTES = 16 << 20
 
 
@@ -76,6 +76,13 @@ class EvoRelativeBias(ctypes.Structure):
         ("pair", ctypes.c_void_p), ("out", ctypes.c_void_p), ("dout", ctypes.c_void_p),
         ("dtable", ctypes.c_void_p), ("dpair", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvoFp8Rounding(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("rows", ctypes.c_int64), ("cols", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("qt", ctypes.c_void_p), ("scales_t", ctypes.c_void_p), ("sums", ctypes.c_void_p),
     ]
 
 
@@ -155,7 +162,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_pair_bias_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i64, i64, i32, i32, i32, vp]
     RB = ctypes.POINTER(EvoRelativeBias)
     for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd",
-           "evoattn_fp8_quantize", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding"):
+           "evoattn_fp8_quantize", "evoattn_fp8_quantize_two", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_sums", "evoattn_fp8_matmul_rounds", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [RB, vp]
     lib.evoattn_relative_bias_bwd_workspace_bytes.restype = ctypes.c_size_t
@@ -168,6 +175,12 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_fp8_matmul_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
     lib.evoattn_fp8_matmul.restype = ctypes.c_int
     lib.evoattn_fp8_matmul.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp]
+    lib.evoattn_fp8_quantize_two.restype = ctypes.c_int
+    lib.evoattn_fp8_quantize_two.argtypes = [ctypes.POINTER(EvoFp8Rounding), ctypes.POINTER(EvoFp8Rounding), i32, vp]
+    lib.evoattn_fp8_matmul_sums.restype = ctypes.c_int
+    lib.evoattn_fp8_matmul_sums.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp, i64, vp, i32, vp]
+    lib.evoattn_fp8_matmul_rounds.restype = ctypes.c_int
+    lib.evoattn_fp8_matmul_rounds.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
     lib.evoattn_fp8_matmul_rounding_workspace_bytes.restype = ctypes.c_size_t
     lib.evoattn_fp8_matmul_rounding_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
     lib.evoattn_fp8_matmul_rounding.restype = ctypes.c_int

@@ -195,7 +195,7 @@ __device__ __forceinline__ void f8_store_scale(uint8_t *s, int64_t k, int64_t bl
 // float at a time through maxima, scaling and conversion 32 768 x 256 along its rows took 7.9 us instead of 7.3.
 // A workgroup rounds R rows x 128 columns, 128 rows where it rounds columns, too: thread t V rows (V (t / 16) ..) of eight columns (8 (t % 16) ..).
 template <typename T, int R, int V, bool ROWS, bool COLS>
-__global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
+__device__ __forceinline__ void f8_quantize(const F8Quantize &p, unsigned id) {
     static_assert(R == 128 || !COLS, "a column's block is 128 rows");
     typedef F8Bits<T> B;
     constexpr int WAVES = R / V / 4, THREADS = R / V * 16;
@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
     __shared__ __attribute__((aligned(16))) float col_scale[COLS ? 128 : 4];
     __shared__ uint8_t row_scale[R];
     const int t = threadIdx.x, cg = t % 16, rg = t / 16, wave = t / 64;
-    const int kt = blockIdx.x % p.tiles_k;
-    const int64_t rt = blockIdx.x / p.tiles_k;
+    const int kt = id % p.tiles_k;
+    const int64_t rt = id / p.tiles_k;
     const int c0 = kt * 128 + cg * 8;
     const int64_t r0 = rt * R + rg * V;
     F8Eight<T> e[V];
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
                 e[i].v[c] = r0 + i < p.rows && c0 + c < p.cols ? one : (T)0.0f;
             }
     }
-    if (ROWS) {
+    if (ROWS && p.q) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             const F8Eight<T> one[1] = {e[i]};
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
             if (cg == 0) row_scale[rg * V + i] = (uint8_t)(ex + 127);
         }
     }
-    if constexpr (COLS) {
+    if constexpr (COLS) if (p.qt) {
         const typename B::V a = f8_max_rows(f8_magnitudes(e));
         float s[8];
 #pragma unroll
@@ -317,10 +317,24 @@ __global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
                 *reinterpret_cast<i32x4f *>(p.qt + (int64_t)(kt * 128 + col) * p.rp + rt * 128 + slot * 16) = *reinterpret_cast<const i32x4f *>(tile + at(col, slot * 16));
         }
     }
-    if constexpr (ROWS) {
-        if (!COLS) __syncthreads();
+    if constexpr (ROWS) if (p.q) {
+        if (!COLS || !p.qt) __syncthreads();
         if (t < R && rt * R + t < p.rows) f8_store_scale(p.s + (rt * R + t) * p.sp, kt, p.tiles_k, p.sp, row_scale[t]);
     }
+}
+template <typename T, int R, int V, bool ROWS, bool COLS>
+__global__ void __launch_bounds__(R / V * 16) fp8_quantize(F8Quantize p) {
+    f8_quantize<T, R, V, ROWS, COLS>(p, blockIdx.x);
+}
+// Two matrices, each both ways or one, in one launch: a weight of a few tiles takes a launch's time (1024 x 256 6 us) beside its input (32 768 x 256 7).
+struct F8Two {
+    F8Quantize p[2];
+    unsigned first;   // tiles of the first
+};
+template <typename T, int V>
+__global__ void __launch_bounds__(128 / V * 16) fp8_quantize_two(F8Two a) {
+    const unsigned second = blockIdx.x >= a.first ? 1 : 0;
+    f8_quantize<T, 128, V, true, true>(a.p[second], blockIdx.x - second * a.first);
 }
 
 __device__ __forceinline__ void f8_store_as(void *out, int64_t i, float v, int dtype) {
@@ -330,21 +344,28 @@ __device__ __forceinline__ void f8_store_as(void *out, int64_t i, float v, int d
 }
 
 // Column sums from those of 128 rows each: 32 columns by 32 slices of the parts.  A launch's time: 256 parts of 1024 columns 3.8 us.
-__global__ void __launch_bounds__(1024) fp8_sums(const float *part, void *out, int cols, int64_t parts, int dtype) {
+template <int THREADS>   // 32 of them, each with 32 / THREADS slices: the same additions
+__device__ __forceinline__ void f8_add_sums(const float *part, void *out, int cols, int64_t parts, int dtype, unsigned id) {
     __shared__ float sums[32][33];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-    float s = 0.0f;
-    if (c < cols) {
+    const int c = id * 32 + (threadIdx.x & 31), first = threadIdx.x >> 5;
+#pragma unroll
+    for (int slice = first; slice < 32; slice += THREADS) {
+        float s = 0.0f;
+        if (c < cols) {
 #pragma unroll 8
-        for (int64_t i = slice; i < parts; i += 32) s += part[i * cols + c];
+            for (int64_t i = slice; i < parts; i += 32) s += part[i * cols + c];
+        }
+        sums[slice][threadIdx.x & 31] = s;
     }
-    sums[slice][threadIdx.x & 31] = s;
     __syncthreads();
-    if (slice || c >= cols) return;
-    s = 0.0f;
+    if (first || c >= cols) return;
+    float s = 0.0f;
 #pragma unroll
     for (int i = 0; i < 32; ++i) s += sums[i][threadIdx.x];
     f8_store_as(out, c, s, dtype);
+}
+__global__ void __launch_bounds__(1024) fp8_sums(const float *part, void *out, int cols, int64_t parts, int dtype) {
+    f8_add_sums<32>(part, out, cols, parts, dtype, blockIdx.x);
 }
 
 // ---- product ----
@@ -906,9 +927,21 @@ __global__ void __launch_bounds__(256, 2) fp8_strip(F8Matmul p) {
     }
 }
 
-// The slices' sums, eight columns per thread, in their order.  16 slices of 1024 x 256: 5 us, a launch and the way to memory.
+// The slices' sums, eight columns per thread, in their order, and column sums that are asked for with them.  16 slices of 1024 x 256: 5 us, a launch and the way to memory;
+// the column sums in one of their own 4 more.
+struct F8Sums {   // the column sums' parts and where their totals go, if there are any
+    const float *part;
+    void *out;
+    int64_t parts;
+    int cols, dtype;
+    unsigned first;   // the first workgroup that adds them up
+};
 template <typename T>
-__global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, const void *bias, int bias_dtype, int64_t M, int N, int64_t ldo, int slices) {
+__global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, const void *bias, int bias_dtype, int64_t M, int N, int64_t ldo, int slices, F8Sums c) {
+    if (c.part && blockIdx.x >= c.first) {
+        f8_add_sums<8>(c.part, c.out, c.cols, c.parts, c.dtype, blockIdx.x - c.first);
+        return;
+    }
     const int pieces = (N + 7) / 8;
     const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / pieces;
     const int o = (int)(id % pieces) * 8;
@@ -1079,7 +1112,7 @@ static int f8_by_dtype(int dtype, F &&f) {
     return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
 }
 
-constexpr int kF8StripBlocks = 4;
+constexpr int kF8StripBlocks = 4, kF8SumsParts = 1024;   // (of more parts a launch of its own, of four times the threads)
 constexpr int64_t kF8MaxK = 1 << 26;   // of the contraction: 32 rows stay within 32-bit offsets
 
 // How a product is cut.  Up to four blocks: strips.  Tiles of 256 x 256 where there is one for each unit, else of 128 x 128 (us, 128 / 256: 8192 x 2048 x 2048, 256 large tiles,
@@ -1117,6 +1150,32 @@ static int f8_check(const EvoFp8Matmul *p) {
     return EVO_OK;
 }
 
+constexpr int kF8QuantizeFew = 512;   // tiles
+static int f8_rounding_check(const void *x, int64_t ldx, const void *q, const void *scales, const void *qt, const void *scales_t, const float *sums, int64_t rows,
+                             int64_t cols, int dtype) {
+    if (!x || rows <= 0 || cols <= 0 || ldx < cols || !f8_dtype(dtype) || !q != !scales || !qt != !scales_t || (!q && !qt) || (sums && !qt)) return EVO_EINVAL;
+    if (cols > kF8MaxK || (qt && rows > ((int64_t)1 << 40))) return EVO_EUNSUPPORTED;
+    return f8_off(q, 16) || f8_off(qt, 16) ? EVO_EALIGN : EVO_OK;
+}
+static F8Quantize f8_rounding(const void *x, int64_t ldx, void *q, void *scales, void *qt, void *scales_t, float *sums, int64_t rows, int64_t cols) {
+    F8Quantize p{};
+    p.x = x;
+    p.ldx = ldx;
+    p.rows = rows;
+    p.cols = (int)cols;
+    p.kp = f8_pitch(cols);
+    p.sp = (int)f8_scale_pitch(cols);
+    p.tiles_k = (int)(p.kp / kF8Block);
+    p.rp = f8_pitch(rows);
+    p.spt = f8_scale_pitch(rows);
+    p.tiles_r = p.rp / kF8Block;
+    p.q = (uint8_t *)q;
+    p.s = (uint8_t *)scales;
+    p.qt = (uint8_t *)qt;
+    p.st = (uint8_t *)scales_t;
+    p.sums = sums;
+    return p;
+}
 static F8Matmul f8_operands(const EvoFp8Matmul &p) {
     F8Matmul a{};
     a.a = (const uint8_t *)p.a;
@@ -1231,10 +1290,11 @@ static int f8_launch_few(const F8Few &a, const F8FewPlan &q, hipStream_t st) {
                                                                                                           : go(std::integral_constant<int, 4>());
 }
 template <typename T>
-static int f8_add_slices(const EvoFp8Matmul &p, int slices, hipStream_t st) {
-    const int64_t pieces = p.m * ((p.n + 7) / 8), groups = (pieces + 255) / 256;
-    if (groups > INT32_MAX) return EVO_EOVERFLOW;
-    fp8_slices<T><<<(unsigned)groups, 256, 0, st>>>((const float *)p.workspace, (T *)p.out, p.bias, p.bias_dtype, p.m, (int)p.n, p.ldo, slices);
+static int f8_add_slices(const EvoFp8Matmul &p, int slices, F8Sums c, hipStream_t st) {
+    const int64_t pieces = p.m * ((p.n + 7) / 8), groups = (pieces + 255) / 256, more = c.part ? (c.cols + 31) / 32 : 0;
+    if (groups + more > INT32_MAX) return EVO_EOVERFLOW;
+    c.first = (unsigned)groups;
+    fp8_slices<T><<<(unsigned)(groups + more), 256, 0, st>>>((const float *)p.workspace, (T *)p.out, p.bias, p.bias_dtype, p.m, (int)p.n, p.ldo, slices, c);
     return f8_rc();
 }
 
@@ -1245,36 +1305,41 @@ extern "C" {
 int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void *qt, void *scales_t, float *sums, int64_t rows, int64_t cols, int32_t dtype,
                          void *hip_stream) {
     using namespace evo;
-    if (!x || rows <= 0 || cols <= 0 || ldx < cols || !f8_dtype(dtype) || !q != !scales || !qt != !scales_t || (!q && !qt) || (sums && !qt)) return EVO_EINVAL;
-    if (cols > kF8MaxK || (qt && rows > ((int64_t)1 << 40))) return EVO_EUNSUPPORTED;
-    if (f8_off(q, 16) || f8_off(qt, 16)) return EVO_EALIGN;
-    F8Quantize p{};
-    p.x = x;
-    p.ldx = ldx;
-    p.rows = rows;
-    p.cols = (int)cols;
-    p.kp = f8_pitch(cols);
-    p.sp = (int)f8_scale_pitch(cols);
-    p.tiles_k = (int)(p.kp / kF8Block);
-    p.rp = f8_pitch(rows);
-    p.spt = f8_scale_pitch(rows);
-    p.tiles_r = p.rp / kF8Block;
-    p.q = (uint8_t *)q;
-    p.s = (uint8_t *)scales;
-    p.qt = (uint8_t *)qt;
-    p.st = (uint8_t *)scales_t;
-    p.sums = sums;
+    if (const int rc = f8_rounding_check(x, ldx, q, scales, qt, scales_t, sums, rows, cols, dtype)) return rc;
+    const F8Quantize p = f8_rounding(x, ldx, q, scales, qt, scales_t, sums, rows, cols);
     if (p.tiles_r > INT32_MAX / p.tiles_k) return EVO_EOVERFLOW;
     const unsigned grid = (unsigned)(p.tiles_r * p.tiles_k);
     hipStream_t st = (hipStream_t)hip_stream;
     return f8_by_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
         // few tiles: more threads for each (us, more / fewer: 1024 x 256 both ways 5.5 / 5.8, 2048 x 4096 rows 6.9 / 7.5; 8192 x 8192 both ways 53.5 / 50.6)
-        const bool few = p.tiles_r * p.tiles_k < 512;
+        const bool few = p.tiles_r * p.tiles_k < kF8QuantizeFew;
         if (q && qt) few ? fp8_quantize<T, 128, 2, true, true><<<grid, 1024, 0, st>>>(p) : fp8_quantize<T, 128, 8, true, true><<<grid, 256, 0, st>>>(p);
         else if (!q) few ? fp8_quantize<T, 128, 2, false, true><<<grid, 1024, 0, st>>>(p) : fp8_quantize<T, 128, 8, false, true><<<grid, 256, 0, st>>>(p);
         else if (few) fp8_quantize<T, 16, 1, true, false><<<(unsigned)((rows + 15) / 16 * p.tiles_k), 256, 0, st>>>(p);
         else fp8_quantize<T, 128, 8, true, false><<<grid, 256, 0, st>>>(p);
+        return f8_rc();
+    });
+}
+
+int evoattn_fp8_quantize_two(const EvoFp8Rounding *a, const EvoFp8Rounding *b, int32_t dtype, void *hip_stream) {
+    using namespace evo;
+    if (!a || !b || !f8_dtype(dtype)) return EVO_EINVAL;
+    F8Two both{};
+    int64_t tiles = 0;
+    for (int i = 0; i < 2; ++i) {
+        const EvoFp8Rounding &r = i ? *b : *a;
+        if (const int rc = f8_rounding_check(r.x, r.ldx, r.q, r.scales, r.qt, r.scales_t, r.sums, r.rows, r.cols, dtype)) return rc;
+        both.p[i] = f8_rounding(r.x, r.ldx, r.q, r.scales, r.qt, r.scales_t, r.sums, r.rows, r.cols);
+        if (both.p[i].tiles_r > INT32_MAX / both.p[i].tiles_k) return EVO_EOVERFLOW;
+        if (i == 0) both.first = (unsigned)(both.p[0].tiles_r * both.p[0].tiles_k);
+        tiles += both.p[i].tiles_r * both.p[i].tiles_k;
+    }
+    if (tiles > INT32_MAX) return EVO_EOVERFLOW;
+    return f8_by_dtype(dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (tiles < kF8QuantizeFew) fp8_quantize_two<T, 2><<<(unsigned)tiles, 1024, 0, (hipStream_t)hip_stream>>>(both);
+        else fp8_quantize_two<T, 8><<<(unsigned)tiles, 256, 0, (hipStream_t)hip_stream>>>(both);
         return f8_rc();
     });
 }
@@ -1294,7 +1359,7 @@ size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p) {
     return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
 
-int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
+static int f8_matmul(const EvoFp8Matmul *p, const evo::F8Sums &c, void *hip_stream, bool *added) {
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
     if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
@@ -1316,9 +1381,32 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
         return p->dtype == EVO_F32 ? f8_launch<float, true>(a, q, st) : p->dtype == EVO_BF16 ? f8_launch<bf16_t, false>(a, q, st) : f8_launch<f16_t, false>(a, q, st);
     }
     if (const int rc = wide ? f8_launch<float, true>(a, q, st) : f8_launch<float, false>(a, q, st)) return rc;
-    return f8_by_dtype(p->dtype, [&](auto t) { return f8_add_slices<decltype(t)>(*p, q.slices, st); });
+    *added = c.part != nullptr;
+    return f8_by_dtype(p->dtype, [&](auto t) { return f8_add_slices<decltype(t)>(*p, q.slices, c, st); });
+}
+int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
+    bool added;
+    return f8_matmul(p, evo::F8Sums{}, hip_stream, &added);
+}
+int evoattn_fp8_matmul_sums(const EvoFp8Matmul *p, const float *sums, int64_t rows, void *out, int32_t dtype, void *hip_stream) {
+    using namespace evo;
+    if (const int rc = f8_check(p)) return rc;
+    if (!sums || !out || rows <= 0 || !f8_dtype(dtype)) return EVO_EINVAL;
+    F8Sums c{};
+    c.parts = (rows + kF8Block - 1) / kF8Block;
+    if (c.parts <= kF8SumsParts) c.part = sums;
+    c.out = out;
+    c.cols = (int)p->m;
+    c.dtype = dtype;
+    bool added = false;
+    const int rc = f8_matmul(p, c, hip_stream, &added);
+    return rc || added ? rc : evoattn_fp8_column_sums(sums, out, rows, p->m, dtype, hip_stream);
 }
 
+int evoattn_fp8_matmul_rounds(const EvoFp8Matmul *p) {
+    using namespace evo;
+    return !f8_check(p) && (p->m <= kF8FewRows || f8_strip_rounds(p->m, p->n, p->k, p->dtype));
+}
 size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p) {
     using namespace evo;
     if (f8_check(p) || p->m > kF8FewRows) return 0;   // (strips need none)
@@ -1330,7 +1418,7 @@ int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ld
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
     const bool few = p->m <= kF8FewRows;
-    if (!few && !f8_strip_rounds(p->m, p->n, p->k, p->dtype)) return EVO_EUNSUPPORTED;
+    if (!evoattn_fp8_matmul_rounds(p)) return EVO_EUNSUPPORTED;
     if (!x || ldx < p->k || !p->b || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->b, 16) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
     hipStream_t st = (hipStream_t)hip_stream;
@@ -1363,7 +1451,7 @@ int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ld
         typedef decltype(t) T;
         if (!cut) return f8_launch_few<T, T>(a, q, st);
         if (const int rc = f8_launch_few<T, float>(a, q, st)) return rc;
-        return f8_add_slices<T>(*p, q.slices, st);
+        return f8_add_slices<T>(*p, q.slices, F8Sums{}, st);
     });
 }
 

@@ -23,14 +23,41 @@ Tensor f8_rows(const Tensor &x) {
 int64_t f8_apart(const Tensor &x) { return x.size(0) == 1 ? std::max(x.stride(0), x.size(1)) : x.stride(0); }   // (one row's stride may be anything)
 
 // x rounded along its rows and its columns, as far as asked for, and the column sums of its blocks of rows.
+EvoFp8Rounding f8_rounded(const Tensor &x, Rounded *along_rows, Rounded *along_cols, Tensor *sums) {
+    EvoFp8Rounding r{};
+    r.x = x.data_ptr();
+    r.ldx = f8_apart(x);
+    r.rows = x.size(0);
+    r.cols = x.size(1);
+    if (along_rows) {
+        *along_rows = Rounded(r.rows, r.cols, x);
+        r.q = along_rows->q;
+        r.scales = along_rows->s;
+    }
+    if (along_cols) {
+        *along_cols = Rounded(r.cols, r.rows, x);
+        r.qt = along_cols->q;
+        r.scales_t = along_cols->s;
+    }
+    if (sums) {
+        *sums = at::empty({(r.rows + 127) / 128, r.cols}, x.options().dtype(at::kFloat));
+        r.sums = (float *)sums->data_ptr();
+    }
+    return r;
+}
 void f8_quantize(const Tensor &x, Rounded *along_rows, Rounded *along_cols, Tensor *sums) {
-    const int64_t rows = x.size(0), cols = x.size(1);
-    if (along_rows) *along_rows = Rounded(rows, cols, x);
-    if (along_cols) *along_cols = Rounded(cols, rows, x);
-    if (sums) *sums = at::empty({(rows + 127) / 128, cols}, x.options().dtype(at::kFloat));
-    check(evoattn_fp8_quantize(x.data_ptr(), f8_apart(x), along_rows ? along_rows->q : nullptr, along_rows ? along_rows->s : nullptr,
-                               along_cols ? along_cols->q : nullptr, along_cols ? along_cols->s : nullptr, sums ? (float *)sums->data_ptr() : nullptr, rows,
-                               cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
+    const EvoFp8Rounding r = f8_rounded(x, along_rows, along_cols, sums);
+    check(evoattn_fp8_quantize(r.x, r.ldx, r.q, r.scales, r.qt, r.scales_t, r.sums, r.rows, r.cols, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize");
+}
+// a weight both ways or along its rows, and x as far as asked for
+void f8_quantize_both(const Tensor &w, Rounded *w_rows, Rounded *w_cols, const Tensor &x, Rounded *x_rows, Rounded *x_cols) {
+    if ((!x_rows && !x_cols) || w.scalar_type() != x.scalar_type()) {
+        f8_quantize(w, w_rows, w_cols, nullptr);
+        if (x_rows || x_cols) f8_quantize(x, x_rows, x_cols, nullptr);
+        return;
+    }
+    const EvoFp8Rounding a = f8_rounded(w, w_rows, w_cols, nullptr), b = f8_rounded(x, x_rows, x_cols, nullptr);
+    check(evoattn_fp8_quantize_two(&a, &b, evo_dtype(x.scalar_type()), stream_of(x)), "evoattn_fp8_quantize_two");
 }
 
 EvoFp8Matmul f8_product(int64_t rows, const Rounded &b, const Tensor &bias, const Tensor &out) {
@@ -49,8 +76,9 @@ EvoFp8Matmul f8_product(int64_t rows, const Rounded &b, const Tensor &bias, cons
     p.out = out.data_ptr();
     return p;
 }
-// a b^T (+ bias), [a.rows, b.rows], on `like`'s device
-Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype, const Tensor &like) {
+// a b^T (+ bias), [a.rows, b.rows], on `like`'s device; and the column sums' totals to `totals`, if given
+Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::ScalarType dtype, const Tensor &like, const Tensor &sums = Tensor(),
+                 const Tensor &totals = Tensor()) {
     Tensor out = at::empty({a.rows, b.rows}, like.options().dtype(dtype)), ws;
     EvoFp8Matmul p = f8_product(a.rows, b, bias, out);
     p.a = a.q;
@@ -60,32 +88,36 @@ Tensor f8_matmul(const Rounded &a, const Rounded &b, const Tensor &bias, at::Sca
         p.workspace = ws.data_ptr();
         p.workspace_bytes = (size_t)ws.numel();
     }
-    check(evoattn_fp8_matmul(&p, stream_of(like)), "evoattn_fp8_matmul");
+    if (totals.defined())
+        check(evoattn_fp8_matmul_sums(&p, (const float *)sums.data_ptr(), b.k, totals.data_ptr(), evo_dtype(totals.scalar_type()), stream_of(like)),
+              "evoattn_fp8_matmul_sums");
+    else check(evoattn_fp8_matmul(&p, stream_of(like)), "evoattn_fp8_matmul");
     return out;
 }
 
-// x b^T (+ bias), x rounded on the way where that is how it is done; not defined for other sizes
-constexpr int64_t kF8FewRows = 64, kF8StripColumns = 512;   // up to so many rows, or so long a contraction
+// whether x [rows, k] times a matrix of n rows is rounded on the way
+bool f8_rounds(const Tensor &x, int64_t n) {
+    EvoFp8Matmul p{};
+    p.m = x.size(0);
+    p.n = n;
+    p.k = x.size(1);
+    p.dtype = evo_dtype(x.scalar_type());
+    return evoattn_fp8_matmul_rounds(&p) != 0;
+}
+// x b^T (+ bias), x rounded on the way
 Tensor f8_rounding(const Tensor &x, const Rounded &b, const Tensor &bias) {
-    Tensor out;
-    if (x.size(0) <= kF8FewRows || x.size(1) <= kF8StripColumns) {
-        Tensor ws;
-        out = at::empty({x.size(0), b.rows}, x.options());
-        EvoFp8Matmul p = f8_product(x.size(0), b, bias, out);
-        if (const size_t bytes = evoattn_fp8_matmul_rounding_workspace_bytes(&p)) {
-            ws = scratch(bytes, x);
-            p.workspace = ws.data_ptr();
-            p.workspace_bytes = (size_t)ws.numel();
-        }
-        const int rc = evoattn_fp8_matmul_rounding(&p, x.data_ptr(), f8_apart(x), stream_of(x));
-        if (rc == EVO_EUNSUPPORTED) return Tensor();
-        check(rc, "evoattn_fp8_matmul_rounding");
+    Tensor out = at::empty({x.size(0), b.rows}, x.options()), ws;
+    EvoFp8Matmul p = f8_product(x.size(0), b, bias, out);
+    if (const size_t bytes = evoattn_fp8_matmul_rounding_workspace_bytes(&p)) {
+        ws = scratch(bytes, x);
+        p.workspace = ws.data_ptr();
+        p.workspace_bytes = (size_t)ws.numel();
     }
+    check(evoattn_fp8_matmul_rounding(&p, x.data_ptr(), f8_apart(x), stream_of(x)), "evoattn_fp8_matmul_rounding");
     return out;
 }
 Tensor f8_times(const Tensor &x, const Rounded &b, const Tensor &bias) {
-    Tensor out = f8_rounding(x, b, bias);
-    if (out.defined()) return out;
+    if (f8_rounds(x, b.rows)) return f8_rounding(x, b, bias);
     Rounded a;
     f8_quantize(x, &a, nullptr, nullptr);
     return f8_matmul(a, b, bias, x.scalar_type(), x);
@@ -135,15 +167,9 @@ Tensor f8_forward(const Tensor &x, const Tensor &w, const Tensor &bias, bool nee
     }
     const Tensor x2 = f8_rows(x), w2 = f8_rows(w), b = bias.defined() ? bias.contiguous() : bias;
     Rounded xr, wr;
-    f8_quantize(w2, &wr, need_x ? &saved->wt : nullptr, nullptr);
-    Tensor y = f8_rounding(x2, wr, b);
-    if (y.defined()) {
-        if (need_w) f8_quantize(x2, nullptr, &saved->xt, nullptr);
-    } else {
-        f8_quantize(x2, &xr, need_w ? &saved->xt : nullptr, nullptr);
-        y = f8_matmul(xr, wr, b, x.scalar_type(), x2);
-    }
-    return y.view(shape);
+    const bool rounds = f8_rounds(x2, n);
+    f8_quantize_both(w2, &wr, need_x ? &saved->wt : nullptr, x2, rounds ? nullptr : &xr, need_w ? &saved->xt : nullptr);
+    return (rounds ? f8_rounding(x2, wr, b) : f8_matmul(xr, wr, b, x.scalar_type(), x2)).view(shape);
 }
 // dx, dw, db from dy [rows, n]
 void f8_backward(const Tensor &dy, const F8Saved &saved, bool need_x, bool need_w, bool need_b, at::ScalarType wtype, at::ScalarType btype, Tensor &dx, Tensor &dw,
@@ -154,9 +180,10 @@ void f8_backward(const Tensor &dy, const F8Saved &saved, bool need_x, bool need_
     const bool cols = need_w || need_b;
     f8_quantize(dy, need_x ? &along_rows : nullptr, cols ? &along_cols : nullptr, need_b ? &sums : nullptr);
     if (need_x) dx = f8_matmul(along_rows, saved.wt, Tensor(), dy.scalar_type(), dy);
-    if (need_w) dw = f8_matmul(along_cols, saved.xt, Tensor(), wtype, dy);
-    if (need_b) {
-        db = at::empty({dy.size(1)}, dy.options().dtype(btype));
+    if (need_b) db = at::empty({dy.size(1)}, dy.options().dtype(btype));
+    if (need_w) {
+        dw = f8_matmul(along_cols, saved.xt, Tensor(), wtype, dy, sums, db);
+    } else if (need_b) {
         check(evoattn_fp8_column_sums((const float *)sums.data_ptr(), db.data_ptr(), dy.size(0), dy.size(1), evo_dtype(btype), stream_of(dy)),
               "evoattn_fp8_column_sums");
     }

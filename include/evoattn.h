@@ -333,6 +333,14 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream);
  * q and qt on 16-byte boundaries.  cols at most 2^26. */
 int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void *qt, void *scales_t, float *sums, int64_t rows, int64_t cols,
                          int32_t dtype, void *hip_stream);
+typedef struct EvoFp8Rounding {
+    const void *x;
+    int64_t ldx, rows, cols;
+    void   *q, *scales, *qt, *scales_t;
+    float  *sums;
+} EvoFp8Rounding;
+/* Two matrices of one dtype in one launch. */
+int evoattn_fp8_quantize_two(const EvoFp8Rounding *a, const EvoFp8Rounding *b, int32_t dtype, void *hip_stream);
 int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t cols, int32_t dtype, void *hip_stream);
 
 /* out [m][n] = a [m][k] b [n][k]^T (+ bias [n]): rounded matrices as above, fp32 sums, rounded once to dtype (EVO_BF16 / _F16 / _F32); out's
@@ -352,10 +360,13 @@ typedef struct EvoFp8Matmul {
 } EvoFp8Matmul;
 size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream);
+/* That and evoattn_fp8_column_sums(sums, out, rows, p->m, dtype), in fewer launches: a weight's gradient and its bias's. */
+int evoattn_fp8_matmul_sums(const EvoFp8Matmul *p, const float *sums, int64_t rows, void *out, int32_t dtype, void *hip_stream);
 
 /* The same with x [m][k], rows ldx elements apart, in the result's dtype, that is rounded on the way (p's a and scales_a are not read): the products
  * of evoattn_fp8_quantize's rows (for more than 64 the same bits as the two calls give).  m at most 64; or k at most 512 where that takes less time than the two calls do, which is whenever k is at
- * most 256: EVO_EUNSUPPORTED for all others, and they go through the two calls.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
+ * most 256 (evoattn_fp8_matmul_rounds says which): EVO_EUNSUPPORTED for all others, and they go through the two calls.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
+int evoattn_fp8_matmul_rounds(const EvoFp8Matmul *p);   /* 1 or 0 */
 size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream);
 

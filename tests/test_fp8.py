@@ -115,6 +115,27 @@ def test_rounding_that_the_c_abi_rejects_before_any_launch(args, code):
     assert _lib.load().evoattn_fp8_quantize(*args, None) == code
 
 
+def test_two_at_once_that_the_c_abi_rejects_before_any_launch():
+    lib = _lib.load()
+
+    def two(a, b, dtype=_lib.EVO_BF16):
+        r = [_lib.EvoFp8Rounding(0x10000, 40, 3, 40, 0x10000, 0x10000, None, None, None) for _ in range(2)]
+        for one, change in zip(r, (a, b)):
+            for k, v in change.items():
+                setattr(one, k, v)
+        return lib.evoattn_fp8_quantize_two(ctypes.byref(r[0]), ctypes.byref(r[1]), dtype, None)
+    for change, code in ((dict(x=None), _lib.EVO_EINVAL), (dict(ldx=39), _lib.EVO_EINVAL), (dict(sums=0x10000), _lib.EVO_EINVAL), (dict(q=0x10004), _lib.EVO_EALIGN), (dict(rows=0), _lib.EVO_EINVAL),
+                         (dict(cols=(1 << 26) + 1, ldx=1 << 27), _lib.EVO_EUNSUPPORTED)):
+        assert two(change, {}) == code and two({}, change) == code
+    assert two({}, {}, 7) == _lib.EVO_EINVAL and lib.evoattn_fp8_quantize_two(None, None, 0, None) == _lib.EVO_EINVAL
+    for change in (dict(sums=None), dict(rows=0), dict(out=None), dict(dtype=4)):
+        args = {**dict(sums=0x10000, rows=300, out=0x10000, dtype=0), **change}
+        assert lib.evoattn_fp8_matmul_sums(ctypes.byref(_product()), *args.values(), None) == _lib.EVO_EINVAL
+    assert lib.evoattn_fp8_matmul_sums(ctypes.byref(_product(workspace=None)), 0x10000, 300, 0x10000, 0, None) == _lib.EVO_EWORKSPACE
+    rounds = [lib.evoattn_fp8_matmul_rounds(ctypes.byref(_product(m=m, n=n, k=k, dtype=t))) for m, n, k, t in ((64, 9, 5000, 0), (65, 9, 5000, 0), (70000, 900, 256, 2), (70000, 900, 257, 2), (70000, 300, 500, 0), (200, 3000, 500, 0))]
+    assert rounds == [1, 0, 1, 0, 1, 0]
+
+
 def test_the_blocks_options():
     plain = GatedAttentionBlock(64, 32, 4, c_z=64)
     block = GatedAttentionBlock(64, 32, 4, c_z=64, fp8=True, relative_distance=16, relative_buckets=8, other_chain=True)
