@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 // pairs x heads, on v_mfma_f32_16x16x32 (lane l, q = l / 16: operands' row or column l % 16, contraction 8q .. 8q + 7; accumulator column l % 16, rows
 // 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones as three bf16 parts, which hold all of their 24 bits.  A
 // product with one is exact, and sums are fp32 in a fixed order.  Zero times an infinity is no number: a workgroup that ends with a
-// sum that is not finite forms its sums again one by one, and so does one whose positions or chains lie 2^30 or more apart.
+// sum that is not finite forms its sums again one by one, and so does one whose positions or chains lie some 2^30 (less 4096) or more from its first query's.
 // Bound by memory: 4 x 32 x 1024^2 in fp32 110 us (537 MB, 4.9 TB/s; with the loads alone 113 where this took 117), after the forward's results have been written
 // 141.  As many additions to sums in LDS: 681 us.  32 heads to a workgroup, whose buckets are then looked up once: 151 instead of 116.
 constexpr int kRbKeys = 64, kRbHeads = 16;   // a workgroup's keys and heads
@@ -210,12 +210,14 @@ __device__ __forceinline__ u16x2r rb_any_bits(u16x2r x) {
     return r;
 }
 
-// A position or chain less the workgroup's first, in 32 bits; false where that is not within 2^30.
+// A position or chain less the workgroup's first, in 32 bits; false where that is not within 2^30 less the largest reach, so that a query's less a key's, and the reach
+// on top of it, fit in 32 bits as well.
 __device__ __forceinline__ bool rb_from(int64_t p, int64_t base, int &d) {
+    constexpr int64_t most = kRbNear - kRbMaxReach;
     int64_t w;
     const bool over = __builtin_sub_overflow(p, base, &w);
     d = (int)w;
-    return !over && rb_near(w);
+    return !over && w > -most && w < most;
 }
 
 // Lanes of a workgroup's keys: group g of 32, a lane's eight from `first` on, of which the first `skip` are another lane's (or none).

@@ -1,0 +1,32 @@
+"""The relative position bias far from zero and at the ends of its numbers: positions and chains as far apart as their type allows, gradients near
+the smallest and without a number."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _sums(bucket, dout, rows):
+    """The table's gradient in 64 bits: bucket [Nq,Nk], dout [B,1,H,Nq,Nk]."""
+    per_pair = dout.double().sum((0, 1)).flatten(1).t()
+    return torch.zeros(rows, dout.shape[2], dtype=torch.float64, device=dout.device).index_add_(0, bucket.flatten(), per_pair)
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("far", [2 ** 30 - 4097, 2 ** 30 - 4096, 2 ** 30 - 5, 2 ** 30 - 2, 2 ** 30 - 1, 2 ** 30])
+@pytest.mark.parametrize("reach", [1, 2, 4, 4096])
+def test_positions_within_a_workgroups_reach(gpu_device, index, far, reach):
+    """Queries and keys on either side of the first query: differences of up to 2^31, in the forward and in the gradient's buckets."""
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    lut = relative_buckets(reach, None if reach < 128 else 64).to(gpu_device)
+    q = torch.tensor([0, far, -far, 3, far - 1], dtype=index, device=gpu_device)
+    k = torch.tensor([-far, far, 0, -far + 1, far - 2, 5, 1, -far + 2, far], dtype=index, device=gpu_device)
+    rows = int(lut.max()) + 1
+    bucket = lut.long()[(q.long()[:, None] - k.long()[None]).clamp(-reach, reach) + reach]
+    table = torch.arange(1.0, 1 + 2 * rows, device=gpu_device).view(rows, 2).requires_grad_()
+    out = relative_position_bias(table, lut, q, k)
+    assert torch.equal(out[0, 0], table.detach()[bucket].permute(2, 0, 1))
+    dout = torch.arange(1.0, 91, device=gpu_device).view(1, 1, 2, 5, 9)
+    assert torch.equal(torch.autograd.grad(out, table, dout)[0].double(), _sums(bucket, dout, rows))
