@@ -140,7 +140,10 @@ const char *f8_linear_wrong(const Tensor &x, const Tensor &w, const OptTensor &b
     return f8_wrong(x, w.size(0), w.size(1), w.device(), bias);
 }
 const char *f8_held_wrong(const Tensor &x, const Tensor &q, const Tensor &s, int64_t k, const OptTensor &bias) {
-    if (q.dim() != 2 || s.dim() != 2 || q.element_size() != 1 || s.element_size() != 1 || k < 0 || q.size(1) != Rounded::pitch(k) ||
+    // (other types of a byte stand for other numbers)
+    if ((q.scalar_type() != at::kFloat8_e4m3fn && q.scalar_type() != at::kByte) || (s.scalar_type() != at::kFloat8_e8m0fnu && s.scalar_type() != at::kByte))
+        return "a weight in 8 bits has values in float8_e4m3fn and scales in float8_e8m0fnu, or their bytes (uint8)";
+    if (q.dim() != 2 || s.dim() != 2 || k < 0 || q.size(1) != Rounded::pitch(k) ||
         s.size(1) != Rounded::scale_pitch(k) || s.size(0) != q.size(0) || !q.is_contiguous() || !s.is_contiguous() || s.device() != q.device())
         return "a weight in 8 bits is values [n, k up to the next 128] and scales [n, k / 128 up to the next 4], both dense, a byte each";
     if (q.numel() && ((uintptr_t)q.data_ptr() % 16 || (uintptr_t)s.data_ptr() % 4)) return "a weight in 8 bits must start on a 16-byte boundary, its scales on one of 4";

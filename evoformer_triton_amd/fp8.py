@@ -40,6 +40,8 @@ class Fp8Weight(NamedTuple):
 
     def dequantize(self) -> torch.Tensor:
         """The values that it stands for, fp32 [n, k]."""
+        if self.values.dtype not in (torch.float8_e4m3fn, torch.uint8) or self.scales.dtype not in (torch.float8_e8m0fnu, torch.uint8):
+            raise ValueError("a weight in 8 bits has values in float8_e4m3fn and scales in float8_e8m0fnu, or their bytes (uint8)")
         v = self.values.view(torch.float8_e4m3fn).float().unflatten(-1, (-1, 128))
         e = self.scales.view(torch.uint8)[:, :v.shape[1]].int() - 127
         return torch.ldexp(v, e.unsqueeze(-1)).flatten(-2)[:, :self.k]
