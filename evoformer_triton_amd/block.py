@@ -189,7 +189,7 @@ _UNBIASED = ("linear_q", "linear_k", "linear_v", "linear_z")
 class Fp8BlockWeights(NamedTuple):
     """A block's projections in 8 bits, for inference: `GatedAttentionBlock.fp8_weights`."""
     projections: Fp8Weight               # Q, K, V (and the gate), stacked
-    bias: Optional[torch.Tensor]         # theirs: zeros but for the gate's
+    bias: Optional[torch.Tensor]         # theirs, zeros for a layer without one
     output: Fp8Weight
 
 
@@ -239,8 +239,8 @@ class GatedAttentionBlock(nn.Module):
     def _stacked_weights(self):
         layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
         weight, bias = torch.cat([l.weight for l in layers], 0), None
-        if self.linear_g is not None:
-            bias = torch.nn.functional.pad(self.linear_g.bias, (weight.shape[0] - self.linear_g.bias.shape[0], 0))
+        if any(l.bias is not None for l in layers):     # (Q, K and V have none as they are made, but a caller's layers may)
+            bias = torch.cat([l.weight.new_zeros(l.weight.shape[0]) if l.bias is None else l.bias for l in layers])
         return weight, bias
 
     @torch.no_grad()

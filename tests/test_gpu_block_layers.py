@@ -1,0 +1,35 @@
+"""The gated block in 8 bits with layers and modes that a caller may bring: biases on Q, K and V, autocast."""
+import pytest
+import torch
+from torch import nn
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def test_every_projections_bias_counts(gpu_device):
+    """A block whose Q, K or V has been given a bias: the stacked product's bias is the layers' biases, one after the other."""
+    from evoformer_triton_amd import evoformer_attention, fp8_linear
+    from evoformer_triton_amd.block import GatedAttentionBlock
+    for dt, gating, names in ((BF16, True, ("linear_k", "linear_v")), (F32, False, ("linear_q",)), (F16, False, ("linear_v",)), (F32, True, ("linear_q", "linear_k", "linear_v"))):
+        torch.manual_seed(5)
+        block = GatedAttentionBlock(64, 32, 2, gating=gating, fp8=True)
+        for name in names:
+            layer = nn.Linear(64, 64)
+            nn.init.normal_(layer.bias, 1.0)
+            setattr(block, name, layer)
+        block = block.to(gpu_device).to(dt)
+        m = torch.randn(1, 4, 40, 64, device=gpu_device).to(dt)
+        y = block(m)
+        grads = torch.autograd.grad(y, [getattr(block, n).bias for n in names], torch.randn_like(y))
+        assert all(g.shape == (64,) and g.any() for n, g in zip(names, grads) if n != "linear_k")      # (K's moves no softmax)
+        x = block.layer_norm_m(m)
+        with torch.no_grad():
+            one = lambda layer: fp8_linear(x, layer.weight, layer.bias).view(1, 4, 40, 2, 32)  # noqa: E731
+            o = evoformer_attention(one(block.linear_q), one(block.linear_k), one(block.linear_v), None, None, layout="ds4sci",
+                                    gate=one(block.linear_g) if gating else None)
+            want = fp8_linear(o.reshape(1, 4, 40, 64), block.linear_o.weight, block.linear_o.bias)
+            # (LayerNorm by torch and by the library, which may round a value to another neighbour and so to another number of 8 bits)
+            assert (y - want).float().norm() <= 3e-2 * want.float().norm()
+            assert torch.equal(block(m, weights=block.fp8_weights()), y)
