@@ -25,7 +25,8 @@ class Fp8Weight(NamedTuple):
     """A weight [n, k] in 8 bits, for inference.
 
     values   [n, k up to the next multiple of 128], dense, e4m3 (float8_e4m3fn or its bytes), zero beyond k
-    scales   [n, number of blocks up to the next multiple of 4], dense, a byte each (uint8 or float8_e8m0fnu): 127 + the block's exponent
+    scales   [n, number of blocks up to the next multiple of 4], dense, a byte each (uint8 or float8_e8m0fnu): 127 + the block's exponent;
+             255 is not a number, and neither are the values of its block
     k        columns of the weight
     """
     values: torch.Tensor
@@ -43,8 +44,10 @@ class Fp8Weight(NamedTuple):
         if self.values.dtype not in (torch.float8_e4m3fn, torch.uint8) or self.scales.dtype not in (torch.float8_e8m0fnu, torch.uint8):
             raise ValueError("a weight in 8 bits has values in float8_e4m3fn and scales in float8_e8m0fnu, or their bytes (uint8)")
         v = self.values.view(torch.float8_e4m3fn).float().unflatten(-1, (-1, 128))
-        e = self.scales.view(torch.uint8)[:, :v.shape[1]].int() - 127
-        return torch.ldexp(v, e.unsqueeze(-1)).flatten(-2)[:, :self.k]
+        e = self.scales.view(torch.uint8)[:, :v.shape[1]].int()
+        # (a power's bits, not torch.ldexp: its powers of two are off by a last bit on the GPU, here and there)
+        power = torch.where(e == 0, 0x400000, torch.where(e == 255, 0x7fc00000, e << 23)).int().view(torch.float32)
+        return (v * power.unsqueeze(-1)).flatten(-2)[:, :self.k]
 
 
 def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Optional[torch.Tensor] = None) -> torch.Tensor:
