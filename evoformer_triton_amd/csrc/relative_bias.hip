@@ -161,7 +161,8 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 // pairs x heads, on v_mfma_f32_16x16x32 (lane l, q = l / 16: operands' row or column l % 16, contraction 8q .. 8q + 7; accumulator column l % 16, rows
 // 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones as three bf16 parts, which hold all of their 24 bits.  A
 // product with one is exact, and sums are fp32 in a fixed order.  Zero times an infinity is no number: a workgroup that ends with a
-// sum that is not finite forms its sums again one by one, and so does one whose positions or chains lie some 2^30 (less 4096) or more from its first query's.
+// sum that is not finite forms its sums again one by one, and so does one whose positions lie some 2^30 (less 4096) or more from its first query's.
+// Chains are names: a query's is compared with those of the workgroup's keys, one to a lane, in all of their bits, and a lane takes its pairs' from the answer.
 // Bound by memory: 4 x 32 x 1024^2 in fp32 110 us (537 MB, 4.9 TB/s; with the loads alone 113 where this took 117), after the forward's results have been written
 // 141.  As many additions to sums in LDS: 681 us.  32 heads to a workgroup, whose buckets are then looked up once: 151 instead of 116.
 constexpr int kRbKeys = 64, kRbHeads = 16;   // a workgroup's keys and heads
@@ -210,7 +211,7 @@ __device__ __forceinline__ u16x2r rb_any_bits(u16x2r x) {
     return r;
 }
 
-// A position or chain less the workgroup's first, in 32 bits; false where that is not within 2^30 less the largest reach, so that a query's less a key's, and the reach
+// A position less the workgroup's first, in 32 bits; false where that is not within 2^30 less the largest reach, so that a query's less a key's, and the reach
 // on top of it, fit in 32 bits as well.
 __device__ __forceinline__ bool rb_from(int64_t p, int64_t base, int &d) {
     constexpr int64_t most = kRbNear - kRbMaxReach;
@@ -240,8 +241,8 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
     const bool whole = a.Nk >= 8, ragged = j0 + kRbKeys > a.Nk;
     const T *rows = dout + (((int64_t)b * a.H + min(h0 + li, a.H - 1)) * a.Nq) * a.Nk;
 
-    const int64_t p0 = qs[r0], c0 = CHAIN ? qc[r0] : 0;
-    int first[G], skip[G], pk[G][8], ck[CHAIN ? G : 1][8];
+    const int64_t p0 = qs[r0], chain = CHAIN ? kc[min(j0 + lane, a.Nk - 1)] : 0;   // of the lane's key of the 64
+    int first[G], skip[G], pk[G][8];
     bool near = true;
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -253,7 +254,6 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
             const int j = min(first[g] + e, a.Nk - 1);
             near = rb_from(ks[j], p0, pk[g][e]) && near;
             pk[g][e] -= a.reach;
-            if (CHAIN) near = rb_from(kc[j], c0, ck[g][e]) && near;
         }
     }
     for (int o = threadIdx.x; o <= 2 * a.reach + 1; o += kRbWaves * 64) lut[o] = o <= 2 * a.reach ? a.lut[o] : a.rows - 1;
@@ -264,13 +264,14 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
     for (int t = 0; t < TILES; ++t) acc[t] = sum[t] = f32x4r{0.0f, 0.0f, 0.0f, 0.0f};
     int steps = 0;
     Row next[U][G];
-    int pq[U], cq[U];
+    int pq[U];
+    int64_t cq[U];
     auto fetch = [&](int base) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = min(base + u * kRbWaves, r1 - 1);
             near = rb_from(qs[i], p0, pq[u]) && near;
-            if (CHAIN) near = rb_from(qc[i], c0, cq[u]) && near;
+            cq[u] = CHAIN ? qc[i] : 0;
             const T *p = rows + (int64_t)i * a.Nk;
 #pragma unroll
             for (int g = 0; g < G; ++g) {
@@ -294,11 +295,12 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
             }
         }
         Row now[U][G];
-        int pn[U], cn[U];
+        int pn[U];
+        int64_t cn[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             pn[u] = pq[u];
-            cn[u] = CHAIN ? cq[u] : 0;
+            cn[u] = cq[u];
 #pragma unroll
             for (int g = 0; g < G; ++g) now[u][g] = next[u][g];
         }
@@ -306,13 +308,17 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (base + u * kRbWaves >= r1) break;
+            const unsigned long long same = CHAIN ? __builtin_amdgcn_ballot_w64(chain == cn[u]) : 0;   // (the whole wave is here)
 #pragma unroll
             for (int g = 0; g < G; ++g) {
                 int o[8];
+                // (a piece that steps back may begin before the workgroup's first key, with keys that are another's)
+                const int at = first[g] - j0;
+                const unsigned mine = (unsigned)(same >> max(at, 0)) << max(-at, 0);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     o[e] = min(max(pn[u] - pk[g][e], 0), 2 * a.reach);
-                    if (CHAIN) o[e] = ck[g][e] == cn[u] ? o[e] : 2 * a.reach + 1;
+                    if (CHAIN) o[e] = mine >> e & 1 ? o[e] : 2 * a.reach + 1;
                 }
                 u16x2r bucket[4];
 #pragma unroll

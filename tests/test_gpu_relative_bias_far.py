@@ -30,3 +30,27 @@ def test_positions_within_a_workgroups_reach(gpu_device, index, far, reach):
     assert torch.equal(out[0, 0], table.detach()[bucket].permute(2, 0, 1))
     dout = torch.arange(1.0, 91, device=gpu_device).view(1, 1, 2, 5, 9)
     assert torch.equal(torch.autograd.grad(out, table, dout)[0].double(), _sums(bucket, dout, rows))
+
+
+@pytest.mark.parametrize("ids,index", [((0, 2 ** 40), torch.int64), ((-2 ** 63, 2 ** 63 - 1), torch.int64), ((5, 5 + 2 ** 32), torch.int64), ((-2 ** 31, 2 ** 31 - 1), torch.int32),
+                                       ((0, 2 ** 30), torch.int32), ((7, 7 + 2 ** 62), torch.int64)])
+@pytest.mark.parametrize("N,dt", [(37, F32), (200, BF16), (203, F16), (5, F32)])
+def test_chains_are_told_apart_by_any_numbers(gpu_device, ids, index, N, dt):
+    """A chain's number is a name: which one it is changes no bit."""
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    g = torch.Generator().manual_seed(N)
+    lut, at = relative_buckets(8).to(gpu_device), torch.arange(N, device=gpu_device).expand(2, N)
+    which = torch.randint(0, 2, (2, N), generator=g).to(gpu_device)
+    named = torch.where(which == 1, torch.tensor(ids[1], device=gpu_device), torch.tensor(ids[0], device=gpu_device)).to(index)
+    table = torch.randn((18, 3), generator=g).to(gpu_device).requires_grad_()
+    dout = torch.randn((2, 1, 3, N, N), generator=g).to(dt).to(gpu_device)
+    results = []
+    for chains in (which, named):
+        out = relative_position_bias(table, lut, at, chains=chains, dtype=dt)
+        results.append((out, torch.autograd.grad(out, table, dout)[0]))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    bucket = torch.where(which[:, :, None] == which[:, None, :], lut.long()[(at[:, :, None] - at[:, None, :]).clamp(-8, 8) + 8], 17)
+    want = _sums(bucket[0], dout[:1], 18) + _sums(bucket[1], dout[1:], 18)
+    size = _sums(bucket[0], dout[:1].abs(), 18) + _sums(bucket[1], dout[1:].abs(), 18)
+    # (each addition may lose half a step of what it has added up: of 203^2 pairs in sums of 64 keys, 203 rows, two batches and strips; a chain of 600 at most)
+    assert ((results[1][1].double() - want).abs() <= 600 * 2.0 ** -24 * size).all()
