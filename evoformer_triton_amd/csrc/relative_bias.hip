@@ -159,7 +159,8 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 
 // Backward: the sums of dout over the pairs of each bucket, as products: buckets x pairs (one where a pair is of the bucket, else zero) times
 // pairs x heads, on v_mfma_f32_16x16x32 (lane l, q = l / 16: operands' row or column l % 16, contraction 8q .. 8q + 7; accumulator column l % 16, rows
-// 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones as three bf16 parts, which hold all of their 24 bits.  A
+// 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones, 2^24 times as large, as three bf16 parts, which hold all of their
+// 24 bits (of one below 2^-110 as it is, the smaller parts run out of exponents: sums of gradients around 3e-36 were 1.6e-5 off).  A
 // product with one is exact, and sums are fp32 in a fixed order.  Zero times an infinity is no number: a workgroup that ends with a
 // sum that is not finite forms its sums again one by one, and so does one whose positions lie some 2^30 (less 4096) or more from its first query's.
 // Chains are names: a query's is compared with those of the workgroup's keys, one to a lane, in all of their bits, and a lane takes its pairs' from the answer.
@@ -180,6 +181,7 @@ struct RbRow {
     typedef typename std::conditional<sizeof(T) == 4, bf16_t, T>::type O;   // operands' type
     typedef typename Mfma<O>::v8 v8;
     static constexpr int PARTS = sizeof(T) == 4 ? 3 : 1;
+    static constexpr float UP = sizeof(T) == 4 ? 0x1p24f : 1.0f, DOWN = 1.0f / UP;   // what products are the sums' times
     static constexpr uint32_t ONE = std::is_same<O, f16_t>::value ? 0x3c00 : 0x3f80;
     T e[8];
     __device__ __forceinline__ void load(const T *p) { __builtin_memcpy(e, p, sizeof e); }
@@ -189,7 +191,7 @@ struct RbRow {
         } else {
             uint32_t x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(e[i]);
+            for (int i = 0; i < 8; ++i) x[i] = __float_as_uint(e[i] * UP);
 #pragma unroll
             for (int k = 0; k < 3; ++k) {   // the upper halves, then what they leave
                 u32x4r h;
@@ -346,7 +348,10 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
         }
     }
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) acc[t] += sum[t];
+    for (int t = 0; t < TILES; ++t) {
+        acc[t] += sum[t];
+        if (sizeof(T) == 4) acc[t] *= Row::DOWN;
+    }
     bool fine = near;
 #pragma unroll
     for (int t = 0; t < TILES; ++t)

@@ -54,3 +54,42 @@ def test_chains_are_told_apart_by_any_numbers(gpu_device, ids, index, N, dt):
     size = _sums(bucket[0], dout[:1].abs(), 18) + _sums(bucket[1], dout[1:].abs(), 18)
     # (each addition may lose half a step of what it has added up: of 203^2 pairs in sums of 64 keys, 203 rows, two batches and strips; a chain of 600 at most)
     assert ((results[1][1].double() - want).abs() <= 600 * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("exponent", [-100, -126, -133, -135, -140, -149])
+def test_small_gradients_keep_their_bits(gpu_device, exponent):
+    """Whole numbers of up to 8 bits in units down to fp32's smallest: their sums are exact."""
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    g = torch.Generator().manual_seed(4)
+    lut, at = relative_buckets(4).to(gpu_device), torch.arange(70, device=gpu_device)
+    whole = torch.randint(-127, 128, (1, 1, 2, 70, 70), generator=g).to(gpu_device)
+    dout = (whole.double() * 2.0 ** exponent).float()
+    assert torch.equal(dout.double() * 2.0 ** -exponent, whole.double())
+    table = torch.zeros(9, 2, device=gpu_device, requires_grad=True)
+    got, = torch.autograd.grad(relative_position_bias(table, lut, at), table, dout)
+    bucket = lut.long()[(at[:, None] - at[None]).clamp(-4, 4) + 4]
+    assert torch.equal(got.double() * 2.0 ** -exponent, _sums(bucket, whole, 9))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** 110, 2.0 ** 120])
+def test_large_gradients_are_no_infinities(gpu_device, size):
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    lut, at = relative_buckets(2).to(gpu_device), torch.arange(9, device=gpu_device)
+    whole = torch.randint(-3, 4, (1, 1, 2, 9, 9), generator=torch.Generator().manual_seed(4)).to(gpu_device)
+    table = torch.zeros(5, 2, device=gpu_device, requires_grad=True)
+    got, = torch.autograd.grad(relative_position_bias(table, lut, at), table, whole.float() * size)
+    bucket = lut.long()[(at[:, None] - at[None]).clamp(-2, 2) + 2]
+    assert torch.equal(got.double() / size, _sums(bucket, whole, 5))
+
+
+@pytest.mark.parametrize("size", [2.0 ** -126, 2.0 ** -118, 2.0 ** -110, 1.0, 2.0 ** 103, 2.0 ** 106, 2.0 ** 126])
+def test_a_gradient_of_one_pair_comes_out_as_it_went_in(gpu_device, size):
+    """Each bucket has one pair: all 24 bits of its gradient, from the smallest normal number to the largest."""
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    g = torch.Generator().manual_seed(7)
+    lut = relative_buckets(50).to(gpu_device)
+    q, k = torch.zeros(1, dtype=torch.int64, device=gpu_device), torch.arange(-50, 51, device=gpu_device)
+    dout = ((1 + torch.rand((1, 1, 5, 1, 101), generator=g)) * (torch.randint(0, 2, (1, 1, 5, 1, 101), generator=g) * 2 - 1)).to(gpu_device) * size
+    table = torch.zeros(101, 5, device=gpu_device, requires_grad=True)
+    got, = torch.autograd.grad(relative_position_bias(table, lut, q, k), table, dout)
+    assert torch.equal(got, dout[0, 0, :, 0].flip(1).t())
