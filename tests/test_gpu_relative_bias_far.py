@@ -93,3 +93,19 @@ def test_a_gradient_of_one_pair_comes_out_as_it_went_in(gpu_device, size):
     table = torch.zeros(101, 5, device=gpu_device, requires_grad=True)
     got, = torch.autograd.grad(relative_position_bias(table, lut, q, k), table, dout)
     assert torch.equal(got, dout[0, 0, :, 0].flip(1).t())
+
+
+def test_sums_beside_one_without_a_number_are_as_good(gpu_device):
+    """One infinity makes its workgroups form their sums one by one.  Of equal numbers the roundings of a single chain of additions all go the same way for long stretches; of sums
+    by rows they stay within what 64 keys, N rows and the workgroups' parts, one after the other, may lose."""
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    N = 2048
+    lut, at = relative_buckets(1).to(gpu_device), torch.arange(N, device=gpu_device)
+    table = torch.zeros(3, 16, device=gpu_device, requires_grad=True)
+    dout = torch.full((1, 1, 16, N, N), 0.1, device=gpu_device)
+    dout[0, 0, 0, ::16, ::16] = float("inf")
+    got, = torch.autograd.grad(relative_position_bias(table, lut, at), table, dout)
+    pairs = torch.tensor([N * (N - 1) // 2, N, N * (N - 1) // 2], dtype=torch.float64, device=gpu_device)
+    want = pairs * dout[0, 0, 1, 0, 0].double()
+    assert torch.isinf(got[:, 0]).all()
+    assert ((got[:, 1:].double() / want[:, None] - 1).abs() <= (64 + 256 + 32) * 2.0 ** -24).all(), (got[:, 1].double() / want - 1).abs()
