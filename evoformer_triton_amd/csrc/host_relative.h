@@ -50,7 +50,8 @@ struct RelativeBias {
         dtype = type ? *type : with ? bias->scalar_type() : table_.scalar_type();
         if (evo_dtype(dtype) == EVO_NONE) return "the result can be bf16, fp16 or fp32";
         if (with && bias->scalar_type() != dtype) return "the pair bias must have the result's dtype";
-        if (B > INT32_MAX || H > INT32_MAX || Nq > INT32_MAX || Nk > INT32_MAX) return "sizes beyond 2^31";
+        constexpr int64_t most = INT32_MAX - 1024;
+        if (B > INT32_MAX || H > INT32_MAX || Nq > most || Nk > most) return "2^31 batches or heads, or queries or keys within 1024 of it, are too many";
 
         table = table_.contiguous();
         lut = lut_.contiguous();

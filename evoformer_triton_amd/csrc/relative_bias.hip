@@ -13,6 +13,7 @@ namespace evo {
 
 constexpr int kRbWaves = 4;
 constexpr int kRbMaxReach = 4096, kRbMaxRows = 256;
+constexpr int kRbMost = INT32_MAX - 1024;      // queries, keys: what is counted up in steps of a workgroup's stays within 32 bits
 constexpr int64_t kRbNear = (int64_t)1 << 30;   // positions in (-2^30, 2^30): differences fit in 32 bits
 
 // V elements of T from any element's address on (global memory takes 16 bytes at any alignment).
@@ -104,7 +105,7 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
     }
     near = __all(near);
     __syncthreads();
-    const int r0 = chunk * a.chunk, r1 = min(r0 + a.chunk, a.Nq);
+    const int r0 = chunk * a.chunk, r1 = r0 + min(a.chunk, a.Nq - r0);
     const int64_t plane = ((int64_t)b * a.H + h) * a.Nq;
     const bool whole = a.Nk >= V;
     for (int base = r0 + wave * per * U; base < r1; base += kRbWaves * per * U) {
@@ -239,7 +240,7 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
     id /= a.chunks;
     const int b = id % a.B, h0 = id / a.B * kRbHeads, j0 = strip * kRbKeys;
     const RbIndex qs = a.queries(a.pos_q, b), ks = a.keys(a.pos_k, b), qc = a.queries(a.chain_q, b), kc = a.keys(a.chain_k, b);
-    const int r0 = chunk * a.chunk, r1 = min(r0 + a.chunk, a.Nq);
+    const int r0 = chunk * a.chunk, r1 = r0 + min(a.chunk, a.Nq - r0);
     const bool whole = a.Nk >= 8, ragged = j0 + kRbKeys > a.Nk;
     const T *rows = dout + (((int64_t)b * a.H + min(h0 + li, a.H - 1)) * a.Nq) * a.Nk;
 
@@ -461,7 +462,7 @@ static void rb_chunks(RbArgs &a, int64_t each, int step, int want) {
     chunk = (chunk + step - 1) / step * step;
     if (chunk > a.Nq) chunk = a.Nq;
     a.chunk = (int)chunk;
-    a.chunks = (a.Nq + a.chunk - 1) / a.chunk;
+    a.chunks = (int)((a.Nq + chunk - 1) / chunk);
 }
 
 static int rb_check(const EvoRelativeBias *p) {
@@ -471,6 +472,7 @@ static int rb_check(const EvoRelativeBias *p) {
     if (p->reach < 0 || p->rows < 1) return EVO_EINVAL;
     if (p->reach > kRbMaxReach || p->rows > kRbMaxRows) return EVO_EUNSUPPORTED;
     if (p->pos_q_stride_b < 0 || p->pos_k_stride_b < 0) return EVO_EINVAL;
+    if (p->Nq > kRbMost || p->Nk > kRbMost) return EVO_EOVERFLOW;
     const int64_t rows = (int64_t)p->B * p->H;
     if (rows > INT32_MAX || rows * p->Nq / p->Nq != rows || rows > INT64_MAX / 8 / p->Nq || rows * p->Nq > INT64_MAX / 8 / p->Nk) return EVO_EOVERFLOW;
     return EVO_OK;
@@ -531,6 +533,7 @@ static RbArgs rb_bwd_args(const EvoRelativeBias &p) {
     return a;
 }
 static int64_t rb_parts(const RbArgs &a) { return (int64_t)a.B * a.chunks * a.strips; }
+static bool rb_bwd_fits(const RbArgs &a) { return rb_parts(a) <= INT32_MAX / a.heads && (int64_t)a.rows * a.H <= INT32_MAX; }
 
 template <typename T, bool CHAIN>
 static int rb_launch_bwd(const RbArgs &a, unsigned grid, const T *dout, float *part, void *dtable, hipStream_t st) {
@@ -579,6 +582,7 @@ size_t evoattn_relative_bias_bwd_workspace_bytes(const EvoRelativeBias *p) {
     using namespace evo;
     if (rb_check(p)) return 0;
     const RbArgs a = rb_bwd_args(*p);
+    if (!rb_bwd_fits(a)) return 0;
     return (size_t)rb_parts(a) * p->rows * p->H * sizeof(float);
 }
 
@@ -590,7 +594,7 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream) {
     if (p->dtable) {
         const RbArgs a = rb_bwd_args(*p);
         const int64_t parts = rb_parts(a), grid = parts * a.heads, entries = (int64_t)a.rows * a.H;
-        if (grid > INT32_MAX || entries > INT32_MAX) return EVO_EOVERFLOW;
+        if (!rb_bwd_fits(a)) return EVO_EOVERFLOW;
         float *part = parts > 1 ? (float *)p->workspace : nullptr;
         if (parts > 1 && (!p->workspace || p->workspace_bytes < evoattn_relative_bias_bwd_workspace_bytes(p))) return EVO_EWORKSPACE;
         const int rc = rb_by_dtype(p->dtype, [&](auto t) {

@@ -297,7 +297,8 @@ int evoattn_pair_bias_bwd(const void *dbias, const void *z, const void *gamma, c
  * table [rows][H] and lut [2 reach + 1] dense; out, dout [B][H][Nq][Nk] dense, dpair [H][Nq][Nk].  pos_*, chain_* [B][N*], rows
  * pos_*_stride_b apart (0: shared by the batches), signed integers of pos_bytes (4 or 8) each, any values.  pair: key contiguous, any
  * strides.  chain_q and chain_k may both be NULL.  dtype (out, pair, dout, dpair) and table_dtype (table, dtable): EVO_BF16 / _F16 /
- * _F32.  Pointers on their elements' boundaries.  reach at most 4096, rows at most 256 (EVO_EUNSUPPORTED beyond).
+ * _F32.  Pointers on their elements' boundaries.  reach at most 4096, rows at most 256 (EVO_EUNSUPPORTED beyond);
+ * Nq and Nk at most 2^31 - 1025 (EVO_EOVERFLOW).
  * Nothing is allocated or synchronised. */
 typedef struct EvoRelativeBias {
     int32_t B, H, Nq, Nk;

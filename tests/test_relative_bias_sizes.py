@@ -1,0 +1,48 @@
+"""The relative position bias at the largest sizes that 32 bits count, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from evoformer_triton_amd import _lib, relative_buckets, relative_position_bias
+
+MOST = 2 ** 31 - 1 - 1024
+
+
+def _block(**change):
+    p = _lib.EvoRelativeBias()
+    p.B, p.H, p.Nq, p.Nk, p.rows, p.reach = 1, 1, 1, 1, 65, 32
+    p.dtype, p.table_dtype, p.pos_bytes = _lib.EVO_BF16, _lib.EVO_F32, 8
+    for f in ("table", "lut", "pos_q", "pos_k", "out", "dout", "dtable"):
+        setattr(p, f, 0x10000)
+    for k, v in change.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("which", ["Nq", "Nk"])
+def test_what_32_bits_do_not_count_is_refused(which):
+    lib = _lib.load()
+    for n in (MOST + 1, 2 ** 31 - 512, 2 ** 31 - 64, 2 ** 31 - 63, 2 ** 31 - 1):
+        p = ctypes.byref(_block(**{which: n}))
+        assert lib.evoattn_relative_bias_bwd_workspace_bytes(p) == 0
+        assert lib.evoattn_relative_bias_bwd(p, None) == lib.evoattn_relative_bias_fwd(p, None) == _lib.EVO_EOVERFLOW
+    many = ctypes.byref(_block(B=2 ** 15, H=2 ** 15, Nk=2 ** 22))             # (more workgroups than a launch has)
+    assert lib.evoattn_relative_bias_bwd_workspace_bytes(many) == 0 and lib.evoattn_relative_bias_bwd(many, None) == _lib.EVO_EOVERFLOW
+
+
+def test_the_largest_has_a_workspace_of_its_size():
+    lib = _lib.load()
+    one = 65 * 4                                                             # bytes of a sum
+    need = lib.evoattn_relative_bias_bwd_workspace_bytes(ctypes.byref(_block(Nk=MOST)))
+    assert need == -(-MOST // 64) * one                                      # one for each 64 keys of the row
+    need = lib.evoattn_relative_bias_bwd_workspace_bytes(ctypes.byref(_block(Nq=MOST)))
+    assert need % one == 0 and 256 <= need // one <= 512                     # rows in as many pieces as there are workgroups
+    assert lib.evoattn_relative_bias_bwd(ctypes.byref(_block(Nk=MOST)), None) == _lib.EVO_EWORKSPACE
+
+
+@pytest.mark.parametrize("positions,keys", [(MOST + 1, 1), (1, MOST + 1), (2 ** 31 + 5, 2)])
+def test_the_call_names_what_is_too_large(positions, keys):
+    at = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="too many"):
+        relative_position_bias(torch.zeros(5, 2), relative_buckets(2), at.expand(positions), at.expand(keys))
