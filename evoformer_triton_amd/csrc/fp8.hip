@@ -1207,6 +1207,7 @@ static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
 template <typename T, bool WIDE>
 static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
     if (q.strip) return f8_launch_strip<T, false>(a, st);
+    if (!grid_fits((int64_t)q.mt * q.nt * q.slices, 512)) return EVO_EOVERFLOW;
     const unsigned grid = (unsigned)(q.mt * q.nt * q.slices);
     if (q.big) {
         constexpr int lds = 4 * 512 * 64 + 2 * 512 * 4 + 256 * 4;
@@ -1276,7 +1277,9 @@ static F8FewPlan f8_few_plan(int64_t n, int64_t k) {
 }
 template <typename T, typename O>
 static int f8_launch_few(const F8Few &a, const F8FewPlan &q, hipStream_t st) {
-    const unsigned grid = (unsigned)((a.N + 16 * q.nt - 1) / (16 * q.nt) * q.slices), threads = 64 * (q.slice < kF8FewWaves ? q.slice : kF8FewWaves);
+    const int64_t groups = ((int64_t)a.N + 16 * q.nt - 1) / (16 * q.nt) * q.slices;
+    const unsigned grid = (unsigned)groups, threads = 64 * (q.slice < kF8FewWaves ? q.slice : kF8FewWaves);
+    if (!grid_fits(groups, (int)threads)) return EVO_EOVERFLOW;
     auto go = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         constexpr int MANY = sizeof(T) == 4 ? 1 : MT > 2 ? 2 : 4;
@@ -1292,7 +1295,7 @@ static int f8_launch_few(const F8Few &a, const F8FewPlan &q, hipStream_t st) {
 template <typename T>
 static int f8_add_slices(const EvoFp8Matmul &p, int slices, F8Sums c, hipStream_t st) {
     const int64_t pieces = p.m * ((p.n + 7) / 8), groups = (pieces + 255) / 256, more = c.part ? (c.cols + 31) / 32 : 0;
-    if (groups + more > INT32_MAX) return EVO_EOVERFLOW;
+    if (!grid_fits(groups + more, 256)) return EVO_EOVERFLOW;
     c.first = (unsigned)groups;
     fp8_slices<T><<<(unsigned)(groups + more), 256, 0, st>>>((const float *)p.workspace, (T *)p.out, p.bias, p.bias_dtype, p.m, (int)p.n, p.ldo, slices, c);
     return f8_rc();
@@ -1307,7 +1310,7 @@ int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void
     using namespace evo;
     if (const int rc = f8_rounding_check(x, ldx, q, scales, qt, scales_t, sums, rows, cols, dtype)) return rc;
     const F8Quantize p = f8_rounding(x, ldx, q, scales, qt, scales_t, sums, rows, cols);
-    if (p.tiles_r > INT32_MAX / p.tiles_k) return EVO_EOVERFLOW;
+    if (p.tiles_r > INT32_MAX / p.tiles_k || !grid_fits(p.tiles_r * p.tiles_k, 256)) return EVO_EOVERFLOW;
     const unsigned grid = (unsigned)(p.tiles_r * p.tiles_k);
     hipStream_t st = (hipStream_t)hip_stream;
     return f8_by_dtype(dtype, [&](auto t) {
@@ -1335,7 +1338,7 @@ int evoattn_fp8_quantize_two(const EvoFp8Rounding *a, const EvoFp8Rounding *b, i
         if (i == 0) both.first = (unsigned)(both.p[0].tiles_r * both.p[0].tiles_k);
         tiles += both.p[i].tiles_r * both.p[i].tiles_k;
     }
-    if (tiles > INT32_MAX) return EVO_EOVERFLOW;
+    if (!grid_fits(tiles, 256)) return EVO_EOVERFLOW;
     return f8_by_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
         if (tiles < kF8QuantizeFew) fp8_quantize_two<T, 2><<<(unsigned)tiles, 1024, 0, (hipStream_t)hip_stream>>>(both);

@@ -6,6 +6,10 @@
 
 namespace evo {
 
+// Whether a launch of so many workgroups takes place as a whole: one of 2^32 threads or more is cut off, without an error.
+inline bool grid_fits(int64_t groups, int threads) { return groups <= (int64_t)UINT32_MAX / threads; }
+
+
 int launch_generic_fwd(const EvoAttnParams &p, hipStream_t st);
 int launch_generic_bwd(const EvoAttnParams &p, const Extra &e, hipStream_t st);
 int launch_f32_fwd(const EvoAttnParams &p, hipStream_t st);

@@ -533,7 +533,7 @@ static RbArgs rb_bwd_args(const EvoRelativeBias &p) {
     return a;
 }
 static int64_t rb_parts(const RbArgs &a) { return (int64_t)a.B * a.chunks * a.strips; }
-static bool rb_bwd_fits(const RbArgs &a) { return rb_parts(a) <= INT32_MAX / a.heads && (int64_t)a.rows * a.H <= INT32_MAX; }
+static bool rb_bwd_fits(const RbArgs &a) { return grid_fits(rb_parts(a) * a.heads, kRbWaves * 64) && (int64_t)a.rows * a.H <= INT32_MAX; }
 
 template <typename T, bool CHAIN>
 static int rb_launch_bwd(const RbArgs &a, unsigned grid, const T *dout, float *part, void *dtable, hipStream_t st) {
@@ -564,7 +564,7 @@ int evoattn_relative_bias_fwd(const EvoRelativeBias *p, void *hip_stream) {
     if (p->pair && (p->pair_stride_row < 0 || p->pair_stride_h < 0 || p->pair_stride_b < 0)) return EVO_EINVAL;
     const RbArgs a = rb_fwd_args(*p);
     const int64_t grid = (int64_t)a.strips * a.chunks * a.H * a.B;
-    if (grid > INT32_MAX) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, kRbWaves * 64)) return EVO_EOVERFLOW;
     const size_t lds = (2 * (size_t)p->reach + 1) * sizeof(float);
     return rb_by_dtype(p->dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -591,10 +591,14 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream) {
     if (const int rc = rb_check(p)) return rc;
     if (!p->dout || (!p->dtable && !p->dpair)) return EVO_EINVAL;
     hipStream_t st = (hipStream_t)hip_stream;
+    // (before any launch)
+    const int64_t n = (int64_t)p->H * p->Nq * p->Nk;
+    const int v = p->dtype == EVO_F32 ? 4 : 8;
+    if (p->dpair && !grid_fits((n + 256 * v - 1) / (256 * v), 256)) return EVO_EOVERFLOW;
     if (p->dtable) {
         const RbArgs a = rb_bwd_args(*p);
-        const int64_t parts = rb_parts(a), grid = parts * a.heads, entries = (int64_t)a.rows * a.H;
         if (!rb_bwd_fits(a)) return EVO_EOVERFLOW;
+        const int64_t parts = rb_parts(a), grid = parts * a.heads, entries = (int64_t)a.rows * a.H;
         float *part = parts > 1 ? (float *)p->workspace : nullptr;
         if (parts > 1 && (!p->workspace || p->workspace_bytes < evoattn_relative_bias_bwd_workspace_bytes(p))) return EVO_EWORKSPACE;
         const int rc = rb_by_dtype(p->dtype, [&](auto t) {
@@ -609,11 +613,9 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream) {
         }
     }
     if (p->dpair) {
-        const int64_t n = (int64_t)p->H * p->Nq * p->Nk;
         return rb_by_dtype(p->dtype, [&](auto t) {
             typedef decltype(t) T;
             const int64_t groups = (n + 256 * RbVec<T>::V - 1) / (256 * RbVec<T>::V);
-            if (groups > INT32_MAX) return (int)EVO_EOVERFLOW;
             relative_bias_batch_sum<T><<<(unsigned)groups, 256, 0, st>>>((const T *)p->dout, (T *)p->dpair, n, p->B);
             return rb_rc();
         });

@@ -34,11 +34,12 @@ def test_what_32_bits_do_not_count_is_refused(which):
 def test_the_largest_has_a_workspace_of_its_size():
     lib = _lib.load()
     one = 65 * 4                                                             # bytes of a sum
-    need = lib.evoattn_relative_bias_bwd_workspace_bytes(ctypes.byref(_block(Nk=MOST)))
-    assert need == -(-MOST // 64) * one                                      # one for each 64 keys of the row
+    most = 64 * (2 ** 24 - 1)                                                # keys of as many workgroups as a launch has
+    need = lib.evoattn_relative_bias_bwd_workspace_bytes(ctypes.byref(_block(Nk=most)))
+    assert need == most // 64 * one                                          # one for each 64 keys of the row
     need = lib.evoattn_relative_bias_bwd_workspace_bytes(ctypes.byref(_block(Nq=MOST)))
     assert need % one == 0 and 256 <= need // one <= 512                     # rows in as many pieces as there are workgroups
-    assert lib.evoattn_relative_bias_bwd(ctypes.byref(_block(Nk=MOST)), None) == _lib.EVO_EWORKSPACE
+    assert lib.evoattn_relative_bias_bwd(ctypes.byref(_block(Nk=most)), None) == _lib.EVO_EWORKSPACE
 
 
 @pytest.mark.parametrize("positions,keys", [(MOST + 1, 1), (1, MOST + 1), (2 ** 31 + 5, 2)])
