@@ -742,6 +742,7 @@ __global__ void __launch_bounds__((64 * DBiasGeo<D, KT>::W), D <= 64 ? 2 : 1) f3
 template <int D, int W, bool BIAS>
 static int fwd_launch(const EvoAttnParams &p, int vec, hipStream_t st) {
     const unsigned grid = (unsigned)((p.N + 32 * W - 1) / (32 * W)) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, 64 * W)) return EVO_EOVERFLOW;
     f32_fwd<D, W, BIAS><<<grid, 64 * W, 0, st>>>(p, vec);
     EVO_LAUNCH_CHECK();
     return EVO_OK;
@@ -757,7 +758,9 @@ static int dbias_launch(const EvoAttnParams &p, const Extra &e, float *out, hipS
     if (R::BYTES > 64 * 1024)   // (more dynamic LDS than a launch may ask for unannounced)
         if (const int rc = ensure_dynamic_lds((const void *)&f32_dbias<D, KT, SPLITS, BIAS>, R::BYTES, done, nullptr)) return rc;
     const unsigned nb = (p.N + R::BLK - 1) / R::BLK;
-    f32_dbias<D, KT, SPLITS, BIAS><<<nb * nb * (unsigned)(p.B * p.H * e.n_chunks), 64 * R::W, R::BYTES, st>>>(p, e.delta, e.shift, out, e.chunk);
+    const int64_t groups = (int64_t)nb * nb * (p.B * p.H) * e.n_chunks;
+    if (!grid_fits(groups, 64 * R::W)) return EVO_EOVERFLOW;
+    f32_dbias<D, KT, SPLITS, BIAS><<<(unsigned)groups, 64 * R::W, R::BYTES, st>>>(p, e.delta, e.shift, out, e.chunk);
     EVO_LAUNCH_CHECK();
     return EVO_OK;
 }
@@ -765,6 +768,7 @@ static int dbias_launch(const EvoAttnParams &p, const Extra &e, float *out, hipS
 template <int D, int W, bool BIAS>
 static int bwd_launch(const EvoAttnParams &p, const Extra &e, int vec, hipStream_t st) {
     const unsigned grid = (unsigned)((p.N + 32 * W - 1) / (32 * W)) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, 64 * W)) return EVO_EOVERFLOW;
     f32_dq<D, W, BIAS><<<grid, 64 * W, 0, st>>>(p, vec, e.delta, e.shift, e.delta_given);
     EVO_LAUNCH_CHECK();
     Extra kv = e;

@@ -255,6 +255,7 @@ __global__ void __launch_bounds__(64) mask_shift_kernel(EvoAttnParams p, float *
 template <typename T, int D>
 static int gen_fwd_bias(const EvoAttnParams &p, hipStream_t st) {
     const unsigned nqb = (p.N + 63) / 64, grid = nqb * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, 64)) return EVO_EOVERFLOW;
     if (p.bias_dtype == EVO_NONE) gen_fwd<T, D, 0><<<grid, 64, 0, st>>>(p);
     else if (p.bias_dtype == EVO_F32) gen_fwd<T, D, 1><<<grid, 64, 0, st>>>(p);
     else gen_fwd<T, D, 2><<<grid, 64, 0, st>>>(p);
@@ -265,6 +266,8 @@ static int gen_fwd_bias(const EvoAttnParams &p, hipStream_t st) {
 template <typename T, int D, int BIASK>
 static int gen_bwd_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned P = (unsigned)(p.B * p.H * p.S), nb = (p.N + 63) / 64;
+    if (!grid_fits((int64_t)nb * P, 64)) return EVO_EOVERFLOW;
+    if (p.dbias && !grid_fits((int64_t)nb * (p.B * p.H) * p.N, 64)) return EVO_EOVERFLOW;
     gen_dq<T, D, BIASK><<<nb * P, 64, 0, st>>>(p, e.delta, e.shift);
     EVO_LAUNCH_CHECK();
     gen_dkdv<T, D, BIASK><<<nb * P, 64, 0, st>>>(p, e.delta, e.shift, p.dmask ? e.dmask_part : nullptr);
@@ -319,6 +322,7 @@ int launch_generic_fwd(const EvoAttnParams &p, hipStream_t st) {
 int launch_delta_generic(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const int64_t rows = (int64_t)p.B * p.H * p.S * p.N;
     const unsigned grid = (unsigned)((rows + 255) / 256);
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     switch (p.dtype) {
         case EVO_F32: gen_delta<float><<<grid, 256, 0, st>>>(p, e.delta); break;
         case EVO_BF16: gen_delta<bf16_t><<<grid, 256, 0, st>>>(p, e.delta); break;
@@ -432,6 +436,7 @@ int launch_gate_bwd(const EvoAttnParams &p, void *dout_ungated, float *delta, hi
 
 int launch_dmask_reduce(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const int64_t n = (int64_t)p.B * p.S * p.N;
+    if (!grid_fits((n + 255) / 256, 256)) return EVO_EOVERFLOW;
     dmask_reduce<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, e.dmask_part);
     EVO_LAUNCH_CHECK();
     return EVO_OK;
@@ -439,12 +444,14 @@ int launch_dmask_reduce(const EvoAttnParams &p, const Extra &e, hipStream_t st) 
 
 int launch_dbias_reduce(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const int64_t n = ((int64_t)p.B * p.H * p.N * p.N + 3) / 4;
+    if (!grid_fits((n + 255) / 256, 256)) return EVO_EOVERFLOW;
     dbias_reduce<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, e.dbias_part, e.n_chunks);
     EVO_LAUNCH_CHECK();
     return EVO_OK;
 }
 
 int launch_mask_shift(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
+    if (!grid_fits((int64_t)p.B * p.S, 64)) return EVO_EOVERFLOW;
     mask_shift_kernel<<<(unsigned)(p.B * p.S), 64, 0, st>>>(p, e.shift);
     EVO_LAUNCH_CHECK();
     return EVO_OK;

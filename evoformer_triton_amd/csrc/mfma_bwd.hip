@@ -653,6 +653,7 @@ template <typename T, int D, bool HAS_BIAS>
 static int dq_ntw(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const int NT = (p.N + 31) / 32;
     const unsigned grid = (unsigned)NT * (unsigned)(p.B * p.H) * (unsigned)e.n_chunks;
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     const int ntw = (NT + 3) / 4;
     if (ntw <= 2) mfma_dq<T, D, HAS_BIAS, 2><<<grid, 256, 0, st>>>(p, e);
     else if (ntw <= 4) mfma_dq<T, D, HAS_BIAS, 4><<<grid, 256, 0, st>>>(p, e);
@@ -675,6 +676,7 @@ int EVO_CAT(launch_mfma_dq_d, EVO_D)(const EvoAttnParams &p, const Extra &e, hip
 template <typename T, int D, int BT, int NW, int ROWS>
 static int dkdv_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned grid = (unsigned)((p.N + NW * 32 - 1) / (NW * 32)) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, NW * 64)) return EVO_EOVERFLOW;
     constexpr int lds = KvGeo<D>::lds_bytes(ROWS);   // at most 56 KB
     mfma_dkdv<T, D, BT, NW, ROWS><<<grid, NW * 64, lds, st>>>(p, e);
     return hip_rc();

@@ -328,6 +328,7 @@ static int fused_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) 
     typedef Fused<KT> R;
     const unsigned grid = (unsigned)mfma_fused_wgs(p), problems = (unsigned)((int64_t)p.B * p.H * p.S);
     const int nb = mfma_fused_blocks(p);
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     auto go = [&](auto kern, PerDevice &done) {
         if (const int rc = ensure_dynamic_lds((const void *)kern, R::BYTES, done, nullptr)) return rc;
         kern<<<grid, 256, R::BYTES, st>>>(p, e, problems, nb);

@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(256, 2) mfma_dbias(EvoAttnParams p, Extra e) {
 int launch_mfma_dbias_d16(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     typedef DbGeo R;
     const int64_t grid = (int64_t)((p.N + R::QB - 1) / R::QB) * ((p.N + R::KB - 1) / R::KB) * p.B * p.H * e.n_chunks;   // one per (query block, key block, batch, head, chunk)
-    if (grid <= 0 || grid > 0x7fffffff) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     const bool bf32 = p.bias_dtype == EVO_F32;
     if (p.dtype == EVO_BF16) {
         if (bf32) mfma_dbias<bf16_t, true><<<(unsigned)grid, 256, 0, st>>>(p, e);

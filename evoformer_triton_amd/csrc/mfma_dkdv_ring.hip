@@ -393,6 +393,7 @@ static int kvr_launch(const EvoAttnParams &p, const Extra &e0, hipStream_t st) {
     const int want = chunks_for_rounds(bh, p.S, cus, 0.0);
     e.chunk = (p.S + want - 1) / want;
     e.n_chunks = (p.S + e.chunk - 1) / e.chunk;
+    if (!grid_fits((int64_t)bh * e.n_chunks, 512)) return EVO_EOVERFLOW;
     kern<<<(unsigned)bh * (unsigned)e.n_chunks, 512, R::LDS_BYTES, st>>>(p, e);
     return hip_rc();
 }

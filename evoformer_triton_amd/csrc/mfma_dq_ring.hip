@@ -692,6 +692,7 @@ static int dqr_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     if (const int rc = ensure_dynamic_lds((const void *)kern, R::LDS_BYTES, done, nullptr)) return rc;
     const int NT = (p.N + 31) / 32, NQP = (NT + QT - 1) / QT;
     const unsigned grid = (unsigned)NQP * (unsigned)(p.B * p.H) * (unsigned)e.n_chunks;
+    if (!grid_fits(grid, 512)) return EVO_EOVERFLOW;
     kern<<<grid, 512, R::LDS_BYTES, st>>>(p, e);
     return hip_rc();
 }

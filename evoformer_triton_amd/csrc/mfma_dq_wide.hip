@@ -287,6 +287,7 @@ template <typename T, int D, int BT, bool WRITE_DS>
 static int dqw_waves(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const int nw = (p.flags & EVO_FLAG_DEBUG_OTHER_WIDTH) ? 8 : 4;
     const unsigned grid = (unsigned)((p.N + nw * 32 - 1) / (nw * 32)) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, nw * 64)) return EVO_EOVERFLOW;
     if (nw == 8) mfma_dq_wide<T, D, BT, 8, WRITE_DS><<<grid, 512, 0, st>>>(p, e);
     else mfma_dq_wide<T, D, BT, 4, WRITE_DS><<<grid, 256, 0, st>>>(p, e);
     return hip_rc();

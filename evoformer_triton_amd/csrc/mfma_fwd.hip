@@ -391,6 +391,7 @@ __global__ void __launch_bounds__(NW * 64, NW == 8 ? 4 : 3) mfma_fwd(EvoAttnPara
 template <typename T, int D, int NW>
 static int fwd_bias(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned nqb = (p.N + NW * 32 - 1) / (NW * 32), grid = nqb * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, NW * 64)) return EVO_EOVERFLOW;
     if (p.bias_dtype == EVO_NONE) mfma_fwd<T, D, 0, NW><<<grid, NW * 64, 0, st>>>(p, e);
     else if (e.bq16 && !e.bias_direct) mfma_fwd<T, D, 2, NW><<<grid, NW * 64, 0, st>>>(p, e);
     else mfma_fwd<T, D, 1, NW><<<grid, NW * 64, 0, st>>>(p, e);

@@ -680,6 +680,7 @@ static int fwdr_launch_g(const EvoAttnParams &p, const Extra &e0, hipStream_t st
     const int want = chunks_for_rounds(bh, p.S, cus, 0.0);
     e.chunk = (p.S + want - 1) / want;
     e.n_chunks = (p.S + e.chunk - 1) / e.chunk;
+    if (!grid_fits((int64_t)bh * e.n_chunks, 512)) return EVO_EOVERFLOW;
     kern<<<(unsigned)bh * (unsigned)e.n_chunks, 512, lds_bytes, st>>>(p, e);
     hipError_t err = hipGetLastError();
     return err == hipSuccess ? EVO_OK : EVO_EHIP - (int)err;

@@ -1428,11 +1428,13 @@ static int fwd_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
 #if EVO_D == 32
     if (mfma_fwd_pair_ok(p, e.bias_direct)) {
         const unsigned pairs = (unsigned)mfma_fwd_pairs(p);
+        if (!grid_fits(pairs, 256)) return EVO_EOVERFLOW;
         if (e.bq16) stream_fwd_pair<T, 2><<<pairs, 256, 0, st>>>(p, e);
         else stream_fwd_pair<T, 1><<<pairs, 256, 0, st>>>(p, e);
         return hip_rc();
     }
 #endif
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     if (p.bias_dtype == EVO_NONE) stream_fwd<T, D, 0><<<grid, 256, 0, st>>>(p, e);
     else if (e.bias_direct && p.bias_dtype == EVO_F32 && ragged_rows(p, e)) stream_fwd<T, D, D == 64 ? 5 : 3><<<grid, 256, 0, st>>>(p, e);
     else if (e.bias_direct && p.bias_dtype == EVO_F32) stream_fwd<T, D, 3><<<grid, 256, 0, st>>>(p, e);
@@ -1449,6 +1451,7 @@ int EVO_CAT(launch_mfma_fwd_d, EVO_D)(const EvoAttnParams &p, const Extra &e, hi
 template <typename T, int D>
 static int split_launch(const EvoAttnParams &p, hipStream_t st) {
     const unsigned grid = (unsigned)((p.N + 31) / 32) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     const int es = p.bias_dtype == EVO_F32 ? 4 : 2;
     const bool vec = p.N % 4 == 0 && ((uintptr_t)p.bias % (4 * es)) == 0 && p.bias_stride_b % 4 == 0 && p.bias_stride_h % 4 == 0 && p.bias_stride_row % 4 == 0;
     auto go = [&](auto kern, PerDevice &done) {
@@ -1470,6 +1473,7 @@ int EVO_CAT(launch_split_fwd_d, EVO_D)(const EvoAttnParams &p, hipStream_t st) {
 template <typename T, int D>
 static int dq_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned grid = (unsigned)((p.N + 127) / 128) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     const bool f32_rows = e.bias_direct && p.bias_dtype == EVO_F32, t16_rows = e.bias_direct && !f32_rows, t16 = e.bq16 != nullptr;
     if (p.dbias && p.S != 1) return EVO_EUNSUPPORTED;   // (a sum over S rows is the other kernels' business)
     if (p.bias_dtype == EVO_NONE) stream_dq<T, D, 0, false><<<grid, 256, 0, st>>>(p, e);
@@ -1493,6 +1497,7 @@ int EVO_CAT(launch_mfma_dqw_d, EVO_D)(const EvoAttnParams &p, const Extra &e, hi
 template <typename T, int D, int BT, int NW>
 static int dkdv_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned grid = (unsigned)((p.N + NW * 32 - 1) / (NW * 32)) * (unsigned)(p.B * p.H * p.S);
+    if (!grid_fits(grid, NW * 64)) return EVO_EOVERFLOW;
     constexpr int lds = KvStream<D, NW>::BYTES;
     auto kern = stream_dkdv<T, D, BT, NW, false>;
     if constexpr (D == 64) {
@@ -1526,6 +1531,7 @@ static int dkdv_waves(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
 template <typename T>
 static int bwd_one_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned grid = 2 * (unsigned)((p.N + 127) / 128) * (unsigned)(p.B * p.H);
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     auto go = [&](auto kern) {
         constexpr int lds = KvStream<64, 4>::BYTES;
         static_assert(lds >= 2 * FwdStream<64>::BYTES + 4 * kDsBytes && lds <= 64 * 1024, "the larger of the two");
@@ -1554,7 +1560,7 @@ template <typename T, int D, bool BF32>
 static int dbias_launch(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     typedef DbStream<D> R;
     const int64_t grid = (int64_t)((p.N + R::QB - 1) / R::QB) * ((p.N + R::KB - 1) / R::KB) * p.B * p.H * e.n_chunks;
-    if (grid <= 0 || grid > 0x7fffffff) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     static PerDevice done{};
     if (const int rc = ensure_dynamic_lds((const void *)&stream_dbias<T, D, BF32>, R::BYTES, done, nullptr)) return rc;
     stream_dbias<T, D, BF32><<<(unsigned)grid, 256, R::BYTES, st>>>(p, e);

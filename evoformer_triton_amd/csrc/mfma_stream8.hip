@@ -330,6 +330,7 @@ __global__ void __launch_bounds__(256, 3) stream_fwd8(EvoAttnParams p, Extra e) 
 
 int launch_stream_fwd8(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned pairs = (unsigned)((p.N + 127) / 128) * (unsigned)(p.B * p.H) * (unsigned)((p.S + 1) / 2);
+    if (!grid_fits(pairs, 256)) return EVO_EOVERFLOW;
     const bool h = p.dtype == EVO_BF16;
     if (e.bq16) h ? stream_fwd8<bf16_t, 2><<<pairs, 256, 0, st>>>(p, e) : stream_fwd8<f16_t, 2><<<pairs, 256, 0, st>>>(p, e);
     else h ? stream_fwd8<bf16_t, 1><<<pairs, 256, 0, st>>>(p, e) : stream_fwd8<f16_t, 1><<<pairs, 256, 0, st>>>(p, e);
@@ -482,7 +483,7 @@ __global__ void __launch_bounds__(256, 2) stream_dbias8(EvoAttnParams p, Extra e
 int launch_mfma_dbias_d8(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     typedef Db8 R;
     const int64_t grid = (int64_t)((p.N + R::QB - 1) / R::QB) * ((p.N + R::KB - 1) / R::KB) * p.B * p.H * e.n_chunks;
-    if (grid <= 0 || grid > 0x7fffffff) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
     const bool f = p.bias_dtype == EVO_F32;
     if (p.dtype == EVO_BF16) {
         if (f) stream_dbias8<bf16_t, true><<<(unsigned)grid, 256, 0, st>>>(p, e);

@@ -204,6 +204,7 @@ int launch_prep(const EvoAttnParams &p, const Extra &e, hipStream_t st) {
     const unsigned NS = (NT + kPrepStrip - 1) / kPrepStrip;
     const unsigned nb = p.bias && !e.bias_direct ? (unsigned)e.bias_batches * p.H * NT * NS + 1u : 0u;
     const unsigned nm = (unsigned)(p.B * p.S);
+    if (!grid_fits((int64_t)nb + nm, 256)) return EVO_EOVERFLOW;
     prep_kernel<<<nb + nm, 256, 0, st>>>(p, e, nb);
     hipError_t err = hipGetLastError();
     return err == hipSuccess ? EVO_OK : EVO_EHIP - (int)err;
