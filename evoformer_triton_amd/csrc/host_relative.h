@@ -30,6 +30,8 @@ struct RelativeBias {
             if (!all[i]) continue;
             const Tensor &t = *all[i];
             if (!at::isIntegralType(t.scalar_type(), false)) return "positions and chains must be whole numbers";
+            // (chains are names, and stay different ones as int64)
+            if (i < 4 && t.scalar_type() == at::kUInt64) return "positions must be whole numbers that int64 holds, not uint64";
             if (t.dim() != 1 && t.dim() != 2) return "positions and chains must be [N] or [B, N]";
             if (t.dim() == 2 && t.size(0) != 1) {
                 if (B != 1 && t.size(0) != B) return "the batches of positions, chains and pair bias do not agree";

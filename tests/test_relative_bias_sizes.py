@@ -47,3 +47,16 @@ def test_the_call_names_what_is_too_large(positions, keys):
     at = torch.zeros(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="too many"):
         relative_position_bias(torch.zeros(5, 2), relative_buckets(2), at.expand(positions), at.expand(keys))
+
+
+@pytest.mark.parametrize("keys", [False, True])
+def test_positions_that_int64_does_not_hold_are_refused(keys):
+    """As int64, 2^63 would be the number farthest below zero."""
+    at, far = torch.zeros(3, dtype=torch.int64), torch.zeros(3, dtype=torch.uint64)
+    with pytest.raises(ValueError, match="uint64"):
+        relative_position_bias(torch.zeros(5, 2), relative_buckets(2), *((at, far) if keys else (far, at)))
+    for dtype in (torch.uint8, torch.int8, torch.uint16, torch.int16, torch.uint32, torch.int32):
+        with pytest.raises(RuntimeError, match="GPU only"):
+            relative_position_bias(torch.zeros(5, 2), relative_buckets(2), torch.zeros(3, dtype=dtype), at)
+    with pytest.raises(RuntimeError, match="GPU only"):
+        relative_position_bias(torch.zeros(5, 2), relative_buckets(2), at, at, chains=far, key_chains=far)
