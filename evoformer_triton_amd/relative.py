@@ -162,10 +162,14 @@ class RelativePositionBias(nn.Module):
     def plain(self, positions: torch.Tensor, *, chains: Optional[torch.Tensor] = None, pair_bias: Optional[torch.Tensor] = None,
               dtype: Optional[torch.dtype] = None):
         """The bias of residues among themselves in plain torch operations, on any device: what the kernel is tested against."""
-        at, reach = positions if positions.dim() == 2 else positions[None], self.buckets.numel() // 2
-        bucket = self.buckets.long()[(at[:, :, None] - at[:, None, :]).clamp(-reach, reach) + reach]
+        at, reach = (positions if positions.dim() == 2 else positions[None]).long(), self.buckets.numel() // 2
+        q, k = at[:, :, None], at[:, None, :]
+        d = q - k
+        # (a difference that int64 does not hold is far; its sign is the query's)
+        far = ((q ^ k) & (q ^ d)) < 0
+        bucket = self.buckets.long()[torch.where(far, torch.where(q < 0, -reach, reach), d.clamp(-reach, reach)) + reach]
         if chains is not None:
-            c = chains if chains.dim() == 2 else chains[None]
+            c = (chains if chains.dim() == 2 else chains[None]).long()
             bucket = torch.where(c[:, :, None] == c[:, None, :], bucket, self.weight.shape[0] - 1)
         out = self.weight.float()[bucket].permute(0, 3, 1, 2).unsqueeze(1)
         if pair_bias is not None:

@@ -109,3 +109,20 @@ def test_sums_beside_one_without_a_number_are_as_good(gpu_device):
     want = pairs * dout[0, 0, 1, 0, 0].double()
     assert torch.isinf(got[:, 0]).all()
     assert ((got[:, 1:].double() / want[:, None] - 1).abs() <= (64 + 256 + 32) * 2.0 ** -24).all(), (got[:, 1].double() / want - 1).abs()
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.uint32, torch.int32, torch.int64], ids=str)
+def test_positions_of_any_whole_type(gpu_device, dtype):
+    from evoformer_triton_amd import RelativePositionBias
+    bias = RelativePositionBias(2, 20, other_chain=True).to(gpu_device)
+    bias.weight.data.normal_()
+    i = torch.iinfo(dtype)
+    values = [0, 1, 5, 100, i.max, i.max - 3] + ([i.min, i.min + 2, -1] if i.min else [])
+    at = torch.tensor(values, dtype=dtype, device=gpu_device)
+    d = torch.tensor([[max(-20, min(20, a - b)) + 20 for b in values] for a in values], device=gpu_device)
+    chains = torch.tensor([2 ** 64 - 1 if k % 2 else 3 for k in range(len(values))], dtype=torch.uint64, device=gpu_device)
+    same = torch.tensor([[(a - b) % 2 == 0 for b in range(len(values))] for a in range(len(values))], device=gpu_device)
+    for given in (None, chains):
+        want = bias.weight[d if given is None else torch.where(same, d, 41)].permute(2, 0, 1)
+        assert torch.equal(bias(at, chains=given)[0, 0], want)
+        assert torch.equal(bias.plain(at, chains=given)[0, 0], want)

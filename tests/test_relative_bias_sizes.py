@@ -60,3 +60,15 @@ def test_positions_that_int64_does_not_hold_are_refused(keys):
             relative_position_bias(torch.zeros(5, 2), relative_buckets(2), torch.zeros(3, dtype=dtype), at)
     with pytest.raises(RuntimeError, match="GPU only"):
         relative_position_bias(torch.zeros(5, 2), relative_buckets(2), at, at, chains=far, key_chains=far)
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64], ids=str)
+def test_the_bias_in_plain_operations_takes_any_whole_type(dtype):
+    """Differences of a byte, or of 64 bits, that their type does not hold."""
+    from evoformer_triton_amd import RelativePositionBias
+    bias = RelativePositionBias(1, 3)
+    bias.weight.data.copy_(torch.arange(7.0).view(7, 1))
+    i = torch.iinfo(dtype)
+    values = [0, 2, 100, i.max, i.max - 1, i.min]
+    want = [[max(-3, min(3, a - b)) + 3.0 for b in values] for a in values]
+    assert bias.plain(torch.tensor(values, dtype=dtype))[0, 0, 0].tolist() == want
