@@ -193,7 +193,7 @@ OptTensor relative_bias(const Tensor &table, const Tensor &lut, const Tensor &q,
         node->p = r.p;
         node->table_type = table.scalar_type();
         node->dtype = r.dtype;
-        node->shared_pair = r.pair.defined() && r.pair.size(0) == 1 && r.p.B > 1;
+        node->shared_pair = r.pair.defined() && r.pair.size(0) == 1 && r.p.B != 1;
         torch::autograd::set_history(out, node);
         for (const Tensor *t : {&r.lut, &r.pos_q, &r.pos_k, &r.chain_q, &r.chain_k}) node->save(*t);
     }
@@ -218,10 +218,10 @@ std::pair<Tensor, Tensor> relative_bias_backward(const Tensor &dout, const Tenso
     r.table_type = table.scalar_type();
     TORCH_CHECK_VALUE(dout.device() == table.device() && dout.dim() == 5 && dout.size(0) == r.p.B && dout.size(1) == 1 && dout.size(2) == r.p.H &&
                           dout.size(3) == r.p.Nq && dout.size(4) == r.p.Nk, "the gradient must have the result's shape and device");
-    const bool shared = r.pair.defined() && r.pair.size(0) == 1 && r.p.B > 1;
+    const bool shared = r.pair.defined() && r.pair.size(0) == 1 && r.p.B != 1;
     Tensor dtable, dpair;
     if (need_table || (need_pair && shared)) r.backward(dout.contiguous(), need_table, need_pair && shared, dtable, dpair);
-    if (need_pair && !shared) dpair = dout.clone();
+    if (need_pair && !shared) dpair = dout.clone(at::MemoryFormat::Contiguous);   // (as the tracer has been told, not with dout's strides)
     const Tensor none = at::empty({0}, dout.options());
     return {dtable.defined() ? dtable : none, dpair.defined() ? dpair : at::empty({0}, dout.options())};
 }

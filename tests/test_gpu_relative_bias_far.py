@@ -126,3 +126,21 @@ def test_positions_of_any_whole_type(gpu_device, dtype):
         want = bias.weight[d if given is None else torch.where(same, d, 41)].permute(2, 0, 1)
         assert torch.equal(bias(at, chains=given)[0, 0], want)
         assert torch.equal(bias.plain(at, chains=given)[0, 0], want)
+
+
+def test_the_registered_backward_gives_what_is_traced(gpu_device):
+    """Shapes and strides of the gradients are those that the compiler has been told, also for a gradient that comes with strides of its own or without a batch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from evoformer_triton_amd import relative_buckets
+    lut, at = relative_buckets(4), torch.arange(24)
+    table = torch.zeros(9, 2)
+    for B, pair_b, crossed in ((1, 1, True), (2, 2, True), (2, 1, True), (2, 1, False), (0, 1, False), (0, 0, False)):
+        dout = torch.randn(B, 1, 2, 24, 24)
+        dout = dout.transpose(3, 4) if crossed else dout
+        args = (dout, table, lut, at.expand(B, 24), at, None, None, torch.zeros(pair_b, 1, 2, 24, 24))
+        real = [t if t is None else t.to(gpu_device) for t in args]
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+            told = torch.ops.evoattn.relative_bias_bwd(*(t if t is None else mode.from_tensor(t) for t in real), True, True)
+        got = torch.ops.evoattn.relative_bias_bwd(*real, True, True)
+        assert [(t.shape, t.stride(), t.dtype) for t in got] == [(t.shape, t.stride(), t.dtype) for t in told], (B, pair_b, crossed)
+        assert torch.equal(got[1], real[0] if pair_b == B else real[0].sum(0, keepdim=True)), (B, pair_b, crossed)
