@@ -288,21 +288,21 @@ std::vector<Tensor> fp8_linear_backward(const Tensor &dy, const Tensor &x, const
                       "the gradient must have the result's shape, dtype and device");
     need_b = need_b && bias && bias->defined();
     c10::DeviceGuard on(x.device());
-    Tensor dx = need_x ? at::zeros_like(x, at::MemoryFormat::Contiguous) : at::empty({0}, x.options()),
-           dw = need_w ? at::zeros_like(weight, at::MemoryFormat::Contiguous) : at::empty({0}, weight.options()),
-           db = need_b ? at::zeros({n}, bias->options()) : at::empty({0}, x.options());
+    Tensor dx, dw, db;
     if (dy.numel() && k && (need_x || need_w || need_b)) {
         F8Saved s;
-        Tensor a, b, c;
         if (need_w) f8_quantize(f8_rows(x), nullptr, &s.xt, nullptr);
         if (need_x) f8_quantize(f8_rows(weight), nullptr, &s.wt, nullptr);
-        f8_backward(f8_rows(dy), s, need_x, need_w, need_b, weight.scalar_type(), need_b ? bias->scalar_type() : at::kFloat, a, b, c);
-        if (need_x) dx = a.view(x.sizes());
-        if (need_w) dw = b;
-        if (need_b) db = c;
-    } else if (dy.numel() && need_b) {
-        db = as_rows(dy).sum(0).to(bias->scalar_type());
+        f8_backward(f8_rows(dy), s, need_x, need_w, need_b, weight.scalar_type(), need_b ? bias->scalar_type() : at::kFloat, dx, dw, db);
+        if (need_x) dx = dx.view(x.sizes());
+    } else {
+        if (need_x) dx = at::zeros(x.sizes(), x.options());
+        if (need_w) dw = at::zeros({n, k}, weight.options());
+        if (need_b) db = dy.numel() ? as_rows(dy).sum(0).to(bias->scalar_type()) : at::zeros({n}, bias->options());
     }
+    if (!need_x) dx = at::empty({0}, x.options());
+    if (!need_w) dw = at::empty({0}, weight.options());
+    if (!need_b) db = at::empty({0}, x.options());
     return {dx, dw, db};
 }
 Tensor fp8_linear_held_forward(const Tensor &x, const Tensor &values, const Tensor &scales, int64_t k, const OptTensor &bias) {

@@ -27,3 +27,22 @@ def test_a_scale_that_is_no_number(gpu_device, rows, k, n, dt):
     with torch.no_grad():
         bad = fp8_linear(torch.zeros(rows, k, device=gpu_device, dtype=dt), w).isnan()
     assert bad[:, 3].all() and bad.sum() == rows
+
+
+@pytest.mark.parametrize("rows", [3000, 9000])
+def test_the_registered_backward_fills_no_memory_twice(gpu_device, rows):
+    """What a compiled or watched step calls takes the gradients' memory once."""
+    import evoformer_triton_amd  # noqa: F401
+    k, n = 1024, 768
+    x, w, b, dy = (torch.randn(s, device=gpu_device).to(torch.bfloat16) for s in ((rows, k), (n, k), (n,), (rows, n)))
+    torch.ops.evoattn.fp8_linear_bwd(dy, x, w, b, True, False, False)
+
+    def taken(need_x):
+        before = torch.cuda.memory_stats()["allocated_bytes.all.allocated"]
+        grads = torch.ops.evoattn.fp8_linear_bwd(dy, x, w, b, need_x, False, False)
+        return torch.cuda.memory_stats()["allocated_bytes.all.allocated"] - before, grads[0]
+
+    total, dx = taken(True)
+    up = lambda v: -(-v // 128) * 128  # noqa: E731
+    rounded = k * up(n) + rows * up(n) + 16 * (k + rows)                     # w^T and dy along their rows, with scales
+    assert dx.shape == x.shape and total < rounded + dx.numel() * 2 * 1.5      # (bytes: less than twice dx's; the product is not cut into slices)
