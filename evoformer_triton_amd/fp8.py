@@ -21,6 +21,9 @@ import torch
 from . import _lib
 
 
+_AUTOCAST = (torch.float32, torch.bfloat16, torch.float16)
+
+
 class Fp8Weight(NamedTuple):
     """A weight [n, k] in 8 bits, for inference.
 
@@ -59,12 +62,15 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
     bias     [n], bf16, fp16 or fp32, added in fp32
 
     Gradients come in the dtype of what they belong to.  A result or weight gradient in fp32 is summed in fp32 throughout; towards
-    16 bits the 8-bit matrix instructions form the sums, to about 1.4e-5 of the result.  Rows, n and k up to 2^26.  Runs on the current
+    16 bits the 8-bit matrix instructions form the sums, to about 1.4e-5 of the result.  Under autocast the input, and so the result, are
+    of its type, as a Linear's; weight and bias stay as they are.  Rows, n and k up to 2^26.  Runs on the current
     stream of the tensors' device; GPU only."""
     held = isinstance(weight, Fp8Weight)
     for name, t in (("x", x), ("bias", bias)) + ((("weight.values", weight.values), ("weight.scales", weight.scales)) if held else (("weight", weight),)):
         if not isinstance(t, torch.Tensor) and not (t is None and name == "bias"):
             raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    if torch.is_autocast_enabled("cuda") and x.is_cuda and x.dtype in _AUTOCAST:
+        x = x.to(torch.get_autocast_dtype("cuda"))
     if torch.compiler.is_compiling():
         if held:
             return torch.ops.evoattn.fp8_linear_held(x, weight.values, weight.scales, weight.k, bias)

@@ -33,3 +33,28 @@ def test_every_projections_bias_counts(gpu_device):
             # (LayerNorm by torch and by the library, which may round a value to another neighbour and so to another number of 8 bits)
             assert (y - want).float().norm() <= 3e-2 * want.float().norm()
             assert torch.equal(block(m, weights=block.fp8_weights()), y)
+
+
+def test_autocast_takes_8_bit_layers_to_its_type(gpu_device):
+    """As torch's Linear: the input in autocast's type, and so the result; parameters and their gradients keep theirs."""
+    from evoformer_triton_amd import Fp8Weight, fp8_linear
+    x, w, b = (torch.randn(s, device=gpu_device) for s in ((100, 256), (64, 256), (64,)))
+    dy = torch.randn(100, 64, device=gpu_device)
+    for to in (BF16, F16):
+        for t in (F32, BF16, F16):
+            leaves = [v.clone().to(t if v is x else F32).requires_grad_() for v in (x, w, b)]
+            with torch.autocast("cuda", to):
+                y = fp8_linear(*leaves)
+                with torch.no_grad():
+                    held = fp8_linear(leaves[0], Fp8Weight.of(w), b)
+                compiled = torch.compile(fp8_linear, fullgraph=True, backend="aot_eager")(*leaves)
+            want_leaves = [leaves[0].detach().to(to).requires_grad_(), *leaves[1:]]
+            want = fp8_linear(*want_leaves)
+            assert y.dtype == to and all(torch.equal(a, want) for a in (y, held, compiled))
+            grads = torch.autograd.grad(y, leaves, dy.to(to))
+            want_grads = torch.autograd.grad(want, want_leaves, dy.to(to))
+            assert [g.dtype for g in grads] == [t, F32, F32] and all(torch.equal(a, c.to(a.dtype)) for a, c in zip(grads, want_grads))
+    with torch.autocast("cuda", BF16, enabled=False):
+        assert fp8_linear(x, w, b).dtype == F32
+    with torch.autocast("cpu", BF16):
+        assert fp8_linear(x, w, b).dtype == F32
