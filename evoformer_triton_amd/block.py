@@ -134,7 +134,17 @@ class _Linear(torch.autograd.Function):
         return dx, dw, db
 
 
+def _recast(layer: nn.Linear, x: torch.Tensor) -> bool:
+    """Whether autocast takes the input or the layer's weight to another type: the layer is torch's then, whose backward knows of it."""
+    if not torch.is_autocast_enabled("cuda") or not x.is_cuda:
+        return False
+    to = torch.get_autocast_dtype("cuda")
+    return x.dtype != to or layer.weight.dtype != to
+
+
 def _linear(layer: nn.Linear, x: torch.Tensor, dx_place: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if _recast(layer, x):
+        return layer(x)
     # (the same in C++)
     y = None if torch.compiler.is_compiling() else _lib.host().linear(x, layer.weight, layer.bias, dx_place)
     return _Linear.apply(x, layer.weight, layer.bias) if y is None else y
@@ -261,7 +271,7 @@ class GatedAttentionBlock(nn.Module):
         lin = (lambda layer, t: layer(t)) if plain else _linear
         x = norm(self.layer_norm_m, m)
         layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
-        if plain:
+        if plain or (not self.fp8 and any(_recast(layer, x) for layer in layers)):
             outs = [layer(x) for layer in layers]
         elif self.fp8:
             outs = self._project(x, weights).unflatten(-1, (len(layers), H * D)).unbind(-2)
@@ -311,6 +321,8 @@ class GatedAttentionBlock(nn.Module):
         """Whether Q, K, V and the gate can come from one GEMM and reach the kernels as slots of its result."""
         if not m.is_cuda or m.dtype not in (torch.bfloat16, torch.float16) or m.numel() == 0 or torch.compiler.is_compiling() \
                 or torch.jit.is_tracing() or self.c_hidden not in _HEAD_DIMS:
+            return False
+        if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") != m.dtype:
             return False
         mods = self._modules
         layers = [mods["linear_q"], mods["linear_k"], mods["linear_v"], mods["linear_o"]] + ([mods["linear_g"]] if mods.get("linear_g") is not None else [])

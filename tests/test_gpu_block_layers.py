@@ -58,3 +58,30 @@ def test_autocast_takes_8_bit_layers_to_its_type(gpu_device):
         assert fp8_linear(x, w, b).dtype == F32
     with torch.autocast("cpu", BF16):
         assert fp8_linear(x, w, b).dtype == F32
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("c_z,relative", [(None, None), (32, None), (32, 8)])
+def test_a_block_in_fp32_under_autocast(gpu_device, fp8, c_z, relative):
+    """Projections and attention in autocast's type, gradients in the parameters': what the same layers of torch give, to that type's roundings."""
+    from evoformer_triton_amd.block import GatedAttentionBlock
+    torch.manual_seed(3)
+    block = GatedAttentionBlock(64, 32, 2, c_z=c_z, fp8=fp8, relative_distance=relative).to(gpu_device)
+    if relative is not None:
+        block.relative.weight.data.normal_()
+    m = torch.randn(1, 6, 40, 64, device=gpu_device, requires_grad=True)
+    z = torch.randn(1, 40, 40, c_z, device=gpu_device, requires_grad=True) if c_z else None
+    at = {"positions": torch.arange(40, device=gpu_device)} if relative else {}
+    dout = torch.randn(1, 6, 40, 64, device=gpu_device)
+    leaves = [m] + ([z] if c_z else []) + [p for n, p in block.named_parameters() if n != "layer_norm_z.bias"]     # (which moves no softmax)
+    with torch.autocast("cuda", BF16):
+        y = block(m, z, None, **at)
+        assert y.dtype == BF16 and all(t.dtype == BF16 for t in block.operands(m, z, None, **at)[:4])
+    grads = torch.autograd.grad(y, leaves, dout.to(BF16))
+    want = block.forward_eager(m, z, None, **at)
+    want_grads = torch.autograd.grad(want, leaves, dout)
+    assert [g.dtype for g in grads] == [F32] * len(grads)
+    # a few parts in a hundred in 8 bits (operands within 2^-4 of themselves), of bf16's in 16
+    assert (y - want).norm() <= (0.15 if fp8 else 2e-2) * want.norm()
+    for a, b in zip(grads, want_grads):
+        assert torch.isfinite(a).all() and (a - b).norm() <= (0.4 if fp8 else 5e-2) * b.norm() + 1e-3 * b.numel() ** 0.5
