@@ -161,8 +161,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_pair_bias_bwd.restype = ctypes.c_int
     lib.evoattn_pair_bias_bwd.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, i64, i64, i32, i32, i32, vp]
     RB = ctypes.POINTER(EvoRelativeBias)
-    for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd",
-           "evoattn_fp8_quantize", "evoattn_fp8_quantize_two", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_sums", "evoattn_fp8_matmul_rounds", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding"):
+    for name in ("evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd"):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = [RB, vp]
     lib.evoattn_relative_bias_bwd_workspace_bytes.restype = ctypes.c_size_t

@@ -13,7 +13,7 @@
 #include <type_traits>
 
 #include "common.h"
-#include "bwd_common.h"
+#include "elements.h"
 #include "kernels.h"
 
 namespace evo {
@@ -337,35 +337,11 @@ __global__ void __launch_bounds__(128 / V * 16) fp8_quantize_two(F8Two a) {
     f8_quantize<T, 128, V, true, true>(a.p[second], blockIdx.x - second * a.first);
 }
 
-__device__ __forceinline__ void f8_store_as(void *out, int64_t i, float v, int dtype) {
-    if (dtype == EVO_F32) ((float *)out)[i] = v;
-    else if (dtype == EVO_BF16) ((bf16_t *)out)[i] = (bf16_t)v;
-    else ((f16_t *)out)[i] = (f16_t)v;
-}
-
-// Column sums from those of 128 rows each: 32 columns by 32 slices of the parts.  A launch's time: 256 parts of 1024 columns 3.8 us.
-template <int THREADS>   // 32 of them, each with 32 / THREADS slices: the same additions
-__device__ __forceinline__ void f8_add_sums(const float *part, void *out, int cols, int64_t parts, int dtype, unsigned id) {
-    __shared__ float sums[32][33];
-    const int c = id * 32 + (threadIdx.x & 31), first = threadIdx.x >> 5;
-#pragma unroll
-    for (int slice = first; slice < 32; slice += THREADS) {
-        float s = 0.0f;
-        if (c < cols) {
-#pragma unroll 8
-            for (int64_t i = slice; i < parts; i += 32) s += part[i * cols + c];
-        }
-        sums[slice][threadIdx.x & 31] = s;
-    }
-    __syncthreads();
-    if (first || c >= cols) return;
-    float s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s += sums[i][threadIdx.x];
-    f8_store_as(out, c, s, dtype);
-}
-__global__ void __launch_bounds__(1024) fp8_sums(const float *part, void *out, int cols, int64_t parts, int dtype) {
-    f8_add_sums<32>(part, out, cols, parts, dtype, blockIdx.x);
+// Column sums from those of 128 rows each.  A launch's time: 256 parts of 1024 columns 3.8 us.
+__global__ void __launch_bounds__(1024) sums_of_parts(const float *part, void *out, int cols, int64_t parts, int dtype) { sum_parts<32>(part, out, cols, parts, dtype, blockIdx.x); }
+int launch_sum_parts(const float *part, void *out, int cols, int64_t parts, int dtype, hipStream_t st) {
+    sums_of_parts<<<(unsigned)((cols + 31) / 32), 1024, 0, st>>>(part, out, cols, parts, dtype);
+    return hip_rc();
 }
 
 // ---- product ----
@@ -426,10 +402,6 @@ __device__ __forceinline__ bf16x8 f8_widen(int lo, int hi, float scale) {
 __device__ __forceinline__ float f8_scale(uint32_t four, int j) {
     const unsigned byte = (four >> (8 * j)) & 0xff;
     return __uint_as_float(byte ? byte << 23 : 0x400000u);
-}
-
-__device__ __forceinline__ float f8_bias(const void *b, int i, int dtype) {
-    return dtype == EVO_F32 ? ((const float *)b)[i] : dtype == EVO_BF16 ? (float)((const bf16_t *)b)[i] : (float)((const f16_t *)b)[i];
 }
 
 // What the lanes of a wave have written to LDS before and read after, or the other way round: LDS takes a wave's accesses in their order, and the compiler, which
@@ -544,7 +516,7 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
             for (int r = 0; r < 16; ++r) acc[t][u][r] = 0.0f;
 
     float *bias = reinterpret_cast<float *>(lds8 + BIAS);
-    for (int i = threadIdx.x; i < BN; i += W * 64) bias[i] = p.bias && n0 + i < p.N ? f8_bias(p.bias, n0 + i, p.bias_dtype) : 0.0f;
+    for (int i = threadIdx.x; i < BN; i += W * 64) bias[i] = p.bias && n0 + i < p.N ? load_as(p.bias, n0 + i, p.bias_dtype) : 0.0f;
     fetch_scales(0);
     fetch(0);
     for (int s4 = 0; s4 < nb; s4 += 4) {
@@ -666,7 +638,7 @@ __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
             for (int r = 0; r < 16; ++r) acc[t][u][r] = 0.0f;
 
     float *bias = reinterpret_cast<float *>(lds8 + BIAS);
-    if (threadIdx.x < BN) bias[threadIdx.x] = p.bias && n0 + (int)threadIdx.x < p.N ? f8_bias(p.bias, n0 + threadIdx.x, p.bias_dtype) : 0.0f;
+    if (threadIdx.x < BN) bias[threadIdx.x] = p.bias && n0 + (int)threadIdx.x < p.N ? load_as(p.bias, n0 + threadIdx.x, p.bias_dtype) : 0.0f;
     fetch_scales(0);
     fetch(0);
     fetch(1);                          // (two steps at least)
@@ -810,7 +782,7 @@ __global__ void __launch_bounds__(256, 2) fp8_strip(F8Matmul p) {
 #pragma unroll
         for (int t = 0; t < TN; ++t) wn[t] = (int)p.sb[(int64_t)min(tile * BN + 32 * t + f8_deal(li), p.N - 1) * p.sd];
         const int n = tile * BN + (int)threadIdx.x;
-        if (threadIdx.x < BN && p.bias) next = n < p.N ? f8_bias(p.bias, n, p.bias_dtype) : 0.0f;
+        if (threadIdx.x < BN && p.bias) next = n < p.N ? load_as(p.bias, n, p.bias_dtype) : 0.0f;
     };
     auto take = [&](int tile) {
 #pragma unroll
@@ -939,7 +911,7 @@ struct F8Sums {   // the column sums' parts and where their totals go, if there 
 template <typename T>
 __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, const void *bias, int bias_dtype, int64_t M, int N, int64_t ldo, int slices, F8Sums c) {
     if (c.part && blockIdx.x >= c.first) {
-        f8_add_sums<8>(c.part, c.out, c.cols, c.parts, c.dtype, blockIdx.x - c.first);
+        sum_parts<8>(c.part, c.out, c.cols, c.parts, c.dtype, blockIdx.x - c.first);
         return;
     }
     const int pieces = (N + 7) / 8;
@@ -966,7 +938,7 @@ __global__ void __launch_bounds__(256) fp8_slices(const float *part, T *out, con
     }
     F8Eight<T> e;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = (T)(bias && o + i < N ? s[i] + f8_bias(bias, o + i, bias_dtype) : s[i]);
+    for (int i = 0; i < 8; ++i) e.v[i] = (T)(bias && o + i < N ? s[i] + load_as(bias, o + i, bias_dtype) : s[i]);
     e.store_some(out + m * ldo + o, N - o);
 }
 
@@ -1096,21 +1068,12 @@ __global__ void __launch_bounds__(kF8FewWaves * 64) fp8_few(F8Few p) {
         if (m < p.M) {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (o + r < p.N) out[m * p.ldo + o + r] = (O)(s[r] + (p.bias ? f8_bias(p.bias, o + r, p.bias_dtype) : 0.0f));
+                if (o + r < p.N) out[m * p.ldo + o + r] = (O)(s[r] + (p.bias ? load_as(p.bias, o + r, p.bias_dtype) : 0.0f));
         }
     }
 }
 
-static int f8_rc() {
-    const hipError_t err = hipGetLastError();
-    return err == hipSuccess ? EVO_OK : EVO_EHIP - (int)err;
-}
-static bool f8_dtype(int d) { return d == EVO_BF16 || d == EVO_F16 || d == EVO_F32; }
 static bool f8_off(const void *p, int n) { return ((uintptr_t)p & (n - 1)) != 0; }
-template <typename F>
-static int f8_by_dtype(int dtype, F &&f) {
-    return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
-}
 
 constexpr int kF8StripBlocks = 4, kF8SumsParts = 1024;   // (of more parts a launch of its own, of four times the threads)
 constexpr int64_t kF8MaxK = 1 << 26;   // of the contraction: 32 rows stay within 32-bit offsets
@@ -1123,7 +1086,7 @@ struct F8Plan {
     int mt, nt, slice, slices;
     bool big, strip;
 };
-static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
+static F8Plan f8_plan(int64_t m, int64_t n, int64_t k) {
     F8Plan q{};
     const int blocks = (int)((k + kF8Block - 1) / kF8Block);
     q.strip = blocks <= kF8StripBlocks;
@@ -1142,10 +1105,10 @@ static F8Plan f8_plan(int64_t m, int64_t n, int64_t k, int dtype) {
 }
 
 static int f8_check(const EvoFp8Matmul *p) {
-    if (!p || p->m <= 0 || p->n <= 0 || p->k <= 0 || !f8_dtype(p->dtype)) return EVO_EINVAL;
+    if (!p || p->m <= 0 || p->n <= 0 || p->k <= 0 || !known_dtype(p->dtype)) return EVO_EINVAL;
     if (p->m > INT32_MAX - 512 || p->n > INT32_MAX - 512) return EVO_EOVERFLOW;
     if (p->k > kF8MaxK) return EVO_EUNSUPPORTED;
-    const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
+    const F8Plan q = f8_plan(p->m, p->n, p->k);
     if ((int64_t)q.mt * q.nt > INT32_MAX || (int64_t)q.mt * q.nt * q.slices > INT32_MAX) return EVO_EOVERFLOW;
     return EVO_OK;
 }
@@ -1153,7 +1116,7 @@ static int f8_check(const EvoFp8Matmul *p) {
 constexpr int kF8QuantizeFew = 512;   // tiles
 static int f8_rounding_check(const void *x, int64_t ldx, const void *q, const void *scales, const void *qt, const void *scales_t, const float *sums, int64_t rows,
                              int64_t cols, int dtype) {
-    if (!x || rows <= 0 || cols <= 0 || ldx < cols || !f8_dtype(dtype) || !q != !scales || !qt != !scales_t || (!q && !qt) || (sums && !qt)) return EVO_EINVAL;
+    if (!x || rows <= 0 || cols <= 0 || ldx < cols || !known_dtype(dtype) || !q != !scales || !qt != !scales_t || (!q && !qt) || (sums && !qt)) return EVO_EINVAL;
     if (cols > kF8MaxK || (qt && rows > ((int64_t)1 << 40))) return EVO_EUNSUPPORTED;
     return f8_off(q, 16) || f8_off(qt, 16) ? EVO_EALIGN : EVO_OK;
 }
@@ -1202,7 +1165,7 @@ static int f8_launch_tiles(const F8Matmul &a, unsigned grid, hipStream_t st) {
     static PerDevice done;
     if (const int rc = ensure_dynamic_lds((const void *)kernel, lds, done, nullptr)) return rc;
     kernel<<<grid, WM * WN * 64, lds, st>>>(a);
-    return f8_rc();
+    return hip_rc();
 }
 template <typename T, bool WIDE>
 static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
@@ -1214,7 +1177,7 @@ static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
         static PerDevice done;
         if (const int rc = ensure_dynamic_lds((const void *)fp8_matmul_big<T, WIDE>, lds, done, nullptr)) return rc;
         fp8_matmul_big<T, WIDE><<<grid, 512, lds, st>>>(a);
-        return f8_rc();
+        return hip_rc();
     }
     return f8_launch_tiles<4, 2, 1, 2, T, WIDE>(a, grid, st);
 }
@@ -1250,7 +1213,7 @@ static int f8_launch_strip(F8Matmul a, hipStream_t st) {
         static PerDevice done;
         if (const int rc = ensure_dynamic_lds((const void *)kernel, lds(NB), done, nullptr)) return rc;
         kernel<<<(unsigned)(q.strips * q.pieces), 256, lds(a.blocks), st>>>(a);
-        return f8_rc();
+        return hip_rc();
     };
     if (a.blocks == 1) return go(std::integral_constant<int, 1>());
     if (a.blocks == 2) return go(std::integral_constant<int, 2>());
@@ -1286,7 +1249,7 @@ static int f8_launch_few(const F8Few &a, const F8FewPlan &q, hipStream_t st) {
         if (q.nt == 4) fp8_few<T, O, MT, 4, 1><<<grid, threads, 0, st>>>(a);
         else if (q.slice <= kF8FewWaves) fp8_few<T, O, MT, 1, 1><<<grid, threads, 0, st>>>(a);
         else fp8_few<T, O, MT, 1, MANY><<<grid, threads, 0, st>>>(a);
-        return f8_rc();
+        return hip_rc();
     };
     const int mt = (a.M + 15) / 16;
     return mt == 1 ? go(std::integral_constant<int, 1>()) : mt == 2 ? go(std::integral_constant<int, 2>()) : mt == 3 ? go(std::integral_constant<int, 3>())
@@ -1298,7 +1261,7 @@ static int f8_add_slices(const EvoFp8Matmul &p, int slices, F8Sums c, hipStream_
     if (!grid_fits(groups + more, 256)) return EVO_EOVERFLOW;
     c.first = (unsigned)groups;
     fp8_slices<T><<<(unsigned)(groups + more), 256, 0, st>>>((const float *)p.workspace, (T *)p.out, p.bias, p.bias_dtype, p.m, (int)p.n, p.ldo, slices, c);
-    return f8_rc();
+    return hip_rc();
 }
 
 }  // namespace evo
@@ -1313,7 +1276,7 @@ int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void
     if (p.tiles_r > INT32_MAX / p.tiles_k || !grid_fits(p.tiles_r * p.tiles_k, 256)) return EVO_EOVERFLOW;
     const unsigned grid = (unsigned)(p.tiles_r * p.tiles_k);
     hipStream_t st = (hipStream_t)hip_stream;
-    return f8_by_dtype(dtype, [&](auto t) {
+    return by_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
         // few tiles: more threads for each (us, more / fewer: 1024 x 256 both ways 5.5 / 5.8, 2048 x 4096 rows 6.9 / 7.5; 8192 x 8192 both ways 53.5 / 50.6)
         const bool few = p.tiles_r * p.tiles_k < kF8QuantizeFew;
@@ -1321,13 +1284,13 @@ int evoattn_fp8_quantize(const void *x, int64_t ldx, void *q, void *scales, void
         else if (!q) few ? fp8_quantize<T, 128, 2, false, true><<<grid, 1024, 0, st>>>(p) : fp8_quantize<T, 128, 8, false, true><<<grid, 256, 0, st>>>(p);
         else if (few) fp8_quantize<T, 16, 1, true, false><<<(unsigned)((rows + 15) / 16 * p.tiles_k), 256, 0, st>>>(p);
         else fp8_quantize<T, 128, 8, true, false><<<grid, 256, 0, st>>>(p);
-        return f8_rc();
+        return hip_rc();
     });
 }
 
 int evoattn_fp8_quantize_two(const EvoFp8Rounding *a, const EvoFp8Rounding *b, int32_t dtype, void *hip_stream) {
     using namespace evo;
-    if (!a || !b || !f8_dtype(dtype)) return EVO_EINVAL;
+    if (!a || !b || !known_dtype(dtype)) return EVO_EINVAL;
     F8Two both{};
     int64_t tiles = 0;
     for (int i = 0; i < 2; ++i) {
@@ -1339,35 +1302,34 @@ int evoattn_fp8_quantize_two(const EvoFp8Rounding *a, const EvoFp8Rounding *b, i
         tiles += both.p[i].tiles_r * both.p[i].tiles_k;
     }
     if (!grid_fits(tiles, 256)) return EVO_EOVERFLOW;
-    return f8_by_dtype(dtype, [&](auto t) {
+    return by_dtype(dtype, [&](auto t) {
         typedef decltype(t) T;
         if (tiles < kF8QuantizeFew) fp8_quantize_two<T, 2><<<(unsigned)tiles, 1024, 0, (hipStream_t)hip_stream>>>(both);
         else fp8_quantize_two<T, 8><<<(unsigned)tiles, 256, 0, (hipStream_t)hip_stream>>>(both);
-        return f8_rc();
+        return hip_rc();
     });
 }
 
 int evoattn_fp8_column_sums(const float *sums, void *out, int64_t rows, int64_t cols, int32_t dtype, void *hip_stream) {
     using namespace evo;
-    if (!sums || !out || rows <= 0 || cols <= 0 || !f8_dtype(dtype)) return EVO_EINVAL;
+    if (!sums || !out || rows <= 0 || cols <= 0 || !known_dtype(dtype)) return EVO_EINVAL;
     if (cols > kF8MaxK) return EVO_EUNSUPPORTED;
-    fp8_sums<<<(unsigned)((cols + 31) / 32), 1024, 0, (hipStream_t)hip_stream>>>(sums, out, (int)cols, (rows + kF8Block - 1) / kF8Block, dtype);
-    return f8_rc();
+    return launch_sum_parts(sums, out, (int)cols, (rows + kF8Block - 1) / kF8Block, dtype, (hipStream_t)hip_stream);
 }
 
 size_t evoattn_fp8_matmul_workspace_bytes(const EvoFp8Matmul *p) {
     using namespace evo;
     if (f8_check(p)) return 0;
-    const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
+    const F8Plan q = f8_plan(p->m, p->n, p->k);
     return q.slices == 1 ? 0 : (size_t)q.slices * p->m * p->n * sizeof(float);
 }
 
 static int f8_matmul(const EvoFp8Matmul *p, const evo::F8Sums &c, void *hip_stream, bool *added) {
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
-    if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
+    if (!p->a || !p->b || !p->scales_a || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !known_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->a, 16) || f8_off(p->b, 16) || f8_off(p->scales_a, 4) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
-    const F8Plan q = f8_plan(p->m, p->n, p->k, p->dtype);
+    const F8Plan q = f8_plan(p->m, p->n, p->k);
     if (q.slices > 1 && (!p->workspace || p->workspace_bytes < evoattn_fp8_matmul_workspace_bytes(p))) return EVO_EWORKSPACE;
     F8Matmul a = f8_operands(*p);
     if (q.slices > 1) {
@@ -1385,7 +1347,7 @@ static int f8_matmul(const EvoFp8Matmul *p, const evo::F8Sums &c, void *hip_stre
     }
     if (const int rc = wide ? f8_launch<float, true>(a, q, st) : f8_launch<float, false>(a, q, st)) return rc;
     *added = c.part != nullptr;
-    return f8_by_dtype(p->dtype, [&](auto t) { return f8_add_slices<decltype(t)>(*p, q.slices, c, st); });
+    return by_dtype(p->dtype, [&](auto t) { return f8_add_slices<decltype(t)>(*p, q.slices, c, st); });
 }
 int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
     bool added;
@@ -1394,7 +1356,7 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream) {
 int evoattn_fp8_matmul_sums(const EvoFp8Matmul *p, const float *sums, int64_t rows, void *out, int32_t dtype, void *hip_stream) {
     using namespace evo;
     if (const int rc = f8_check(p)) return rc;
-    if (!sums || !out || rows <= 0 || !f8_dtype(dtype)) return EVO_EINVAL;
+    if (!sums || !out || rows <= 0 || !known_dtype(dtype)) return EVO_EINVAL;
     F8Sums c{};
     c.parts = (rows + kF8Block - 1) / kF8Block;
     if (c.parts <= kF8SumsParts) c.part = sums;
@@ -1422,14 +1384,14 @@ int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ld
     if (const int rc = f8_check(p)) return rc;
     const bool few = p->m <= kF8FewRows;
     if (!evoattn_fp8_matmul_rounds(p)) return EVO_EUNSUPPORTED;
-    if (!x || ldx < p->k || !p->b || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !f8_dtype(p->bias_dtype))) return EVO_EINVAL;
+    if (!x || ldx < p->k || !p->b || !p->scales_b || !p->out || p->ldo < p->n || (p->bias && !known_dtype(p->bias_dtype))) return EVO_EINVAL;
     if (f8_off(p->b, 16) || f8_off(p->scales_b, 4)) return EVO_EALIGN;
     hipStream_t st = (hipStream_t)hip_stream;
     if (!few) {
         F8Matmul a = f8_operands(*p);
         a.x = x;
         a.ldx = ldx;
-        return f8_by_dtype(p->dtype, [&](auto t) { return f8_launch_strip<decltype(t), true>(a, st); });
+        return by_dtype(p->dtype, [&](auto t) { return f8_launch_strip<decltype(t), true>(a, st); });
     }
     const F8FewPlan q = f8_few_plan(p->n, p->k);
     const bool cut = q.slices > 1;
@@ -1450,7 +1412,7 @@ int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ld
     a.slice = q.slice;
     a.sd = (int)(f8_scale_pitch(p->k) / 4);
     a.bias_dtype = p->bias_dtype;
-    return f8_by_dtype(p->dtype, [&](auto t) {
+    return by_dtype(p->dtype, [&](auto t) {
         typedef decltype(t) T;
         if (!cut) return f8_launch_few<T, T>(a, q, st);
         if (const int rc = f8_launch_few<T, float>(a, q, st)) return rc;

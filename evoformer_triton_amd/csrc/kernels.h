@@ -21,6 +21,7 @@ int launch_dbias_reduce(const EvoAttnParams &p, const Extra &e, hipStream_t st);
 int launch_gate_bwd(const EvoAttnParams &p, void *dout_ungated, float *delta, hipStream_t st);  // dO, dgate and delta from the gradient of the gated output
 int launch_mask_shift(const EvoAttnParams &p, const Extra &e, hipStream_t st);
 
+int launch_sum_parts(const float *part, void *out, int cols, int64_t parts, int dtype, hipStream_t st);  // out[c] = sum of part[i][c] (elements.h)
 int launch_prep(const EvoAttnParams &p, const Extra &e, hipStream_t st);
 int launch_mfma_fwd(const EvoAttnParams &p, const Extra &e, hipStream_t st);
 constexpr int kSplitFwdMaxN = 4096;   // (its mask row lies in LDS)

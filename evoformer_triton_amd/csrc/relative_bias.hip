@@ -6,7 +6,7 @@
 #include <type_traits>
 
 #include "common.h"
-#include "bwd_common.h"
+#include "elements.h"
 #include "kernels.h"
 
 namespace evo {
@@ -52,16 +52,6 @@ struct RbArgs {
     __device__ __forceinline__ RbIndex keys(const void *t, int b) const { return {t, b * pos_k_b, wide}; }
 };
 
-__device__ __forceinline__ float rb_entry(const void *t, int64_t i, int dtype) {
-    return dtype == EVO_F32 ? ((const float *)t)[i] : dtype == EVO_BF16 ? (float)((const bf16_t *)t)[i] : (float)((const f16_t *)t)[i];
-}
-
-__device__ __forceinline__ void rb_store(void *t, int64_t i, float v, int dtype) {
-    if (dtype == EVO_F32) ((float *)t)[i] = v;
-    else if (dtype == EVO_BF16) ((bf16_t *)t)[i] = (bf16_t)v;
-    else ((f16_t *)t)[i] = (f16_t)v;
-}
-
 __device__ __forceinline__ bool rb_near(int64_t p) { return p > -kRbNear && p < kRbNear; }
 
 // The clipped distance from 0 on.  Positions near zero in 32 bits, any others in 64, where a difference may overflow.
@@ -87,9 +77,9 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
     const int h = id % a.H, b = id / a.H;
     for (int o = threadIdx.x; o <= 2 * a.reach; o += kRbWaves * 64) {
         const int r = a.lut[o];
-        val[o] = r < a.rows ? rb_entry(a.table, (int64_t)r * a.H + h, a.table_dtype) : 0.0f;
+        val[o] = r < a.rows ? load_as(a.table, (int64_t)r * a.H + h, a.table_dtype) : 0.0f;
     }
-    const float other = CHAIN ? rb_entry(a.table, (int64_t)(a.rows - 1) * a.H + h, a.table_dtype) : 0.0f;
+    const float other = CHAIN ? load_as(a.table, (int64_t)(a.rows - 1) * a.H + h, a.table_dtype) : 0.0f;
     const RbIndex qs = a.queries(a.pos_q, b), ks = a.keys(a.pos_k, b), qc = a.queries(a.chain_q, b), kc = a.keys(a.chain_k, b);
     // The last lane of a row that is no whole number of pieces steps back: two lanes write the same values there.
     const int col = (strip * 64 + lane % a.lanes) * V, first = min(col, max(a.Nk - V, 0)), sub = lane / a.lanes, per = 64 / a.lanes;
@@ -368,7 +358,7 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
     const int64_t at = ((int64_t)b * a.chunks + chunk) * a.strips + strip;
     auto write = [&](int row, int h, float s) {
         if (part) part[(at * a.rows + row) * a.H + h] = s;
-        else rb_store(dtable, (int64_t)row * a.H + h, s, a.table_dtype);
+        else store_as(dtable, (int64_t)row * a.H + h, s, a.table_dtype);
     };
     if (!again) {
         if (wave > 0 || h0 + li >= a.H) return;
@@ -402,24 +392,6 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_bwd(RbArgs a, con
     }
 }
 
-// The workgroups' sums: 32 entries of the table by 32 slices of the parts, in their order.  512 parts: 4 to 5 us, a launch and the way to memory.
-__global__ void __launch_bounds__(1024) relative_bias_sum(const float *part, void *dtable, int entries, int parts, int dtype) {
-    __shared__ float sums[32][33];
-    const int e = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-    float s = 0.0f;
-    if (e < entries) {
-#pragma unroll 8
-        for (int i = slice; i < parts; i += 32) s += part[(int64_t)i * entries + e];
-    }
-    sums[slice][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (slice || e >= entries) return;
-    s = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s += sums[i][threadIdx.x];
-    rb_store(dtable, e, s, dtype);
-}
-
 // The gradient of a pair bias that all batches share: the sum of the output's over them.  Bound by memory: 4 x 32 x 1024^2 in fp32 124 us (671 MB, 5.4 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) relative_bias_batch_sum(const T *dout, T *dpair, int64_t n, int batches) {
@@ -449,13 +421,6 @@ __global__ void __launch_bounds__(256) relative_bias_batch_sum(const T *dout, T 
     }
 }
 
-static int rb_rc() {
-    const hipError_t err = hipGetLastError();
-    return err == hipSuccess ? EVO_OK : EVO_EHIP - (int)err;
-}
-
-static bool rb_dtype(int d) { return d == EVO_BF16 || d == EVO_F16 || d == EVO_F32; }
-
 // Rows of a workgroup, a multiple of `step`, so that `want` workgroups cover a call of `each` strips of rows.
 static void rb_chunks(RbArgs &a, int64_t each, int step, int want) {
     int64_t chunk = (each * a.Nq + want - 1) / want;
@@ -467,7 +432,7 @@ static void rb_chunks(RbArgs &a, int64_t each, int step, int want) {
 
 static int rb_check(const EvoRelativeBias *p) {
     if (!p) return EVO_EINVAL;
-    if (p->B <= 0 || p->H <= 0 || p->Nq <= 0 || p->Nk <= 0 || !rb_dtype(p->dtype) || !rb_dtype(p->table_dtype)) return EVO_EINVAL;
+    if (p->B <= 0 || p->H <= 0 || p->Nq <= 0 || p->Nk <= 0 || !known_dtype(p->dtype) || !known_dtype(p->table_dtype)) return EVO_EINVAL;
     if (!p->lut || !p->pos_q || !p->pos_k || (p->pos_bytes != 4 && p->pos_bytes != 8) || !p->chain_q != !p->chain_k) return EVO_EINVAL;
     if (p->reach < 0 || p->rows < 1) return EVO_EINVAL;
     if (p->reach > kRbMaxReach || p->rows > kRbMaxRows) return EVO_EUNSUPPORTED;
@@ -502,10 +467,6 @@ static RbArgs rb_args(const EvoRelativeBias &p) {
     return a;
 }
 
-template <typename F>
-static int rb_by_dtype(int dtype, F &&f) {
-    return dtype == EVO_BF16 ? f(bf16_t()) : dtype == EVO_F16 ? f(f16_t()) : f(float());
-}
 // Workgroups.  Forward: one for every 64 KB, since each looks its table and positions up first, two for each unit at least and eight at most, that enough is under
 // way.  Of 512 / 1024 / 2048 / 4096, us: 2 x 64 x 256^2 with a bias in bf16 12.1 / 12.7 / 17.6 / 24.5, 1 x 32 x 1024^2 in fp32 81 / 58 / 47 / 47.
 // Backward: two for each unit, whose parts are few to add up.  Of 256 / 384 / 512 / 1024 / 2048: 4 x 32 x 1024^2 in fp32 140 / 131 / 107 / 116 / 121,
@@ -544,7 +505,7 @@ static int rb_launch_bwd(const RbArgs &a, unsigned grid, const T *dout, float *p
         static PerDevice done;
         if (const int rc = ensure_dynamic_lds((const void *)kernel, most, done, nullptr)) return rc;
         kernel<<<grid, kRbWaves * 64, sums + (2 * a.reach + 2) * sizeof(uint16_t), st>>>(a, dout, part, dtable);
-        return rb_rc();
+        return hip_rc();
     };
     if (a.rows <= 32) return go(std::integral_constant<int, 2>());
     if (a.rows <= 48) return go(std::integral_constant<int, 3>());
@@ -566,11 +527,11 @@ int evoattn_relative_bias_fwd(const EvoRelativeBias *p, void *hip_stream) {
     const int64_t grid = (int64_t)a.strips * a.chunks * a.H * a.B;
     if (!grid_fits(grid, kRbWaves * 64)) return EVO_EOVERFLOW;
     const size_t lds = (2 * (size_t)p->reach + 1) * sizeof(float);
-    return rb_by_dtype(p->dtype, [&](auto t) {
+    return by_dtype(p->dtype, [&](auto t) {
         typedef decltype(t) T;
         auto go = [&](auto pair, auto chain) {
             relative_bias_fwd<T, decltype(pair)::value, decltype(chain)::value><<<(unsigned)grid, kRbWaves * 64, lds, (hipStream_t)hip_stream>>>(a, (const T *)p->pair, (T *)p->out);
-            return rb_rc();
+            return hip_rc();
         };
         const std::true_type yes;
         const std::false_type no;
@@ -601,23 +562,23 @@ int evoattn_relative_bias_bwd(const EvoRelativeBias *p, void *hip_stream) {
         const int64_t parts = rb_parts(a), grid = parts * a.heads, entries = (int64_t)a.rows * a.H;
         float *part = parts > 1 ? (float *)p->workspace : nullptr;
         if (parts > 1 && (!p->workspace || p->workspace_bytes < evoattn_relative_bias_bwd_workspace_bytes(p))) return EVO_EWORKSPACE;
-        const int rc = rb_by_dtype(p->dtype, [&](auto t) {
+        const int rc = by_dtype(p->dtype, [&](auto t) {
             typedef decltype(t) T;
             return p->chain_q ? rb_launch_bwd<T, true>(a, (unsigned)grid, (const T *)p->dout, part, p->dtable, st)
                               : rb_launch_bwd<T, false>(a, (unsigned)grid, (const T *)p->dout, part, p->dtable, st);
         });
         if (rc) return rc;
         if (part) {
-            relative_bias_sum<<<(unsigned)((entries + 31) / 32), 1024, 0, st>>>(part, p->dtable, (int)entries, (int)parts, p->table_dtype);
-            if (const int rc2 = rb_rc()) return rc2;
+            // (512 parts: 4 to 5 us, a launch and the way to memory)
+            if (const int rc2 = launch_sum_parts(part, p->dtable, (int)entries, parts, p->table_dtype, st)) return rc2;
         }
     }
     if (p->dpair) {
-        return rb_by_dtype(p->dtype, [&](auto t) {
+        return by_dtype(p->dtype, [&](auto t) {
             typedef decltype(t) T;
             const int64_t groups = (n + 256 * RbVec<T>::V - 1) / (256 * RbVec<T>::V);
             relative_bias_batch_sum<T><<<(unsigned)groups, 256, 0, st>>>((const T *)p->dout, (T *)p->dpair, n, p->B);
-            return rb_rc();
+            return hip_rc();
         });
     }
     return EVO_OK;
