@@ -1183,22 +1183,29 @@ static int f8_launch(const F8Matmul &a, const F8Plan &q, hipStream_t st) {
 }
 
 // Strips of 128 rows, their columns in pieces for two workgroups on each unit (one: 32 768 x 1024 x 256 27.3 us instead of 20.1, 8192 x 4096 x 256 26.1 instead of 20.8).
+constexpr int kF8StripGroups = 512;
 struct F8StripPlan {
     int strips, tiles, pieces;
 };
 static F8StripPlan f8_strip_plan(int64_t m, int64_t n) {
     F8StripPlan q{};
     q.strips = (int)((m + 127) / 128);
-    const int nt = (int)((n + 63) / 64), want = std::min((512 + q.strips - 1) / q.strips, nt);
+    const int nt = (int)((n + 63) / 64), want = std::min((kF8StripGroups + q.strips - 1) / q.strips, nt);
     q.tiles = (nt + want - 1) / want;
     q.pieces = (nt + q.tiles - 1) / q.tiles;
     return q;
 }
-// Whether a strip is rounded by its workgroups: where there are few of them to do that again, or little of it.  us, on the way / before: two blocks 100 x 1024 x 256
-// 5.6 / 7.4, 4096 x 1024 x 256 (16 pieces) 8.8 / 8.4, 8192 x 4096 x 256 20.8 / 23.7; more 65 536 x 512 x 512 (one piece) 32.5 / 46.1, 16 384 x 768 x 384 (four) 16.7 / 18.8,
-// 8192 x 1024 x 512 (eight) 16.4 / 15.5, 300 x 8192 x 512 (128) 12.6 / 9.1; in fp32, which has to spare registers, 4096 x 4096 x 512 43.6 / 29.5.
+// Whether a strip is rounded by its workgroups.  Up to two blocks: always (us, on the way / before, in bf16: 1000 x 1024 x 256 6.5 / 11.0, 4096 x 1024 x 256 in 16 pieces 8.9 /
+// 10.9, 17 000 x 700 x 256 15.6 / 16.4, 33 000 x 333 x 256 16.4 / 20.5; 12 000 x 384 x 256 11.4 / 11.1; in fp32 it takes up to a third longer where there are many pieces, 4096 x 1024 x 256
+// 15.8 / 12.2, and as long for one or two).  More, which fp32 has no registers for: where a strip is one piece, or up to six are all under way at once, two workgroups to a unit (one piece: 65 536 x
+// 512 x 512 30.6 / 42.2, 100 000 x 1024 x 384 75 / 92; at once: 16 384 x 768 x 384, 512 workgroups, 15.6 / 17.7, 11 000 x 320 x 384, 430 in five pieces, 10.6 / 11.2); with a second
+// round of them, or more pieces, before (17 000 x 700 x 300, 532 workgroups, 24.4 / 19.5, 13 312 x 1280 x 384 in five pieces 26.0 / 20.2, 22 000 x 1536 x 300 in three 39.0 / 30.9; 8192 x 1024 x 512,
+// 512 in eight, 16.4 / 15.2, 300 x 8192 x 512 12.6 / 9.1).
 static bool f8_strip_rounds(int64_t m, int64_t n, int64_t k, int dtype) {
-    return k <= 2 * kF8Block || (k <= kF8StripBlocks * kF8Block && dtype != EVO_F32 && f8_strip_plan(m, n).pieces <= 6);
+    if (k <= 2 * kF8Block) return true;
+    if (k > kF8StripBlocks * kF8Block || dtype == EVO_F32) return false;
+    const F8StripPlan q = f8_strip_plan(m, n);
+    return q.pieces == 1 || (q.pieces <= 6 && q.strips * q.pieces <= kF8StripGroups);
 }
 template <typename T, bool ROUND>
 static int f8_launch_strip(F8Matmul a, hipStream_t st) {

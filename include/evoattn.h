@@ -365,8 +365,8 @@ int evoattn_fp8_matmul(const EvoFp8Matmul *p, void *hip_stream);
 int evoattn_fp8_matmul_sums(const EvoFp8Matmul *p, const float *sums, int64_t rows, void *out, int32_t dtype, void *hip_stream);
 
 /* The same with x [m][k], rows ldx elements apart, in the result's dtype, that is rounded on the way (p's a and scales_a are not read): the products
- * of evoattn_fp8_quantize's rows (for more than 64 the same bits as the two calls give).  m at most 64; or k at most 512 where that takes less time than the two calls do, which is whenever k is at
- * most 256 (evoattn_fp8_matmul_rounds says which): EVO_EUNSUPPORTED for all others, and they go through the two calls.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
+ * of evoattn_fp8_quantize's rows (for more than 64 the same bits as the two calls give).  m at most 64; or k at most 256; or k at most 512 in 16 bits where that takes less time than the two
+ * calls do, as measured (evoattn_fp8_matmul_rounds says which): EVO_EUNSUPPORTED for all others, and they go through the two calls.  `workspace` of evoattn_fp8_matmul_rounding_workspace_bytes(). */
 int evoattn_fp8_matmul_rounds(const EvoFp8Matmul *p);   /* 1 or 0 */
 size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream);
