@@ -1111,6 +1111,7 @@ PYBIND11_MODULE(_host, m) {
     m.def("pair_bias", &pair_bias, no_gil, py::arg("z"), py::arg("ln_weight"), py::arg("ln_bias"), py::arg("eps"), py::arg("weight"));
     m.def("block", &block, no_gil, py::arg("inputs"), py::arg("keep"), py::arg("heads"), py::arg("eps_m"), py::arg("eps_z"), py::arg("inf"),
           py::arg("flags"));
+    m.def("has_tangent", &dual, no_gil);
     m.def("relative_bias", &relative_bias, no_gil);
     m.def("relative_bias_forward", &relative_bias_forward, no_gil);
     m.def("relative_bias_backward", &relative_bias_backward, no_gil);

@@ -277,6 +277,7 @@ Tensor fp8_linear_forward(const Tensor &x, const Tensor &weight, const OptTensor
     const char *wrong = f8_linear_wrong(x, weight, bias);
     TORCH_CHECK_VALUE(!wrong, wrong);
     TORCH_CHECK(x.is_cuda(), "fp8_linear runs on the GPU only");
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual(x) && !dual(weight) && !(bias && dual(*bias)), "fp8_linear has no formula for forward mode differentiation");
     return f8_forward(x, weight, bias ? *bias : Tensor(), false, false, nullptr);
 }
 std::vector<Tensor> fp8_linear_backward(const Tensor &dy, const Tensor &x, const Tensor &weight, const OptTensor &bias, bool need_x, bool need_w, bool need_b) {
@@ -309,6 +310,7 @@ Tensor fp8_linear_held_forward(const Tensor &x, const Tensor &values, const Tens
     const char *wrong = f8_held_wrong(x, values, scales, k, bias);
     TORCH_CHECK_VALUE(!wrong, wrong);
     TORCH_CHECK(x.is_cuda(), "fp8_linear runs on the GPU only");
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual(x) && !(bias && dual(*bias)), "fp8_linear has no formula for forward mode differentiation");
     return f8_held_forward(x, values, scales, k, bias ? *bias : Tensor());
 }
 // values and scales of a matrix rounded along its rows

@@ -207,6 +207,7 @@ Tensor relative_bias_forward(const Tensor &table, const Tensor &lut, const Tenso
     const char *wrong = r.take(table, lut, q, k, cq, ck, bias, dtype);
     TORCH_CHECK_VALUE(!wrong, wrong);
     TORCH_CHECK(table.is_cuda(), "the relative position bias runs on the GPU only");
+    TORCH_CHECK_NOT_IMPLEMENTED(!dual(table) && !(bias && dual(*bias)), "relative_position_bias has no formula for forward mode differentiation");
     return r.forward();
 }
 std::pair<Tensor, Tensor> relative_bias_backward(const Tensor &dout, const Tensor &table, const Tensor &lut, const Tensor &q, const Tensor &k, const OptTensor &cq,

@@ -19,6 +19,7 @@ from typing import List, NamedTuple, Optional, Union
 import torch
 
 from . import _lib
+from ._transforms import refuse_tangents
 
 
 _AUTOCAST = (torch.float32, torch.bfloat16, torch.float16)
@@ -84,6 +85,7 @@ def fp8_linear(x: torch.Tensor, weight: Union[torch.Tensor, Fp8Weight], bias: Op
         raise ValueError(wrong)
     if not x.is_cuda:
         raise RuntimeError("fp8_linear runs on the GPU only (no CPU implementation); move its tensors to one cuda device")
+    refuse_tangents("fp8_linear", x, bias, *(() if held else (weight,)))
     if not held:
         return torch.ops.evoattn.fp8_linear(x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):

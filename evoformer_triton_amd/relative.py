@@ -12,6 +12,7 @@ import torch
 from torch import nn
 
 from . import _lib
+from ._transforms import refuse_tangents
 
 _MAX_REACH = 4096
 
@@ -84,6 +85,7 @@ def relative_position_bias(table: torch.Tensor, buckets: torch.Tensor, positions
             raise ValueError(wrong)
         if not table.is_cuda:
             raise RuntimeError("relative_position_bias runs on the GPU only (no CPU implementation); move its tensors to one cuda device")
+        refuse_tangents("relative_position_bias", table, pair_bias)
     return torch.ops.evoattn.relative_bias(table, buckets, positions, key_positions, chains, key_chains, pair_bias, dtype)
 
 
