@@ -6,11 +6,11 @@ struct RelativeBias {
     Tensor table, lut, pos_q, pos_k, chain_q, chain_k, pair;
     at::ScalarType dtype = at::kFloat;
 
-    // Positions of the queries and of the keys, then chains, [B or 1, N], in one integer type and each side's two laid out alike.
+    // Positions of the queries and of the keys, then chains, [B or 1, N] or [N], in one integer type and each side's two laid out alike.  What need not be copied is the caller's
+    // tensor itself, not a view: one made here would have a version of its own, and what is saved for the backward could be changed in place unseen.
     static Tensor indices(const Tensor &t, at::ScalarType type, int64_t batches) {
-        Tensor r = t.dim() == 1 ? t.unsqueeze(0) : t;
-        if (r.size(0) != batches) r = r.expand({batches, r.size(1)});
-        return r.to(type).contiguous();
+        const bool fits = t.dim() == 1 ? batches == 1 : t.size(0) == batches;
+        return (fits ? t : t.expand({batches, t.size(-1)})).to(type).contiguous();
     }
     // What is wrong with the call, or nothing; then the parameter block is filled.
     const char *take(const Tensor &table_, const Tensor &lut_, const Tensor &q, const Tensor &k, const OptTensor &cq, const OptTensor &ck, const OptTensor &bias,

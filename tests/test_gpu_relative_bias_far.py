@@ -144,3 +144,28 @@ def test_the_registered_backward_gives_what_is_traced(gpu_device):
         got = torch.ops.evoattn.relative_bias_bwd(*real, True, True)
         assert [(t.shape, t.stride(), t.dtype) for t in got] == [(t.shape, t.stride(), t.dtype) for t in told], (B, pair_b, crossed)
         assert torch.equal(got[1], real[0] if pair_b == B else real[0].sum(0, keepdim=True)), (B, pair_b, crossed)
+
+
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+@pytest.mark.parametrize("which", ["positions", "key_positions", "chains", "key_chains", "buckets"])
+@pytest.mark.parametrize("shape", [(24,), (1, 24), (2, 24)], ids=str)
+def test_what_is_saved_and_changed_before_the_backward_is_noticed(gpu_device, which, shape, index):
+    """As of any tensor that a backward needs; what was copied for it may change."""
+    from evoformer_triton_amd import relative_buckets, relative_position_bias
+    g = torch.Generator().manual_seed(1)
+    args = {n: torch.randint(0, 9, shape, generator=g).to(index).to(gpu_device) for n in ("positions", "key_positions", "chains", "key_chains")}
+    args["buckets"] = relative_buckets(3).to(gpu_device)
+    table = torch.randn(8, 2, device=gpu_device, requires_grad=True)
+    dout = torch.randn(shape[0] if len(shape) == 2 else 1, 1, 2, 24, 24, device=gpu_device)
+    out = relative_position_bias(table, **args)
+    args[which].copy_(args[which].flip(-1))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, table, dout)
+    # one row of chains for two batches of positions is copied
+    if shape == (2, 24) and which == "chains":
+        short = args["chains"][0].clone()
+        call = lambda: relative_position_bias(table, **{**args, "chains": short, "key_chains": short})  # noqa: E731
+        want, = torch.autograd.grad(call(), table, dout)
+        out = call()
+        short.zero_()
+        assert torch.equal(torch.autograd.grad(out, table, dout)[0], want)
