@@ -236,6 +236,14 @@ struct SavingNode : Node {
         for (auto &s : saved) s.reset_data();
     }
     void save(const Tensor &t, bool is_output = false) { saved.emplace_back(t, is_output); }
+    // What was saved (`output`: the one that is the node's own output), asked for before a backward goes below autograd: a hook may run the forward again, as checkpointing
+    // does, and that has to be recorded.
+    variable_list unpacked(int output = -1) {
+        variable_list t;
+        t.reserve(saved.size());
+        for (size_t i = 0; i < saved.size(); ++i) t.push_back(saved[i].unpack((int)i == output ? shared_from_this() : nullptr));
+        return t;
+    }
     template <typename... T>
     static bool wanted(const T &...t) {
         return at::GradMode::is_enabled() && ((t.defined() && t.requires_grad()) || ...);
@@ -261,11 +269,10 @@ struct AttentionNode : SavingNode {
         const bool rec = at::GradMode::is_enabled();
         variable_list out(6);
         {
+            const variable_list t = unpacked(6);
             at::AutoDispatchBelowADInplaceOrView guard;
-            const Tensor q = saved[0].unpack().contiguous(), k = saved[1].unpack().contiguous(), v = saved[2].unpack().contiguous(),
-                         mask = saved[3].unpack(), bias = saved[4].unpack(), aux = saved[5].unpack(),
-                         o = saved[6].unpack(shared_from_this()).contiguous();
-            const Tensor gate = c.gated ? saved[7].unpack().contiguous() : Tensor();
+            const Tensor q = t[0].contiguous(), k = t[1].contiguous(), v = t[2].contiguous(), mask = t[3], bias = t[4], aux = t[5], o = t[6].contiguous();
+            const Tensor gate = c.gated ? t[7].contiguous() : Tensor();
             c10::DeviceGuard on(q.device());
             Tensor dO = grads[0].defined() ? grads[0].contiguous() : at::zeros_like(q);
             if (dO.scalar_type() != q.scalar_type()) dO = dO.to(q.scalar_type());
@@ -481,8 +488,8 @@ struct SlotAttention : torch::autograd::Function<SlotAttention> {
         const bool rec = at::GradMode::is_enabled();
         variable_list res(5);
         {
+            const auto saved = ctx->get_saved_variables();   // (before going below autograd, as SavingNode::unpacked)
             at::AutoDispatchBelowADInplaceOrView guard;
-            const auto saved = ctx->get_saved_variables();
             const Tensor P = saved[0].contiguous(), &mask = saved[1], &bias = saved[2], &aux = saved[3];
             Call c;
             const std::string bytes = ctx->saved_data["call"].toStringRef();
@@ -657,8 +664,9 @@ struct LinearNode : SavingNode {
         variable_list out(3);
         if (!grads[0].defined()) return out;
         {
+            const variable_list t = unpacked();
             at::AutoDispatchBelowADInplaceOrView guard;
-            const Tensor x = saved[0].unpack(), w = saved[1].unpack(), dy2 = as_rows(grads[0]);
+            const Tensor x = t[0], w = t[1], dy2 = as_rows(grads[0]);
             if (task_should_compute_output(0)) {
                 out[0] = dx_place.defined() ? dx_place : at::empty_like(x, at::MemoryFormat::Contiguous);
                 Tensor rows = out[0].view({-1, x.size(-1)});
@@ -711,10 +719,10 @@ struct StackedNode : SavingNode {
         variable_list out(2 + sizes.size());
         if (!grads[0].defined()) return out;
         {
+            const variable_list t = unpacked();
             at::AutoDispatchBelowADInplaceOrView guard;
-            const Tensor x = saved[0].unpack(), dp2 = as_rows(grads[0]);
-            std::vector<Tensor> w;
-            for (size_t i = 0; i < sizes.size(); ++i) w.push_back(saved[1 + i].unpack());
+            const Tensor x = t[0], dp2 = as_rows(grads[0]);
+            const std::vector<Tensor> w(t.begin() + 1, t.begin() + 1 + sizes.size());
             if (task_should_compute_output(0)) {
                 out[0] = at::empty_like(x, at::MemoryFormat::Contiguous);
                 Tensor rows = as_rows(out[0]);
@@ -825,8 +833,9 @@ struct LayerNormNode : SavingNode {
         variable_list out(3);
         if (!grads[0].defined()) return out;
         {
+            const variable_list t = unpacked();
             at::AutoDispatchBelowADInplaceOrView guard;
-            const Tensor x = saved[0].unpack().contiguous(), w = saved[1].unpack(), stats = saved[2].unpack();
+            const Tensor x = t[0].contiguous(), w = t[1], stats = t[2];
             ln_backward(grads[0].contiguous(), x, w, stats, task_should_compute_output(0), w.defined() && task_should_compute_output(1),
                         has_bias && task_should_compute_output(2), out[0], out[1], out[2]);
         }
@@ -922,11 +931,12 @@ struct PairBiasNode : SavingNode {
         variable_list out(4);
         if (!grads[0].defined()) return out;
         {
+            const variable_list t = unpacked();
             at::AutoDispatchBelowADInplaceOrView guard;
-            const PairOperands o(PairOperands::ready(saved[0].unpack()), saved[1].unpack(), saved[2].unpack(), PairOperands::ready(saved[3].unpack()));
+            const PairOperands o(PairOperands::ready(t[0]), t[1], t[2], PairOperands::ready(t[3]));
             const bool lw = task_should_compute_output(1), lb = task_should_compute_output(2), w = task_should_compute_output(3);
             Tensor dparams;
-            o.backward(grads[0].contiguous(), saved[4].unpack(), task_should_compute_output(0), lw || lb || w, out[0], dparams);
+            o.backward(grads[0].contiguous(), t[4], task_should_compute_output(0), lw || lb || w, out[0], dparams);
             if (lw) out[1] = dparams.select(0, 0);
             if (lb) out[2] = dparams.select(0, 1);
             if (w) out[3] = dparams.narrow(0, 2, o.H);
@@ -973,9 +983,8 @@ struct BlockNode : SavingNode {
         variable_list out(kBlockInputs);
         if (!grads[0].defined()) return out;
         {
+            variable_list t = unpacked();
             at::AutoDispatchBelowADInplaceOrView guard;
-            Tensor t[kSaved];
-            for (int i = 0; i < kSaved; ++i) t[i] = saved[i].unpack();
             for (int i : {(int)kM, (int)kX, (int)kP, (int)kOut}) t[i] = t[i].contiguous();   // (after a hook on saved tensors)
             bool want[kBlockInputs], inner = false;
             for (int i = 0; i < kBlockInputs; ++i) {
@@ -1014,7 +1023,7 @@ struct BlockNode : SavingNode {
                 }
                 if (want[kM] || want[kNormMW] || want[kNormMB]) {
                     Tensor dx = at::empty_like(x2);
-                    std::vector<Tensor> w(t + kQ, t + kQ + W);
+                    std::vector<Tensor> w(t.begin() + kQ, t.begin() + kQ + W);
                     if (!lin_input_grad(dp2, w, dx)) at::mm_out(dx, dp2, at::cat(w, 0));
                     ln_backward(dx, t[kM], t[kNormMW], t[kStatsM], want[kM], want[kNormMW], want[kNormMB], out[kM], out[kNormMW], out[kNormMB]);
                 }

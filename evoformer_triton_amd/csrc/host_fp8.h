@@ -205,9 +205,10 @@ struct Fp8LinearNode : SavingNode {
         variable_list out(3);
         if (!grads[0].defined()) return out;
         {
+            const variable_list t = unpacked();
             at::AutoDispatchBelowADInplaceOrView guard;
             const Tensor d = grads[0].scalar_type() == x_type ? grads[0] : grads[0].to(x_type);
-            const Tensor xt = saved[0].unpack(), wt = saved[1].unpack();
+            const Tensor xt = t[0], wt = t[1];
             const bool need_x = task_should_compute_output(0), need_w = task_should_compute_output(1), need_b = has_bias && task_should_compute_output(2);
             if (d.numel() == 0 || k == 0) {
                 if (need_x) out[0] = at::zeros(x_shape, d.options());

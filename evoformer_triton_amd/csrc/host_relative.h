@@ -147,18 +147,19 @@ struct RelativeBiasNode : SavingNode {
         variable_list out(2);
         if (!grads[0].defined()) return out;
         {
+            const bool need_table = task_should_compute_output(0), need_pair = task_should_compute_output(1), sums = need_table || (need_pair && shared_pair);
+            const variable_list t = sums ? unpacked() : variable_list();
             at::AutoDispatchBelowADInplaceOrView guard;
-            const bool need_table = task_should_compute_output(0), need_pair = task_should_compute_output(1);
             Tensor d = grads[0].scalar_type() == dtype ? grads[0] : grads[0].to(dtype), dpair;
-            if (need_table || (need_pair && shared_pair)) {
+            if (sums) {
                 RelativeBias r;
                 r.p = p;
                 r.table_type = table_type;
-                r.lut = saved[0].unpack().contiguous();
-                r.pos_q = saved[1].unpack().contiguous();
-                r.pos_k = saved[2].unpack().contiguous();
-                r.chain_q = saved[3].unpack();
-                r.chain_k = saved[4].unpack();
+                r.lut = t[0].contiguous();
+                r.pos_q = t[1].contiguous();
+                r.pos_k = t[2].contiguous();
+                r.chain_q = t[3];
+                r.chain_k = t[4];
                 if (r.chain_q.defined()) {
                     r.chain_q = r.chain_q.contiguous();
                     r.chain_k = r.chain_k.contiguous();
