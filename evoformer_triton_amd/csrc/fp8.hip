@@ -1,14 +1,16 @@
 // Linear layers in 8 bits: e4m3 operands with a power-of-two scale (E8M0, the exponent + 127) for each block of 128 along the
-// contraction, y = Q(x) Q(w)^T + b.  Two kernels: the rounding of a matrix, along its rows, its columns or both in one pass, and the product of two
-// rounded matrices that both lie with the contraction along their rows.  A training step's products are all of that form:
+// contraction, y = Q(x) Q(w)^T + b.  The rounding of a matrix (fp8_quantize, fp8_quantize_two: along its rows, its columns or both in one pass), and products of two
+// rounded matrices that both lie with the contraction along their rows: tiles of 128 x 128 (fp8_matmul) and of 256 x 256 (fp8_matmul_big), strips of 128 rows for up to four
+// blocks (fp8_strip), up to 64 rows (fp8_few), and the sum of a contraction's slices (fp8_slices).  A training step's products are all of that form:
 //   y = Qk(x) Qk(w)^T,  dx = Qn(dy) Qn(w^T)^T,  dw = Qm(dy^T) Qm(x^T)^T
 // each operand rounded along the axis that its product contracts.  A copy of 1 GB runs at 5.1 TB/s both ways here, of 67 MB at up to 7.9; the bf16 product of 8192^3 at
-// 1211 TFLOP/s, the library's 8-bit one (one scale for a matrix) at 2790 to 2900: on such data these are limited by power (the kernel below takes 528 us, 407 without
-// loads, 385 without LDS reads as well; with operands of zeros 391, 301 and 292).
+// 1211 TFLOP/s, the library's 8-bit one (one scale for a matrix) at 2790 to 2900.
 //
 // Sums.  On gfx950 all 8-bit products add eight neighbouring values of a lane with what lies 13 bits below the largest of them cut off; between those groups, and to the
-// accumulator, 24 bits count.  That is 1.4e-5 of a result on normal data, where the roundings to 8 bits are up to 2^-4 each and that of a bf16 result up to 2^-8 of what
-// they round, for half the time that bf16 products take.  fp32 results are not given that: their operands are widened to bf16, exactly, and take its products, whose sums are fp32 (WIDE).
+// accumulator, 24 bits count.  That is 1.4e-5 of a result on normal data, where the roundings to 8 bits are up to 2^-4 each and that of a bf16 result up to 2^-9 of what
+// they round, for half the time that bf16 products take: a bf16 result is another one than with fp32 sums in one entry of 25 to 75, an fp16 one in one of 7 to 13, mostly by a last bit, and
+// as far from 64 bits (1.7e-3 and 2.1e-4).  fp32 results are not given that: their operands are widened to bf16, exactly for values from 2^-133 on (a smaller one, of a block
+// whose largest is below 2^-115, loses bits) and below 2^128, and take its products, whose sums are fp32 (WIDE).
 #include <algorithm>
 #include <type_traits>
 
@@ -461,8 +463,8 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
 // out[m][n] (+ slice M N) = sum over the slice's blocks of a[m] . b[n], times the scales, + bias[n].  WM x WN waves of TM x TN tiles
 // of 32 x 32; outputs (rows of b) are the accumulators' rows, rows of a their columns: a lane then holds 16 outputs side by side.  128 x 128 with two stages of a block each:
 // 64 KB, two workgroups to a unit, one of which multiplies while the other waits for its loads or stores; eight waves of 32 x 64, two of a SIMD in turn (us, instead of four of
-// 64 x 64: 2048^3 13.0 / 14.4, 1024 x 4096 x 1024 9.0 / 9.8, 32 768 x 256 x 1024 15.1 / 15.0; four stages for the one workgroup that then fits: 14.8, 9.8, 14.7).  Bound by those: 32 768 x 256 x 1024 in 14.4 us (1190 TFLOP/s; 50 MB,
-// 3.5 TB/s); results written two bytes at a time instead of 16 made 32 768 x 1024 x 256 30 us instead of 23.
+// 64 x 64, on one box: 2048^3 13.0 / 14.4, 1024 x 4096 x 1024 9.0 / 9.8, 32 768 x 256 x 1024 15.1 / 15.0; four stages for the one workgroup that then fits: 14.8, 9.8, 14.7).  Bound by those
+// loads and stores: 32 768 x 256 x 1024 in 13.6 us on another (1260 TFLOP/s; 50 MB, 3.7 TB/s); results written two bytes at a time instead of 16 made 32 768 x 1024 x 256 30 us instead of 23.
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {
     constexpr int W = WM * WN, BM = WM * TM * 32, BN = WN * TN * 32, STAGE = (BM + BN) * 128, PIECES = (BM + BN) / 8 / W, SCALES = 2 * STAGE,
@@ -586,9 +588,11 @@ struct F8Wide {   // 16 of a lane's values of a row as operands of two products
 // barrier; eight products; barrier.  Stage s + 1 is first read by waves 0 to 3 after their step s: before that barrier every wave's loads of it
 // have landed.  That is the end of step s for waves 0 to 3 and the middle of it for waves 4 to 7, when stages s + 2 and s + 3 are still under way.
 //
-// 8192 x 4096 x 4096 in 111 us, 2480 TFLOP/s (128 x 128: 139; 124 on another card), 8192^3 in 478 to 528, 2300 to 2080, where power is the bound.  fp32 results (WIDE): 224 us, 1230 TFLOP/s, the rate of
-// the library's bf16 product (216); widened in one piece before the products instead of by halves 285.  Four waves of 128 x 128 over several tiles in turn, with the next tile's
-// loads under the last one's stores: 528 and, for short contractions, 36 us instead of 32.  Loads asked for between the products: no change.
+// 8192 x 4096 x 4096 in 111 to 114 us, 2480 TFLOP/s (128 x 128: 139; 124 on another card), 8192^3 in 417 to 528 by card, 2640 to 2080.  Two bounds share the rest: power (with operands of
+// zeros 391 us instead of 528 on one card) and the loads (without them 407 of those 528, 301 of the 391; without LDS reads as well 385 and 292).  The matrix cores are busy for 0.59 to 0.61 of
+// the cycles.  9 loads of 10 find L2: 1.07 GB for 8192 x 4096 x 4096, 9.7 TB/s of requests of 64 bytes, some 400 cycles each; 99 MB come from past it, 50 are needed.  fp32 results (WIDE): 224 us,
+// 1230 TFLOP/s, the rate of the library's bf16 product (216); widened in one piece before the products instead of by halves 285.  Four waves of 128 x 128 over several tiles in
+// turn, with the next tile's loads under the last one's stores: 528 and, for short contractions, 36 us instead of 32.  Loads asked for between the products: no change.
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(512, 2) fp8_matmul_big(F8Matmul p) {
     constexpr int W = 8, TM = 4, TN = 2, BM = 256, BN = 256, STAGE = (BM + BN) * 64, RING = 4, PIECES = 4;

@@ -153,10 +153,11 @@ __global__ void __launch_bounds__(kRbWaves * 64) relative_bias_fwd(RbArgs a, con
 // 4q .. 4q + 3).  16-bit gradients are operands as they lie; fp32 ones, 2^24 times as large, as three bf16 parts, which hold all of their
 // 24 bits (of one below 2^-110 as it is, the smaller parts run out of exponents: sums of gradients around 3e-36 were 1.6e-5 off).  A
 // product with one is exact, and sums are fp32 in a fixed order.  Zero times an infinity is no number: a workgroup that ends with a
-// sum that is not finite forms its sums again one by one, and so does one whose positions lie some 2^30 (less 4096) or more from its first query's.
+// sum that is not finite (2^24 times as large, in fp32: from 2^104 on) forms its sums again one by one, and so does one whose positions lie some 2^30 (less 4096) or more from its first query's.
+// Such a workgroup takes 40 to 100 times as long (with infinities in all of them 2 x 8 x 251^2 in fp16 0.57 ms instead of 14 us, 4 x 32 x 1024^2 in fp32 11 ms instead of 0.11).
 // Chains are names: a query's is compared with those of the workgroup's keys, one to a lane, in all of their bits, and a lane takes its pairs' from the answer.
-// Bound by memory: 4 x 32 x 1024^2 in fp32 110 us (537 MB, 4.9 TB/s; with the loads alone 113 where this took 117), after the forward's results have been written
-// 141.  As many additions to sums in LDS: 681 us.  32 heads to a workgroup, whose buckets are then looked up once: 151 instead of 116.
+// Bound by memory: 4 x 32 x 1024^2 in fp32 107 to 109 us (537 MB, 5.0 TB/s), after the forward's results have been written 141 to 148.  As many additions to sums in LDS: 681 us.  32 heads to a
+// workgroup, whose buckets are then looked up once: 151 where this took 116.
 constexpr int kRbKeys = 64, kRbHeads = 16;   // a workgroup's keys and heads
 
 typedef float f32x4r __attribute__((ext_vector_type(4)));
