@@ -463,7 +463,7 @@ __device__ __forceinline__ void f8_store_tile(const f32x16 (&acc)[TN][TM], const
 // out[m][n] (+ slice M N) = sum over the slice's blocks of a[m] . b[n], times the scales, + bias[n].  WM x WN waves of TM x TN tiles
 // of 32 x 32; outputs (rows of b) are the accumulators' rows, rows of a their columns: a lane then holds 16 outputs side by side.  128 x 128 with two stages of a block each:
 // 64 KB, two workgroups to a unit, one of which multiplies while the other waits for its loads or stores; eight waves of 32 x 64, two of a SIMD in turn (us, instead of four of
-// 64 x 64, on one box: 2048^3 13.0 / 14.4, 1024 x 4096 x 1024 9.0 / 9.8, 32 768 x 256 x 1024 15.1 / 15.0; four stages for the one workgroup that then fits: 14.8, 9.8, 14.7).  Bound by those
+// 64 x 64, on one card: 2048^3 13.0 / 14.4, 1024 x 4096 x 1024 9.0 / 9.8, 32 768 x 256 x 1024 15.1 / 15.0; four stages for the one workgroup that then fits: 14.8, 9.8, 14.7).  Bound by those
 // loads and stores: 32 768 x 256 x 1024 in 13.6 us on another (1260 TFLOP/s; 50 MB, 3.7 TB/s); results written two bytes at a time instead of 16 made 32 768 x 1024 x 256 30 us instead of 23.
 template <int WM, int WN, int TM, int TN, typename T, bool WIDE>
 __global__ void __launch_bounds__(WM * WN * 64, 2) fp8_matmul(F8Matmul p) {

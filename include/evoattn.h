@@ -103,7 +103,7 @@ enum {
     EVO_EUNSUPPORTED  = -2,  /* head dim or size outside what the kernels cover */
     EVO_EALIGN        = -3,  /* pointer or stride not aligned for the requested dtype */
     EVO_EWORKSPACE    = -4,  /* workspace missing or too small */
-    EVO_EOVERFLOW     = -5,  /* extents overflow the index type */
+    EVO_EOVERFLOW     = -5,  /* extents overflow the index type, or a launch would have 2^32 threads */
     EVO_EHIP          = -100 /* EVO_EHIP - hipError_t from a launch */
 };
 
