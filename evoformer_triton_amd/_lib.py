@@ -37,7 +37,8 @@ EXPORTS = ("evoattn_version", "evoattn_strerror", "evoattn_check", "evoattn_prep
            "evoattn_pair_bias_workspace_bytes", "evoattn_pair_bias_fwd", "evoattn_pair_bias_bwd",
            "evoattn_keep_mask", "evoattn_linear_fwd", "evoattn_linear_dx", "evoattn_linear_dw_workspace_bytes", "evoattn_linear_dw",
            "evoattn_relative_bias_fwd", "evoattn_relative_bias_bwd_workspace_bytes", "evoattn_relative_bias_bwd",
-           "evoattn_fp8_quantize", "evoattn_fp8_quantize_two", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_sums", "evoattn_fp8_matmul_rounds", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding")
+           "evoattn_fp8_quantize", "evoattn_fp8_quantize_two", "evoattn_fp8_column_sums", "evoattn_fp8_matmul_workspace_bytes", "evoattn_fp8_matmul", "evoattn_fp8_matmul_sums", "evoattn_fp8_matmul_rounds", "evoattn_fp8_matmul_rounding_workspace_bytes", "evoattn_fp8_matmul_rounding",
+           "evoattn_rotary", "evoattn_packed_fwd_workspace_bytes", "evoattn_packed_fwd", "evoattn_packed_bwd_workspace_bytes", "evoattn_packed_bwd")
 EVOATTN_STATIC_PREP_BYTES = 16 << 20
 
 
@@ -92,6 +93,31 @@ class EvoFp8Matmul(ctypes.Structure):
         ("dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
         ("a", ctypes.c_void_p), ("scales_a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("scales_b", ctypes.c_void_p),
         ("bias", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class EvoRotary(ctypes.Structure):
+    _fields_ = [
+        ("B", ctypes.c_int32), ("S", ctypes.c_int32), ("N", ctypes.c_int32), ("H", ctypes.c_int32), ("Hk", ctypes.c_int32), ("D", ctypes.c_int32), ("R", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("inverse", ctypes.c_int32), ("pos_bytes", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("pos_stride_b", ctypes.c_int64),
+        ("q_stride", ctypes.c_int64 * 4), ("k_stride", ctypes.c_int64 * 4), ("out_q_stride", ctypes.c_int64 * 4), ("out_k_stride", ctypes.c_int64 * 4),
+        ("pos", ctypes.c_void_p), ("turns", ctypes.c_void_p), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p),
+        ("out_q", ctypes.c_void_p), ("out_k", ctypes.c_void_p),
+    ]
+
+
+class EvoPacked(ctypes.Structure):
+    _fields_ = [
+        ("n", ctypes.c_int32), ("H", ctypes.c_int32), ("Hk", ctypes.c_int32), ("D", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("offset_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("scale", ctypes.c_float), ("reserved2", ctypes.c_int32), ("Tq", ctypes.c_int64), ("Tk", ctypes.c_int64),
+        ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64), ("k_stride_t", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v_stride_t", ctypes.c_int64), ("v_stride_h", ctypes.c_int64), ("dout_stride_t", ctypes.c_int64), ("dout_stride_h", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("key_offsets", ctypes.c_void_p),
+        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("dout", ctypes.c_void_p),
+        ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]
 
@@ -184,6 +210,13 @@ def load(path: str | None = None) -> ctypes.CDLL:
     lib.evoattn_fp8_matmul_rounding_workspace_bytes.argtypes = [ctypes.POINTER(EvoFp8Matmul)]
     lib.evoattn_fp8_matmul_rounding.restype = ctypes.c_int
     lib.evoattn_fp8_matmul_rounding.argtypes = [ctypes.POINTER(EvoFp8Matmul), vp, i64, vp]
+    lib.evoattn_rotary.restype = ctypes.c_int
+    lib.evoattn_rotary.argtypes = [ctypes.POINTER(EvoRotary), vp]
+    for name in ("evoattn_packed_fwd", "evoattn_packed_bwd"):
+        getattr(lib, name).restype = ctypes.c_int
+        getattr(lib, name).argtypes = [ctypes.POINTER(EvoPacked), vp]
+        getattr(lib, name + "_workspace_bytes").restype = ctypes.c_size_t
+        getattr(lib, name + "_workspace_bytes").argtypes = [ctypes.POINTER(EvoPacked)]
     lib.evoattn_path.restype = ctypes.c_char_p
     lib.evoattn_kernels.restype = ctypes.c_char_p
     lib.evoattn_path.argtypes = [P, ctypes.c_int]

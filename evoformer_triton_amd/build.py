@@ -40,6 +40,7 @@ def _units():
     units = [("api", "api.hip", []), ("generic", "generic.hip", []), ("dispatch", "dispatch.hip", []),
              ("prep", "prep.hip", []), ("layernorm", "layernorm.hip", []), ("pair_bias", "pair_bias.hip", VGPR_FORM[:2]),
              ("linear", "linear.hip", VGPR_FORM[:2]), ("relative_bias", "relative_bias.hip", VGPR_FORM[:2]), ("fp8", "fp8.hip", VGPR_FORM[:2]),
+             ("rotary", "rotary.hip", []), ("packed", "packed.hip", []),
              ("f32", "f32.hip", VGPR_FORM[:2]), ("mfma_bwd_fused", "mfma_bwd_fused.hip", VGPR_FORM),
              ("mfma_bwd_fused8", "mfma_bwd_fused8.hip", VGPR_FORM), ("mfma_stream8", "mfma_stream8.hip", VGPR_FORM), ("mfma_dbias", "mfma_dbias.hip", VGPR_FORM)]
     for d in HEAD_DIMS:

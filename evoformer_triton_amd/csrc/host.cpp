@@ -20,6 +20,8 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cfloat>
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -1105,6 +1107,8 @@ OptTensor block(const std::vector<OptTensor> &in, const OptTensor &keep, int64_t
 
 #include "host_relative.h"
 #include "host_fp8.h"
+#include "host_rotary.h"
+#include "host_packed.h"
 
 }  // namespace
 
@@ -1133,4 +1137,11 @@ PYBIND11_MODULE(_host, m) {
     m.def("fp8_linear_wrong", &fp8_linear_wrong, no_gil);
     m.def("fp8_linear_held_wrong", &fp8_linear_held_wrong, no_gil);
     m.def("fp8_round", &fp8_round, no_gil);
+    m.def("rotary", &rotary, no_gil);
+    m.def("rotary_forward", &rotary_forward, no_gil);
+    m.def("rotary_wrong", &rotary_wrong, no_gil);
+    m.def("packed_attention", &packed_attention, no_gil);
+    m.def("packed_forward", &packed_forward, no_gil);
+    m.def("packed_backward", &packed_backward, no_gil);
+    m.def("packed_wrong", &packed_wrong, no_gil);
 }

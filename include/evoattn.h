@@ -371,6 +371,56 @@ int evoattn_fp8_matmul_rounds(const EvoFp8Matmul *p);   /* 1 or 0 */
 size_t evoattn_fp8_matmul_rounding_workspace_bytes(const EvoFp8Matmul *p);
 int evoattn_fp8_matmul_rounding(const EvoFp8Matmul *p, const void *x, int64_t ldx, void *hip_stream);
 
+/* Rotary positions (no counterpart in the reference): the first R values of each row of q and k as R / 2 pairs, each turned by an angle that grows with the row's position,
+ *   y[i] = scale * (x[i] cos a - x[j] sin a),  y[j] = scale * (x[j] cos a + x[i] sin a),  a = 2 pi (pos * turns[pair] mod 2^64) / 2^64,
+ *   pair (i, j) = (i, i + R / 2), or with `interleaved` (2 i, 2 i + 1); values from R on are copied.  `inverse`: by -a, which is also the gradient's formula.
+ * q [B][S][N][H][D] and k [B][S][N][Hk][D] (Hk may be 0), the last dimension contiguous, any strides; out_q and out_k likewise, either apart from what is read or exactly
+ * in its place.  pos [B][N], rows pos_stride_b apart (0: shared by the batches), signed integers of pos_bytes (4 or 8); the S rows share them.  turns [R / 2]:
+ * the fraction of a turn per position as a 64-bit whole number.  dtype EVO_BF16 / _F16 / _F32; rounded once.  Nothing is allocated or synchronised. */
+typedef struct EvoRotary {
+    int32_t B, S, N, H, Hk, D, R;
+    int32_t dtype, interleaved, inverse, pos_bytes;
+    float   scale;
+    int64_t pos_stride_b;
+    int64_t q_stride[4], k_stride[4];          /* b, s, n, h */
+    int64_t out_q_stride[4], out_k_stride[4];
+    const void *pos, *turns;
+    const void *q, *k;
+    void       *out_q, *out_k;
+} EvoRotary;
+int evoattn_rotary(const EvoRotary *p, void *hip_stream);
+
+/* Attention within sequences that lie one after the other (no counterpart in the reference, whose rows all have N residues):
+ *   o[i][h] = sum_j softmax_j(scale * q[i][h] . k[j][h / (H / Hk)]) v[j][h / (H / Hk)],  j over the keys of i's sequence,
+ *   causal: those with (keys behind j) >= (queries behind i), so that the last query sees every key.
+ * q [Tq][H][D], k and v [Tk][Hk][D], dout [Tq][H][D], the last dimension contiguous, rows and heads *_stride_t and *_stride_h apart; o, dq, dk, dv dense.  Hk divides H.
+ * offsets, key_offsets [n + 1], signed integers of offset_bytes (4 or 8): sequence s has queries offsets[s] .. offsets[s + 1] - 1 and keys likewise; ascending, within
+ * [0, T] (others are brought there: no access is out of bounds, what such rows hold is not specified).  Rows of no sequence and rows that see no key get zeros, in o and in the gradients.
+ *   lse  [H][Tq] fp32: log2 of the row's sum of 2^(scale log2(e) q . k), for the backward (+inf: no key); may be NULL in the forward
+ *   dk, dv  both may be NULL (not wanted)
+ * D at most 128; scale positive.  16-bit: D and all strides multiples of 8, pointers on 16-byte boundaries (EVO_EALIGN otherwise), row strides below 2^23.  `workspace`
+ * of evoattn_packed_fwd_workspace_bytes() (0: none needed) and evoattn_packed_bwd_workspace_bytes().  The backward is deterministic.  Nothing is allocated or synchronised. */
+typedef struct EvoPacked {
+    int32_t n, H, Hk, D;
+    int32_t dtype, causal, offset_bytes, reserved;
+    float   scale;
+    int32_t reserved2;
+    int64_t Tq, Tk;
+    int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, dout_stride_t, dout_stride_h;
+    const void *q, *k, *v;
+    const void *offsets, *key_offsets;
+    void       *o;
+    float      *lse;
+    const void *dout;
+    void       *dq, *dk, *dv;
+    void       *workspace;
+    size_t      workspace_bytes;
+} EvoPacked;
+size_t evoattn_packed_fwd_workspace_bytes(const EvoPacked *p);
+int    evoattn_packed_fwd(const EvoPacked *p, void *hip_stream);
+size_t evoattn_packed_bwd_workspace_bytes(const EvoPacked *p);
+int    evoattn_packed_bwd(const EvoPacked *p, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif
