@@ -10,12 +10,14 @@ struct Packed {
         const bool wide = t.scalar_type() == at::kFloat;
         if (t.size(2) != Dp) return at::constant_pad_nd(t, {0, Dp - t.size(2)});
         if (!t.numel()) return t;
-        const int64_t st = t.size(0) > 1 ? t.stride(0) : 0, sh = t.size(1) > 1 ? t.stride(1) : 0;
-        const bool taken = (t.stride(2) == 1 || t.size(2) == 1) && (wide || (st % 8 == 0 && sh % 8 == 0 && st < 1 << 23 && (uintptr_t)t.data_ptr() % 16 == 0));
+        int64_t st, sh;
+        stride(t, st, sh);
+        // (rows of 16 bits lie apart, so that what is beyond a sequence is out of range)
+        const bool taken = (t.stride(2) == 1 || t.size(2) == 1) && (wide || (st >= Dp && st % 8 == 0 && sh % 8 == 0 && st < 1 << 23 && (uintptr_t)t.data_ptr() % 16 == 0));
         return taken ? t : t.clone(at::MemoryFormat::Contiguous);
     }
     static void stride(const Tensor &t, int64_t &st, int64_t &sh) {
-        st = t.size(0) > 1 ? t.stride(0) : 0;
+        st = t.size(0) > 1 ? t.stride(0) : t.size(2);
         sh = t.size(1) > 1 ? t.stride(1) : 0;
     }
     // What is wrong with the call, or nothing; then the parameter block is filled.

@@ -1,4 +1,4 @@
-// Attention within packed sequences: its entry points, and a kernel of one row per wave.
+// Attention within packed sequences: its entry points, and fp32's kernels, of one row per wave.
 //
 // Forward: a wave keeps a query row and walks over the keys that it sees, 64 at a time, a key to a lane: scores, the running maximum m and sum l of 2^(score - m), then
 // o += p_j v_j with the row's values in the lanes.  Backward with p_ij = 2^(score - lse_i) formed again, delta_i = sum do_i o_i: ds_ij = p_ij (do_i v_j - delta_i) scale,
@@ -31,6 +31,15 @@ __global__ void __launch_bounds__(256) packed_rows_dkdv(EvoPacked p, const float
     row_dkdv<T>(p, segment_of_row<true>(p, j), j, hk, delta);
 }
 
+int launch_packed_fwd_d32(const EvoPacked &, hipStream_t);
+int launch_packed_fwd_d64(const EvoPacked &, hipStream_t);
+int launch_packed_fwd_d96(const EvoPacked &, hipStream_t);
+int launch_packed_fwd_d128(const EvoPacked &, hipStream_t);
+int launch_packed_bwd_d32(const EvoPacked &, float *, hipStream_t);
+int launch_packed_bwd_d64(const EvoPacked &, float *, hipStream_t);
+int launch_packed_bwd_d96(const EvoPacked &, float *, hipStream_t);
+int launch_packed_bwd_d128(const EvoPacked &, float *, hipStream_t);
+
 static int packed_check(const EvoPacked *p) {
     if (!p || p->n < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1 || !known_dtype(p->dtype) || (p->offset_bytes != 4 && p->offset_bytes != 8) || p->Tq < 0 ||
         p->Tk < 0 || !(p->scale > 0.0f && p->scale <= FLT_MAX))
@@ -38,7 +47,21 @@ static int packed_check(const EvoPacked *p) {
     if (p->D > 128) return EVO_EUNSUPPORTED;
     // (row numbers and the positions of tiles are formed in 32 bits)
     if (p->Tq > INT32_MAX / 2 || p->Tk > INT32_MAX / 2 || p->n > INT32_MAX / 4 || (int64_t)p->H > 1 << 20) return EVO_EOVERFLOW;
+    if (p->dtype != EVO_F32 && p->D % 8) return EVO_EALIGN;
     return EVO_OK;
+}
+// The matrix kernels move pieces of 16 bytes, address the rows of a stage by 32 bits, and take what is beyond a sequence for out of range, which rows have to lie apart for.
+static bool packed_aligned(const EvoPacked &p, bool backward) {
+    if (p.dtype == EVO_F32) return true;
+    for (const void *x : {p.q, p.k, p.v, (const void *)p.o, backward ? p.dout : nullptr, backward ? (const void *)p.dq : nullptr, backward ? (const void *)p.dk : nullptr,
+                          backward ? (const void *)p.dv : nullptr})
+        if ((uintptr_t)x % 16) return false;
+    for (int64_t x : {p.q_stride_t, p.k_stride_t, p.v_stride_t, backward ? p.dout_stride_t : 0})
+        if (x % 8 || x >= 1 << 23) return false;
+    if ((p.Tq && p.q_stride_t < p.D) || (p.Tk && (p.k_stride_t < p.D || p.v_stride_t < p.D)) || (backward && p.Tq && p.dout_stride_t < p.D)) return false;
+    for (int64_t x : {p.q_stride_h, p.k_stride_h, p.v_stride_h, backward ? p.dout_stride_h : 0})
+        if (x % 8) return false;
+    return true;
 }
 static int packed_pointers(const EvoPacked &p, bool backward) {
     if (!p.offsets || !p.key_offsets) return EVO_EINVAL;
@@ -46,7 +69,7 @@ static int packed_pointers(const EvoPacked &p, bool backward) {
     if (p.Tk && (!p.k || !p.v || (backward && !p.dk != !p.dv))) return EVO_EINVAL;
     if (backward && p.Tq && p.workspace_bytes < evoattn_packed_bwd_workspace_bytes(&p)) return EVO_EWORKSPACE;
     if (!backward && p.workspace_bytes < evoattn_packed_fwd_workspace_bytes(&p)) return EVO_EWORKSPACE;
-    return EVO_OK;
+    return packed_aligned(p, backward) ? EVO_OK : EVO_EALIGN;
 }
 
 }  // namespace evo
@@ -64,12 +87,13 @@ int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
     if (const int rc = packed_check(p)) return rc;
     if (!p->Tq) return EVO_OK;
     if (const int rc = packed_pointers(*p, false)) return rc;
+    const hipStream_t st = (hipStream_t)hip_stream;
+    if (p->dtype != EVO_F32)
+        return p->D <= 32 ? launch_packed_fwd_d32(*p, st) : p->D <= 64 ? launch_packed_fwd_d64(*p, st) : p->D <= 96 ? launch_packed_fwd_d96(*p, st) : launch_packed_fwd_d128(*p, st);
     const int64_t rows = p->Tq * p->H;
     if (rows > INT32_MAX || !grid_fits((rows + 3) / 4, 256)) return EVO_EOVERFLOW;
-    return by_dtype(p->dtype, [&](auto t) {
-        packed_rows_fwd<decltype(t)><<<(unsigned)((rows + 3) / 4), 256, 0, (hipStream_t)hip_stream>>>(*p, (unsigned)rows);
-        return hip_rc();
-    });
+    packed_rows_fwd<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, (unsigned)rows);
+    return hip_rc();
 }
 
 size_t evoattn_packed_bwd_workspace_bytes(const EvoPacked *p) {
@@ -83,19 +107,21 @@ int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
     if (const int rc = packed_check(p)) return rc;
     if (!p->Tq && !p->Tk) return EVO_OK;
     if (const int rc = packed_pointers(*p, true)) return rc;
-    const int64_t rows = p->Tq * p->H, keys = p->Tk * p->Hk;
-    if (rows > INT32_MAX || keys > INT32_MAX || !grid_fits((rows + 3) / 4, 256) || !grid_fits((keys + 3) / 4, 256)) return EVO_EOVERFLOW;
     const hipStream_t st = (hipStream_t)hip_stream;
     float *delta = (float *)p->workspace;
-    return by_dtype(p->dtype, [&](auto t) {
-        typedef decltype(t) T;
-        if (rows) {
-            packed_rows_dq<T><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, delta, (unsigned)rows);
-            if (const int rc = hip_rc()) return rc;
-        }
-        if (keys && p->dk) packed_rows_dkdv<T><<<(unsigned)((keys + 3) / 4), 256, 0, st>>>(*p, delta, (unsigned)keys);
-        return hip_rc();
-    });
+    if (p->dtype != EVO_F32)
+        return p->D <= 32   ? launch_packed_bwd_d32(*p, delta, st)
+               : p->D <= 64 ? launch_packed_bwd_d64(*p, delta, st)
+               : p->D <= 96 ? launch_packed_bwd_d96(*p, delta, st)
+                            : launch_packed_bwd_d128(*p, delta, st);
+    const int64_t rows = p->Tq * p->H, keys = p->Tk * p->Hk;
+    if (rows > INT32_MAX || keys > INT32_MAX || !grid_fits((rows + 3) / 4, 256) || !grid_fits((keys + 3) / 4, 256)) return EVO_EOVERFLOW;
+    if (rows) {
+        packed_rows_dq<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, delta, (unsigned)rows);
+        if (const int rc = hip_rc()) return rc;
+    }
+    if (keys && p->dk) packed_rows_dkdv<float><<<(unsigned)((keys + 3) / 4), 256, 0, st>>>(*p, delta, (unsigned)keys);
+    return hip_rc();
 }
 
 }  // extern "C"

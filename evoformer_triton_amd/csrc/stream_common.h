@@ -40,6 +40,12 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned char *
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : : "s"(base), "v"(off), "s"(rs) : "m0", "memory");
 }
 
+// 4 bytes per lane, likewise
+__device__ __forceinline__ void dma4(__amdgpu_buffer_rsrc_t rs, unsigned char *dst, int off) {
+    const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" : : "s"(base), "v"(off), "s"(rs) : "m0", "memory");
+}
+
 // The first N of `x`, loaded above, are wanted from here on: all are under way by now.  A load written where a condition decides about its use
 // (`dead ? zeros : scaled(load)`) is put into that branch, asked for there and waited for at once: KSD round trips to memory one after the other
 // ahead of a workgroup's first stage.  Training step, S = 64, N = 512, H = 4, D = 128 303 -> 294 us; S = 200, N = 640, H = 5, D = 64, fp32 bias 925 -> 921.
