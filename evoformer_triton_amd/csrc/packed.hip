@@ -31,14 +31,22 @@ __global__ void __launch_bounds__(256) packed_rows_dkdv(EvoPacked p, const float
     row_dkdv<T>(p, segment_of_row<true>(p, j), j, hk, delta);
 }
 
-int launch_packed_fwd_d32(const EvoPacked &, hipStream_t);
-int launch_packed_fwd_d64(const EvoPacked &, hipStream_t);
-int launch_packed_fwd_d96(const EvoPacked &, hipStream_t);
-int launch_packed_fwd_d128(const EvoPacked &, hipStream_t);
-int launch_packed_bwd_d32(const EvoPacked &, float *, hipStream_t);
-int launch_packed_bwd_d64(const EvoPacked &, float *, hipStream_t);
-int launch_packed_bwd_d96(const EvoPacked &, float *, hipStream_t);
-int launch_packed_bwd_d128(const EvoPacked &, float *, hipStream_t);
+#define EVO_PACKED(D)                                                              \
+    int launch_packed_fwd_d##D(const EvoPacked &, hipStream_t);                    \
+    int launch_packed_bwd_d##D(const EvoPacked &, float *, hipStream_t);           \
+    size_t packed_few_bytes_d##D(const EvoPacked &);                               \
+    int launch_packed_few_d##D(const EvoPacked &, hipStream_t);
+EVO_PACKED(32)
+EVO_PACKED(64)
+EVO_PACKED(96)
+EVO_PACKED(128)
+#undef EVO_PACKED
+// One of the four by the head dim
+#define EVO_BY_HEAD_DIM(name, p, ...) \
+    ((p).D <= 32 ? name##_d32(__VA_ARGS__) : (p).D <= 64 ? name##_d64(__VA_ARGS__) : (p).D <= 96 ? name##_d96(__VA_ARGS__) : name##_d128(__VA_ARGS__))
+
+// Whether the kernel that splits the keys serves the forward: where a key head has few queries of few heads in a sequence.
+static bool few_queries(const EvoPacked &p) { return p.dtype != EVO_F32 && p.Tq * (p.H / p.Hk) <= (int64_t)64 * p.n; }
 
 static int packed_check(const EvoPacked *p) {
     if (!p || p->n < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1 || !known_dtype(p->dtype) || (p->offset_bytes != 4 && p->offset_bytes != 8) || p->Tq < 0 ||
@@ -78,8 +86,8 @@ extern "C" {
 
 size_t evoattn_packed_fwd_workspace_bytes(const EvoPacked *p) {
     using namespace evo;
-    if (packed_check(p)) return 0;
-    return 0;
+    if (packed_check(p) || !few_queries(*p)) return 0;
+    return EVO_BY_HEAD_DIM(packed_few_bytes, *p, *p);
 }
 
 int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
@@ -88,8 +96,8 @@ int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
     if (!p->Tq) return EVO_OK;
     if (const int rc = packed_pointers(*p, false)) return rc;
     const hipStream_t st = (hipStream_t)hip_stream;
-    if (p->dtype != EVO_F32)
-        return p->D <= 32 ? launch_packed_fwd_d32(*p, st) : p->D <= 64 ? launch_packed_fwd_d64(*p, st) : p->D <= 96 ? launch_packed_fwd_d96(*p, st) : launch_packed_fwd_d128(*p, st);
+    if (few_queries(*p)) return EVO_BY_HEAD_DIM(launch_packed_few, *p, *p, st);
+    if (p->dtype != EVO_F32) return EVO_BY_HEAD_DIM(launch_packed_fwd, *p, *p, st);
     const int64_t rows = p->Tq * p->H;
     if (rows > INT32_MAX || !grid_fits((rows + 3) / 4, 256)) return EVO_EOVERFLOW;
     packed_rows_fwd<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, (unsigned)rows);
@@ -109,11 +117,7 @@ int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
     if (const int rc = packed_pointers(*p, true)) return rc;
     const hipStream_t st = (hipStream_t)hip_stream;
     float *delta = (float *)p->workspace;
-    if (p->dtype != EVO_F32)
-        return p->D <= 32   ? launch_packed_bwd_d32(*p, delta, st)
-               : p->D <= 64 ? launch_packed_bwd_d64(*p, delta, st)
-               : p->D <= 96 ? launch_packed_bwd_d96(*p, delta, st)
-                            : launch_packed_bwd_d128(*p, delta, st);
+    if (p->dtype != EVO_F32) return EVO_BY_HEAD_DIM(launch_packed_bwd, *p, *p, delta, st);
     const int64_t rows = p->Tq * p->H, keys = p->Tk * p->Hk;
     if (rows > INT32_MAX || keys > INT32_MAX || !grid_fits((rows + 3) / 4, 256) || !grid_fits((keys + 3) / 4, 256)) return EVO_EOVERFLOW;
     if (rows) {

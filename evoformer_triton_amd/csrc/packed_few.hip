@@ -1,0 +1,313 @@
+// Attention within packed sequences where a sequence has few queries: tokens that are added to sequences.  16-bit, compiled once per head dim (-DEVO_D=32|64|96|128).
+//
+// Bound by memory: keys and values are read once and little is computed with them.  So the keys are split: a workgroup takes a chunk of one sequence's keys and one key head,
+// its waves take 32 keys at a time each, and the queries of all heads that share the key head are the 16 columns of a matrix instruction (v_mfma_f32_16x16x32, S^T = K Q^T and O^T = V^T P^T as
+// in packed_mfma.hip; more than 16 of them: 16 after 16).  A wave brings its keys and values into LDS of its own by the load path itself and waits for nobody: the next keys are asked for when
+// the scores are formed, the next values when they have been multiplied; many waves with 16 KB (head dim 128) under way each are what memory's latency takes.  The waves' maxima, sums and
+// outputs are joined in LDS; with more than one chunk to a sequence a second kernel joins the chunks', in their order.
+//
+// Which chunk: as for the tiles of packed_mfma.hip, chunk t of the launch belongs to the last segment j with key_begin(j) / chunk + j <= t, so that sequences of any lengths are spread evenly.
+#include "packed_tiles.h"
+
+namespace evo {
+
+namespace EVO_CAT(packed_d, EVO_D) {
+
+template <typename T> struct Mfma16;
+template <> struct Mfma16<bf16_t> {
+    static __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mfma16<f16_t> {
+    static __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+struct Few {
+    typedef PackedGeo::G G;
+    static constexpr int KEYS = 32, ROWS = 16;                       // keys of a wave's step; columns
+    static constexpr int ARRAY = KEYS * G::ROW, PIECES = ARRAY / 1024, RPP = 1024 / G::ROW;
+    static constexpr int WAVES = PackedGeo::GD == 128 ? 8 : 16;      // (two arrays each: 128 KB of LDS, head dim 32: 64)
+    static constexpr int KS = EVO_D / 32, DT = EVO_D / 16;
+    static constexpr int PITCH = EVO_D + 4;                          // of a joined row, fp32
+    static constexpr int JOIN = WAVES * ROWS * (PITCH + 2) * 4;
+    static constexpr int LDS = 2 * ARRAY * WAVES > JOIN ? 2 * ARRAY * WAVES : JOIN;
+};
+
+// Scratch of chunks: [chunk][token][head] rows of D fp32 relative to 2^m, and (m, l)
+struct Parts {
+    float *o;
+    float2 *ml;
+    int chunk;   // keys of one
+    int chunks;  // the most of a sequence
+};
+
+template <typename T, bool PART>
+__global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts parts) {
+    typedef PackedGeo R;
+    typedef R::G G;
+    typedef typename Mfma<T>::v8 v8;
+    typedef typename Mfma<T>::v4 v4;
+    __shared__ __attribute__((aligned(1024))) unsigned char lds[Few::LDS];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, gq = lane >> 4;
+    const int group = p.H / p.Hk, D = p.D;
+    const int hk = (int)(blockIdx.x % (unsigned)p.Hk), t = (int)(blockIdx.x / (unsigned)p.Hk);
+    const int j = last_where(p.n + 2, [&](int x) { return keys_begin(p, x) / parts.chunk + x <= t; });
+    const Segment s = segment(p, j);
+    const int index = t - (s.k0 / parts.chunk + j);
+    if (index < 0) return;
+    const int64_t c0 = (int64_t)index * parts.chunk;
+    const int nk = s.gap ? 0 : s.nk();
+    if (c0 >= nk && (PART || index > 0)) return;
+    const int key_from = (int)c0, key_to = (int)min((int64_t)nk, c0 + parts.chunk);   // (none: zeros, by the only chunk)
+    const int64_t rows = (int64_t)s.nq() * group;
+    const int kst = (int)p.k_stride_t * 2, vst = (int)p.v_stride_t * 2;
+    const char *kbase = (const char *)head_row<T>(p.k, s.k0, p.k_stride_t, hk, p.k_stride_h), *vbase = (const char *)head_row<T>(p.v, s.k0, p.v_stride_t, hk, p.v_stride_h);
+    unsigned char *const kbuf = lds + wave * 2 * Few::ARRAY, *const vbuf = kbuf + Few::ARRAY;
+    auto fetch = [&](const char *base, int stride, unsigned char *dst, int key) {
+        const __amdgpu_buffer_rsrc_t rs = rows_at(base + (int64_t)key * stride, min(Few::KEYS, nk - key), stride, D);
+#pragma unroll
+        for (int i = 0; i < Few::PIECES; ++i) {
+            const int r = i * Few::RPP + lane / G::C, c = (lane % G::C) ^ G::x(r);
+            dma16(rs, dst + i * 1024, c * 8 < D ? r * stride + c * 16 : kFarOff);
+        }
+    };
+    v8 one;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) one[i] = (T)1.0f;
+    const float c = p.scale * kLog2e;
+
+    for (int64_t r0 = 0; r0 < rows; r0 += Few::ROWS) {
+        // this lane's column: a query and a head
+        const int64_t pr = min(r0 + col, rows - 1);
+        const int i = s.q0 + (int)(pr / group), h = hk * group + (int)(pr % group), seen = s.gap ? 0 : s.seen(i, p.causal);
+        float m = kMaskFloor, l = 0.0f;
+        f32x4 o[Few::DT];
+#pragma unroll
+        for (int dt = 0; dt < Few::DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        int key = key_from + wave * Few::KEYS;
+        if (key < key_to) {
+            fetch(kbase, kst, kbuf, key);
+            fetch(vbase, vst, vbuf, key);
+            v8 qf[Few::KS];
+            const T *q = head_row<T>(p.q, i, p.q_stride_t, h, p.q_stride_h);
+#pragma unroll
+            for (int ks = 0; ks < Few::KS; ++ks) qf[ks] = ks * 32 + gq * 8 < D ? ld8(q + ks * 32 + gq * 8) : zero8<T>();
+            asked_together<Few::KS>(qf);   // (waited for here, with the first keys and values: what is counted below are the rows' loads alone)
+            for (;;) {
+                const int next = key + Few::WAVES * Few::KEYS;
+                const bool more = next < key_to;   // (uniform)
+                wait_loads_but<Few::PIECES>();      // the keys (the values are younger)
+                f32x4 a[2];
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt) {
+                    a[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < Few::KS; ++ks) a[tt] = Mfma16<T>::mma(*reinterpret_cast<const v8 *>(kbuf + G::at(16 * tt + col, 4 * ks + gq)), qf[ks], a[tt]);
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        a[tt][r] = key + 16 * tt + 4 * gq + r < seen ? a[tt][r] : -INFINITY;
+                        top = fmaxf(top, a[tt][r]);
+                    }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the keys have been read
+                if (more) fetch(kbase, kst, kbuf, next);
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float mn = fmaxf(m, top * c), alpha = fast_exp2(m - mn);
+                m = mn;
+                v8 pf;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) pf[x] = (T)fast_exp2(fmaf(a[x >> 2][x & 3], c, -m));
+                l = dot8<T>(pf, one, l * alpha);
+#pragma unroll
+                for (int dt = 0; dt < Few::DT; ++dt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
+                if (more) wait_loads_but<Few::PIECES>();   // the values (the next keys are younger)
+                else wait_loads();
+#pragma unroll
+                for (int dt = 0; dt < Few::DT; ++dt) {
+                    v8 vt;   // V^T: row 16 dt + col, the keys in the order in which a lane holds their probabilities
+#pragma unroll
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        const int row = 16 * h2 + 4 * gq + (col >> 2), at = dt * 16 + 4 * (lane & 3);
+                        const s16x4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4s __attribute__((address_space(3))) *)(vbuf + G::at(row, at >> 3) + (at & 7) * 2));
+                        const v4 x = __builtin_bit_cast(v4, w);
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) vt[4 * h2 + y] = x[y];
+                    }
+                    o[dt] = Mfma16<T>::mma(vt, pf, o[dt]);
+                }
+                if (!more) break;
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the values have been read
+                fetch(vbase, vst, vbuf, next);
+                key = next;
+            }
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        // The waves' parts joined, every thread four columns of a row
+        __syncthreads();
+        float *const jo = reinterpret_cast<float *>(lds), *const jm = jo + Few::WAVES * Few::ROWS * Few::PITCH, *const jl = jm + Few::WAVES * Few::ROWS;
+#pragma unroll
+        for (int dt = 0; dt < Few::DT; ++dt) *reinterpret_cast<f32x4 *>(jo + (wave * Few::ROWS + col) * Few::PITCH + dt * 16 + gq * 4) = o[dt];
+        if (gq == 0) {
+            jm[wave * Few::ROWS + col] = m;
+            jl[wave * Few::ROWS + col] = l;
+        }
+        __syncthreads();
+        const int jr = threadIdx.x / (EVO_D / 4), d = threadIdx.x % (EVO_D / 4) * 4;
+        const bool mine = jr < Few::ROWS && r0 + jr < rows;
+        bool nan = false;
+        if (mine) {
+            float M = kMaskFloor, L = 0.0f;
+#pragma unroll 4
+            for (int w = 0; w < Few::WAVES; ++w) M = fmaxf(M, jm[w * Few::ROWS + jr]);
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (int w = 0; w < Few::WAVES; ++w) {
+                const float f = fast_exp2(jm[w * Few::ROWS + jr] - M);
+                L = fmaf(jl[w * Few::ROWS + jr], f, L);
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(jo + (w * Few::ROWS + jr) * Few::PITCH + d);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum[y] = fmaf(x[y], f, sum[y]);
+            }
+            const int64_t own = r0 + jr;
+            const int oi = s.q0 + (int)(own / group), oh = hk * group + (int)(own % group);
+            const int64_t row = (int64_t)oi * p.H + oh;
+            if (PART) {
+                const int64_t at = (int64_t)index * p.Tq * p.H + row;
+                if (d < D) *reinterpret_cast<f32x4 *>(parts.o + at * D + d) = sum;
+                if (d == 0) parts.ml[at] = make_float2(M, L);
+            } else {
+                const bool sees = nk > 0 && s.seen(oi, p.causal) > 0;
+                const float inv = sees ? 1.0f / L : 0.0f;
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    sum[y] = sees ? sum[y] * inv : 0.0f;
+                    nan |= d < D && !(sum[y] == sum[y]);
+                }
+                if (d < D) store4<T>((T *)p.o + row * D + d, sum[0], sum[1], sum[2], sum[3]);
+                if (d == 0 && p.lse) p.lse[(int64_t)oh * p.Tq + oi] = sees ? M + __log2f(L) : INFINITY;
+            }
+        }
+        const bool again = __syncthreads_or(!PART && nan);
+        if (again) {   // some row holds something that is no number: all of them once more, with the rows that are seen alone
+            for (int x = wave; x < Few::ROWS && r0 + x < rows; x += Few::WAVES)
+                row_forward<T>(p, s, s.q0 + (int)((r0 + x) / group), hk * group + (int)((r0 + x) % group));
+        }
+    }
+}
+
+// The chunks of a row joined: `per` waves (1 or 4) take every per-th of them.
+template <typename T>
+__global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int per, unsigned rows) {
+    __shared__ float sums[4][128], rest[4];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), own = wave % per;
+    const unsigned row = blockIdx.x * (4 / per) + wave / per;
+    const bool mine = row < rows;   // (uniform over the wave; over the workgroup where waves share a row)
+    const int i = (int)(min(row, rows - 1) / (unsigned)p.H), h = (int)(min(row, rows - 1) % (unsigned)p.H), D = p.D;
+    const Segment s = segment_of_row<false>(p, i);
+    const int chunks = s.gap ? 0 : min(parts.chunks, (s.nk() + parts.chunk - 1) / parts.chunk);
+    const int64_t step = p.Tq * p.H;
+    const float2 *ml = parts.ml + (int64_t)i * p.H + h;
+    const float *o = parts.o + ((int64_t)i * p.H + h) * D;
+    float M = kMaskFloor;
+    for (int x = lane; x < chunks; x += 64) M = fmaxf(M, ml[x * step].x);
+    M = wave_max(M);
+    float L = 0.0f, a = 0.0f, b = 0.0f;
+    const int d = min(lane * 2, D - 2);
+#pragma unroll 4
+    for (int x = own; x < chunks; x += per) {
+        const float2 y = ml[x * step], z = *reinterpret_cast<const float2 *>(o + x * step * D + d);
+        const float f = fast_exp2(y.x - M);
+        L = fmaf(y.y, f, L);
+        a = fmaf(z.x, f, a);
+        b = fmaf(z.y, f, b);
+    }
+    if (per > 1) {
+        if (lane * 2 < 128) {
+            sums[wave][lane * 2] = a;
+            sums[wave][lane * 2 + 1] = b;
+        }
+        if (lane == 0) rest[wave] = L;
+        __syncthreads();
+        if (own) return;
+        for (int w = 1; w < per; ++w) {
+            a += sums[w][lane * 2];
+            b += sums[w][lane * 2 + 1];
+            L += rest[w];
+        }
+    }
+    if (!mine) return;
+    const bool sees = !s.gap && s.seen(i, p.causal) > 0;
+    const float inv = sees ? 1.0f / L : 0.0f;
+    a = sees ? a * inv : 0.0f;
+    b = sees ? b * inv : 0.0f;
+    const bool used = lane * 2 < D;
+    if (__any(used && (!(a == a) || !(b == b)))) {
+        row_forward<T>(p, s, i, h);
+        return;
+    }
+    if (used) {
+        T *out = (T *)p.o + ((int64_t)i * p.H + h) * D + lane * 2;
+        typename Mfma<T>::v2 x;
+        x[0] = (T)a;
+        x[1] = (T)b;
+        *reinterpret_cast<typename Mfma<T>::v2 *>(out) = x;
+    }
+    if (lane == 0 && p.lse) p.lse[(int64_t)h * p.Tq + i] = sees ? M + __log2f(L) : INFINITY;
+}
+
+// Keys of a chunk: as many as make some kFewWorkgroups workgroups of all keys and key heads, at least four steps of every wave (a workgroup that has only one spends its time on finding its place and
+// joining), all of them where one workgroup's walk over them takes less time than a second launch does.  And not so few that the parts take more than kFewScratch bytes.
+constexpr int64_t kFewWorkgroups = 512, kFewScratch = 64 << 20;
+static Parts few_parts(const EvoPacked &p, void *workspace, size_t *bytes) {
+    constexpr int64_t unit = Few::WAVES * Few::KEYS;
+    const int64_t part = p.Tq * p.H * ((int64_t)p.D + 2) * (int64_t)sizeof(float), most = kFewScratch / (part ? part : 1);
+    int64_t chunk = p.Tk * p.Hk / kFewWorkgroups;
+    if (chunk < 4 * unit) chunk = 4 * unit;
+    if (most < 2) chunk = p.Tk;
+    else if (chunk < (p.Tk + most - 1) / most) chunk = (p.Tk + most - 1) / most;
+    chunk = (chunk + unit - 1) / unit * unit;
+    if (chunk < unit) chunk = unit;
+    if (p.Tk <= 8 * unit && chunk < p.Tk) chunk = (p.Tk + unit - 1) / unit * unit;
+    Parts r;
+    r.chunk = (int)chunk;
+    r.chunks = (int)((p.Tk + chunk - 1) / chunk);
+    r.o = (float *)workspace;
+    r.ml = (float2 *)(r.o + (int64_t)r.chunks * p.Tq * p.H * p.D);
+    if (bytes) *bytes = r.chunks > 1 ? (size_t)(r.chunks * part) : 0;
+    return r;
+}
+
+}  // namespace
+
+size_t EVO_CAT(packed_few_bytes_d, EVO_D)(const EvoPacked &p) {
+    size_t bytes;
+    EVO_CAT(packed_d, EVO_D)::few_parts(p, nullptr, &bytes);
+    return bytes;
+}
+int EVO_CAT(launch_packed_few_d, EVO_D)(const EvoPacked &p, hipStream_t st) {
+    using namespace EVO_CAT(packed_d, EVO_D);
+    const Parts parts = few_parts(p, p.workspace, nullptr);
+    const int64_t grid = (p.Tk / parts.chunk + p.n + 2) * p.Hk, rows = p.Tq * p.H;
+    if (rows > INT32_MAX || !grid_fits(grid, Few::WAVES * 64) || !grid_fits(rows, 256)) return EVO_EOVERFLOW;
+    return by_half(p.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        if (parts.chunks <= 1) {
+            packed_few<T, false><<<(unsigned)grid, Few::WAVES * 64, 0, st>>>(p, parts);
+            return hip_rc();
+        }
+        packed_few<T, true><<<(unsigned)grid, Few::WAVES * 64, 0, st>>>(p, parts);
+        if (const int rc = hip_rc()) return rc;
+        const int per = parts.chunks > 8 ? 4 : 1;
+        packed_join<T><<<(unsigned)((rows * per + 3) / 4), 256, 0, st>>>(p, parts, per, (unsigned)rows);
+        return hip_rc();
+    });
+}
+
+}  // namespace evo

@@ -11,32 +11,14 @@
 //
 // A row of V beyond the sequence's end is read as zeros (the load is out of range).  One that causal queries do not see may hold an infinity or a NaN, which a probability of
 // zero does not keep out of the sums: results that are no numbers are formed anew, row by row (row_forward and its like), with the rows that are seen alone.
-#include "packed_common.h"
-#include "stream_common.h"
-
-#ifndef EVO_D
-#error "compile with -DEVO_D=<head dim>"
-#endif
+#include "packed_tiles.h"
 
 namespace evo {
 
-namespace EVO_CAT(packed_d, EVO_D) {   // (one name for each head dim's kernels)
+namespace EVO_CAT(packed_d, EVO_D) {
 
 constexpr int kPackedRows = 128;   // of a workgroup
-constexpr int kFarOff = 0x7fffff00;   // an offset past the end of every array
 
-struct PackedGeo {
-    static constexpr int GD = EVO_D == 96 ? 128 : EVO_D;   // rows in LDS (96: three quarters of them used)
-    typedef StreamGeo<GD> G;
-    static constexpr int KSD = EVO_D / 16, DT = EVO_D / 32;
-    static constexpr int STAGE = 64;
-    static constexpr int ARRAY = STAGE * G::ROW;
-};
-
-// Rows at `base`, `rows` of them, stride_t bytes apart, as a resource whose end is the end of the last: what is asked for beyond reads as zeros.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void *base, int rows, int stride, int D) {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, rows > 0 ? (rows - 1) * stride + D * 2 : 0, 0x00020000);
-}
 // This lane's offset of its first piece of a stage of rows; its further pieces are kPieceRows rows on each.
 template <int NW>
 struct StagePieces {
@@ -481,11 +463,6 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 3 : 2) packed_dkdv(EvoPacke
 // ------------------------------------------------------------------ launches
 
 static int64_t packed_tiles(int64_t rows, int n) { return rows / kPackedRows + n + 2; }
-
-template <typename F>
-static int by_half(int dtype, F &&f) {
-    return dtype == EVO_BF16 ? f(bf16_t()) : f(f16_t());
-}
 
 }  // namespace
 
