@@ -42,7 +42,7 @@ struct Packed {
         if (ko.size(0) != offsets_.size(0)) return "key_offsets must be as long as offsets";
         if (!own && k_.size(0) != q_.size(0)) return "keys that are not as many as queries need key_offsets";
         const double s = scale ? *scale : 1.0 / std::sqrt((double)D);
-        if (!((float)s > 0.0f && (float)s <= FLT_MAX)) return "scale must be a positive number";
+        if (!((float)s >= 0x1p-64f && (float)s <= 0x1p64f)) return "scale must be a positive number, 2^-64 to 2^64";
         const int64_t Tq = q_.size(0), Tk = k_.size(0), most = INT32_MAX / 2;
         if (Tq > most || Tk > most || offsets_.size(0) > INT32_MAX / 4 || H > 1 << 20) return "2^30 rows, 2^29 sequences or more than 2^20 heads are too many";
         p.n = (int32_t)(offsets_.size(0) - 1);

@@ -20,7 +20,7 @@ __global__ void __launch_bounds__(256) packed_rows_dq(EvoPacked p, float *delta,
     if (row >= rows) return;
     const int i = row / (unsigned)p.H, h = row % (unsigned)p.H;
     const float d = row_delta<T>(p, i, h);
-    if ((threadIdx.x & 63) == 0) delta[(int64_t)h * p.Tq + i] = d;
+    if ((threadIdx.x & 63) == 0) delta[(int64_t)h * p.Tq + i] = -d;
     row_dq<T>(p, segment_of_row<false>(p, i), i, h, d);
 }
 template <typename T>
@@ -33,7 +33,8 @@ __global__ void __launch_bounds__(256) packed_rows_dkdv(EvoPacked p, const float
 
 #define EVO_PACKED(D)                                                              \
     int launch_packed_fwd_d##D(const EvoPacked &, hipStream_t);                    \
-    int launch_packed_bwd_d##D(const EvoPacked &, float *, hipStream_t);           \
+    int launch_packed_dq_d##D(const EvoPacked &, const BackwardRows &, hipStream_t);\
+    int launch_packed_dkdv_d##D(const EvoPacked &, const BackwardRows &, hipStream_t);\
     size_t packed_few_bytes_d##D(const EvoPacked &);                               \
     int launch_packed_few_d##D(const EvoPacked &, hipStream_t);
 EVO_PACKED(32)
@@ -50,7 +51,7 @@ static bool few_queries(const EvoPacked &p) { return p.dtype != EVO_F32 && p.Tq 
 
 static int packed_check(const EvoPacked *p) {
     if (!p || p->n < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1 || !known_dtype(p->dtype) || (p->offset_bytes != 4 && p->offset_bytes != 8) || p->Tq < 0 ||
-        p->Tk < 0 || !(p->scale > 0.0f && p->scale <= FLT_MAX))
+        p->Tk < 0 || !(p->scale >= 0x1p-64f && p->scale <= 0x1p64f))   // (the backward divides sums of exponents by it)
         return EVO_EINVAL;
     if (p->D > 128) return EVO_EUNSUPPORTED;
     // (row numbers and the positions of tiles are formed in 32 bits)
@@ -107,7 +108,7 @@ int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
 size_t evoattn_packed_bwd_workspace_bytes(const EvoPacked *p) {
     using namespace evo;
     if (packed_check(p)) return 0;
-    return (size_t)p->H * p->Tq * sizeof(float);
+    return (size_t)p->H * p->Tq * sizeof(float) * (p->dtype == EVO_F32 ? 1 : 2);
 }
 
 int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
@@ -116,15 +117,20 @@ int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
     if (!p->Tq && !p->Tk) return EVO_OK;
     if (const int rc = packed_pointers(*p, true)) return rc;
     const hipStream_t st = (hipStream_t)hip_stream;
-    float *delta = (float *)p->workspace;
-    if (p->dtype != EVO_F32) return EVO_BY_HEAD_DIM(launch_packed_bwd, *p, *p, delta, st);
+    const BackwardRows saved = {(float *)p->workspace, (float *)p->workspace + (int64_t)p->H * p->Tq};
+    if (p->dtype != EVO_F32) {
+        if (p->Tq) {
+            if (const int rc = EVO_BY_HEAD_DIM(launch_packed_dq, *p, *p, saved, st)) return rc;
+        }
+        return p->Tk && p->dk ? EVO_BY_HEAD_DIM(launch_packed_dkdv, *p, *p, saved, st) : EVO_OK;
+    }
     const int64_t rows = p->Tq * p->H, keys = p->Tk * p->Hk;
     if (rows > INT32_MAX || keys > INT32_MAX || !grid_fits((rows + 3) / 4, 256) || !grid_fits((keys + 3) / 4, 256)) return EVO_EOVERFLOW;
     if (rows) {
-        packed_rows_dq<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, delta, (unsigned)rows);
+        packed_rows_dq<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, saved.delta, (unsigned)rows);
         if (const int rc = hip_rc()) return rc;
     }
-    if (keys && p->dk) packed_rows_dkdv<float><<<(unsigned)((keys + 3) / 4), 256, 0, st>>>(*p, delta, (unsigned)keys);
+    if (keys && p->dk) packed_rows_dkdv<float><<<(unsigned)((keys + 3) / 4), 256, 0, st>>>(*p, saved.delta, (unsigned)keys);
     return hip_rc();
 }
 

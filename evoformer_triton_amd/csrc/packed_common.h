@@ -103,6 +103,11 @@ __device__ __forceinline__ const T *head_row(const void *x, int64_t row, int64_t
     return (const T *)x + row * stride_t + h * stride_h;
 }
 
+// What dQ's kernel leaves for that of dK and dV, [H][Tq] each: -delta, and the row's log-sum -lse in units of q . k (16 bits: what their products begin with).
+struct BackwardRows {
+    float *delta, *base;
+};
+
 // ---- One row by one wave, products and sums in fp32: the kernels for fp32, and what the matrix kernels leave for rows whose result is no
 // number: there a masked key or query may hold an infinity or a NaN, which a product with a probability of zero does not keep out.
 
@@ -157,7 +162,7 @@ __device__ __forceinline__ void row_dq(const EvoPacked &p, const Segment &s, int
 }
 
 template <typename T>
-__device__ __forceinline__ void row_dkdv(const EvoPacked &p, const Segment &s, int j, int hk, const float *delta) {
+__device__ __forceinline__ void row_dkdv(const EvoPacked &p, const Segment &s, int j, int hk, const float *minus_delta) {
     const int lane = threadIdx.x & 63, G = p.H / p.Hk;
     const float c = p.scale * kLog2e;
     const Row k = load_row(head_row<T>(p.k, j, p.k_stride_t, hk, p.k_stride_h), p.D), v = load_row(head_row<T>(p.v, j, p.v_stride_t, hk, p.v_stride_h), p.D);
@@ -171,7 +176,7 @@ __device__ __forceinline__ void row_dkdv(const EvoPacked &p, const Segment &s, i
             if (lane < n) {
                 const int i = i0 + lane;
                 e = fast_exp2(own_dot(k, head_row<T>(p.q, i, p.q_stride_t, h, p.q_stride_h), p.D) * c - p.lse[(int64_t)h * p.Tq + i]);
-                ds = e * (own_dot(v, head_row<T>(p.dout, i, p.dout_stride_t, h, p.dout_stride_h), p.D) - delta[(int64_t)h * p.Tq + i]) * p.scale;
+                ds = e * (own_dot(v, head_row<T>(p.dout, i, p.dout_stride_t, h, p.dout_stride_h), p.D) + minus_delta[(int64_t)h * p.Tq + i]) * p.scale;
             }
             for (int i = 0; i < n; ++i) {
                 add_row(dv, lane_value(e, i), load_row(head_row<T>(p.dout, i0 + i, p.dout_stride_t, h, p.dout_stride_h), p.D));

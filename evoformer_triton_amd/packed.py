@@ -23,7 +23,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     offsets      int32 or int64 [sequences + 1] on the same device, ascending from 0 to at most Tq: sequence s has the queries offsets[s] .. offsets[s + 1] - 1
     key_offsets  likewise for the keys; the queries' if not given
     causal       a sequence's queries are its last ones: the last sees every key, the one before all but the last key, and so on
-    scale        positive; D^-0.5 if not given
+    scale        positive (2^-64 to 2^64); D^-0.5 if not given
 
     Rows of no sequence (behind the last) and rows without a key get zeros, as do their gradients; what lies in rows that a query does not see, infinities and NaN among
     it, does not reach its result.  Probabilities multiply the values, and the scores' gradients queries and keys, rounded to the inputs' type; sums are in fp32.  Gradients: q, k and v, the same bits

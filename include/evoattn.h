@@ -398,7 +398,7 @@ int evoattn_rotary(const EvoRotary *p, void *hip_stream);
  * [0, T] (others are brought there: no access is out of bounds, what such rows hold is not specified).  Rows of no sequence and rows that see no key get zeros, in o and in the gradients.
  *   lse  [H][Tq] fp32: log2 of the row's sum of 2^(scale log2(e) q . k), for the backward (+inf: no key); may be NULL in the forward
  *   dk, dv  both may be NULL (not wanted)
- * D at most 128; scale positive.  16-bit: D and all strides multiples of 8, pointers on 16-byte boundaries, row strides from D to 2^23 (EVO_EALIGN
+ * D at most 128; scale 2^-64 to 2^64.  16-bit: D and all strides multiples of 8, pointers on 16-byte boundaries, row strides from D to 2^23 (EVO_EALIGN
  * otherwise).  `workspace` of evoattn_packed_fwd_workspace_bytes() (0: none needed) and evoattn_packed_bwd_workspace_bytes().  The backward is
  * deterministic.  Nothing is allocated or synchronised. */
 typedef struct EvoPacked {
