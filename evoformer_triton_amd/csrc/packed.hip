@@ -33,8 +33,11 @@ __global__ void __launch_bounds__(256) packed_rows_dkdv(EvoPacked p, const float
 
 #define EVO_PACKED(D)                                                              \
     int launch_packed_fwd_d##D(const EvoPacked &, hipStream_t);                    \
-    int launch_packed_dq_d##D(const EvoPacked &, const BackwardRows &, hipStream_t);\
-    int launch_packed_dkdv_d##D(const EvoPacked &, const BackwardRows &, hipStream_t);\
+    int launch_packed_dq_d##D(const EvoPacked &, const BackwardRows &, float *, hipStream_t);   \
+    int launch_packed_dkdv_d##D(const EvoPacked &, const BackwardRows &, float *, hipStream_t); \
+    size_t packed_dq_bytes_d##D(const EvoPacked &);                                \
+    size_t packed_dkdv_bytes_d##D(const EvoPacked &);                              \
+    size_t packed_fwd_bytes_d##D(const EvoPacked &);                               \
     size_t packed_few_bytes_d##D(const EvoPacked &);                               \
     int launch_packed_few_d##D(const EvoPacked &, hipStream_t);
 EVO_PACKED(32)
@@ -48,6 +51,8 @@ EVO_PACKED(128)
 
 // Whether the kernel that splits the keys serves the forward: where a key head has few queries of few heads in a sequence.
 static bool few_queries(const EvoPacked &p) { return p.dtype != EVO_F32 && p.Tq * (p.H / p.Hk) <= (int64_t)64 * p.n; }
+
+static int64_t align_rows(int64_t n) { return (n + 63) / 64 * 64; }   // (16-byte pieces behind them)
 
 static int packed_check(const EvoPacked *p) {
     if (!p || p->n < 0 || p->H < 1 || p->Hk < 1 || p->H % p->Hk || p->D < 1 || !known_dtype(p->dtype) || (p->offset_bytes != 4 && p->offset_bytes != 8) || p->Tq < 0 ||
@@ -76,7 +81,7 @@ static int packed_pointers(const EvoPacked &p, bool backward) {
     if (!p.offsets || !p.key_offsets) return EVO_EINVAL;
     if (p.Tq && (!p.q || !p.o || (backward && (!p.dout || !p.dq || !p.lse)))) return EVO_EINVAL;
     if (p.Tk && (!p.k || !p.v || (backward && !p.dk != !p.dv))) return EVO_EINVAL;
-    if (backward && p.Tq && p.workspace_bytes < evoattn_packed_bwd_workspace_bytes(&p)) return EVO_EWORKSPACE;
+    if (backward && p.workspace_bytes < evoattn_packed_bwd_workspace_bytes(&p)) return EVO_EWORKSPACE;
     if (!backward && p.workspace_bytes < evoattn_packed_fwd_workspace_bytes(&p)) return EVO_EWORKSPACE;
     return packed_aligned(p, backward) ? EVO_OK : EVO_EALIGN;
 }
@@ -87,8 +92,8 @@ extern "C" {
 
 size_t evoattn_packed_fwd_workspace_bytes(const EvoPacked *p) {
     using namespace evo;
-    if (packed_check(p) || !few_queries(*p)) return 0;
-    return EVO_BY_HEAD_DIM(packed_few_bytes, *p, *p);
+    if (packed_check(p) || p->dtype == EVO_F32) return 0;
+    return few_queries(*p) ? EVO_BY_HEAD_DIM(packed_few_bytes, *p, *p) : EVO_BY_HEAD_DIM(packed_fwd_bytes, *p, *p);
 }
 
 int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
@@ -108,7 +113,10 @@ int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
 size_t evoattn_packed_bwd_workspace_bytes(const EvoPacked *p) {
     using namespace evo;
     if (packed_check(p)) return 0;
-    return (size_t)p->H * p->Tq * sizeof(float) * (p->dtype == EVO_F32 ? 1 : 2);
+    const size_t rows = (size_t)align_rows((int64_t)p->H * p->Tq) * sizeof(float);
+    if (p->dtype == EVO_F32) return rows;
+    const size_t dq = EVO_BY_HEAD_DIM(packed_dq_bytes, *p, *p), dkdv = EVO_BY_HEAD_DIM(packed_dkdv_bytes, *p, *p);
+    return 2 * rows + (dq > dkdv ? dq : dkdv);
 }
 
 int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
@@ -117,12 +125,13 @@ int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
     if (!p->Tq && !p->Tk) return EVO_OK;
     if (const int rc = packed_pointers(*p, true)) return rc;
     const hipStream_t st = (hipStream_t)hip_stream;
-    const BackwardRows saved = {(float *)p->workspace, (float *)p->workspace + (int64_t)p->H * p->Tq};
+    const BackwardRows saved = {(float *)p->workspace, (float *)p->workspace + align_rows((int64_t)p->H * p->Tq)};
     if (p->dtype != EVO_F32) {
+        float *const sums = saved.base + align_rows((int64_t)p->H * p->Tq);   // (dQ's parts, then dK's and dV's)
         if (p->Tq) {
-            if (const int rc = EVO_BY_HEAD_DIM(launch_packed_dq, *p, *p, saved, st)) return rc;
+            if (const int rc = EVO_BY_HEAD_DIM(launch_packed_dq, *p, *p, saved, sums, st)) return rc;
         }
-        return p->Tk && p->dk ? EVO_BY_HEAD_DIM(launch_packed_dkdv, *p, *p, saved, st) : EVO_OK;
+        return p->Tk && p->dk ? EVO_BY_HEAD_DIM(launch_packed_dkdv, *p, *p, saved, sums, st) : EVO_OK;
     }
     const int64_t rows = p->Tq * p->H, keys = p->Tk * p->Hk;
     if (rows > INT32_MAX || keys > INT32_MAX || !grid_fits((rows + 3) / 4, 256) || !grid_fits((keys + 3) / 4, 256)) return EVO_EOVERFLOW;

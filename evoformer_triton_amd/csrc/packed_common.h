@@ -14,6 +14,8 @@ struct Segment {
     __device__ __forceinline__ int nk() const { return k1 - k0; }
     // the keys that query i (of the tensor) sees: k0 .. k0 + seen(i) - 1
     __device__ __forceinline__ int seen(int i, bool causal) const { return causal ? max(0, min(nk(), nk() - nq() + (i - q0) + 1)) : nk(); }
+    // the first query (of the tensor) that sees key j (of the tensor); q1 or beyond: none does
+    __device__ __forceinline__ int first_query(int j, bool causal) const { return causal ? q0 + max(0, (j - k0) - (nk() - nq())) : q0; }
 };
 
 // Where segment j of n + 2 begins: 0 before the first sequence, then the sequences, then what is behind the last.  Brought into [0, T] whatever the offsets hold.
@@ -168,7 +170,7 @@ __device__ __forceinline__ void row_dkdv(const EvoPacked &p, const Segment &s, i
     const Row k = load_row(head_row<T>(p.k, j, p.k_stride_t, hk, p.k_stride_h), p.D), v = load_row(head_row<T>(p.v, j, p.v_stride_t, hk, p.v_stride_h), p.D);
     Row dk = {0.0f, 0.0f}, dv = {0.0f, 0.0f};
     // the first query that sees this key
-    const int first = s.gap ? s.q1 : p.causal ? s.q0 + max(0, (j - s.k0) - (s.nk() - s.nq())) : s.q0;
+    const int first = s.gap ? s.q1 : s.first_query(j, p.causal);
     for (int h = hk * G; h < (hk + 1) * G; ++h) {
         for (int i0 = first; i0 < s.q1; i0 += 64) {
             const int n = min(64, s.q1 - i0);

@@ -32,14 +32,6 @@ struct Few {
     static constexpr int LDS = 2 * ARRAY * WAVES > JOIN ? 2 * ARRAY * WAVES : JOIN;
 };
 
-// Scratch of chunks: [chunk][token][head] rows of D fp32 relative to 2^m, and (m, l)
-struct Parts {
-    float *o;
-    float2 *ml;
-    int chunk;   // keys of one
-    int chunks;  // the most of a sequence
-};
-
 template <typename T, bool PART>
 __global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts parts) {
     typedef PackedGeo R;
@@ -211,7 +203,7 @@ __global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int
     const bool mine = row < rows;   // (uniform over the wave; over the workgroup where waves share a row)
     const int i = (int)(min(row, rows - 1) / (unsigned)p.H), h = (int)(min(row, rows - 1) % (unsigned)p.H), D = p.D;
     const Segment s = segment_of_row<false>(p, i);
-    const int chunks = s.gap ? 0 : min(parts.chunks, (s.nk() + parts.chunk - 1) / parts.chunk);
+    const int chunks = s.gap || s.seen(i, p.causal) == 0 ? 0 : parts.chunk ? min(parts.chunks, (s.nk() + parts.chunk - 1) / parts.chunk) : parts.chunks;
     const int64_t step = p.Tq * p.H;
     const float2 *ml = parts.ml + (int64_t)i * p.H + h;
     const float *o = parts.o + ((int64_t)i * p.H + h) * D;
@@ -262,6 +254,14 @@ __global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int
     if (lane == 0 && p.lse) p.lse[(int64_t)h * p.Tq + i] = sees ? M + __log2f(L) : INFINITY;
 }
 
+template <typename T>
+static int join(const EvoPacked &p, const Parts &parts, hipStream_t st) {
+    const int64_t rows = p.Tq * p.H;
+    const int per = parts.chunks > 8 ? 4 : 1;
+    packed_join<T><<<(unsigned)((rows * per + 3) / 4), 256, 0, st>>>(p, parts, per, (unsigned)rows);
+    return hip_rc();
+}
+
 // Keys of a chunk: as many as make some kFewWorkgroups workgroups of all keys and key heads, at least four steps of every wave (a workgroup that has only one spends its time on finding its place and
 // joining), all of them where one workgroup's walk over them takes less time than a second launch does.  And not so few that the parts take more than kFewScratch bytes.
 constexpr int64_t kFewWorkgroups = 512, kFewScratch = 64 << 20;
@@ -303,11 +303,13 @@ int EVO_CAT(launch_packed_few_d, EVO_D)(const EvoPacked &p, hipStream_t st) {
             return hip_rc();
         }
         packed_few<T, true><<<(unsigned)grid, Few::WAVES * 64, 0, st>>>(p, parts);
-        if (const int rc = hip_rc()) return rc;
-        const int per = parts.chunks > 8 ? 4 : 1;
-        packed_join<T><<<(unsigned)((rows * per + 3) / 4), 256, 0, st>>>(p, parts, per, (unsigned)rows);
-        return hip_rc();
+        const int rc = hip_rc();
+        return rc ? rc : join<T>(p, parts, st);
     });
+}
+int EVO_CAT(launch_packed_join_d, EVO_D)(const EvoPacked &p, float *o, float2 *ml, int parts, hipStream_t st) {
+    using namespace EVO_CAT(packed_d, EVO_D);
+    return by_half(p.dtype, [&](auto t) { return join<decltype(t)>(p, Parts{o, ml, 0, parts}, st); });
 }
 
 }  // namespace evo

@@ -17,43 +17,52 @@ namespace evo {
 
 namespace EVO_CAT(packed_d, EVO_D) {
 
+// Stages in LDS: one that is computed on and the others under way
+template <int KG> constexpr int kStageBuffers = KG == 2 ? (EVO_D > 64 ? 2 : 3) : EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2;
+
 // ------------------------------------------------------------------ forward
 
-template <typename T>
-__global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) packed_fwd(EvoPacked p, int tiles) {
+// KG: groups of four waves that share the queries and take 64 keys of a stage each, joined at the end.  PART: a part of the stages, of which packed_join makes the result.
+template <typename T, int KG, bool PART>
+__global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) packed_fwd(EvoPacked p, Parts parts, int tiles) {
     typedef PackedGeo R;
     typedef R::G G;
-    typedef StagePieces<4> Pieces;
+    typedef StagePieces<4 * KG> Pieces;
     typedef typename Mfma<T>::v8 v8;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2 * R::ARRAY];
+    constexpr int BUFS = kStageBuffers<KG>, KEYS = R::STAGE * KG, ARRAY = R::ARRAY * KG;   // of a stage
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
-    // A key head's query heads follow each other, then its tiles, the last (under a causal mask the longest) first; consecutive workgroups run on one XCD.
-    const int group = p.H / p.Hk;
-    const unsigned lid = xcd_remap(blockIdx.x, gridDim.x), per = (unsigned)tiles * (unsigned)group;
-    const int hk = (int)(lid / per), h = hk * group + (int)(lid % per % (unsigned)group);
-    const Place at = place_of<false>(p, tiles - 1 - (int)(lid % per / (unsigned)group));
+    const int heads = p.H / p.Hk;
+    const Unit unit(blockIdx.x, tiles, p.Hk, heads * (PART ? parts.chunks : 1));
+    if (unit.none) return;
+    const int hk = unit.hk, h = hk * heads + unit.member % heads, part = PART ? unit.member / heads : 0;
+    const Place at = place_of<false>(p, tiles - 1 - unit.tile);   // (a sequence's last queries, which under a causal mask see most, first)
     const Segment &s = at.s;
     if (at.first >= s.q1) return;
     const int D = p.D, rows = min(kPackedRows, s.q1 - at.first);
     const int seen_most = s.gap ? 0 : s.seen(at.first + rows - 1, p.causal);
-    if (seen_most == 0) {
+    if (seen_most == 0) {   // (with parts: packed_join's)
+        if (PART) return;
         zero_rows((T *)p.o, at.first, rows, p.H, h, D);
         if (p.lse && (int)threadIdx.x < rows) p.lse[(int64_t)h * p.Tq + at.first + threadIdx.x] = INFINITY;
         return;
     }
+    const int all = (seen_most + KEYS - 1) / KEYS, from = PART ? part_begin(part, parts.chunks, all) : 0, to = PART ? part_begin(part + 1, parts.chunks, all) : all;
     const int kst = (int)p.k_stride_t * 2, vst = (int)p.v_stride_t * 2;
     const char *kbase = (const char *)head_row<T>(p.k, s.k0, p.k_stride_t, hk, p.k_stride_h), *vbase = (const char *)head_row<T>(p.v, s.k0, p.v_stride_t, hk, p.v_stride_h);
     const int koff = Pieces::first(wave, lane, kst, D), voff = Pieces::first(wave, lane, vst, D);
-    auto fetch = [&](int stage) {
-        const int row = stage * R::STAGE, n = min(R::STAGE, s.nk() - row);
-        unsigned char *dst = lds[stage & 1];
-        Pieces::fetch<R::STAGE>(rows_at(kbase + (int64_t)row * kst, n, kst, D), dst, koff, kst, wave);
-        Pieces::fetch<R::STAGE>(rows_at(vbase + (int64_t)row * vst, n, vst, D), dst + R::ARRAY, voff, vst, wave);
+    auto fetch = [&](int stage) {   // (a stage past the last reads zeros: a wave's loads are as many in every stage)
+        const int row = stage * KEYS, n = min(KEYS, s.nk() - row);
+        unsigned char *dst = lds + stage % BUFS * (2 * ARRAY);
+        Pieces::template fetch<KEYS>(rows_at(kbase + (int64_t)row * kst, n, kst, D), dst, koff, kst, wave);
+        Pieces::template fetch<KEYS>(rows_at(vbase + (int64_t)row * vst, n, vst, D), dst + ARRAY, voff, vst, wave);
     };
-    fetch(0);
+#pragma unroll
+    for (int i = 0; i < BUFS - 1; ++i) fetch(from + i);
 
-    const int q0 = at.first + wave * 32, qrow = min(q0 + li, s.q1 - 1);
+    const int own = KG == 1 ? wave : wave & 3, key_group = KG == 1 ? 0 : wave >> 2;
+    const int q0 = at.first + own * 32, qrow = min(q0 + li, s.q1 - 1);
     const bool active = q0 < s.q1;   // uniform
     v8 qf[R::KSD];
     load_operands(head_row<T>(p.q, qrow, p.q_stride_t, h, p.q_stride_h), D, g, qf);
@@ -71,14 +80,26 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
 
     const Staged staged(lane);
     auto step = [&](const unsigned char *buf, int key0) __attribute__((always_inline)) {
-        const unsigned at = Staged::base(buf);
+        const unsigned at = Staged::base(buf) + key_group * R::ARRAY;
+        // All operands of a product are asked for together (left to itself the compiler asks for one, waits for it and multiplies), the values' before the softmax
+        v8 kf[2][R::KSD], vf[4][R::DT];
+#pragma unroll
+        for (int ks = 0; ks < R::KSD; ++ks)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) kf[t][ks] = staged.rows<T>(at, 32 * t, ks);
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 a[2];
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            a[t] = filled(0.0f);
+        for (int t = 0; t < 2; ++t) a[t] = filled(0.0f);
 #pragma unroll
-            for (int ks = 0; ks < R::KSD; ++ks) a[t] = Mfma<T>::mma(staged.rows<T>(at, 32 * t, ks), qf[ks], a[t]);
-        }
+        for (int ks = 0; ks < R::KSD; ++ks)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) a[t] = Mfma<T>::mma(kf[t][ks], qf[ks], a[t]);
+#pragma unroll
+        for (int ts = 0; ts < 4; ++ts)
+#pragma unroll
+            for (int dt = 0; dt < R::DT; ++dt) vf[ts][dt] = staged.cols<T>(at + ARRAY, (ts / 2) * 32, ts & 1, dt);
+        __builtin_amdgcn_sched_barrier(0);
         if (key0 + R::STAGE > wave_least) {   // (uniform)
             asm volatile("");                 // (a branch: not computed where it is not needed)
 #pragma unroll
@@ -86,49 +107,82 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
 #pragma unroll
                 for (int r = 0; r < 16; ++r) a[t][r] = key0 + 32 * t + crow(r, g) < seen ? a[t][r] : -INFINITY;
         }
-        float top = a[0][0];
+        // Probabilities relative to the maximum so far, which is looked for only when their sum shows that some score stands far above it (at first any does)
+        v8 pf[4];
+        auto probabilities = [&] {
+            float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+            for (int ts = 0; ts < 4; ++ts) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, a[t][r]);
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-        // (not below the floor: a query that sees none of these keys has -inf here, and -inf less -inf is no number)
-        const float cand = fmaxf(fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c, kMaskFloor);
-        const bool grow = cand > m + 8.0f;
-        if (__any(grow)) {
-            const float mn = grow ? cand : m, alpha = fast_exp2(m - mn);
+                for (int i = 0; i < 8; ++i) pf[ts][i] = (T)fast_exp2(fmaf(a[ts / 2][8 * (ts & 1) + i], c, -m));
+                sum[ts & 1] = dot8<T>(pf[ts], one, sum[ts & 1]);
+            }
+            return sum[0] + sum[1];
+        };
+        float sum = probabilities();
+        if (__builtin_expect(__any(!(sum <= 8192.0f)), 0)) {
+            float top = a[0][0];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, a[t][r]);
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            const float mn = fmaxf(fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * c, m), alpha = fast_exp2(m - mn);
             m = mn;
             l *= alpha;
 #pragma unroll
             for (int dt = 0; dt < R::DT; ++dt)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[dt][r] *= alpha;
+            sum = probabilities();
         }
-        v8 pf[4];
-#pragma unroll
-        for (int ts = 0; ts < 4; ++ts) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pf[ts][i] = (T)fast_exp2(fmaf(a[ts / 2][8 * (ts & 1) + i], c, -m));
-            l = dot8<T>(pf[ts], one, l);
-        }
+        l += sum;
 #pragma unroll
         for (int ts = 0; ts < 4; ++ts)
 #pragma unroll
-            for (int dt = 0; dt < R::DT; ++dt) o[dt] = Mfma<T>::mma(staged.cols<T>(at + R::ARRAY, (ts / 2) * 32, ts & 1, dt), pf[ts], o[dt]);
+            for (int dt = 0; dt < R::DT; ++dt) o[dt] = Mfma<T>::mma(vf[ts][dt], pf[ts], o[dt]);
     };
-    const int stages = (seen_most + R::STAGE - 1) / R::STAGE;
-    wait_loads();
-    wait_lds_barrier();
-    for (int st = 0; st < stages; ++st) {
-        if (st + 1 < stages) fetch(st + 1);
-        if (st * R::STAGE < wave_most) step(lds[st & 1], st * R::STAGE);
-        if (st + 1 < stages) {
-            wait_loads();
-            wait_lds_barrier();
+    for (int st = from; st < to; ++st) {
+        // this stage is there, and everybody has read the one before, whose place the next one to be asked for takes
+        wait_loads_but<(BUFS - 2) * 2 * Pieces::each(KEYS)>();
+        wait_lds_barrier();
+        fetch(st + BUFS - 1);
+        const int key0 = st * KEYS + key_group * R::STAGE;
+        if (key0 < wave_most) step(lds + st % BUFS * (2 * ARRAY), key0);
+    }
+    wait_loads();   // (LDS is the next workgroup's from here on)
+    if constexpr (KG == 2) {
+        // Both groups' sums relative to the larger maximum, the second's added to the first's
+        float *const x = reinterpret_cast<float *>(lds) + own * (R::DT * 16 + 3) * 64, *const ml = x + R::DT * 16 * 64;
+        wait_lds_barrier();
+        ml[key_group * 64 + lane] = m;
+        wait_lds_barrier();
+        const float mn = fmaxf(ml[lane], ml[64 + lane]), f = fast_exp2(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < R::DT; ++dt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] *= f;
+        if (key_group) {
+            give(o, x, lane);
+            ml[128 + lane] = l;
         }
+        wait_lds_barrier();
+        if (key_group) return;
+        take(o, x, lane);
+        l += ml[128 + lane];
     }
     if (!active) return;
     l += __shfl_xor(l, 32);
+    const bool mine = q0 + li < s.q1;
+    if constexpr (PART) {
+        const int64_t row = ((int64_t)part * p.Tq + qrow) * p.H + h;
+#pragma unroll
+        for (int dt = 0; dt < R::DT; ++dt) store_row_part(parts.o + row * D, dt * 32, mine ? D : 0, o[dt], g);
+        if (mine && g == 0) parts.ml[row] = make_float2(m, l);
+        return;
+    }
     const float inv = seen ? 1.0f / l : 0.0f;
     bool nan = false;
 #pragma unroll
@@ -138,9 +192,8 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
             o[dt][r] = seen ? o[dt][r] * inv : 0.0f;
             nan |= !(o[dt][r] == o[dt][r]);
         }
-    const bool own = q0 + li < s.q1;
-    unsigned again = rows_without_number(nan && own);
-    const bool whole = own && !(again >> li & 1);
+    unsigned again = rows_without_number(nan && mine);
+    const bool whole = mine && !(again >> li & 1);
     if (p.lse && whole && g == 0) p.lse[(int64_t)h * p.Tq + qrow] = seen ? m + __log2f(l) : INFINITY;
     T *out = (T *)p.o + ((int64_t)qrow * p.H + h) * D;
 #pragma unroll
@@ -150,40 +203,46 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
 
 // ------------------------------------------------------------------ dQ
 
-template <typename T>
-__global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) packed_dq(EvoPacked p, BackwardRows out_rows, int tiles) {
+template <typename T, int KG, bool PART>
+__global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) packed_dq(EvoPacked p, BackwardRows out_rows, Parts parts, int tiles) {
     typedef PackedGeo R;
     typedef R::G G;
-    typedef StagePieces<4> Pieces;
+    typedef StagePieces<4 * KG> Pieces;
     typedef typename Mfma<T>::v8 v8;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[2][2 * R::ARRAY];
+    constexpr int BUFS = kStageBuffers<KG>, KEYS = R::STAGE * KG, ARRAY = R::ARRAY * KG;   // of a stage
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, g = lane >> 5;
-    const int group = p.H / p.Hk;
-    const unsigned lid = xcd_remap(blockIdx.x, gridDim.x), per = (unsigned)tiles * (unsigned)group;
-    const int hk = (int)(lid / per), h = hk * group + (int)(lid % per % (unsigned)group);
-    const Place at = place_of<false>(p, tiles - 1 - (int)(lid % per / (unsigned)group));
+    const int heads = p.H / p.Hk;
+    const Unit unit(blockIdx.x, tiles, p.Hk, heads * (PART ? parts.chunks : 1));
+    if (unit.none) return;
+    const int hk = unit.hk, h = hk * heads + unit.member % heads, part = PART ? unit.member / heads : 0;
+    const Place at = place_of<false>(p, tiles - 1 - unit.tile);
     const Segment &s = at.s;
     if (at.first >= s.q1) return;
     const int D = p.D, rows = min(kPackedRows, s.q1 - at.first);
     const int seen_most = s.gap ? 0 : s.seen(at.first + rows - 1, p.causal);
     if (seen_most == 0) {
-        zero_rows((T *)p.dq, at.first, rows, p.H, h, D);
+        if (!PART) zero_rows((T *)p.dq, at.first, rows, p.H, h, D);
         return;
     }
+    const int all = (seen_most + KEYS - 1) / KEYS, from = PART ? part_begin(part, parts.chunks, all) : 0, to = PART ? part_begin(part + 1, parts.chunks, all) : all;
     const int kst = (int)p.k_stride_t * 2, vst = (int)p.v_stride_t * 2;
     const char *kbase = (const char *)head_row<T>(p.k, s.k0, p.k_stride_t, hk, p.k_stride_h), *vbase = (const char *)head_row<T>(p.v, s.k0, p.v_stride_t, hk, p.v_stride_h);
     const int koff = Pieces::first(wave, lane, kst, D), voff = Pieces::first(wave, lane, vst, D);
-    auto fetch = [&](int stage) {
-        const int row = stage * R::STAGE, n = min(R::STAGE, s.nk() - row);
-        unsigned char *dst = lds[stage & 1];
-        Pieces::fetch<R::STAGE>(rows_at(kbase + (int64_t)row * kst, n, kst, D), dst, koff, kst, wave);
-        Pieces::fetch<R::STAGE>(rows_at(vbase + (int64_t)row * vst, n, vst, D), dst + R::ARRAY, voff, vst, wave);
+    auto fetch = [&](int stage) {   // (a stage past the last reads zeros: a wave's loads are as many in every stage)
+        const int row = stage * KEYS, n = min(KEYS, s.nk() - row);
+        unsigned char *dst = lds + stage % BUFS * (2 * ARRAY);
+        Pieces::template fetch<KEYS>(rows_at(kbase + (int64_t)row * kst, n, kst, D), dst, koff, kst, wave);
+        Pieces::template fetch<KEYS>(rows_at(vbase + (int64_t)row * vst, n, vst, D), dst + ARRAY, voff, vst, wave);
     };
-    fetch(0);
+#pragma unroll
+    for (int i = 0; i < BUFS - 1; ++i) fetch(from + i);
 
-    const int q0 = at.first + wave * 32, qrow = min(q0 + li, s.q1 - 1);
-    const bool active = q0 < s.q1, own = q0 + li < s.q1;
+    const int own = KG == 1 ? wave : wave & 3, key_group = KG == 1 ? 0 : wave >> 2;
+    const int q0 = at.first + own * 32, qrow = min(q0 + li, s.q1 - 1);
+    const bool active = q0 < s.q1;   // uniform
+    const bool mine = q0 + li < s.q1;
     v8 qf[R::KSD], df[R::KSD];
     load_operands(head_row<T>(p.q, qrow, p.q_stride_t, h, p.q_stride_h), D, g, qf);
     load_operands(head_row<T>(p.dout, qrow, p.dout_stride_t, h, p.dout_stride_h), D, g, df);
@@ -196,7 +255,7 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
     }
     dl += __shfl_xor(dl, 32);
     const float c = p.scale * kLog2e, lse = p.lse[(int64_t)h * p.Tq + qrow];
-    if (own && g == 0) {
+    if (mine && g == 0 && part == 0 && key_group == 0) {
         out_rows.delta[(int64_t)h * p.Tq + qrow] = -dl;
         out_rows.base[(int64_t)h * p.Tq + qrow] = -lse / c;
     }
@@ -208,13 +267,21 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
 
     const Staged staged(lane);
     auto step = [&](const unsigned char *buf, int kb, int key0) __attribute__((always_inline)) {
-        const unsigned at = Staged::base(buf);
+        const unsigned at = Staged::base(buf) + key_group * R::ARRAY;
+        v8 kf[R::KSD], kt[2][R::DT];
+#pragma unroll
+        for (int ks = 0; ks < R::KSD; ++ks) kf[ks] = staged.rows<T>(at, kb, ks);
+        __builtin_amdgcn_sched_barrier(0);
         f32x16 a = filled(0.0f), d = filled(-dl);
 #pragma unroll
-        for (int ks = 0; ks < R::KSD; ++ks) {
-            a = Mfma<T>::mma(staged.rows<T>(at, kb, ks), qf[ks], a);
-            d = Mfma<T>::mma(staged.rows<T>(at + R::ARRAY, kb, ks), df[ks], d);
-        }
+        for (int ks = 0; ks < R::KSD; ++ks) a = Mfma<T>::mma(kf[ks], qf[ks], a);
+#pragma unroll
+        for (int ks = 0; ks < R::KSD; ++ks) d = Mfma<T>::mma(staged.rows<T>(at + ARRAY, kb, ks), df[ks], d);
+#pragma unroll
+        for (int ts = 0; ts < 2; ++ts)
+#pragma unroll
+            for (int dt = 0; dt < R::DT; ++dt) kt[ts][dt] = staged.cols<T>(at, kb, ts, dt);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 16; ++r) d[r] *= fast_exp2(fmaf(a[r], c, -lse));
         if (key0 + 32 > wave_least) {   // (uniform)
@@ -230,29 +297,41 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
 #pragma unroll
         for (int ts = 0; ts < 2; ++ts)
 #pragma unroll
-            for (int dt = 0; dt < R::DT; ++dt) dq[dt] = Mfma<T>::mma(staged.cols<T>(at, kb, ts, dt), pf[ts], dq[dt]);
+            for (int dt = 0; dt < R::DT; ++dt) dq[dt] = Mfma<T>::mma(kt[ts][dt], pf[ts], dq[dt]);
     };
-    const int stages = (seen_most + R::STAGE - 1) / R::STAGE;
-    wait_loads();
-    wait_lds_barrier();
-    for (int st = 0; st < stages; ++st) {
-        if (st + 1 < stages) fetch(st + 1);
+    for (int st = from; st < to; ++st) {
+        wait_loads_but<(BUFS - 2) * 2 * Pieces::each(KEYS)>();
+        wait_lds_barrier();
+        fetch(st + BUFS - 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-            if (st * R::STAGE + 32 * t < wave_most) step(lds[st & 1], 32 * t, st * R::STAGE + 32 * t);
-        if (st + 1 < stages) {
-            wait_loads();
-            wait_lds_barrier();
+        for (int t = 0; t < 2; ++t) {
+            const int key0 = st * KEYS + key_group * R::STAGE + 32 * t;
+            if (key0 < wave_most) step(lds + st % BUFS * (2 * ARRAY), 32 * t, key0);
         }
     }
+    wait_loads();
+    if constexpr (KG == 2) {
+        float *const x = reinterpret_cast<float *>(lds) + own * R::DT * 16 * 64;
+        wait_lds_barrier();
+        if (key_group) give(dq, x, lane);
+        wait_lds_barrier();
+        if (key_group) return;
+        take(dq, x, lane);
+    }
     if (!active) return;
+    if constexpr (PART) {
+        const int64_t row = ((int64_t)part * p.Tq + qrow) * p.H + h;
+#pragma unroll
+        for (int dt = 0; dt < R::DT; ++dt) store_row_part(parts.o + row * D, dt * 32, mine ? D : 0, dq[dt], g);
+        return;
+    }
     bool nan = false;
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) nan |= !(dq[dt][r] == dq[dt][r]);
-    unsigned again = rows_without_number(nan && own);
-    const bool whole = own && !(again >> li & 1);
+    unsigned again = rows_without_number(nan && mine);
+    const bool whole = mine && !(again >> li & 1);
     T *out = (T *)p.dq + ((int64_t)qrow * p.H + h) * D;
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>(out, dt * 32, whole ? D : 0, dq[dt], p.scale, g);
@@ -266,22 +345,48 @@ __global__ void __launch_bounds__(256, EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) pa
 
 }  // namespace
 
+size_t EVO_CAT(packed_fwd_bytes_d, EVO_D)(const EvoPacked &p) { return EVO_CAT(packed_d, EVO_D)::query_plan(p).bytes(p.Tq * p.H, p.D + 2); }
+int EVO_CAT(launch_packed_join_d, EVO_D)(const EvoPacked &p, float *o, float2 *ml, int parts, hipStream_t st);
 int EVO_CAT(launch_packed_fwd_d, EVO_D)(const EvoPacked &p, hipStream_t st) {
     using namespace EVO_CAT(packed_d, EVO_D);
-    const int64_t tiles = packed_tiles(p.Tq, p.n), grid = tiles * p.H;
-    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
+    const Plan plan = query_plan(p);
+    const int64_t tiles = packed_tiles(p.Tq, p.n), grid = Unit::grid(tiles, p.Hk, p.H / p.Hk * plan.parts), rows = p.Tq * p.H;
+    if (!grid_fits(grid, 256 * plan.groups) || (plan.parts > 1 && (rows > INT32_MAX || !grid_fits(rows, 256)))) return EVO_EOVERFLOW;
     return by_half(p.dtype, [&](auto t) {
-        packed_fwd<decltype(t)><<<(unsigned)grid, 256, 0, st>>>(p, (int)tiles);
-        return hip_rc();
+        typedef decltype(t) T;
+        return plan.run([&](auto groups, auto part) {
+            constexpr int KG = decltype(groups)::value, LDS = kStageBuffers<KG> * 2 * PackedGeo::ARRAY * KG;
+            constexpr auto kern = packed_fwd<T, KG, decltype(part)::value>;
+            static PerDevice done;
+            if (const int rc = ensure_dynamic_lds((const void *)kern, LDS, done, nullptr)) return rc;
+            float *const o = (float *)p.workspace;
+            const Parts parts = {o, (float2 *)(o + plan.parts * rows * p.D), 0, plan.parts};
+            kern<<<(unsigned)grid, 256 * KG, LDS, st>>>(p, parts, (int)tiles);
+            const int rc = hip_rc();
+            return rc || !decltype(part)::value ? rc : EVO_CAT(launch_packed_join_d, EVO_D)(p, parts.o, parts.ml, parts.chunks, st);
+        });
     });
 }
-int EVO_CAT(launch_packed_dq_d, EVO_D)(const EvoPacked &p, const BackwardRows &rows, hipStream_t st) {
+size_t EVO_CAT(packed_dq_bytes_d, EVO_D)(const EvoPacked &p) { return EVO_CAT(packed_d, EVO_D)::query_plan(p).bytes(p.Tq * p.H, p.D); }
+int EVO_CAT(launch_packed_dq_d, EVO_D)(const EvoPacked &p, const BackwardRows &saved, float *sums, hipStream_t st) {
     using namespace EVO_CAT(packed_d, EVO_D);
-    const int64_t tiles = packed_tiles(p.Tq, p.n), grid = tiles * p.H;
-    if (!grid_fits(grid, 256)) return EVO_EOVERFLOW;
+    const Plan plan = query_plan(p);
+    const int64_t tiles = packed_tiles(p.Tq, p.n), grid = Unit::grid(tiles, p.Hk, p.H / p.Hk * plan.parts), rows = p.Tq * p.H;
+    if (!grid_fits(grid, 256 * plan.groups) || (plan.parts > 1 && (rows > INT32_MAX || !grid_fits(rows, 64)))) return EVO_EOVERFLOW;
     return by_half(p.dtype, [&](auto t) {
-        packed_dq<decltype(t)><<<(unsigned)grid, 256, 0, st>>>(p, rows, (int)tiles);
-        return hip_rc();
+        typedef decltype(t) T;
+        return plan.run([&](auto groups, auto part) {
+            constexpr int KG = decltype(groups)::value, LDS = kStageBuffers<KG> * 2 * PackedGeo::ARRAY * KG;
+            constexpr auto kern = packed_dq<T, KG, decltype(part)::value>;
+            static PerDevice done;
+            if (const int rc = ensure_dynamic_lds((const void *)kern, LDS, done, nullptr)) return rc;
+            const Parts parts = {sums, nullptr, 0, plan.parts};
+            kern<<<(unsigned)grid, 256 * KG, LDS, st>>>(p, saved, parts, (int)tiles);
+            if (const int rc = hip_rc()) return rc;
+            if (!decltype(part)::value) return (int)EVO_OK;
+            packed_sum<T, false><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(p, saved, parts, (unsigned)rows);
+            return hip_rc();
+        });
     });
 }
 

@@ -35,6 +35,7 @@ struct StagePieces {
     static constexpr int RPP = 1024 / G::ROW;        // rows to a piece of 1 KB
     static constexpr int STEP = RPP * NW;            // rows from one of a wave's pieces to its next
     static_assert(STEP % 16 == 0, "a lane's chunk is the same in all of its pieces");
+    static constexpr int each(int rows) { return rows / RPP / NW; }   // pieces of a wave (where they are shared out evenly)
     static __device__ __forceinline__ int first(int wave, int lane, int stride, int D) {
         const int r = wave * RPP + lane / G::C, c = (lane % G::C) ^ G::x(r);
         return c * 8 < D ? r * stride + c * 16 : kFarOff;
@@ -107,7 +108,7 @@ __device__ __forceinline__ Place place_of(const EvoPacked &p, int t) {
 template <typename T>
 __device__ __forceinline__ void zero_rows(T *x, int first, int rows, int heads, int h, int D) {
     const int per = D / 8, n = rows * per;
-    for (int i = threadIdx.x; i < n; i += 256) *reinterpret_cast<uint4 *>(x + ((int64_t)(first + i / per) * heads + h) * D + i % per * 8) = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) *reinterpret_cast<uint4 *>(x + ((int64_t)(first + i / per) * heads + h) * D + i % per * 8) = make_uint4(0, 0, 0, 0);
 }
 
 // The lanes (low 32 bits: the rows of the wave) whose accumulators hold something that is no number
@@ -123,7 +124,133 @@ __device__ __forceinline__ f32x16 filled(float v) {
     return x;
 }
 
+// Which tile and heads a workgroup takes.  Workgroups go round the eight XCDs, each with an L2 of its own; a unit, a tile and a key head, goes to one of them with all of its query heads, and units follow
+// each other by tiles first: with a multiple of eight key heads an XCD keeps to its own, with fewer the tiles of one are dealt out one by one, so that all XCDs have long and short ones.  (In runs of units, a half of a key head's tiles
+// to an XCD: seven prompts of 90 to 2011, 16 / 4 heads of 64, 39.7 us.)
+struct Unit {
+    int tile, hk, member;   // member: of the unit's workgroups
+    bool none;              // past the last unit
+    __device__ __forceinline__ Unit(unsigned id, int tiles, int heads, int members) {
+        const unsigned slot = id / 8, u = slot / (unsigned)members * 8 + id % 8;
+        member = (int)(slot % (unsigned)members);
+        tile = (int)(u / (unsigned)heads);
+        hk = (int)(u % (unsigned)heads);
+        none = tile >= tiles;
+    }
+    static int64_t grid(int64_t tiles, int64_t heads, int64_t members) { return (tiles * heads + 7) / 8 * 8 * members; }
+};
+
+// Results in parts: [part][row][head] rows of D fp32 (of a softmax: relative to 2^m) and, of a softmax, (m, l).
+struct Parts {
+    float *o;
+    float2 *ml;
+    int chunk;   // keys of a part (packed_few), or 0: each row has `chunks` of them
+    int chunks;  // the most of a row
+};
+// What part `x` of `parts` takes of n steps
+__device__ __forceinline__ int part_begin(int x, int parts, int n) { return (int)((int64_t)n * x / parts); }
+
+// The accumulators of two waves that have the same rows, through LDS, a register of all lanes after the other: given by one, added by the other
+template <int N>
+__device__ __forceinline__ void give(const f32x16 (&x)[N], float *to, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) to[(i * 16 + r) * 64 + lane] = x[i][r];
+}
+template <int N>
+__device__ __forceinline__ void take(f32x16 (&x)[N], const float *from, int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[i][r] += from[(i * 16 + r) * 64 + lane];
+}
+// A tile's row as fp32 (store_row_tile's, unrounded): columns 8 (r / 4) + 4 g + r % 4
+__device__ __forceinline__ void store_row_part(float *row, int c0, int ncols, const f32x16 &x, int g) {
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr) {
+        const int c = c0 + 8 * rr + 4 * g;
+        if (c < ncols) *reinterpret_cast<f32x4 *>(row + c) = f32x4{x[4 * rr], x[4 * rr + 1], x[4 * rr + 2], x[4 * rr + 3]};
+    }
+}
+__device__ __forceinline__ void zero_parts(float *x, int first, int rows, int heads, int h, int D) {
+    const int per = D / 4, n = rows * per;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) *reinterpret_cast<f32x4 *>(x + ((int64_t)(first + i / per) * heads + h) * D + i % per * 4) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+
 static int64_t packed_tiles(int64_t rows, int n, int tile = kPackedRows) { return rows / tile + n + 2; }
+
+// The sums of a row's parts, by a wave for each row: dQ, or (KEYS) dK and dV, whose parts follow those of dK.
+template <typename T, bool KEYS>
+__global__ void __launch_bounds__(256) packed_sum(EvoPacked p, BackwardRows saved, Parts parts, unsigned rows) {
+    const int lane = threadIdx.x & 63;
+    const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (row >= rows) return;
+    const int heads = KEYS ? p.Hk : p.H, i = (int)(row / (unsigned)heads), h = (int)(row % (unsigned)heads), D = p.D, d = min(lane * 2, D - 2);
+    const Segment s = segment_of_row<KEYS>(p, i);
+    const bool any = !s.gap && (KEYS ? s.first_query(i, p.causal) < s.q1 : s.seen(i, p.causal) > 0);
+    bool nan = false;
+    float2 sum[KEYS ? 2 : 1];
+#pragma unroll
+    for (int y = 0; y < (KEYS ? 2 : 1); ++y) {
+        const float *x = parts.o + ((int64_t)y * parts.chunks * rows + row) * D + d;
+        sum[y] = make_float2(0.0f, 0.0f);
+        if (any) {
+#pragma unroll 4
+            for (int c = 0; c < parts.chunks; ++c) {
+                const float2 v = *reinterpret_cast<const float2 *>(x + (int64_t)c * rows * D);
+                sum[y].x += v.x;
+                sum[y].y += v.y;
+            }
+        }
+        nan |= !(sum[y].x == sum[y].x) || !(sum[y].y == sum[y].y);
+    }
+    if (__any(nan)) {
+        if constexpr (KEYS) row_dkdv<T>(p, s, i, h, saved.delta);
+        else row_dq<T>(p, s, i, h, -saved.delta[(int64_t)h * p.Tq + i]);
+        return;
+    }
+    if (lane * 2 >= D) return;
+#pragma unroll
+    for (int y = 0; y < (KEYS ? 2 : 1); ++y) {
+        const float f = y ? 1.0f : p.scale;
+        typename Mfma<T>::v2 v;
+        v[0] = (T)(sum[y].x * f);
+        v[1] = (T)(sum[y].y * f);
+        *reinterpret_cast<typename Mfma<T>::v2 *>((T *)(KEYS ? (y ? p.dv : p.dk) : p.dq) + (int64_t)row * D + lane * 2) = v;
+    }
+}
+
+// How a launch fills the chip: `groups` (1 or 2) of four waves to a tile of rows, that share its walk over the other side, and `parts` of it, workgroups of their own whose results are joined by a kernel more.
+struct Plan {
+    int groups, parts;
+    size_t bytes(int64_t rows, int columns) const { return parts > 1 ? (size_t)(parts * rows * columns * (int64_t)sizeof(float)) : 0; }
+    template <typename F>
+    int run(F &&f) const {
+        const std::integral_constant<int, 1> one;
+        const std::integral_constant<int, 2> two;
+        if (parts > 1) return f(two, std::true_type());
+        return groups == 2 ? f(two, std::false_type()) : f(one, std::false_type());
+    }
+};
+// units: tiles and heads; steps: of an average sequence's walk, 64 rows each.
+static Plan plan_for(int64_t units, int64_t steps) {
+    Plan r;
+    r.groups = steps >= 12 && units <= (EVO_D == 32 ? 768 : 400) ? 2 : 1;
+    r.parts = 1;
+    if (units && units <= 256) {
+        const int64_t fill = 512 / units, worth = steps / (units <= 64 ? 8 : 16), most = fill < worth ? fill : worth;
+        r.parts = (int)(most < 1 ? 1 : most > 16 ? 16 : most);
+    }
+    return r;
+}
+static Plan query_plan(const EvoPacked &p) {
+    return plan_for((p.Tq / kPackedRows + (p.n + 1) / 2) * p.H, p.Tk / (p.n ? p.n : 1) / 64);
+}
+// (a key's walk is over the queries of all heads that share it)
+static Plan key_plan(const EvoPacked &p) {
+    return plan_for((p.Tk / kPackedRows + (p.n + 1) / 2) * p.Hk, p.Tq / (p.n ? p.n : 1) * (p.H / p.Hk) / 64);
+}
 
 template <typename F>
 static int by_half(int dtype, F &&f) {
