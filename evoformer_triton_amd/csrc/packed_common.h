@@ -56,10 +56,29 @@ __device__ __forceinline__ Segment segment(const EvoPacked &p, int j) {
     s.k1 = __builtin_amdgcn_readfirstlane(s.k1);
     return s;
 }
+// The last segment j for which before(begin(j), j) holds, begin(j) being its first query (KEYS: key) and `before` as last_where takes it.  Where a wave has a lane for every segment's begin, those of queries and of
+// keys are loaded at once and the segment's own are taken from the lanes: one trip to memory, not two or three.
+template <bool KEYS, typename F>
+__device__ __forceinline__ Segment find_segment(const EvoPacked &p, F before, int &j) {
+    if (p.n + 3 > 64) {
+        j = last_where(p.n + 2, [&](int x) { return before(KEYS ? keys_begin(p, x) : queries_begin(p, x), x); });
+        return segment(p, j);
+    }
+    const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x);
+    j = __builtin_amdgcn_readfirstlane(max(1, (int)__popcll(__ballot(lane < p.n + 2 && before(KEYS ? k : q, lane)))) - 1);
+    Segment s;
+    s.gap = j == 0 || j == p.n + 1;
+    s.q0 = __builtin_amdgcn_readlane(q, j);
+    s.q1 = __builtin_amdgcn_readfirstlane(max(s.q0, (int)__builtin_amdgcn_readlane(q, j + 1)));
+    s.k0 = __builtin_amdgcn_readlane(k, j);
+    s.k1 = __builtin_amdgcn_readfirstlane(max(s.k0, (int)__builtin_amdgcn_readlane(k, j + 1)));
+    return s;
+}
 // The segment that a row of the queries (or, KEYS, of the keys) lies in.
 template <bool KEYS>
 __device__ __forceinline__ Segment segment_of_row(const EvoPacked &p, int row) {
-    return segment(p, last_where(p.n + 2, [&](int j) { return (KEYS ? keys_begin(p, j) : queries_begin(p, j)) <= row; }));
+    int j;
+    return find_segment<KEYS>(p, [&](int begin, int) { return begin <= row; }, j);
 }
 
 __device__ __forceinline__ float lane_value(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }

@@ -43,14 +43,15 @@ __global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, gq = lane >> 4;
     const int group = p.H / p.Hk, D = p.D;
     const int hk = (int)(blockIdx.x % (unsigned)p.Hk), t = (int)(blockIdx.x / (unsigned)p.Hk);
-    const int j = last_where(p.n + 2, [&](int x) { return keys_begin(p, x) / parts.chunk + x <= t; });
-    const Segment s = segment(p, j);
+    int j;
+    const Segment s = find_segment<true>(p, [&](int begin, int x) { return begin / parts.chunk + x <= t; }, j);
     const int index = t - (s.k0 / parts.chunk + j);
     if (index < 0) return;
     const int64_t c0 = (int64_t)index * parts.chunk;
     const int nk = s.gap ? 0 : s.nk();
     if (c0 >= nk && (PART || index > 0)) return;
-    const int key_from = (int)c0, key_to = (int)min((int64_t)nk, c0 + parts.chunk);   // (none: zeros, by the only chunk)
+    // (none: zeros, by the only chunk; in scalar registers, where 64-bit comparisons are not formed by themselves)
+    const int key_from = __builtin_amdgcn_readfirstlane((int)c0), key_to = __builtin_amdgcn_readfirstlane((int)min((int64_t)nk, c0 + parts.chunk));
     const int64_t rows = (int64_t)s.nq() * group;
     const int kst = (int)p.k_stride_t * 2, vst = (int)p.v_stride_t * 2;
     const char *kbase = (const char *)head_row<T>(p.k, s.k0, p.k_stride_t, hk, p.k_stride_h), *vbase = (const char *)head_row<T>(p.v, s.k0, p.v_stride_t, hk, p.v_stride_h);

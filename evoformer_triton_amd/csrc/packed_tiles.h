@@ -96,10 +96,9 @@ struct Place {
 };
 template <bool KEYS, int ROWS = kPackedRows>
 __device__ __forceinline__ Place place_of(const EvoPacked &p, int t) {
-    auto begin = [&](int j) { return KEYS ? keys_begin(p, j) : queries_begin(p, j); };
-    const int j = last_where(p.n + 2, [&](int x) { return begin(x) / ROWS + x <= t; });
     Place r;
-    r.s = segment(p, j);
+    int j;
+    r.s = find_segment<KEYS>(p, [&](int begin, int x) { return begin / ROWS + x <= t; }, j);
     const int b = KEYS ? r.s.k0 : r.s.q0, i = t - (b / ROWS + j);
     r.first = i < 0 ? INT32_MAX : (int)min((int64_t)INT32_MAX, b + (int64_t)i * ROWS);   // (below zero: offsets that do not ascend)
     return r;
@@ -233,23 +232,22 @@ struct Plan {
         return groups == 2 ? f(two, std::false_type()) : f(one, std::false_type());
     }
 };
-// units: tiles and heads; steps: of an average sequence's walk, 64 rows each.
-static Plan plan_for(int64_t units, int64_t steps) {
-    Plan r;
-    r.groups = steps >= 12 && units <= (EVO_D == 32 ? 768 : 400) ? 2 : 1;
-    r.parts = 1;
-    if (units && units <= 256) {
-        const int64_t fill = 512 / units, worth = steps / (units <= 64 ? 8 : 16), most = fill < worth ? fill : worth;
-        r.parts = (int)(most < 1 ? 1 : most > 16 ? 16 : most);
+// units: tiles and heads; steps: of an average sequence's walk, 64 rows each.  Parts: as many as make some `fill` workgroups, of `few` steps at least where a CU is left to itself (up to 64 units),
+// of `more` up to 256 and of 32 beyond; for `most` units and fewer.
+static Plan plan_for(int64_t units, int64_t steps, int64_t fill, int64_t most, int64_t few, int64_t more) {
+    Plan r = {steps >= 12 && units <= (EVO_D == 32 ? 768 : 400) ? 2 : 1, 1};
+    if (units && units <= most) {
+        const int64_t room = fill / units, worth = steps / (units <= 64 ? few : units <= 256 ? more : 32), n = room < worth ? room : worth;
+        r.parts = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
     }
     return r;
 }
 static Plan query_plan(const EvoPacked &p) {
-    return plan_for((p.Tq / kPackedRows + (p.n + 1) / 2) * p.H, p.Tk / (p.n ? p.n : 1) / 64);
+    return plan_for((p.Tq / kPackedRows + (p.n + 1) / 2) * p.H, p.Tk / (p.n ? p.n : 1) / 64, 512, 256, 8, 32);
 }
 // (a key's walk is over the queries of all heads that share it)
 static Plan key_plan(const EvoPacked &p) {
-    return plan_for((p.Tk / kPackedRows + (p.n + 1) / 2) * p.Hk, p.Tq / (p.n ? p.n : 1) * (p.H / p.Hk) / 64);
+    return plan_for((p.Tk / kPackedRows + (p.n + 1) / 2) * p.Hk, p.Tq / (p.n ? p.n : 1) * (p.H / p.Hk) / 64, 768, 400, 4, 8);
 }
 
 template <typename F>
