@@ -21,24 +21,28 @@ template <> struct Mfma16<f16_t> {
     static __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
-struct Few {
+template <int NW, int CT> struct FewGeo {
     typedef PackedGeo::G G;
-    static constexpr int KEYS = 32, ROWS = 16;                       // keys of a wave's step; columns
+    static constexpr int KEYS = 32, ROWS = 16 * CT;                  // keys of a wave's step; columns
     static constexpr int ARRAY = KEYS * G::ROW, PIECES = ARRAY / 1024, RPP = 1024 / G::ROW;
-    static constexpr int WAVES = PackedGeo::GD == 128 ? 8 : 16;      // (two arrays each: 128 KB of LDS, head dim 32: 64)
+    static constexpr int WAVES = NW;
     static constexpr int KS = EVO_D / 32, DT = EVO_D / 16;
     static constexpr int PITCH = EVO_D + 4;                          // of a joined row, fp32
     static constexpr int JOIN = WAVES * ROWS * (PITCH + 2) * 4;
     static constexpr int LDS = 2 * ARRAY * WAVES > JOIN ? 2 * ARRAY * WAVES : JOIN;
 };
+// Waves of a workgroup: 128 KB of LDS (head dim 32: 64), a CU's worth, where there are few workgroups; four where there are many, so that a CU has several and one does not wait for all of its waves.
+constexpr int kFewWaves = PackedGeo::GD == 128 ? 8 : 16;
 
-template <typename T, bool PART>
-__global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts parts) {
+// CT: tiles of 16 columns that are multiplied with keys and values in LDS
+template <typename T, bool PART, int NW, int CT>
+__global__ void __launch_bounds__(NW * 64) packed_few(EvoPacked p, Parts parts) {
+    typedef FewGeo<NW, CT> Few;
     typedef PackedGeo R;
     typedef R::G G;
     typedef typename Mfma<T>::v8 v8;
     typedef typename Mfma<T>::v4 v4;
-    __shared__ __attribute__((aligned(1024))) unsigned char lds[Few::LDS];
+    extern __shared__ __attribute__((aligned(1024))) unsigned char lds[];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, gq = lane >> 4;
     const int group = p.H / p.Hk, D = p.D;
@@ -70,55 +74,78 @@ __global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts
     const float c = p.scale * kLog2e;
 
     for (int64_t r0 = 0; r0 < rows; r0 += Few::ROWS) {
-        // this lane's column: a query and a head
-        const int64_t pr = min(r0 + col, rows - 1);
-        const int i = s.q0 + (int)(pr / group), h = hk * group + (int)(pr % group), seen = s.gap ? 0 : s.seen(i, p.causal);
-        float m = kMaskFloor, l = 0.0f;
-        f32x4 o[Few::DT];
+        // this lane's columns: a query and a head each
+        int seen[CT];
+        const T *q[CT];
 #pragma unroll
-        for (int dt = 0; dt < Few::DT; ++dt) o[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int ct = 0; ct < CT; ++ct) {
+            const int64_t pr = min(r0 + 16 * ct + col, rows - 1);
+            const int i = s.q0 + (int)(pr / group), h = hk * group + (int)(pr % group);
+            seen[ct] = s.gap ? 0 : s.seen(i, p.causal);
+            q[ct] = head_row<T>(p.q, i, p.q_stride_t, h, p.q_stride_h);
+        }
+        float m[CT], l[CT];
+        f32x4 o[CT][Few::DT];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+            m[ct] = kMaskFloor;
+            l[ct] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < Few::DT; ++dt) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
         int key = key_from + wave * Few::KEYS;
         if (key < key_to) {
             fetch(kbase, kst, kbuf, key);
             fetch(vbase, vst, vbuf, key);
-            v8 qf[Few::KS];
-            const T *q = head_row<T>(p.q, i, p.q_stride_t, h, p.q_stride_h);
+            v8 qf[CT][Few::KS];
 #pragma unroll
-            for (int ks = 0; ks < Few::KS; ++ks) qf[ks] = ks * 32 + gq * 8 < D ? ld8(q + ks * 32 + gq * 8) : zero8<T>();
-            asked_together<Few::KS>(qf);   // (waited for here, with the first keys and values: what is counted below are the rows' loads alone)
+            for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+                for (int ks = 0; ks < Few::KS; ++ks) qf[ct][ks] = ks * 32 + gq * 8 < D ? ld8(q[ct] + ks * 32 + gq * 8) : zero8<T>();
+            }
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) asked_together<Few::KS>(qf[ct]);   // (waited for here, with the first keys and values: what is counted below are the rows' loads alone)
             for (;;) {
                 const int next = key + Few::WAVES * Few::KEYS;
                 const bool more = next < key_to;   // (uniform)
                 wait_loads_but<Few::PIECES>();      // the keys (the values are younger)
-                f32x4 a[2];
+                f32x4 a[CT][2];
 #pragma unroll
                 for (int tt = 0; tt < 2; ++tt) {
-                    a[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int ks = 0; ks < Few::KS; ++ks) a[tt] = Mfma16<T>::mma(*reinterpret_cast<const v8 *>(kbuf + G::at(16 * tt + col, 4 * ks + gq)), qf[ks], a[tt]);
-                }
-                float top = -INFINITY;
+                    for (int ct = 0; ct < CT; ++ct) a[ct][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int tt = 0; tt < 2; ++tt)
+                    for (int ks = 0; ks < Few::KS; ++ks) {
+                        const v8 x = *reinterpret_cast<const v8 *>(kbuf + G::at(16 * tt + col, 4 * ks + gq));
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        a[tt][r] = key + 16 * tt + 4 * gq + r < seen ? a[tt][r] : -INFINITY;
-                        top = fmaxf(top, a[tt][r]);
+                        for (int ct = 0; ct < CT; ++ct) a[ct][tt] = Mfma16<T>::mma(x, qf[ct][ks], a[ct][tt]);
                     }
+                }
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the keys have been read
                 if (more) fetch(kbase, kst, kbuf, next);
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float mn = fmaxf(m, top * c), alpha = fast_exp2(m - mn);
-                m = mn;
-                v8 pf;
+                v8 pf[CT];
 #pragma unroll
-                for (int x = 0; x < 8; ++x) pf[x] = (T)fast_exp2(fmaf(a[x >> 2][x & 3], c, -m));
-                l = dot8<T>(pf, one, l * alpha);
+                for (int ct = 0; ct < CT; ++ct) {
+                    float top = -INFINITY;
 #pragma unroll
-                for (int dt = 0; dt < Few::DT; ++dt)
+                    for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[dt][r] *= alpha;
+                        for (int r = 0; r < 4; ++r) {
+                            a[ct][tt][r] = key + 16 * tt + 4 * gq + r < seen[ct] ? a[ct][tt][r] : -INFINITY;
+                            top = fmaxf(top, a[ct][tt][r]);
+                        }
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const float mn = fmaxf(m[ct], top * c), alpha = fast_exp2(m[ct] - mn);
+                    m[ct] = mn;
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) pf[ct][x] = (T)fast_exp2(fmaf(a[ct][x >> 2][x & 3], c, -mn));
+                    l[ct] = dot8<T>(pf[ct], one, l[ct] * alpha);
+#pragma unroll
+                    for (int dt = 0; dt < Few::DT; ++dt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[ct][dt][r] *= alpha;
+                }
                 if (more) wait_loads_but<Few::PIECES>();   // the values (the next keys are younger)
                 else wait_loads();
 #pragma unroll
@@ -132,7 +159,8 @@ __global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts
 #pragma unroll
                         for (int y = 0; y < 4; ++y) vt[4 * h2 + y] = x[y];
                     }
-                    o[dt] = Mfma16<T>::mma(vt, pf, o[dt]);
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) o[ct][dt] = Mfma16<T>::mma(vt, pf[ct], o[ct][dt]);
                 }
                 if (!more) break;
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the values have been read
@@ -140,22 +168,24 @@ __global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts
                 key = next;
             }
         }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
         // The waves' parts joined, every thread four columns of a row
         __syncthreads();
         float *const jo = reinterpret_cast<float *>(lds), *const jm = jo + Few::WAVES * Few::ROWS * Few::PITCH, *const jl = jm + Few::WAVES * Few::ROWS;
 #pragma unroll
-        for (int dt = 0; dt < Few::DT; ++dt) *reinterpret_cast<f32x4 *>(jo + (wave * Few::ROWS + col) * Few::PITCH + dt * 16 + gq * 4) = o[dt];
-        if (gq == 0) {
-            jm[wave * Few::ROWS + col] = m;
-            jl[wave * Few::ROWS + col] = l;
+        for (int ct = 0; ct < CT; ++ct) {
+            l[ct] += __shfl_xor(l[ct], 16);
+            l[ct] += __shfl_xor(l[ct], 32);
+            const int row = wave * Few::ROWS + 16 * ct + col;
+#pragma unroll
+            for (int dt = 0; dt < Few::DT; ++dt) *reinterpret_cast<f32x4 *>(jo + row * Few::PITCH + dt * 16 + gq * 4) = o[ct][dt];
+            if (gq == 0) {
+                jm[row] = m[ct];
+                jl[row] = l[ct];
+            }
         }
         __syncthreads();
-        const int jr = threadIdx.x / (EVO_D / 4), d = threadIdx.x % (EVO_D / 4) * 4;
-        const bool mine = jr < Few::ROWS && r0 + jr < rows;
         bool nan = false;
-        if (mine) {
+        for (int jr = threadIdx.x / (EVO_D / 4), d = threadIdx.x % (EVO_D / 4) * 4; jr < Few::ROWS && r0 + jr < rows; jr += NW * 64 / (EVO_D / 4)) {
             float M = kMaskFloor, L = 0.0f;
 #pragma unroll 4
             for (int w = 0; w < Few::WAVES; ++w) M = fmaxf(M, jm[w * Few::ROWS + jr]);
@@ -195,12 +225,13 @@ __global__ void __launch_bounds__(Few::WAVES * 64) packed_few(EvoPacked p, Parts
     }
 }
 
-// The chunks of a row joined: `per` waves (1 or 4) take every per-th of them.
-template <typename T>
-__global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int per, unsigned rows) {
-    __shared__ float sums[4][128], rest[4];
+// The parts of a row joined: PER waves take every PER-th of them.
+template <typename T, int PER>
+__global__ void __launch_bounds__(PER > 4 ? PER * 64 : 256) packed_join(EvoPacked p, Parts parts, unsigned rows) {
+    constexpr int WAVES = PER > 4 ? PER : 4, per = PER;
+    __shared__ float sums[WAVES][128], rest[WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), own = wave % per;
-    const unsigned row = blockIdx.x * (4 / per) + wave / per;
+    const unsigned row = blockIdx.x * (WAVES / per) + wave / per;
     const bool mine = row < rows;   // (uniform over the wave; over the workgroup where waves share a row)
     const int i = (int)(min(row, rows - 1) / (unsigned)p.H), h = (int)(min(row, rows - 1) % (unsigned)p.H), D = p.D;
     const Segment s = segment_of_row<false>(p, i);
@@ -213,7 +244,7 @@ __global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int
     M = wave_max(M);
     float L = 0.0f, a = 0.0f, b = 0.0f;
     const int d = min(lane * 2, D - 2);
-#pragma unroll 4
+#pragma unroll 8
     for (int x = own; x < chunks; x += per) {
         const float2 y = ml[x * step], z = *reinterpret_cast<const float2 *>(o + x * step * D + d);
         const float f = fast_exp2(y.x - M);
@@ -221,11 +252,9 @@ __global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int
         a = fmaf(z.x, f, a);
         b = fmaf(z.y, f, b);
     }
-    if (per > 1) {
-        if (lane * 2 < 128) {
-            sums[wave][lane * 2] = a;
-            sums[wave][lane * 2 + 1] = b;
-        }
+    if constexpr (per > 1) {
+        sums[wave][lane * 2] = a;
+        sums[wave][lane * 2 + 1] = b;
         if (lane == 0) rest[wave] = L;
         __syncthreads();
         if (own) return;
@@ -256,61 +285,75 @@ __global__ void __launch_bounds__(256) packed_join(EvoPacked p, Parts parts, int
 }
 
 template <typename T>
-static int join(const EvoPacked &p, const Parts &parts, hipStream_t st) {
+static int join(const EvoPacked &p, const Parts &parts, int64_t average, hipStream_t st) {
     const int64_t rows = p.Tq * p.H;
-    const int per = parts.chunks > 8 ? 4 : 1;
-    packed_join<T><<<(unsigned)((rows * per + 3) / 4), 256, 0, st>>>(p, parts, per, (unsigned)rows);
+    if (average > 16) packed_join<T, 16><<<(unsigned)rows, 1024, 0, st>>>(p, parts, (unsigned)rows);
+    else if (parts.chunks > 8) packed_join<T, 4><<<(unsigned)rows, 256, 0, st>>>(p, parts, (unsigned)rows);
+    else packed_join<T, 1><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(p, parts, (unsigned)rows);
     return hip_rc();
 }
 
-// Keys of a chunk: as many as make some kFewWorkgroups workgroups of all keys and key heads, at least four steps of every wave (a workgroup that has only one spends its time on finding its place and
-// joining), all of them where one workgroup's walk over them takes less time than a second launch does.  And not so few that the parts take more than kFewScratch bytes.
-constexpr int64_t kFewWorkgroups = 512, kFewScratch = 64 << 20;
-static Parts few_parts(const EvoPacked &p, void *workspace, size_t *bytes) {
-    constexpr int64_t unit = Few::WAVES * Few::KEYS;
+// Keys of a chunk: as many as make some 256 workgroups of all sequences, keys and key heads (1024 of four waves), at least two (four) steps of every wave, since a workgroup that has only one spends its time
+// on finding its place and joining; all of them where the longest sequence's walk, taken for up to four times the average's, is no longer than a second launch's way.  And not so few that the parts take
+// more than kFewScratch bytes.
+constexpr int64_t kFewScratch = 64 << 20;
+struct FewPlan {
+    Parts parts;
+    bool many, wide;   // workgroups; columns
+    size_t bytes;
+};
+static FewPlan few_plan(const EvoPacked &p, void *workspace) {
+    FewPlan r;
+    r.many = (int64_t)p.n * p.Hk >= 128;
+    r.wide = p.Tq * (p.H / p.Hk) > (int64_t)16 * p.n;
+    const int64_t unit = (r.many ? 4 : kFewWaves) * 32, room = (r.many ? 1024 : 256) / p.Hk - p.n, least = (r.many ? 4 : 2) * unit;
     const int64_t part = p.Tq * p.H * ((int64_t)p.D + 2) * (int64_t)sizeof(float), most = kFewScratch / (part ? part : 1);
-    int64_t chunk = p.Tk * p.Hk / kFewWorkgroups;
-    if (chunk < 4 * unit) chunk = 4 * unit;
-    if (most < 2) chunk = p.Tk;
-    else if (chunk < (p.Tk + most - 1) / most) chunk = (p.Tk + most - 1) / most;
-    chunk = (chunk + unit - 1) / unit * unit;
-    if (chunk < unit) chunk = unit;
-    if (p.Tk <= 8 * unit && chunk < p.Tk) chunk = (p.Tk + unit - 1) / unit * unit;
-    Parts r;
-    r.chunk = (int)chunk;
-    r.chunks = (int)((p.Tk + chunk - 1) / chunk);
-    r.o = (float *)workspace;
-    r.ml = (float2 *)(r.o + (int64_t)r.chunks * p.Tq * p.H * p.D);
-    if (bytes) *bytes = r.chunks > 1 ? (size_t)(r.chunks * part) : 0;
+    const int64_t longest = p.n < 4 ? p.Tk : 4 * p.Tk / p.n;
+    int64_t chunk = room > 1 ? p.Tk / room : p.Tk;
+    if (chunk < least) chunk = least;
+    if (most > 1 && chunk < p.Tk / most + unit) chunk = p.Tk / most + unit;
+    chunk = (chunk + unit / 2) / unit * unit;   // (to the nearest: workgroups that all CUs can begin at once)
+    if (most < 2 || longest <= 5 * unit || chunk >= p.Tk) chunk = p.Tk < 1 ? unit : (p.Tk + unit - 1) / unit * unit;
+    r.parts.chunk = (int)chunk;
+    r.parts.chunks = (int)((p.Tk + chunk - 1) / chunk);
+    r.parts.o = (float *)workspace;
+    r.parts.ml = (float2 *)(r.parts.o + (int64_t)r.parts.chunks * p.Tq * p.H * p.D);
+    r.bytes = r.parts.chunks > 1 ? (size_t)(r.parts.chunks * part) : 0;
     return r;
 }
 
 }  // namespace
 
-size_t EVO_CAT(packed_few_bytes_d, EVO_D)(const EvoPacked &p) {
-    size_t bytes;
-    EVO_CAT(packed_d, EVO_D)::few_parts(p, nullptr, &bytes);
-    return bytes;
-}
+size_t EVO_CAT(packed_few_bytes_d, EVO_D)(const EvoPacked &p) { return EVO_CAT(packed_d, EVO_D)::few_plan(p, nullptr).bytes; }
 int EVO_CAT(launch_packed_few_d, EVO_D)(const EvoPacked &p, hipStream_t st) {
     using namespace EVO_CAT(packed_d, EVO_D);
-    const Parts parts = few_parts(p, p.workspace, nullptr);
+    const FewPlan plan = few_plan(p, p.workspace);
+    const Parts &parts = plan.parts;
     const int64_t grid = (p.Tk / parts.chunk + p.n + 2) * p.Hk, rows = p.Tq * p.H;
-    if (rows > INT32_MAX || !grid_fits(grid, Few::WAVES * 64) || !grid_fits(rows, 256)) return EVO_EOVERFLOW;
+    if (rows > INT32_MAX || !grid_fits(grid, kFewWaves * 64) || !grid_fits(rows, 1024)) return EVO_EOVERFLOW;
     return by_half(p.dtype, [&](auto t) {
         typedef decltype(t) T;
-        if (parts.chunks <= 1) {
-            packed_few<T, false><<<(unsigned)grid, Few::WAVES * 64, 0, st>>>(p, parts);
-            return hip_rc();
-        }
-        packed_few<T, true><<<(unsigned)grid, Few::WAVES * 64, 0, st>>>(p, parts);
-        const int rc = hip_rc();
-        return rc ? rc : join<T>(p, parts, st);
+        auto go = [&](auto part, auto waves, auto tiles) {
+            constexpr int NW = decltype(waves)::value, CT = decltype(tiles)::value, LDS = FewGeo<NW, CT>::LDS;
+            constexpr auto kern = packed_few<T, decltype(part)::value, NW, CT>;
+            static PerDevice done;
+            if (const int rc = ensure_dynamic_lds((const void *)kern, LDS, done, nullptr)) return rc;
+            kern<<<(unsigned)grid, NW * 64, LDS, st>>>(p, parts);
+            const int rc = hip_rc();
+            return rc || !decltype(part)::value ? rc : join<T>(p, parts, p.Tk / p.n / parts.chunk, st);
+        };
+        auto by_tiles = [&](auto part, auto waves) {
+            return plan.wide ? go(part, waves, std::integral_constant<int, 2>()) : go(part, waves, std::integral_constant<int, 1>());
+        };
+        auto by_waves = [&](auto part) {
+            return plan.many ? by_tiles(part, std::integral_constant<int, 4>()) : by_tiles(part, std::integral_constant<int, kFewWaves>());
+        };
+        return parts.chunks > 1 ? by_waves(std::true_type()) : by_waves(std::false_type());
     });
 }
 int EVO_CAT(launch_packed_join_d, EVO_D)(const EvoPacked &p, float *o, float2 *ml, int parts, hipStream_t st) {
     using namespace EVO_CAT(packed_d, EVO_D);
-    return by_half(p.dtype, [&](auto t) { return join<decltype(t)>(p, Parts{o, ml, 0, parts}, st); });
+    return by_half(p.dtype, [&](auto t) { return join<decltype(t)>(p, Parts{o, ml, 0, parts}, parts, st); });
 }
 
 }  // namespace evo
