@@ -116,7 +116,7 @@ class EvoPacked(ctypes.Structure):
         ("q_stride_t", ctypes.c_int64), ("q_stride_h", ctypes.c_int64), ("k_stride_t", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
         ("v_stride_t", ctypes.c_int64), ("v_stride_h", ctypes.c_int64), ("dout_stride_t", ctypes.c_int64), ("dout_stride_h", ctypes.c_int64),
         ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("key_offsets", ctypes.c_void_p),
-        ("o", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("dout", ctypes.c_void_p),
+        ("o", ctypes.c_void_p), ("o_low", ctypes.c_void_p), ("lse", ctypes.c_void_p), ("dout", ctypes.c_void_p),
         ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p),
         ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
     ]

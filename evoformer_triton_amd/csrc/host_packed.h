@@ -79,15 +79,17 @@ struct Packed {
         p.key_offsets = key_offsets.data_ptr();
     }
     Tensor cut(const Tensor &t) const { return t.size(2) == D ? t : t.narrow(2, 0, D).contiguous(); }
-    // o, and lse if it is wanted
-    Tensor forward(Tensor *lse) {
+    // o, and, if they are wanted, lse and (16 bits) what rounding left of o
+    Tensor forward(Tensor *lse, Tensor *low) {
         c10::DeviceGuard on(q.device());
         point();
         Tensor o = at::empty({p.Tq, p.H, p.D}, q.options()), ws;
         if (lse) *lse = at::empty({p.H, p.Tq}, q.options().dtype(at::kFloat));
+        if (low) *low = at::empty(p.dtype == EVO_F32 ? at::IntArrayRef({0, p.H, p.D}) : at::IntArrayRef({p.Tq, p.H, p.D}), q.options());
         if (p.Tq) {
             p.o = o.data_ptr();
             p.lse = lse ? (float *)lse->data_ptr() : nullptr;
+            p.o_low = low && low->numel() ? low->data_ptr() : nullptr;
             if (const size_t bytes = evoattn_packed_fwd_workspace_bytes(&p)) {
                 ws = scratch(bytes, q);
                 p.workspace = ws.data_ptr();
@@ -97,10 +99,10 @@ struct Packed {
         }
         return cut(o);
     }
-    void backward(const Tensor &dout_, const Tensor &o_, const Tensor &lse_, bool need_kv, Tensor &dq, Tensor &dk, Tensor &dv) {
+    void backward(const Tensor &dout_, const Tensor &o_, const Tensor &lse_, const Tensor &low_, bool need_kv, Tensor &dq, Tensor &dk, Tensor &dv) {
         c10::DeviceGuard on(q.device());
         point();
-        const Tensor dout = ready(dout_, p.D), lse = lse_.contiguous();
+        const Tensor dout = ready(dout_, p.D), lse = lse_.contiguous(), low = low_.contiguous();
         Tensor o = ready(o_, p.D);
         if (!o.is_contiguous()) o = o.contiguous();
         dq = at::empty({p.Tq, p.H, p.D}, q.options());
@@ -113,6 +115,7 @@ struct Packed {
             p.dout = ptr_or_null(dout);
             p.o = const_cast<void *>(ptr_or_null(o));
             p.lse = (float *)const_cast<void *>(ptr_or_null(lse));
+            p.o_low = low.numel() ? low.data_ptr() : nullptr;
             p.dq = const_cast<void *>(ptr_or_null(dq));
             p.dk = const_cast<void *>(ptr_or_null(dk));
             p.dv = const_cast<void *>(ptr_or_null(dv));
@@ -133,7 +136,7 @@ struct PackedNode : SavingNode {
     EvoPacked p{};
     int64_t D = 0;
     std::string name() const override { return "PackedAttentionBackward"; }
-    // saved: queries, keys, values, offsets, key offsets, lse, the output; results: queries, keys, values
+    // saved: queries, keys, values, offsets, key offsets, lse, the output, what rounding left of it; results: queries, keys, values
     variable_list apply(variable_list &&grads) override {
         std::lock_guard<std::mutex> lock(mutex_);
         const bool rec = at::GradMode::is_enabled();
@@ -151,7 +154,7 @@ struct PackedNode : SavingNode {
             c.offsets = t[3];
             c.key_offsets = t[4];
             const Tensor dout = grads[0].scalar_type() == c.q.scalar_type() ? grads[0] : grads[0].to(c.q.scalar_type());
-            c.backward(dout, t[6], t[5], task_should_compute_output(1) || task_should_compute_output(2), out[0], out[1], out[2]);
+            c.backward(dout, t[6], t[5], t[7], task_should_compute_output(1) || task_should_compute_output(2), out[0], out[1], out[2]);
             for (int i = 0; i < 3; ++i)
                 if (!task_should_compute_output(i)) out[i] = Tensor();
         }
@@ -167,11 +170,11 @@ OptTensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
     if (key_offsets && key_offsets->defined() && !plain(*key_offsets)) return std::nullopt;
     const bool wanted = SavingNode::wanted(q, k, v);
     Packed c;
-    Tensor o, lse;
+    Tensor o, lse, low;
     {
         at::AutoDispatchBelowADInplaceOrView guard;
         if (c.take(q, k, v, offsets, key_offsets, causal, scale)) return std::nullopt;
-        o = c.forward(wanted ? &lse : nullptr);
+        o = c.forward(wanted ? &lse : nullptr, wanted ? &low : nullptr);
     }
     if (wanted) {
         auto node = make_node<PackedNode>(q, k, v);
@@ -183,32 +186,35 @@ OptTensor packed_attention(const Tensor &q, const Tensor &k, const Tensor &v, co
         node->save(c.key_offsets);
         node->save(lse);
         node->save(o, true);
+        node->save(low);
     }
     return o;
 }
 
 // The same launches without a node, for the registered operators.
-std::pair<Tensor, Tensor> packed_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, const OptTensor &key_offsets, bool causal,
+std::tuple<Tensor, Tensor, Tensor> packed_forward(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, const OptTensor &key_offsets, bool causal,
                                          std::optional<double> scale) {
     Packed c;
     const char *wrong = c.take(q, k, v, offsets, key_offsets, causal, scale);
     TORCH_CHECK_VALUE(!wrong, wrong);
     TORCH_CHECK(q.is_cuda(), "packed attention runs on the GPU only");
     TORCH_CHECK_NOT_IMPLEMENTED(!dual(q) && !dual(k) && !dual(v), "packed_attention has no formula for forward mode differentiation");
-    Tensor lse, o = c.forward(&lse);
-    return {o, lse};
+    Tensor lse, low, o = c.forward(&lse, &low);
+    return {o, lse, low};
 }
 std::tuple<Tensor, Tensor, Tensor> packed_backward(const Tensor &dout, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, const OptTensor &key_offsets,
-                                                   const Tensor &o, const Tensor &lse, bool causal, std::optional<double> scale) {
+                                                   const Tensor &o, const Tensor &lse, const Tensor &low, bool causal, std::optional<double> scale) {
     Packed c;
     const char *wrong = c.take(q, k, v, offsets, key_offsets, causal, scale);
     TORCH_CHECK_VALUE(!wrong, wrong);
     TORCH_CHECK(q.is_cuda(), "packed attention runs on the GPU only");
     TORCH_CHECK_VALUE(dout.device() == q.device() && dout.sizes().equals(q.sizes()) && dout.scalar_type() == q.scalar_type() && o.device() == q.device() &&
                           o.sizes().equals(q.sizes()) && o.scalar_type() == q.scalar_type() && lse.device() == q.device() && lse.scalar_type() == at::kFloat &&
-                          lse.dim() == 2 && lse.size(0) == q.size(1) && lse.size(1) == q.size(0), "the output, its gradient and lse must be as the forward gave them");
+                          lse.dim() == 2 && lse.size(0) == q.size(1) && lse.size(1) == q.size(0) && low.device() == q.device() && low.scalar_type() == q.scalar_type() &&
+                          low.dim() == 3 && low.size(0) == (c.p.dtype == EVO_F32 ? 0 : q.size(0)) && low.size(1) == q.size(1) && low.size(2) == c.p.D,
+                      "the output, its gradient, lse and what rounding left must be as the forward gave them");
     Tensor dq, dk, dv;
-    c.backward(dout, o, lse, true, dq, dk, dv);
+    c.backward(dout, o, lse, low, true, dq, dk, dv);
     return {dq, dk, dv};
 }
 std::optional<std::string> packed_wrong(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &offsets, const OptTensor &key_offsets, bool causal,

@@ -67,7 +67,7 @@ static int packed_check(const EvoPacked *p) {
 // The matrix kernels move pieces of 16 bytes, address the rows of a stage by 32 bits, and take what is beyond a sequence for out of range, which rows have to lie apart for.
 static bool packed_aligned(const EvoPacked &p, bool backward) {
     if (p.dtype == EVO_F32) return true;
-    for (const void *x : {p.q, p.k, p.v, (const void *)p.o, backward ? p.dout : nullptr, backward ? (const void *)p.dq : nullptr, backward ? (const void *)p.dk : nullptr,
+    for (const void *x : {p.q, p.k, p.v, (const void *)p.o, (const void *)p.o_low, backward ? p.dout : nullptr, backward ? (const void *)p.dq : nullptr, backward ? (const void *)p.dk : nullptr,
                           backward ? (const void *)p.dv : nullptr})
         if ((uintptr_t)x % 16) return false;
     for (int64_t x : {p.q_stride_t, p.k_stride_t, p.v_stride_t, backward ? p.dout_stride_t : 0})

@@ -124,10 +124,17 @@ __device__ __forceinline__ const T *head_row(const void *x, int64_t row, int64_t
     return (const T *)x + row * stride_t + h * stride_h;
 }
 
-// What dQ's kernel leaves for that of dK and dV, [H][Tq] each: -delta, and the row's log-sum -lse in units of q . k (16 bits: what their products begin with).
+// What dQ's kernel leaves for that of dK and dV, [H][Tq] each: -delta and -lse, the latter in units of q . k (16 bits: what their products begin with).
 struct BackwardRows {
     float *delta, *base;
 };
+// The forward's lse is that of rounded probabilities, and its output, of which delta is formed, theirs too.  The sums that dQ's kernel has of probabilities (`sum`, 1 but for that) and of ds (`rest`, 0 but for that) say by how
+// much: what dK and dV are formed with is put right by them.
+__device__ __forceinline__ void save_row(const BackwardRows &to, int64_t at, float lse, float delta, float sum, float rest, float c) {
+    const bool any = sum > 0.0f;
+    to.delta[at] = -(any ? delta + rest / sum : delta);
+    to.base[at] = -(any ? lse + __log2f(sum) : lse) / c;
+}
 
 // ---- One row by one wave, products and sums in fp32: the kernels for fp32, and what the matrix kernels leave for rows whose result is no
 // number: there a masked key or query may hold an infinity or a NaN, which a product with a probability of zero does not keep out.
@@ -154,6 +161,7 @@ __device__ __forceinline__ void row_forward(const EvoPacked &p, const Segment &s
     o.a *= inv;
     o.b *= inv;
     store_row((T *)p.o + ((int64_t)i * p.H + h) * p.D, o, p.D);
+    if (p.o_low) store_row((T *)p.o_low + ((int64_t)i * p.H + h) * p.D, Row{o.a - (float)(T)o.a, o.b - (float)(T)o.b}, p.D);
     if (p.lse && lane == 0) p.lse[(int64_t)h * p.Tq + i] = seen ? m + __log2f(l) : INFINITY;
 }
 

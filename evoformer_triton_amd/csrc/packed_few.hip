@@ -214,6 +214,7 @@ __global__ void __launch_bounds__(NW * 64) packed_few(EvoPacked p, Parts parts) 
                     nan |= d < D && !(sum[y] == sum[y]);
                 }
                 if (d < D) store4<T>((T *)p.o + row * D + d, sum[0], sum[1], sum[2], sum[3]);
+                if (d < D && p.o_low) store4<T>((T *)p.o_low + row * D + d, left<T>(sum[0]), left<T>(sum[1]), left<T>(sum[2]), left<T>(sum[3]));
                 if (d == 0 && p.lse) p.lse[(int64_t)oh * p.Tq + oi] = sees ? M + __log2f(L) : INFINITY;
             }
         }
@@ -280,6 +281,11 @@ __global__ void __launch_bounds__(PER > 4 ? PER * 64 : 256) packed_join(EvoPacke
         x[0] = (T)a;
         x[1] = (T)b;
         *reinterpret_cast<typename Mfma<T>::v2 *>(out) = x;
+        if (p.o_low) {
+            x[0] = (T)left<T>(a);
+            x[1] = (T)left<T>(b);
+            *reinterpret_cast<typename Mfma<T>::v2 *>((T *)p.o_low + ((int64_t)i * p.H + h) * D + lane * 2) = x;
+        }
     }
     if (lane == 0 && p.lse) p.lse[(int64_t)h * p.Tq + i] = sees ? M + __log2f(L) : INFINITY;
 }

@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
     if (seen_most == 0) {   // (with parts: packed_join's)
         if (PART) return;
         zero_rows((T *)p.o, at.first, rows, p.H, h, D);
+        if (p.o_low) zero_rows((T *)p.o_low, at.first, rows, p.H, h, D);
         if (p.lse && (int)threadIdx.x < rows) p.lse[(int64_t)h * p.Tq + at.first + threadIdx.x] = INFINITY;
         return;
     }
@@ -195,16 +196,24 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
     unsigned again = rows_without_number(nan && mine);
     const bool whole = mine && !(again >> li & 1);
     if (p.lse && whole && g == 0) p.lse[(int64_t)h * p.Tq + qrow] = seen ? m + __log2f(l) : INFINITY;
-    T *out = (T *)p.o + ((int64_t)qrow * p.H + h) * D;
+    const int64_t row = ((int64_t)qrow * p.H + h) * D;
 #pragma unroll
-    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>(out, dt * 32, whole ? D : 0, o[dt], 1.0f, g);
+    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>((T *)p.o + row, dt * 32, whole ? D : 0, o[dt], 1.0f, g);
+    if (p.o_low) {
+#pragma unroll
+        for (int dt = 0; dt < R::DT; ++dt) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] = left<T>(o[dt][r]);
+            store_row_tile<T>((T *)p.o_low + row, dt * 32, whole ? D : 0, o[dt], 1.0f, g);
+        }
+    }
     for (; again; again &= again - 1) row_forward<T>(p, s, q0 + __builtin_ctz(again), h);
 }
 
 // ------------------------------------------------------------------ dQ
 
 template <typename T, int KG, bool PART>
-__global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2) packed_dq(EvoPacked p, BackwardRows out_rows, Parts parts, int tiles) {
+__global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) packed_dq(EvoPacked p, BackwardRows out_rows, Parts parts, int tiles) {
     typedef PackedGeo R;
     typedef R::G G;
     typedef StagePieces<4 * KG> Pieces;
@@ -252,23 +261,25 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
         load_operands((const T *)p.o + ((int64_t)qrow * p.H + h) * D, D, g, of);
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) dl = dot8<T>(df[ks], of[ks], dl);
+        if (p.o_low) {
+            load_operands((const T *)p.o_low + ((int64_t)qrow * p.H + h) * D, D, g, of);
+#pragma unroll
+            for (int ks = 0; ks < R::KSD; ++ks) dl = dot8<T>(df[ks], of[ks], dl);
+        }
     }
     dl += __shfl_xor(dl, 32);
     const float c = p.scale * kLog2e, lse = p.lse[(int64_t)h * p.Tq + qrow];
-    if (mine && g == 0 && part == 0 && key_group == 0) {
-        out_rows.delta[(int64_t)h * p.Tq + qrow] = -dl;
-        out_rows.base[(int64_t)h * p.Tq + qrow] = -lse / c;
-    }
     const int seen = s.seen(qrow, p.causal);
     const int wave_least = active ? s.seen(q0, p.causal) : 0, wave_most = active ? s.seen(min(q0 + 31, s.q1 - 1), p.causal) : 0;
     f32x16 dq[R::DT];
+    float sum[2] = {0.0f, 0.0f}, rest[2] = {0.0f, 0.0f};   // of the probabilities, which should be 1, and of ds, which should be 0
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt) dq[dt] = filled(0.0f);
 
     const Staged staged(lane);
     auto step = [&](const unsigned char *buf, int kb, int key0) __attribute__((always_inline)) {
         const unsigned at = Staged::base(buf) + key_group * R::ARRAY;
-        v8 kf[R::KSD], kt[2][R::DT];
+        v8 kf[R::KSD];
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) kf[ks] = staged.rows<T>(at, kb, ks);
         __builtin_amdgcn_sched_barrier(0);
@@ -277,54 +288,80 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
         for (int ks = 0; ks < R::KSD; ++ks) a = Mfma<T>::mma(kf[ks], qf[ks], a);
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) d = Mfma<T>::mma(staged.rows<T>(at + ARRAY, kb, ks), df[ks], d);
-#pragma unroll
-        for (int ts = 0; ts < 2; ++ts)
-#pragma unroll
-            for (int dt = 0; dt < R::DT; ++dt) kt[ts][dt] = staged.cols<T>(at, kb, ts, dt);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) d[r] *= fast_exp2(fmaf(a[r], c, -lse));
         if (key0 + 32 > wave_least) {   // (uniform)
             asm volatile("");
 #pragma unroll
-            for (int r = 0; r < 16; ++r) d[r] = key0 + crow(r, g) < seen ? d[r] : 0.0f;
+            for (int r = 0; r < 16; ++r) {
+                const bool sees = key0 + crow(r, g) < seen;
+                a[r] = sees ? a[r] : -INFINITY;
+                d[r] = sees ? d[r] : 0.0f;
+            }
         }
-        v8 pf[2];
 #pragma unroll
-        for (int ts = 0; ts < 2; ++ts)
+        for (int r = 0; r < 16; ++r) {
+            const float e = fast_exp2(fmaf(a[r], c, -lse));
+            sum[r & 1] += e;
+            d[r] *= e;
+            rest[r & 1] += d[r];
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) pf[ts][i] = (T)d[8 * ts + i];
+        for (int ts = 0; ts < 2; ++ts) {
+            v8 hi, lo, kt[R::DT];
 #pragma unroll
-        for (int ts = 0; ts < 2; ++ts)
+            for (int dt = 0; dt < R::DT; ++dt) kt[dt] = staged.cols<T>(at, kb, ts, dt);
 #pragma unroll
-            for (int dt = 0; dt < R::DT; ++dt) dq[dt] = Mfma<T>::mma(kt[ts][dt], pf[ts], dq[dt]);
+            for (int i = 0; i < 8; ++i) {
+                hi[i] = (T)d[8 * ts + i];
+                lo[i] = (T)left<T>(d[8 * ts + i]);
+            }
+#pragma unroll
+            for (int dt = 0; dt < R::DT; ++dt) dq[dt] = Mfma<T>::mma(kt[dt], hi, dq[dt]);
+#pragma unroll
+            for (int dt = 0; dt < R::DT; ++dt) dq[dt] = Mfma<T>::mma(kt[dt], lo, dq[dt]);
+        }
     };
     for (int st = from; st < to; ++st) {
         wait_loads_but<(BUFS - 2) * 2 * Pieces::each(KEYS)>();
         wait_lds_barrier();
         fetch(st + BUFS - 1);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
+#pragma unroll 1
+        for (int t = 0; t < 2; ++t) {   // (one after the other: interleaved they have too few registers)
             const int key0 = st * KEYS + key_group * R::STAGE + 32 * t;
             if (key0 < wave_most) step(lds + st % BUFS * (2 * ARRAY), 32 * t, key0);
         }
     }
     wait_loads();
+    sum[0] += sum[1];
+    rest[0] += rest[1];
     if constexpr (KG == 2) {
-        float *const x = reinterpret_cast<float *>(lds) + own * R::DT * 16 * 64;
+        float *const x = reinterpret_cast<float *>(lds) + own * (R::DT * 16 + 2) * 64, *const more = x + R::DT * 16 * 64;
         wait_lds_barrier();
-        if (key_group) give(dq, x, lane);
+        if (key_group) {
+            give(dq, x, lane);
+            more[lane] = sum[0];
+            more[64 + lane] = rest[0];
+        }
         wait_lds_barrier();
         if (key_group) return;
         take(dq, x, lane);
+        sum[0] += more[lane];
+        rest[0] += more[64 + lane];
     }
     if (!active) return;
+    sum[0] += __shfl_xor(sum[0], 32);
+    rest[0] += __shfl_xor(rest[0], 32);
     if constexpr (PART) {
         const int64_t row = ((int64_t)part * p.Tq + qrow) * p.H + h;
 #pragma unroll
         for (int dt = 0; dt < R::DT; ++dt) store_row_part(parts.o + row * D, dt * 32, mine ? D : 0, dq[dt], g);
+        if (mine && g == 0) {
+            parts.ml[row] = make_float2(sum[0], rest[0]);
+            if (part == 0) out_rows.delta[(int64_t)h * p.Tq + qrow] = dl;
+        }
         return;
     }
+    const float inv = seen ? 1.0f / sum[0] : 0.0f;
+    if (mine && g == 0) save_row(out_rows, (int64_t)h * p.Tq + qrow, lse, dl, sum[0], rest[0], c);
     bool nan = false;
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt)
@@ -334,7 +371,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
     const bool whole = mine && !(again >> li & 1);
     T *out = (T *)p.dq + ((int64_t)qrow * p.H + h) * D;
 #pragma unroll
-    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>(out, dt * 32, whole ? D : 0, dq[dt], p.scale, g);
+    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>(out, dt * 32, whole ? D : 0, dq[dt], p.scale * inv, g);
     for (; again; again &= again - 1) {
         const int b = __builtin_ctz(again);
         row_dq<T>(p, s, q0 + b, h, lane_value(dl, b));
@@ -367,7 +404,7 @@ int EVO_CAT(launch_packed_fwd_d, EVO_D)(const EvoPacked &p, hipStream_t st) {
         });
     });
 }
-size_t EVO_CAT(packed_dq_bytes_d, EVO_D)(const EvoPacked &p) { return EVO_CAT(packed_d, EVO_D)::query_plan(p).bytes(p.Tq * p.H, p.D); }
+size_t EVO_CAT(packed_dq_bytes_d, EVO_D)(const EvoPacked &p) { return EVO_CAT(packed_d, EVO_D)::query_plan(p).bytes(p.Tq * p.H, p.D + 2); }
 int EVO_CAT(launch_packed_dq_d, EVO_D)(const EvoPacked &p, const BackwardRows &saved, float *sums, hipStream_t st) {
     using namespace EVO_CAT(packed_d, EVO_D);
     const Plan plan = query_plan(p);
@@ -380,7 +417,7 @@ int EVO_CAT(launch_packed_dq_d, EVO_D)(const EvoPacked &p, const BackwardRows &s
             constexpr auto kern = packed_dq<T, KG, decltype(part)::value>;
             static PerDevice done;
             if (const int rc = ensure_dynamic_lds((const void *)kern, LDS, done, nullptr)) return rc;
-            const Parts parts = {sums, nullptr, 0, plan.parts};
+            const Parts parts = {sums, (float2 *)(sums + plan.parts * rows * p.D), 0, plan.parts};
             kern<<<(unsigned)grid, 256 * KG, LDS, st>>>(p, saved, parts, (int)tiles);
             if (const int rc = hip_rc()) return rc;
             if (!decltype(part)::value) return (int)EVO_OK;

@@ -116,6 +116,10 @@ __device__ __forceinline__ unsigned rows_without_number(bool nan) {
     return (unsigned)b | (unsigned)(b >> 32);
 }
 
+// What rounding leaves
+template <typename T>
+__device__ __forceinline__ float left(float v) { return v - (float)(T)v; }
+
 __device__ __forceinline__ f32x16 filled(float v) {
     f32x16 x;
 #pragma unroll
@@ -204,15 +208,33 @@ __global__ void __launch_bounds__(256) packed_sum(EvoPacked p, BackwardRows save
         }
         nan |= !(sum[y].x == sum[y].x) || !(sum[y].y == sum[y].y);
     }
+    float scale = p.scale;
+    if constexpr (!KEYS) {   // (of the probabilities and of ds: see packed_dq)
+        const int64_t at = (int64_t)h * p.Tq + i;
+        const float delta = any ? saved.delta[at] : 0.0f, c = p.scale * kLog2e;
+        float total = 0.0f, rest = 0.0f;
+        if (any) {
+            for (int x = 0; x < parts.chunks; ++x) {
+                const float2 y = parts.ml[(int64_t)x * rows + row];
+                total += y.x;
+                rest += y.y;
+            }
+        }
+        if (lane == 0 && any) save_row(saved, at, p.lse[at], delta, total, rest, c);
+        scale = any ? scale / total : 0.0f;
+        if (__any(nan)) {
+            row_dq<T>(p, s, i, h, delta);
+            return;
+        }
+    }
     if (__any(nan)) {
         if constexpr (KEYS) row_dkdv<T>(p, s, i, h, saved.delta);
-        else row_dq<T>(p, s, i, h, -saved.delta[(int64_t)h * p.Tq + i]);
         return;
     }
     if (lane * 2 >= D) return;
 #pragma unroll
     for (int y = 0; y < (KEYS ? 2 : 1); ++y) {
-        const float f = y ? 1.0f : p.scale;
+        const float f = y ? 1.0f : scale;
         typename Mfma<T>::v2 v;
         v[0] = (T)(sum[y].x * f);
         v[1] = (T)(sum[y].y * f);
@@ -233,9 +255,10 @@ struct Plan {
     }
 };
 // units: tiles and heads; steps: of an average sequence's walk, 64 rows each.  Parts: as many as make some `fill` workgroups, of `few` steps at least where a CU is left to itself (up to 64 units),
-// of `more` up to 256 and of 32 beyond; for `most` units and fewer.
+// of `more` up to 256 and of 32 beyond; for `most` units and fewer.  Two groups while the workgroups of eight waves all fit at once, two or (D = 32) three of them to a CU:
+// 2048 causal rows of 24 heads and D = 128 43 us (53 with one group), of 40 heads 73 (59).
 static Plan plan_for(int64_t units, int64_t steps, int64_t fill, int64_t most, int64_t few, int64_t more) {
-    Plan r = {steps >= 12 && units <= (EVO_D == 32 ? 768 : 400) ? 2 : 1, 1};
+    Plan r = {steps >= 12 && units <= (EVO_D == 32 ? 768 : 512) ? 2 : 1, 1};
     if (units && units <= most) {
         const int64_t room = fill / units, worth = steps / (units <= 64 ? few : units <= 256 ? more : 32), n = room < worth ? room : worth;
         r.parts = (int)(n < 1 ? 1 : n > 16 ? 16 : n);

@@ -58,40 +58,41 @@ def packed_positions(offsets: torch.Tensor, rows: int) -> torch.Tensor:
 
 @torch.library.custom_op("evoattn::packed", mutates_args=(), device_types="cuda")
 def _op_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, key_offsets: Optional[torch.Tensor], causal: bool,
-               scale: Optional[float]) -> Tuple[torch.Tensor, torch.Tensor]:
-    """(o, lse)"""
+               scale: Optional[float]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(o, lse, what rounding left of o)"""
     return _lib.host().packed_forward(q, k, v, offsets, key_offsets, causal, scale)
 
 
 @_op_packed.register_fake
 def _(q, k, v, offsets, key_offsets, causal, scale):
-    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32)
+    low = (0, q.shape[1], q.shape[2]) if q.dtype == torch.float32 else (q.shape[0], q.shape[1], (q.shape[2] + 7) // 8 * 8)
+    return q.new_empty(q.shape), q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32), q.new_empty(low)
 
 
 @torch.library.custom_op("evoattn::packed_bwd", mutates_args=(), device_types="cuda")
 def _op_packed_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, key_offsets: Optional[torch.Tensor],
-                   o: torch.Tensor, lse: torch.Tensor, causal: bool, scale: Optional[float]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _lib.host().packed_backward(dout, q, k, v, offsets, key_offsets, o, lse, causal, scale)
+                   o: torch.Tensor, lse: torch.Tensor, low: torch.Tensor, causal: bool, scale: Optional[float]) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return _lib.host().packed_backward(dout, q, k, v, offsets, key_offsets, o, lse, low, causal, scale)
 
 
 @_op_packed_bwd.register_fake
-def _(dout, q, k, v, offsets, key_offsets, o, lse, causal, scale):
+def _(dout, q, k, v, offsets, key_offsets, o, lse, low, causal, scale):
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
 
 
 def _setup_context(ctx, inputs, output):
     q, k, v, offsets, key_offsets, ctx.causal, ctx.scale = inputs
-    o, lse = output
-    ctx.save_for_backward(q, k, v, offsets, key_offsets, o, lse)
-    ctx.mark_non_differentiable(lse)
+    o, lse, low = output
+    ctx.save_for_backward(q, k, v, offsets, key_offsets, o, lse, low)
+    ctx.mark_non_differentiable(lse, low)
     ctx.set_materialize_grads(False)
 
 
-def _backward(ctx, dout, _):
+def _backward(ctx, dout, *_):
     if dout is None:
         return (None,) * 7
-    q, k, v, offsets, key_offsets, o, lse = ctx.saved_tensors
-    grads = torch.ops.evoattn.packed_bwd(dout.to(q.dtype), q, k, v, offsets, key_offsets, o, lse, ctx.causal, ctx.scale)
+    q, k, v, offsets, key_offsets, o, lse, low = ctx.saved_tensors
+    grads = torch.ops.evoattn.packed_bwd(dout.to(q.dtype), q, k, v, offsets, key_offsets, o, lse, low, ctx.causal, ctx.scale)
     return *(g if n else None for g, n in zip(grads, ctx.needs_input_grad)), None, None, None, None
 
 
