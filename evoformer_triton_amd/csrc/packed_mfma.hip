@@ -324,8 +324,9 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
         wait_loads_but<(BUFS - 2) * 2 * Pieces::each(KEYS)>();
         wait_lds_barrier();
         fetch(st + BUFS - 1);
-#pragma unroll 1
-        for (int t = 0; t < 2; ++t) {   // (one after the other: interleaved they have too few registers)
+        // (interleaved for D = 64 they would need more than the 168 registers of three waves to a SIMD: 10 of them would live in memory)
+#pragma unroll (EVO_D == 64 ? 1 : 2)
+        for (int t = 0; t < 2; ++t) {
             const int key0 = st * KEYS + key_group * R::STAGE + 32 * t;
             if (key0 < wave_most) step(lds + st % BUFS * (2 * ARRAY), 32 * t, key0);
         }
