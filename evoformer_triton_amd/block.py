@@ -22,6 +22,9 @@ idle), and lays the results out so that the attention kernels read them as they 
   * the pair bias Linear(LayerNorm(z)) comes from one kernel as [B,1,H,N,N] in the dtype of Q, so the attention kernels
     take it from 16-bit tiles; for shapes that kernel does not take, from the separate steps and a permute;
   * a learned relative position bias (`relative.py`) is added to the pair bias, or stands for it, if the block has one;
+  * queries and keys are turned by their positions (`rotary.py`), in place in the GEMM's result, if the block is made so;
+  * sequences of different lengths can come one after the other instead of padded to the longest (`packed.py`,
+    `GatedAttentionBlock.packed`);
   * the projections run in 8 bits (`fp8.py`) if the block is made so.
 """
 from __future__ import annotations
@@ -35,7 +38,9 @@ from . import _lib
 from . import evoformer as _evoformer
 from .evoformer import _DTYPES, _HEAD_DIMS, _SlotAttention, _alloc_bytes, _on_device, _ptr, _stream, evoformer_attention
 from .fp8 import Fp8Weight, fp8_linear
+from .packed import packed_attention, packed_positions
 from .relative import RelativePositionBias
+from .rotary import RotaryPositions
 
 
 def _row_slices(rows: int, n_out: int, n_in: int) -> int:
@@ -210,19 +215,20 @@ class GatedAttentionBlock(nn.Module):
     m    [B,S,N,c_m]   the representation attended over (S rows of N residues)
     z    [B,N,N,c_z]   optional pair representation; its projection to H channels is the bias
     mask [B,S,N]       optional, 1 = keep, 0 = drop the key (bool or float)
-    positions [B,N] or [N], chains alike (optional): the residues' numbers and chains, for a block with a relative position bias
+    positions [B,N] or [N], chains alike (optional): the residues' numbers and chains, for a block with a relative position bias; the positions for one with rotary positions too
     weights            Fp8BlockWeights of `fp8_weights()`, for inference with a block in 8 bits; else the weights are rounded with each call
     ->   [B,S,N,c_m]
 
     fp8                       the projections in 8 bits (fp8_linear): operands rounded to e4m3 with a scale for each block of 128, forward and backward
     relative_distance, relative_buckets, other_chain   a learned relative position bias, as RelativePositionBias takes them
+    rotary                    a RotaryPositions of head dim c_hidden: what queries and keys are turned by
     """
 
     fp8 = False
 
     def __init__(self, c_m: int, c_hidden: int, no_heads: int, c_z: Optional[int] = None, gating: bool = True,
                  inf: float = 1e9, fp8: bool = False, relative_distance: Optional[int] = None, relative_buckets: Optional[int] = None,
-                 other_chain: bool = False):
+                 other_chain: bool = False, rotary: Optional[RotaryPositions] = None):
         super().__init__()
         if fp8:
             self.fp8 = True
@@ -245,6 +251,9 @@ class GatedAttentionBlock(nn.Module):
             raise ValueError("relative_buckets and other_chain need relative_distance")
         else:
             self.relative = None
+        if rotary is not None and rotary.head_dim != c_hidden:
+            raise ValueError(f"rotary positions of head dim {rotary.head_dim} in a block of head dim {c_hidden}")
+        self.rotary = rotary
 
     def _stacked_weights(self):
         layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
@@ -265,11 +274,15 @@ class GatedAttentionBlock(nn.Module):
         bias [B,1,H,N,N].  `plain`: the framework's LayerNorm and Linear throughout (what
         `forward_eager` uses), else the library's LayerNorm kernels and the projections with
         their weight gradients summed over slices of the rows."""
-        B, S, N, _ = m.shape
-        H, D = self.no_heads, self.c_hidden
         norm = (lambda layer, t: layer(t)) if plain or not m.is_cuda else _layer_norm
         lin = (lambda layer, t: layer(t)) if plain else _linear
-        x = norm(self.layer_norm_m, m)
+        q, k, v, g = self._heads(norm(self.layer_norm_m, m), positions, plain, weights)
+        bias, add_mask = self._bias_and_mask(z, mask, q.dtype, m.shape[:3], norm, lin, positions, chains, plain)
+        return q, k, v, g, add_mask, bias
+
+    def _heads(self, x, positions, plain, weights):
+        """Q, K (turned by their positions), V and the gate of a normalised input [..., c_m], [..., H, D] each."""
+        H, D = self.no_heads, self.c_hidden
         layers = [self.linear_q, self.linear_k, self.linear_v] + ([self.linear_g] if self.linear_g is not None else [])
         if plain or (not self.fp8 and any(_recast(layer, x) for layer in layers)):
             outs = [layer(x) for layer in layers]
@@ -277,10 +290,24 @@ class GatedAttentionBlock(nn.Module):
             outs = self._project(x, weights).unflatten(-1, (len(layers), H * D)).unbind(-2)
         else:
             outs = _Projections.apply(x, *(t for layer in layers for t in (layer.weight, layer.bias)))
-        q, k, v = (t.view(B, S, N, H, D) for t in outs[:3])
-        g = outs[3].view(B, S, N, H, D) if self.linear_g is not None else None
-        bias, add_mask = self._bias_and_mask(z, mask, q.dtype, (B, S, N), norm, lin, positions, chains, plain)
-        return q, k, v, g, add_mask, bias
+        q, k, v, *g = (t.view(*x.shape[:-1], H, D) for t in outs)
+        rotary = self._modules.get("rotary")
+        if rotary is not None:
+            q, k = (rotary.plain if plain else rotary)(q, k, positions)
+        return q, k, v, g[0] if g else None
+
+    def _slots(self, x, positions, weights):
+        """The same, [..., slots, H, D], from one GEMM (see `_slots_ok`)."""
+        gated = self.linear_g is not None
+        if self.fp8:
+            y = self._project(x, weights)
+        else:
+            projections = [self.linear_q.weight, self.linear_k.weight, self.linear_v.weight] + ([self.linear_g.weight] if gated else [])
+            y = _StackedProjection.apply(x, self.linear_g.bias if gated else None, *projections)
+        shape, rotary = (*x.shape[:-1], 4 if gated else 3, self.no_heads, self.c_hidden), self._modules.get("rotary")
+        if rotary is not None:
+            y = rotary.rotate_slots(y, shape, positions)
+        return y.view(shape)
 
     def _project(self, x: torch.Tensor, weights: Optional[Fp8BlockWeights]) -> torch.Tensor:
         """Q, K, V (and the gate) side by side, in 8 bits."""
@@ -308,10 +335,10 @@ class GatedAttentionBlock(nn.Module):
         return bias, add_mask
 
     def _check(self, positions, chains, weights):
-        relative = self._modules.get("relative")      # (a block that was saved before it could have one has none)
-        if (positions is None) != (relative is None):
-            raise ValueError("a block with a relative position bias needs the residues' positions" if positions is None else
-                             "positions are for a block with a relative position bias (relative_distance)")
+        relative, rotary = self._modules.get("relative"), self._modules.get("rotary")      # (a block that was saved before it could have one has none)
+        if (positions is None) != (relative is None and rotary is None):
+            raise ValueError("a block with a relative position bias or rotary positions needs the residues' positions" if positions is None else
+                             "positions are for a block with a relative position bias (relative_distance) or rotary positions (rotary)")
         if chains is not None and (relative is None or not relative.other_chain):
             raise ValueError("chains are for a block with a bucket for pairs of different chains (other_chain=True)")
         if weights is not None and not self.fp8:
@@ -350,7 +377,8 @@ class GatedAttentionBlock(nn.Module):
     def forward(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None, chains: Optional[torch.Tensor] = None, weights: Optional[Fp8BlockWeights] = None):
         B, S, N, _ = m.shape
-        simple = not self.fp8 and self._modules.get("relative") is None and positions is None and chains is None and weights is None
+        mods = self._modules
+        simple = not self.fp8 and mods.get("relative") is None and mods.get("rotary") is None and positions is None and chains is None and weights is None
         if not simple:
             self._check(positions, chains, weights)
         if self._slots_ok(m):
@@ -358,19 +386,41 @@ class GatedAttentionBlock(nn.Module):
             if out is not None:
                 return out
             H, D = self.no_heads, self.c_hidden
-            gated = self.linear_g is not None
-            x = _layer_norm(self.layer_norm_m, m)
-            if self.fp8:
-                P = self._project(x, weights).view(B, S, N, 4 if gated else 3, H, D)
-            else:
-                projections = [self.linear_q.weight, self.linear_k.weight, self.linear_v.weight] + ([self.linear_g.weight] if gated else [])
-                P = _StackedProjection.apply(x, self.linear_g.bias if gated else None, *projections).view(B, S, N, len(projections), H, D)
+            P = self._slots(_layer_norm(self.layer_norm_m, m), positions, weights)
             bias, add_mask = self._bias_and_mask(z, mask, m.dtype, (B, S, N), _layer_norm, _linear, positions, chains)
-            o, grad_slot = _SlotAttention.apply(P, add_mask, bias, gated)
+            o, grad_slot = _SlotAttention.apply(P, add_mask, bias, self.linear_g is not None)
             return self._output(o.reshape(B, S, N, H * D), weights, grad_slot.view(B, S, N, H * D))
         q, k, v, g, add_mask, bias = self.operands(m, z, mask, positions=positions, chains=chains, weights=weights)
         o = evoformer_attention(q, k, v, add_mask, bias, layout="ds4sci", gate=g)
         return self._output(o.reshape(B, S, N, self.no_heads * self.c_hidden), weights)
+
+    def packed(self, m: torch.Tensor, offsets: torch.Tensor, positions: Optional[torch.Tensor] = None, causal: bool = False,
+               weights: Optional[Fp8BlockWeights] = None) -> torch.Tensor:
+        """The block without pair bias on sequences of different lengths that lie one after the other: m [T, c_m] -> [T, c_m].
+
+        offsets    int32 or int64 [sequences + 1], as packed_attention takes them; each sequence attends within itself
+        positions  [T], for rotary positions: each row's number within its sequence if not given
+        causal     a row sees those up to itself only
+
+        Rows behind the last sequence attend to nothing: theirs is the output projection's bias.  GPU only."""
+        if m.dim() != 2:
+            raise ValueError(f"packed rows must be [T, c_m], got {tuple(m.shape)}")
+        if self._modules.get("relative") is not None:
+            raise ValueError("a relative position bias is for rows of one length, not for packed ones")
+        if self._modules.get("rotary") is not None and positions is None:
+            positions = packed_positions(offsets, m.shape[0])
+        self._check(positions, None, weights)
+        if not m.is_cuda:
+            raise RuntimeError("packed rows run on the GPU only (no CPU implementation)")
+        x = _layer_norm(self.layer_norm_m, m)
+        if self._slots_ok(m):
+            q, k, v, *g = self._slots(x, positions, weights).unbind(1)
+        else:
+            q, k, v, *g = self._heads(x, positions, False, weights)
+        o = packed_attention(q, k, v, offsets, causal=causal)
+        if self.linear_g is not None:
+            o = torch.sigmoid(g[0]) * o
+        return self._output(o.reshape(m.shape[0], self.no_heads * self.c_hidden), weights)
 
     def forward_eager(self, m: torch.Tensor, z: Optional[torch.Tensor] = None, mask: Optional[torch.Tensor] = None,
                       positions: Optional[torch.Tensor] = None, chains: Optional[torch.Tensor] = None):
