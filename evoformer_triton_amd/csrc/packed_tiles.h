@@ -254,23 +254,25 @@ struct Plan {
         return groups == 2 ? f(two, std::false_type()) : f(one, std::false_type());
     }
 };
-// units: tiles and heads; steps: of an average sequence's walk, 64 rows each.  Parts: as many as make some `fill` workgroups, of `few` steps at least where a CU is left to itself (up to 64 units),
-// of `more` up to 256 and of 32 beyond; for `most` units and fewer.  Two groups while the workgroups of eight waves all fit at once, two or (D = 32) three of them to a CU:
-// 2048 causal rows of 24 heads and D = 128 43 us (53 with one group), of 40 heads 73 (59).
-static Plan plan_for(int64_t units, int64_t steps, int64_t fill, int64_t most, int64_t few, int64_t more) {
-    Plan r = {steps >= 12 && units <= (EVO_D == 32 ? 768 : 512) ? 2 : 1, 1};
+// units: tiles and heads; steps: of an average sequence's walk, 64 rows each.  Two groups while the workgroups of eight waves all fit at once, two or (D = 32) three of them to a CU: 2048 causal rows
+// of 24 heads and D = 128 43 us (53 with one group), of 40 heads 73 (59).  Parts: for `most` units and fewer, as many as make workgroups that all fit at once, two (the keys' side) at least, each of
+// `few` steps where a CU is left to itself (up to 64 units), of `more` up to 256 and of 32 beyond: dK and dV of 12 heads (4 for keys) of D = 80, five sequences of up to 1777 rows, 55 us with 3 parts
+// and 59 with 5.
+constexpr int kAtOnce = EVO_D == 32 ? 768 : 512;
+static Plan plan_for(int64_t units, int64_t steps, int64_t least, int64_t most, int64_t few, int64_t more) {
+    Plan r = {steps >= 12 && units <= kAtOnce ? 2 : 1, 1};
     if (units && units <= most) {
-        const int64_t room = fill / units, worth = steps / (units <= 64 ? few : units <= 256 ? more : 32), n = room < worth ? room : worth;
+        const int64_t room = kAtOnce / units < least ? least : kAtOnce / units, worth = steps / (units <= 64 ? few : units <= 256 ? more : 32), n = room < worth ? room : worth;
         r.parts = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
     }
     return r;
 }
 static Plan query_plan(const EvoPacked &p) {
-    return plan_for((p.Tq / kPackedRows + (p.n + 1) / 2) * p.H, p.Tk / (p.n ? p.n : 1) / 64, 512, 256, 8, 32);
+    return plan_for((p.Tq / kPackedRows + (p.n + 1) / 2) * p.H, p.Tk / (p.n ? p.n : 1) / 64, 1, 256, 8, 32);
 }
 // (a key's walk is over the queries of all heads that share it)
 static Plan key_plan(const EvoPacked &p) {
-    return plan_for((p.Tk / kPackedRows + (p.n + 1) / 2) * p.Hk, p.Tq / (p.n ? p.n : 1) * (p.H / p.Hk) / 64, 768, 400, 4, 8);
+    return plan_for((p.Tk / kPackedRows + (p.n + 1) / 2) * p.Hk, p.Tq / (p.n ? p.n : 1) * (p.H / p.Hk) / 64, 2, 400, 4, 8);
 }
 
 template <typename F>
