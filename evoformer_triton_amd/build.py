@@ -41,7 +41,7 @@ def _units():
              ("prep", "prep.hip", []), ("layernorm", "layernorm.hip", []), ("pair_bias", "pair_bias.hip", VGPR_FORM[:2]),
              ("linear", "linear.hip", VGPR_FORM[:2]), ("relative_bias", "relative_bias.hip", VGPR_FORM[:2]), ("fp8", "fp8.hip", VGPR_FORM[:2]),
              ("rotary", "rotary.hip", []), ("packed", "packed.hip", []),
-             *((f"{name}_d{d}", f"{name}.hip", [f"-DEVO_D={d}", *VGPR_FORM[:2]]) for name in ("packed_mfma", "packed_dkdv", "packed_few") for d in (32, 64, 96, 128)),
+             *((f"{name}_d{d}", f"{name}.hip", [f"-DEVO_D={d}", *VGPR_FORM[:2]]) for name in ("packed_mfma", "packed_dkdv", "packed_few", "packed_f32") for d in (32, 64, 96, 128)),
              ("f32", "f32.hip", VGPR_FORM[:2]), ("mfma_bwd_fused", "mfma_bwd_fused.hip", VGPR_FORM),
              ("mfma_bwd_fused8", "mfma_bwd_fused8.hip", VGPR_FORM), ("mfma_stream8", "mfma_stream8.hip", VGPR_FORM), ("mfma_dbias", "mfma_dbias.hip", VGPR_FORM)]
     for d in HEAD_DIMS:

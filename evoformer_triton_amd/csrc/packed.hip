@@ -1,35 +1,7 @@
-// Attention within packed sequences: its entry points, and fp32's kernels, of one row per wave.
-//
-// Forward: a wave keeps a query row and walks over the keys that it sees, 64 at a time, a key to a lane: scores, the running maximum m and sum l of 2^(score - m), then
-// o += p_j v_j with the row's values in the lanes.  Backward with p_ij = 2^(score - lse_i) formed again, delta_i = sum do_i o_i: ds_ij = p_ij (do_i v_j - delta_i) scale,
-// dq_i = sum_j ds_ij k_j by a wave per query, dk_j = sum_i ds_ij q_i and dv_j = sum_i p_ij do_i by a wave per key, over the heads that share it in their order.
+// Attention within packed sequences: its entry points.
 #include "packed_common.h"
 
 namespace evo {
-
-template <typename T>
-__global__ void __launch_bounds__(256) packed_rows_fwd(EvoPacked p, unsigned rows) {
-    const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (row >= rows) return;
-    const int i = row / (unsigned)p.H, h = row % (unsigned)p.H;
-    row_forward<T>(p, segment_of_row<false>(p, i), i, h);
-}
-template <typename T>
-__global__ void __launch_bounds__(256) packed_rows_dq(EvoPacked p, float *delta, unsigned rows) {
-    const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (row >= rows) return;
-    const int i = row / (unsigned)p.H, h = row % (unsigned)p.H;
-    const float d = row_delta<T>(p, i, h);
-    if ((threadIdx.x & 63) == 0) delta[(int64_t)h * p.Tq + i] = -d;
-    row_dq<T>(p, segment_of_row<false>(p, i), i, h, d);
-}
-template <typename T>
-__global__ void __launch_bounds__(256) packed_rows_dkdv(EvoPacked p, const float *delta, unsigned rows) {
-    const unsigned row = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (row >= rows) return;
-    const int j = row / (unsigned)p.Hk, hk = row % (unsigned)p.Hk;
-    row_dkdv<T>(p, segment_of_row<true>(p, j), j, hk, delta);
-}
 
 #define EVO_PACKED(D)                                                              \
     int launch_packed_fwd_d##D(const EvoPacked &, hipStream_t);                    \
@@ -39,7 +11,13 @@ __global__ void __launch_bounds__(256) packed_rows_dkdv(EvoPacked p, const float
     size_t packed_dkdv_bytes_d##D(const EvoPacked &);                              \
     size_t packed_fwd_bytes_d##D(const EvoPacked &);                               \
     size_t packed_few_bytes_d##D(const EvoPacked &);                               \
-    int launch_packed_few_d##D(const EvoPacked &, hipStream_t);
+    int launch_packed_few_d##D(const EvoPacked &, hipStream_t);                    \
+    size_t packed_f32_few_bytes_d##D(const EvoPacked &);                           \
+    int launch_packed_f32_few_d##D(const EvoPacked &, hipStream_t);                \
+    size_t packed_f32_fwd_bytes_d##D(const EvoPacked &);                           \
+    int launch_packed_f32_fwd_d##D(const EvoPacked &, hipStream_t);                \
+    size_t packed_f32_bwd_bytes_d##D(const EvoPacked &);                           \
+    int launch_packed_f32_bwd_d##D(const EvoPacked &, const BackwardRows &, float *, hipStream_t);
 EVO_PACKED(32)
 EVO_PACKED(64)
 EVO_PACKED(96)
@@ -50,7 +28,7 @@ EVO_PACKED(128)
     ((p).D <= 32 ? name##_d32(__VA_ARGS__) : (p).D <= 64 ? name##_d64(__VA_ARGS__) : (p).D <= 96 ? name##_d96(__VA_ARGS__) : name##_d128(__VA_ARGS__))
 
 // Whether the kernel that splits the keys serves the forward: where a key head has few queries of few heads in a sequence.
-static bool few_queries(const EvoPacked &p) { return p.dtype != EVO_F32 && p.Tq * (p.H / p.Hk) <= (int64_t)64 * p.n; }
+static bool few_queries(const EvoPacked &p) { return p.Tq * (p.H / p.Hk) <= (int64_t)64 * p.n; }
 
 static int64_t align_rows(int64_t n) { return (n + 63) / 64 * 64; }   // (16-byte pieces behind them)
 
@@ -92,7 +70,8 @@ extern "C" {
 
 size_t evoattn_packed_fwd_workspace_bytes(const EvoPacked *p) {
     using namespace evo;
-    if (packed_check(p) || p->dtype == EVO_F32) return 0;
+    if (packed_check(p)) return 0;
+    if (p->dtype == EVO_F32) return few_queries(*p) ? EVO_BY_HEAD_DIM(packed_f32_few_bytes, *p, *p) : EVO_BY_HEAD_DIM(packed_f32_fwd_bytes, *p, *p);
     return few_queries(*p) ? EVO_BY_HEAD_DIM(packed_few_bytes, *p, *p) : EVO_BY_HEAD_DIM(packed_fwd_bytes, *p, *p);
 }
 
@@ -102,19 +81,15 @@ int evoattn_packed_fwd(const EvoPacked *p, void *hip_stream) {
     if (!p->Tq) return EVO_OK;
     if (const int rc = packed_pointers(*p, false)) return rc;
     const hipStream_t st = (hipStream_t)hip_stream;
-    if (few_queries(*p)) return EVO_BY_HEAD_DIM(launch_packed_few, *p, *p, st);
-    if (p->dtype != EVO_F32) return EVO_BY_HEAD_DIM(launch_packed_fwd, *p, *p, st);
-    const int64_t rows = p->Tq * p->H;
-    if (rows > INT32_MAX || !grid_fits((rows + 3) / 4, 256)) return EVO_EOVERFLOW;
-    packed_rows_fwd<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, (unsigned)rows);
-    return hip_rc();
+    if (few_queries(*p)) return p->dtype == EVO_F32 ? EVO_BY_HEAD_DIM(launch_packed_f32_few, *p, *p, st) : EVO_BY_HEAD_DIM(launch_packed_few, *p, *p, st);
+    return p->dtype == EVO_F32 ? EVO_BY_HEAD_DIM(launch_packed_f32_fwd, *p, *p, st) : EVO_BY_HEAD_DIM(launch_packed_fwd, *p, *p, st);
 }
 
 size_t evoattn_packed_bwd_workspace_bytes(const EvoPacked *p) {
     using namespace evo;
     if (packed_check(p)) return 0;
     const size_t rows = (size_t)align_rows((int64_t)p->H * p->Tq) * sizeof(float);
-    if (p->dtype == EVO_F32) return rows;
+    if (p->dtype == EVO_F32) return rows + EVO_BY_HEAD_DIM(packed_f32_bwd_bytes, *p, *p);
     const size_t dq = EVO_BY_HEAD_DIM(packed_dq_bytes, *p, *p), dkdv = EVO_BY_HEAD_DIM(packed_dkdv_bytes, *p, *p);
     return 2 * rows + (dq > dkdv ? dq : dkdv);
 }
@@ -126,21 +101,12 @@ int evoattn_packed_bwd(const EvoPacked *p, void *hip_stream) {
     if (const int rc = packed_pointers(*p, true)) return rc;
     const hipStream_t st = (hipStream_t)hip_stream;
     const BackwardRows saved = {(float *)p->workspace, (float *)p->workspace + align_rows((int64_t)p->H * p->Tq)};
-    if (p->dtype != EVO_F32) {
-        float *const sums = saved.base + align_rows((int64_t)p->H * p->Tq);   // (dQ's parts, then dK's and dV's)
-        if (p->Tq) {
-            if (const int rc = EVO_BY_HEAD_DIM(launch_packed_dq, *p, *p, saved, sums, st)) return rc;
-        }
-        return p->Tk && p->dk ? EVO_BY_HEAD_DIM(launch_packed_dkdv, *p, *p, saved, sums, st) : EVO_OK;
+    if (p->dtype == EVO_F32) return EVO_BY_HEAD_DIM(launch_packed_f32_bwd, *p, *p, saved, saved.base, st);   // (`base` is 16 bits': sums begin there)
+    float *const sums = saved.base + align_rows((int64_t)p->H * p->Tq);   // (dQ's parts, then dK's and dV's)
+    if (p->Tq) {
+        if (const int rc = EVO_BY_HEAD_DIM(launch_packed_dq, *p, *p, saved, sums, st)) return rc;
     }
-    const int64_t rows = p->Tq * p->H, keys = p->Tk * p->Hk;
-    if (rows > INT32_MAX || keys > INT32_MAX || !grid_fits((rows + 3) / 4, 256) || !grid_fits((keys + 3) / 4, 256)) return EVO_EOVERFLOW;
-    if (rows) {
-        packed_rows_dq<float><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(*p, saved.delta, (unsigned)rows);
-        if (const int rc = hip_rc()) return rc;
-    }
-    if (keys && p->dk) packed_rows_dkdv<float><<<(unsigned)((keys + 3) / 4), 256, 0, st>>>(*p, saved.delta, (unsigned)keys);
-    return hip_rc();
+    return p->Tk && p->dk ? EVO_BY_HEAD_DIM(launch_packed_dkdv, *p, *p, saved, sums, st) : EVO_OK;
 }
 
 }  // extern "C"

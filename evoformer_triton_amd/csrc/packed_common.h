@@ -136,8 +136,8 @@ __device__ __forceinline__ void save_row(const BackwardRows &to, int64_t at, flo
     to.base[at] = -(any ? lse + __log2f(sum) : lse) / c;
 }
 
-// ---- One row by one wave, products and sums in fp32: the kernels for fp32, and what the matrix kernels leave for rows whose result is no
-// number: there a masked key or query may hold an infinity or a NaN, which a product with a probability of zero does not keep out.
+// ---- One row by one wave, products and sums in fp32: what the matrix kernels leave for rows whose result is no number.  A masked key or query may hold an infinity or a NaN there, which a product
+// with a probability of zero does not keep out; here a wave takes the rows alone that are seen, 64 at a time, a row of the other side to a lane.
 
 template <typename T>
 __device__ __forceinline__ void row_forward(const EvoPacked &p, const Segment &s, int i, int h) {
@@ -163,12 +163,6 @@ __device__ __forceinline__ void row_forward(const EvoPacked &p, const Segment &s
     store_row((T *)p.o + ((int64_t)i * p.H + h) * p.D, o, p.D);
     if (p.o_low) store_row((T *)p.o_low + ((int64_t)i * p.H + h) * p.D, Row{o.a - (float)(T)o.a, o.b - (float)(T)o.b}, p.D);
     if (p.lse && lane == 0) p.lse[(int64_t)h * p.Tq + i] = seen ? m + __log2f(l) : INFINITY;
-}
-
-template <typename T>
-__device__ __forceinline__ float row_delta(const EvoPacked &p, int i, int h) {
-    const Row d = load_row(head_row<T>(p.dout, i, p.dout_stride_t, h, p.dout_stride_h), p.D), o = load_row((const T *)p.o + ((int64_t)i * p.H + h) * p.D, p.D);
-    return wave_sum(fmaf(d.a, o.a, d.b * o.b));
 }
 
 template <typename T>

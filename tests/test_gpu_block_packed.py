@@ -200,3 +200,40 @@ def test_a_prompt_and_its_tokens_one_by_one(gpu_device, dt):
         kc[rows], vc[rows] = kt, v[rows]
         koff = torch.tensor([x for b, n in zip(ends, lengths) for x in (b, b + n + t + 1)] + [ends[-1]], device=gpu_device)
         _close([packed_attention(qt, kc, vc, off, koff)], [want[0][rows]], [bound[0][rows]], [f"token {t}"])
+
+
+def test_checkpointed_in_inference_mode_and_without_gradients(gpu_device):
+    from torch.utils.checkpoint import checkpoint
+    block = _block(gpu_device, BF16, rotary={})
+    m, dout, off = _packed_case(gpu_device, BF16)
+    m.requires_grad_()
+    rows, at = m.detach().view(1, 1, *m.shape).requires_grad_(), torch.arange(m.shape[0], device=gpu_device)
+    for call, x, d in ((lambda x: block.packed(x, off), m, dout), (lambda x: block(x, None, None, at), rows, dout.view(rows.shape))):
+        leaves = [x, *block.parameters()]
+        y = call(x)
+        want = torch.autograd.grad(y, leaves, d)
+        for again in (checkpoint(call, x, use_reentrant=False), checkpoint(call, x, use_reentrant=True)):
+            assert torch.equal(again, y)
+        y2 = checkpoint(call, x, use_reentrant=False)
+        for a, w in zip(torch.autograd.grad(y2, leaves, d), want):
+            assert torch.equal(a, w)
+        with torch.inference_mode():
+            assert torch.equal(call(x), y)
+        with torch.no_grad():
+            assert torch.equal(call(x.detach()), y)
+
+
+def test_two_streams_at_once(gpu_device):
+    block = _block(gpu_device, F16, rotary={})
+    m, _, off = _packed_case(gpu_device, F16)
+    with torch.no_grad():
+        want = [block.packed(m, off), block.packed(m * 2, off, causal=True)]
+        streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+        twice = m * 2
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for i, s in enumerate(streams):
+                with torch.cuda.stream(s):
+                    got[i] = block.packed(twice if i else m, off, causal=bool(i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

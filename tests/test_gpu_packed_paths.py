@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from oracle.packed import packed
-from test_gpu_packed import BF16, F16, _check, _close, _inputs, _offsets
+from test_gpu_packed import BF16, F16, F32, _check, _close, _inputs, _offsets
 
 pytestmark = pytest.mark.gpu
 
@@ -24,6 +24,14 @@ LONG = [
     # one
     (F16, [300] * 9, None, 12, 4, 128, True),
     (BF16, [520, 3, 700] * 4, None, 12, 12, 64, False),
+    # fp32: in parts, in many of them for one token, without parts, vectors that are not 16 bytes long
+    (F32, [2200], None, 2, 1, 128, True),
+    (F32, [300, 0, 700, 1], None, 4, 2, 64, False),
+    (F32, [1], [20000], 2, 1, 96, True),
+    (F32, [130], [4100], 2, 2, 40, True),
+    (F32, [2000], [90], 2, 1, 32, False),
+    (F32, [700] * 12, None, 16, 8, 32, True),
+    (F32, [1000, 33], None, 3, 3, 77, True),
 ]
 
 
@@ -34,7 +42,8 @@ def test_long_walks(gpu_device, case):
     _check(*_inputs(dtype, queries, keys, H, Hk, D, padding=3), queries, keys, causal)
 
 
-@pytest.mark.parametrize("dtype,D,H,Hk,lengths", [(BF16, 64, 2, 1, [2200, 40]), (F16, 128, 2, 2, [1500, 40]), (BF16, 96, 12, 12, [1200, 1300]), (F16, 32, 2, 1, [2000, 9])])
+@pytest.mark.parametrize("dtype,D,H,Hk,lengths", [(BF16, 64, 2, 1, [2200, 40]), (F16, 128, 2, 2, [1500, 40]), (BF16, 96, 12, 12, [1200, 1300]), (F16, 32, 2, 1, [2000, 9]),
+                                                   (F32, 64, 2, 1, [1500, 40]), (F32, 33, 12, 12, [1200, 1300])])
 def test_long_walks_past_infinities_and_nan(gpu_device, dtype, D, H, Hk, lengths):
     """In rows of no sequence and in the second sequence: the same bits.  In the first one's last key: the queries that do not see it stay within their bounds."""
     from evoformer_triton_amd import packed_attention
@@ -67,7 +76,8 @@ def test_long_walks_past_infinities_and_nan(gpu_device, dtype, D, H, Hk, lengths
 FEW = [(dtype, [q] * n, [1 + (i * 37) % most for i in range(n)], H, Hk, D)
        for dtype, q, n, most, H, Hk, D in [
            (BF16, 1, 2, 9000, 4, 2, 64), (F16, 1, 2, 9000, 32, 1, 128), (BF16, 3, 3, 5000, 8, 1, 96), (F16, 1, 1, 20000, 8, 8, 32), (BF16, 5, 2, 700, 8, 2, 80),
-           (F16, 1, 70, 300, 8, 2, 64), (BF16, 1, 70, 3000, 8, 2, 128), (F16, 2, 70, 2000, 32, 2, 96), (BF16, 1, 200, 1000, 24, 1, 32), (F16, 1, 64, 5000, 2, 2, 40)]]
+           (F16, 1, 70, 300, 8, 2, 64), (BF16, 1, 70, 3000, 8, 2, 128), (F16, 2, 70, 2000, 32, 2, 96), (BF16, 1, 200, 1000, 24, 1, 32), (F16, 1, 64, 5000, 2, 2, 40),
+           (F32, 1, 2, 9000, 4, 2, 64), (F32, 3, 3, 5000, 16, 1, 96), (F32, 1, 70, 300, 40, 2, 13), (F32, 1, 300, 100, 8, 8, 128), (F32, 2, 1, 33, 2, 2, 30)]]
 
 
 @pytest.mark.parametrize("case", FEW, ids=lambda c: f"{c[0]}-{c[1][0]}x{len(c[1])}-{c[3:]}".replace("torch.", "").replace(" ", ""))
@@ -142,3 +152,18 @@ def test_rows_beyond_32_bits_and_their_gradients(gpu_device):
         want, bound = packed(*(t.detach()[-last:] for t in (q, k, v)), [0, last], [0, last], True, D ** -0.5, dout[-last:])
         _close([t[-last:] for t in got], want, bound, ("o", "dq", "dk", "dv"))
         assert not any(t[:-last].any() for t in got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_side_is_empty(gpu_device, dtype):
+    """No queries, no keys, and neither: zeros of the right shapes."""
+    from evoformer_triton_amd import packed_attention
+    for Tq, Tk in ((0, 70), (200, 0), (3, 0), (0, 0)):
+        for n in (0, 1, 70):
+            q, k, v, dout = _inputs(dtype, [Tq], [Tk], 4, 2, 40)
+            dout = dout[:Tq]
+            off, koff = (torch.tensor([0] + [t] * n, device="cuda:0") for t in (Tq, Tk))
+            leaves = [t[:m].requires_grad_() for t, m in ((q, Tq), (k, Tk), (v, Tk))]
+            out = packed_attention(*leaves, off, koff)
+            got = [out, *torch.autograd.grad(out, leaves, dout)]
+            assert [g.shape for g in got] == [t.shape for t in (leaves[0], *leaves)] and not any(g.any() for g in got)
