@@ -1,4 +1,9 @@
 // Attention within packed sequences on the matrix cores: dK and dV (see packed_mfma.hip).
+//
+// A wave has 32 keys, a column of the products' each, and walks over the queries of all heads that share the key head: S = Q K^T and dP = dO V^T begin with what is subtracted from them (-lse in units of
+// q . k, -delta; staged in LDS beside the rows), P and dS as they lie are operands of dV^T = dO^T P and dK^T = Q^T dS.  Four products for each pair of rows, their other operands from LDS: for head dims
+// above 64 V's too, since with K's, dK and dV in registers (2 waves to a SIMD) there is no room for them.  4 x 4096 causal rows, 32 heads (8) of 128: 1.33 ms, 0.83 Pflop/s; what is left of the rate of
+// a large product goes into LDS's reads, of which each product needs two, and into exponentials.
 #include "packed_tiles.h"
 
 namespace evo {

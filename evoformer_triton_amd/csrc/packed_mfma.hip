@@ -3,8 +3,18 @@
 // A workgroup of four waves takes 128 rows of a sequence and head (forward, dQ: queries; dK/dV: keys), a wave 32 of them, and the other side's rows stream through LDS, a
 // stage ahead of the one that is computed on, brought there by the load path itself.  Scores are formed transposed, S^T = K Q^T: a lane then holds 16 keys of one query, the softmax
 // needs one exchange with the lane's other half, and the tile is as it lies the operand of O^T = V^T P^T (common.h), whose other operand, V^T, is read from row-major V by
-// transposing reads.  The running maximum moves only when it grows by more than 2^8, so that the sums are rarely multiplied again; probabilities are rounded to the inputs' type to
+// transposing reads.  Probabilities are formed relative to the maximum so far, which is looked for again only when a lane's sum of 32 of them passes 2^13; they are rounded to the inputs' type to
 // multiply V and summed as rounded.
+//
+// dQ: P again from the forward's lse, dP^T = V dO^T, dS = P (dP - delta), delta = sum of dO times the output and what rounding left of it (the forward keeps both: the output alone is off by half a
+// step, and with it every dS of its row by P times that).  dS multiplies K as two values of the inputs' type, what rounding leaves of it as the second: rounded once its share of the error is as large
+// as that of rounding the result.  P's and dS's sums over a row, which should be 1 and 0, put right what the rounded probabilities of the forward left in lse and delta: by them dQ is divided, and dK's
+// kernel gets both mended.  Errors of dQ and dK next to the formula's in 64 bits, of their norms (chains of 51 to 768 rows, 8 heads of 32, bf16): 0.0019 and 0.0023, where rounding the exact result gives
+// 0.0017; without any of this 0.0035 and 0.0033.
+//
+// What bounds them: the matrix instructions and, at the same time on the same SIMD, exponentials (a quarter of the rate of other instructions) and additions.  Forward, one causal prompt of 16384 rows,
+// 32 heads (8 for keys) of 128: 1.98 ms, 1.1 Pflop/s of the 1.2 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.64 ms, dQ 1.03 (its product of K twice), dK and dV 1.33.
+// Inputs of zeros take a quarter less time than random ones: the power that the products take has its part in it.
 //
 // Which rows: tile t of the launch belongs to the last segment j (packed_common.h) with begin(j) / 128 + j <= t; begin(j + 1) / 128 + j + 1 leaves room for all of j's tiles, so that every workgroup finds
 // its place by itself, without a sum over the sequences before it and whatever the lengths are; at most one tile per segment finds nothing to do.

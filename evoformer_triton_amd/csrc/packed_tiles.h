@@ -28,7 +28,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void *base, int 
     return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, rows > 0 ? (rows - 1) * stride + D * 2 : 0, 0x00020000);
 }
 
-// This lane's offset of its first piece of a stage of rows; its further pieces are kPieceRows rows on each.
+// This lane's offset of its first piece of a stage of rows; its further pieces are STEP rows on each.
 template <int NW>
 struct StagePieces {
     typedef PackedGeo::G G;
@@ -94,13 +94,13 @@ struct Place {
     Segment s;
     int first;   // its first row (of the tensor), or, where there is nothing to do, s's end or beyond
 };
-template <bool KEYS, int ROWS = kPackedRows>
+template <bool KEYS>
 __device__ __forceinline__ Place place_of(const EvoPacked &p, int t) {
     Place r;
     int j;
-    r.s = find_segment<KEYS>(p, [&](int begin, int x) { return begin / ROWS + x <= t; }, j);
-    const int b = KEYS ? r.s.k0 : r.s.q0, i = t - (b / ROWS + j);
-    r.first = i < 0 ? INT32_MAX : (int)min((int64_t)INT32_MAX, b + (int64_t)i * ROWS);   // (below zero: offsets that do not ascend)
+    r.s = find_segment<KEYS>(p, [&](int begin, int x) { return begin / kPackedRows + x <= t; }, j);
+    const int b = KEYS ? r.s.k0 : r.s.q0, i = t - (b / kPackedRows + j);
+    r.first = i < 0 ? INT32_MAX : (int)min((int64_t)INT32_MAX, b + (int64_t)i * kPackedRows);   // (below zero: offsets that do not ascend)
     return r;
 }
 
@@ -128,8 +128,8 @@ __device__ __forceinline__ f32x16 filled(float v) {
 }
 
 // Which tile and heads a workgroup takes.  Workgroups go round the eight XCDs, each with an L2 of its own; a unit, a tile and a key head, goes to one of them with all of its query heads, and units follow
-// each other by tiles first: with a multiple of eight key heads an XCD keeps to its own, with fewer the tiles of one are dealt out one by one, so that all XCDs have long and short ones.  (In runs of units, a half of a key head's tiles
-// to an XCD: seven prompts of 90 to 2011, 16 / 4 heads of 64, 39.7 us.)
+// each other by tiles first: with a multiple of eight key heads an XCD keeps to its own, with fewer the tiles of one are dealt out one by one, so that all XCDs have long and short ones.  (Seven prompts of 90 to 2011, 16 / 4 heads of 64:
+// 36.6 us; in runs of units, a half of a key head's tiles to an XCD, 39.7.)
 struct Unit {
     int tile, hk, member;   // member: of the unit's workgroups
     bool none;              // past the last unit
@@ -181,7 +181,7 @@ __device__ __forceinline__ void zero_parts(float *x, int first, int rows, int he
     for (int i = threadIdx.x; i < n; i += blockDim.x) *reinterpret_cast<f32x4 *>(x + ((int64_t)(first + i / per) * heads + h) * D + i % per * 4) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 
-static int64_t packed_tiles(int64_t rows, int n, int tile = kPackedRows) { return rows / tile + n + 2; }
+static int64_t packed_tiles(int64_t rows, int n) { return rows / kPackedRows + n + 2; }
 
 // The sums of a row's parts, by a wave for each row: dQ, or (KEYS) dK and dV, whose parts follow those of dK.
 template <typename T, bool KEYS>

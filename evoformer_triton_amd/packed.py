@@ -2,7 +2,7 @@
 
 The reference's rows all have N residues (evoformer.py:640-651); chains of different lengths are padded to the longest there.  Here they are packed: rows
 [T, H, D] and the row at which each sequence begins.  Causal or not, query heads in groups that share a key and value head, as many queries as keys
-(training, a prompt) or the last few of them (tokens that are added to a sequence).  Kernels: csrc/packed.hip.
+(training, a prompt) or the last few of them (tokens that are added to a sequence).  Kernels: csrc/packed_mfma.hip, packed_dkdv.hip, packed_few.hip, packed_f32.hip.
 """
 from __future__ import annotations
 
@@ -26,9 +26,13 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     scale        positive (2^-64 to 2^64); D^-0.5 if not given
 
     Rows of no sequence (behind the last) and rows without a key get zeros, as do their gradients; what lies in rows that a query does not see, infinities and NaN among
-    it, does not reach its result.  Probabilities multiply the values, and the scores' gradients queries and keys, rounded to the inputs' type; sums are in fp32.  Gradients: q, k and v, the same bits
-    with every call.  The offsets' values are not looked at on the host (no synchronisation): where they are not ascending, results are not specified.  Runs on the current stream of the tensors'
-    device; GPU only."""
+    it, does not reach its result.  Sums are in fp32.  In 16 bits probabilities are rounded to the inputs' type to multiply values, and scores' gradients to multiply queries (to multiply keys:
+    as two values); for the backward the call keeps, beside its inputs, the output, what rounding left of it, and a number for each row and head.  Gradients: q, k and v, the same bits with every call.
+
+    Room that a cache leaves between its sequences is a sequence without queries: offsets [0, 1, 1, 2, 2], key_offsets [0, n0, room, room + n1, 2 room].  Calls whose sequences have few queries each
+    (by the average of queries times H / Hk) and others are served by different kernels: prompts and single tokens are best in calls of their own.
+
+    The offsets' values are not looked at on the host (no synchronisation): where they are not ascending, results are not specified.  Runs on the current stream of the tensors' device; GPU only."""
     for name, t in (("q", q), ("k", k), ("v", v), ("offsets", offsets), ("key_offsets", key_offsets)):
         if not isinstance(t, torch.Tensor) and not (t is None and name == "key_offsets"):
             raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
