@@ -56,6 +56,16 @@ __device__ __forceinline__ Segment segment(const EvoPacked &p, int j) {
     s.k1 = __builtin_amdgcn_readfirstlane(s.k1);
     return s;
 }
+// Segment j where lane x holds the first query q and the first key k of segment x (up to n + 2).
+__device__ __forceinline__ Segment segment_of_lanes(const EvoPacked &p, int q, int k, int j) {
+    Segment s;
+    s.gap = j == 0 || j == p.n + 1;
+    s.q0 = __builtin_amdgcn_readlane(q, j);
+    s.q1 = __builtin_amdgcn_readfirstlane(max(s.q0, (int)__builtin_amdgcn_readlane(q, j + 1)));
+    s.k0 = __builtin_amdgcn_readlane(k, j);
+    s.k1 = __builtin_amdgcn_readfirstlane(max(s.k0, (int)__builtin_amdgcn_readlane(k, j + 1)));
+    return s;
+}
 // The last segment j for which before(begin(j), j) holds, begin(j) being its first query (KEYS: key) and `before` as last_where takes it.  Where a wave has a lane for every segment's begin, those of queries and of
 // keys are loaded at once and the segment's own are taken from the lanes: one trip to memory, not two or three.
 template <bool KEYS, typename F>
@@ -66,13 +76,7 @@ __device__ __forceinline__ Segment find_segment(const EvoPacked &p, F before, in
     }
     const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x);
     j = __builtin_amdgcn_readfirstlane(max(1, (int)__popcll(__ballot(lane < p.n + 2 && before(KEYS ? k : q, lane)))) - 1);
-    Segment s;
-    s.gap = j == 0 || j == p.n + 1;
-    s.q0 = __builtin_amdgcn_readlane(q, j);
-    s.q1 = __builtin_amdgcn_readfirstlane(max(s.q0, (int)__builtin_amdgcn_readlane(q, j + 1)));
-    s.k0 = __builtin_amdgcn_readlane(k, j);
-    s.k1 = __builtin_amdgcn_readfirstlane(max(s.k0, (int)__builtin_amdgcn_readlane(k, j + 1)));
-    return s;
+    return segment_of_lanes(p, q, k, j);
 }
 // The segment that a row of the queries (or, KEYS, of the keys) lies in.
 template <bool KEYS>

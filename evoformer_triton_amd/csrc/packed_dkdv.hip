@@ -2,7 +2,7 @@
 //
 // A wave has 32 keys, a column of the products' each, and walks over the queries of all heads that share the key head: S = Q K^T and dP = dO V^T begin with what is subtracted from them (-lse in units of
 // q . k, -delta; staged in LDS beside the rows), P and dS as they lie are operands of dV^T = dO^T P and dK^T = Q^T dS.  Four products for each pair of rows, their other operands from LDS: for head dims
-// above 64 V's too, since with K's, dK and dV in registers (2 waves to a SIMD) there is no room for them.  4 x 4096 causal rows, 32 heads (8) of 128: 1.33 ms, 0.83 Pflop/s; what is left of the rate of
+// above 64 V's too, since with K's, dK and dV in registers (2 waves to a SIMD) there is no room for them.  4 x 4096 causal rows, 32 heads (8) of 128: 1.19 ms, 0.93 Pflop/s; what is left of the rate of
 // a large product goes into LDS's reads, of which each product needs two, and into exponentials.
 #include "packed_tiles.h"
 
@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
     const Unit unit(blockIdx.x, tiles, p.Hk, PART ? parts.chunks : 1);
     if (unit.none) return;
     const int hk = unit.hk;
-    const Place at = place_of<true>(p, unit.tile);   // (a sequence's first keys, which causal queries see most of, first)
+    const Place at = place_of<true>(p, unit.tile, tiles);
     const Segment &s = at.s;
     if (at.first >= s.k1) return;
     const int D = p.D, rows = min(kPackedRows, s.k1 - at.first);

@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(256, 2) packed_f32_fwd(EvoPacked p, Parts part
     const Unit unit(blockIdx.x, tiles, p.Hk, heads * (PART ? parts.chunks : 1));
     if (unit.none) return;
     const int hk = unit.hk, h = hk * heads + unit.member % heads, part = PART ? unit.member / heads : 0;
-    const Place at = place_of<false>(p, tiles - 1 - unit.tile);
+    const Place at = place_of<false>(p, unit.tile, tiles);
     const Segment &s = at.s;
     if (at.first >= s.q1) return;
     const int rows = min(kPackedRows, s.q1 - at.first);
@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(256, EVO_D <= 64 ? 2 : 1) packed_f32_dq(EvoPac
     const Unit unit(blockIdx.x, tiles, p.Hk, heads * (PART ? parts.chunks : 1));
     if (unit.none) return;
     const int hk = unit.hk, h = hk * heads + unit.member % heads, part = PART ? unit.member / heads : 0;
-    const Place at = place_of<false>(p, tiles - 1 - unit.tile);
+    const Place at = place_of<false>(p, unit.tile, tiles);
     const Segment &s = at.s;
     if (at.first >= s.q1) return;
     const int rows = min(kPackedRows, s.q1 - at.first);
@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(256, EVO_D <= 64 ? 2 : 1) packed_f32_dkdv(EvoP
     const Unit unit(blockIdx.x, tiles, p.Hk, PART ? parts.chunks : 1);
     if (unit.none) return;
     const int hk = unit.hk;
-    const Place at = place_of<true>(p, unit.tile);
+    const Place at = place_of<true>(p, unit.tile, tiles);
     const Segment &s = at.s;
     if (at.first >= s.k1) return;
     const int rows = min(kPackedRows, s.k1 - at.first);

@@ -13,11 +13,12 @@
 // 0.0017; without any of this 0.0035 and 0.0033.
 //
 // What bounds them: the matrix instructions and, at the same time on the same SIMD, exponentials (a quarter of the rate of other instructions) and additions.  Forward, one causal prompt of 16384 rows,
-// 32 heads (8 for keys) of 128: 1.98 ms, 1.1 Pflop/s of the 1.2 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.64 ms, dQ 1.03 (its product of K twice), dK and dV 1.33.
+// 32 heads (8 for keys) of 128: 1.98 ms, 1.1 Pflop/s of the 1.2 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.64 ms, dQ 1.06 (its product of K twice), dK and dV 1.19.
 // Inputs of zeros take a quarter less time than random ones: the power that the products take has its part in it.
 //
 // Which rows: tile t of the launch belongs to the last segment j (packed_common.h) with begin(j) / 128 + j <= t; begin(j + 1) / 128 + j + 1 leaves room for all of j's tiles, so that every workgroup finds
-// its place by itself, without a sum over the sequences before it and whatever the lengths are; at most one tile per segment finds nothing to do.
+// its place by itself, without a sum over the sequences before it and whatever the lengths are; at most one tile per segment finds nothing to do.  A sequence's last queries (first keys), which under a
+// causal mask have the longest walks, begin first; of few long sequences all of them by their walks (place_of).
 //
 // A row of V beyond the sequence's end is read as zeros (the load is out of range).  One that causal queries do not see may hold an infinity or a NaN, which a probability of
 // zero does not keep out of the sums: results that are no numbers are formed anew, row by row (row_forward and its like), with the rows that are seen alone.
@@ -47,7 +48,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
     const Unit unit(blockIdx.x, tiles, p.Hk, heads * (PART ? parts.chunks : 1));
     if (unit.none) return;
     const int hk = unit.hk, h = hk * heads + unit.member % heads, part = PART ? unit.member / heads : 0;
-    const Place at = place_of<false>(p, tiles - 1 - unit.tile);   // (a sequence's last queries, which under a causal mask see most, first)
+    const Place at = place_of<false>(p, unit.tile, tiles);
     const Segment &s = at.s;
     if (at.first >= s.q1) return;
     const int D = p.D, rows = min(kPackedRows, s.q1 - at.first);
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
     const Unit unit(blockIdx.x, tiles, p.Hk, heads * (PART ? parts.chunks : 1));
     if (unit.none) return;
     const int hk = unit.hk, h = hk * heads + unit.member % heads, part = PART ? unit.member / heads : 0;
-    const Place at = place_of<false>(p, tiles - 1 - unit.tile);
+    const Place at = place_of<false>(p, unit.tile, tiles);
     const Segment &s = at.s;
     if (at.first >= s.q1) return;
     const int D = p.D, rows = min(kPackedRows, s.q1 - at.first);

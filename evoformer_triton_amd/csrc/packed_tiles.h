@@ -89,15 +89,50 @@ __device__ __forceinline__ void load_operands(const T *row, int D, int g, typena
     for (int ks = 0; ks < PackedGeo::KSD; ++ks) x[ks] = ks * 16 + g * 8 < D ? ld8(row + ks * 16 + g * 8) : zero8<T>();
 }
 
-// Where a workgroup is: a tile of a segment, and a head.
+// Where a workgroup is: a tile of a segment.
 struct Place {
     Segment s;
     int first;   // its first row (of the tensor), or, where there is nothing to do, s's end or beyond
 };
+// The tile that is the `rank`th of `tiles` to begin.  KEYS: of keys, else of queries.
 template <bool KEYS>
-__device__ __forceinline__ Place place_of(const EvoPacked &p, int t) {
+__device__ __forceinline__ Place place_of(const EvoPacked &p, int rank, int tiles) {
     Place r;
     int j;
+    // Under a causal mask of few long sequences those with the longest walks begin first: a tile of queries i before a sequence's own first one sees i + 1 tiles of keys, one of keys is seen from
+    // as many tiles as are behind it and its own.  Of c_j tiles of sequence j max(0, c_j - w) have walks longer than w; the rank is that of walks of w where the sum of these reaches it.  4 x 4096 rows,
+    // 32 heads (8) of 128: dK and dV 1.19 ms (1.34 with one sequence after the other), forward 0.635 (0.66), dQ 1.08 (1.06: more sequences' keys at once in an L2).  Sequences of 7 tiles on average:
+    // forward 40.8 us (43.9); of 5: 38.1 (37.4), the search costs what it gains.
+    if (p.causal && p.n + 3 <= 64 && (KEYS ? p.Tk : p.Tq) >= (int64_t)6 * kPackedRows * p.n) {
+        const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x), b = KEYS ? k : q;
+        const int rows = max(0, __shfl_down(b, 1) - b), own = lane < p.n + 2 ? (rows + kPackedRows - 1) / kPackedRows : 0;
+        auto longer = [&](int w) {
+            int sum = 0;
+            for (int y = 0; y < p.n + 2; ++y) sum += max(0, __builtin_amdgcn_readlane(own, y) - w);
+            return sum;
+        };
+        int lo = -1, hi = tiles, at = 0;   // longer(hi) <= rank, and not of lo
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 63) / 64, w = min(hi, lo + (lane + 1) * step), n = longer(w);
+            const int f = __builtin_ctzll(__ballot(n <= rank));   // (the last lane's w is hi)
+            hi = __builtin_amdgcn_readlane(w, f);
+            at = __builtin_amdgcn_readlane(n, f);
+            lo = hi - step;
+        }
+        const uint64_t those = __ballot(own >= hi && own > 0);
+        const bool chosen = hi > 0 && (those >> lane & 1) && __popcll(those & ((1ull << lane) - 1)) == rank - at;
+        const uint64_t found = __ballot(chosen);
+        if (!found) {   // (past the last)
+            r.s = Segment{0, 0, 0, 0, true};
+            r.first = INT32_MAX;
+            return r;
+        }
+        j = __builtin_ctzll(found);
+        r.s = segment_of_lanes(p, q, k, j);
+        r.first = KEYS ? r.s.k0 + (__builtin_amdgcn_readlane(own, j) - hi) * kPackedRows : r.s.q0 + (hi - 1) * kPackedRows;
+        return r;
+    }
+    const int t = KEYS ? rank : tiles - 1 - rank;
     r.s = find_segment<KEYS>(p, [&](int begin, int x) { return begin / kPackedRows + x <= t; }, j);
     const int b = KEYS ? r.s.k0 : r.s.q0, i = t - (b / kPackedRows + j);
     r.first = i < 0 ? INT32_MAX : (int)min((int64_t)INT32_MAX, b + (int64_t)i * kPackedRows);   // (below zero: offsets that do not ascend)
