@@ -305,9 +305,7 @@ class GatedAttentionBlock(nn.Module):
             projections = [self.linear_q.weight, self.linear_k.weight, self.linear_v.weight] + ([self.linear_g.weight] if gated else [])
             y = _StackedProjection.apply(x, self.linear_g.bias if gated else None, *projections)
         shape, rotary = (*x.shape[:-1], 4 if gated else 3, self.no_heads, self.c_hidden), self._modules.get("rotary")
-        if rotary is not None:
-            y = rotary.rotate_slots(y, shape, positions)
-        return y.view(shape)
+        return y.view(shape) if rotary is None else rotary.rotate_slots(y, shape, positions)
 
     def _project(self, x: torch.Tensor, weights: Optional[Fp8BlockWeights]) -> torch.Tensor:
         """Q, K, V (and the gate) side by side, in 8 bits."""

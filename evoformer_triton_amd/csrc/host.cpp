@@ -1139,6 +1139,7 @@ PYBIND11_MODULE(_host, m) {
     m.def("fp8_round", &fp8_round, no_gil);
     m.def("rotary", &rotary, no_gil);
     m.def("rotary_forward", &rotary_forward, no_gil);
+    m.def("rotary_slots", &rotary_slots, no_gil);
     m.def("rotary_wrong", &rotary_wrong, no_gil);
     m.def("packed_attention", &packed_attention, no_gil);
     m.def("packed_forward", &packed_forward, no_gil);

@@ -129,22 +129,80 @@ std::optional<std::pair<Tensor, OptTensor>> rotary(const Tensor &q, const OptTen
     return std::make_pair(out.first, out.second.defined() ? OptTensor(out.second) : std::nullopt);
 }
 
-// The same launch without a node, for the registered operator and, in place, for slices of a projection's result.
-std::pair<Tensor, Tensor> rotary_forward(const Tensor &q, const OptTensor &k, const Tensor &positions, const Tensor &turns, bool interleaved, double scale, bool inverse,
-                                         bool in_place) {
+// The same launch without a node, for the registered operator.
+std::pair<Tensor, Tensor> rotary_forward(const Tensor &q, const OptTensor &k, const Tensor &positions, const Tensor &turns, bool interleaved, double scale, bool inverse) {
     Rotary r;
     const char *wrong = r.take(q, k, positions, turns, interleaved, scale);
     TORCH_CHECK_VALUE(!wrong, wrong);
     TORCH_CHECK(q.is_cuda(), "rotary positions run on the GPU only");
     TORCH_CHECK_NOT_IMPLEMENTED(!dual(q) && !(k && dual(*k)), "rotary_positions has no formula for forward mode differentiation");
-    if (in_place) {
-        TORCH_CHECK_VALUE(r.q.is_same(q) && (!k || r.k.is_same(*k)), "in place: the last dimension must be contiguous");
-        c10::DeviceGuard on(q.device());
-        r.run(r.q, r.k, inverse);
-        return {q, k ? *k : at::empty({0}, q.options())};
-    }
     auto out = r.turned(inverse);
     return {out.first, out.second.defined() ? out.second : at::empty({0}, q.options())};
+}
+
+// Queries and keys that are the first two slices of a projection's result y [..., N, slots, H, D], turned where they lie.
+struct RotarySlots {
+    static Tensor slot(const Tensor &y, int64_t i) { return y.select(-3, i); }
+    static const char *turn(const Tensor &y, const Tensor &positions, const Tensor &turns, bool interleaved, double scale, bool inverse) {
+        Rotary r;
+        const Tensor q = slot(y, 0), k = slot(y, 1);
+        if (const char *wrong = r.take(q, k, positions, turns, interleaved, scale)) return wrong;
+        c10::DeviceGuard on(y.device());
+        r.run(r.q, r.k, inverse);
+        return nullptr;
+    }
+};
+struct RotarySlotsNode : SavingNode {
+    std::vector<int64_t> shape;   // the projection's result's
+    at::ScalarType dtype = at::kFloat;
+    bool interleaved = false;
+    double scale = 1.0;
+    std::string name() const override { return "RotarySlotsBackward"; }
+    // saved: positions, turns
+    variable_list apply(variable_list &&grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        const bool rec = at::GradMode::is_enabled();
+        variable_list out(1);
+        if (!grads[0].defined()) return out;
+        {
+            const variable_list t = unpacked();
+            at::AutoDispatchBelowADInplaceOrView guard;
+            Tensor g = std::move(grads[0]);
+            // turned where it lies if nobody else has it (a hook, a gradient that is kept, a view), else in a copy
+            const bool alone = !rec && g.use_count() == 1 && g.has_storage() && g.storage().use_count() == 1;
+            if (g.scalar_type() != dtype) g = g.to(dtype).contiguous();
+            else if (!alone || !g.is_contiguous()) g = g.clone(at::MemoryFormat::Contiguous);
+            const char *wrong = RotarySlots::turn(g, t[0], t[1], interleaved, scale, true);
+            TORCH_INTERNAL_ASSERT(!wrong, wrong);
+            out[0] = g.view(shape);
+        }
+        return once_differentiable(std::move(out), rec);
+    }
+};
+// y as its slices with the first two turned where they lie: y itself is not to be used again (autograd says so where something kept it).  None for a call that the node does not stand for.
+OptTensor rotary_slots(const Tensor &y, const std::vector<int64_t> &shape, const Tensor &positions, const Tensor &turns, bool interleaved, double scale) {
+    if (!plain_modes()) return std::nullopt;
+    for (const Tensor *t : {&y, &positions, &turns})
+        if (!t->defined() || !plain(*t) || !t->is_cuda()) return std::nullopt;
+    if (!y.is_contiguous() || y.is_view() || (y.requires_grad() && y.is_leaf()) || shape.size() < 4) return std::nullopt;
+    Tensor slots;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        slots = y.view(shape);
+        if (RotarySlots::turn(slots, positions, turns, interleaved, scale, false)) return std::nullopt;
+    }
+    if (!y.is_inference()) torch::autograd::impl::bump_version(y);
+    if (SavingNode::wanted(y)) {
+        auto node = make_node<RotarySlotsNode>(y);
+        node->shape = y.sizes().vec();
+        node->dtype = y.scalar_type();
+        node->interleaved = interleaved;
+        node->scale = scale;
+        node->save(positions);
+        node->save(turns);
+        torch::autograd::set_history(slots, node);
+    }
+    return slots;
 }
 std::optional<std::string> rotary_wrong(const Tensor &q, const OptTensor &k, const Tensor &positions, const Tensor &turns, bool interleaved, double scale) {
     Rotary r;

@@ -91,7 +91,7 @@ def rotary_positions(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
 def _op_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, turns: torch.Tensor, interleaved: bool, scale: float,
                inverse: bool) -> Tuple[torch.Tensor, torch.Tensor]:
     """(q, k) turned; k empty if there is none."""
-    return _lib.host().rotary_forward(q, k, positions, turns, interleaved, scale, inverse, False)
+    return _lib.host().rotary_forward(q, k, positions, turns, interleaved, scale, inverse)
 
 
 @_op_rotary.register_fake
@@ -113,32 +113,6 @@ def _backward(ctx, dq, dk):
 
 
 _op_rotary.register_autograd(_backward, setup_context=_setup_context)
-
-
-class _RotateSlots(torch.autograd.Function):
-    """The first two of `slots` slices of a projection's result y [..., N, slots * H * D], queries and keys, turned in place: nothing else of y is moved.
-    (The gradient is turned in a copy: it may be somebody else's.)"""
-
-    @staticmethod
-    def _turn(y, shape, positions, turns, interleaved, scale, inverse):
-        P = y.view(*shape)
-        _lib.host().rotary_forward(P[..., 0, :, :], P[..., 1, :, :], positions, turns, interleaved, scale, inverse, True)
-
-    @staticmethod
-    def forward(ctx, y, shape, positions, turns, interleaved, scale):
-        _RotateSlots._turn(y, shape, positions, turns, interleaved, scale, False)
-        ctx.save_for_backward(positions, turns)
-        ctx.rest = shape, interleaved, scale
-        ctx.mark_dirty(y)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        shape, interleaved, scale = ctx.rest
-        dy = dy.clone(memory_format=torch.contiguous_format)
-        _RotateSlots._turn(dy, shape, *ctx.saved_tensors, interleaved, scale, True)
-        return dy, None, None, None, None, None
 
 
 class RotaryPositions(nn.Module):
@@ -168,8 +142,12 @@ class RotaryPositions(nn.Module):
         return rotary_positions(q, k, positions, self.turns, interleaved=self.interleaved, scale=self.magnitude)
 
     def rotate_slots(self, y: torch.Tensor, shape, positions: torch.Tensor) -> torch.Tensor:
-        """y, a projection's result, with the queries and keys among its slices [..., N, slots, H, D] (`shape`) turned in place."""
-        return _RotateSlots.apply(y, tuple(shape), positions, self.turns, self.interleaved, self.magnitude)
+        """A projection's result y as its slices [..., N, slots, H, D] (`shape`) with the first two, queries and keys, turned: where they lie if that can be, so y is not to be used again."""
+        slots = _lib.host().rotary_slots(y, list(shape), positions, self.turns, self.interleaved, self.magnitude)
+        if slots is not None:
+            return slots
+        q, k, *rest = y.view(shape).unbind(-3)
+        return torch.stack((*self(q, k, positions), *rest), -3)
 
     def plain(self, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor):
         """The same in plain torch operations, on any device: what the kernel is tested against.  (In 64 bits for inputs in 64 bits, else in 32.)"""

@@ -237,3 +237,45 @@ def test_two_streams_at_once(gpu_device):
                     got[i] = block.packed(twice if i else m, off, causal=bool(i))
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_slots_gradient_that_somebody_else_has_stays(gpu_device):
+    """The queries' and keys' gradient is turned back where it lies only if nobody else sees it."""
+    from evoformer_triton_amd import RotaryPositions, packed_positions, rotary_positions
+    rotary = RotaryPositions(32).to(gpu_device)
+    T, shape = 40, (40, 3, 4, 32)
+    at = torch.arange(T, device=gpu_device)
+    x = torch.randn(T, 384, device=gpu_device, requires_grad=True)
+    d = torch.randn(shape, device=gpu_device)
+    kept = d.clone()
+
+    def plain():
+        q, k, v = (x * 2).view(shape).unbind(1)
+        return torch.stack((*rotary_positions(q, k, at, rotary.turns), v), 1)
+
+    want, = torch.autograd.grad(plain(), x, d)
+    y = x * 2
+    out = rotary.rotate_slots(y, shape, at)
+    assert torch.equal(out, plain()) and out.data_ptr() == y.data_ptr()
+    assert torch.equal(torch.autograd.grad(out, x, d)[0], want) and torch.equal(d, kept)      # the caller's own
+    seen = []
+    y = x * 2
+    out = rotary.rotate_slots(y, shape, at)
+    out.register_hook(lambda g: seen.append(g))
+    out.retain_grad()
+    (out * 1.0).backward(d)
+    assert torch.equal(seen[0], kept) and torch.equal(out.grad, kept) and torch.equal(x.grad, want)
+    # a leaf and a view cannot be turned where they lie: in a copy
+    leaf = x.detach().clone().requires_grad_()
+    base = leaf.detach().clone()
+    out = rotary.rotate_slots(leaf, shape, at)
+    assert torch.equal(leaf, base)
+    assert torch.equal(2 * torch.autograd.grad(out, leaf, d)[0], want)
+    view = torch.cat((x * 2, x))[:T]
+    assert torch.equal(rotary.rotate_slots(view, shape, at), plain())
+    # what is in use for another gradient is not overwritten unnoticed
+    y = x * 2
+    z = y * y
+    rotary.rotate_slots(y, shape, at)
+    with pytest.raises(RuntimeError, match="inplace"):
+        z.sum().backward()
