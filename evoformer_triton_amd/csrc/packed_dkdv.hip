@@ -73,6 +73,8 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
     v8 kf[R::KSD], vf[K::VLDS ? 1 : R::KSD];
     load_operands(head_row<T>(p.k, krow, p.k_stride_t, hk, p.k_stride_h), D, g, kf);
     if constexpr (!K::VLDS) load_operands(head_row<T>(p.v, krow, p.v_stride_t, hk, p.v_stride_h), D, g, vf);
+    asked_together<R::KSD>(kf);   // (and waited for: see packed_fwd)
+    if constexpr (!K::VLDS) asked_together<R::KSD>(vf);
     // the first query that sees this lane's key, the wave's first one and its last one
     const int key_from = s.first_query(krow, p.causal), wave_from = s.first_query(k0, p.causal), wave_to = s.first_query(min(k0 + 31, s.k1 - 1), p.causal);
     const float c = p.scale * kLog2e;

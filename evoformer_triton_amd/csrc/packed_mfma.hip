@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
     const bool active = q0 < s.q1;   // uniform
     v8 qf[R::KSD];
     load_operands(head_row<T>(p.q, qrow, p.q_stride_t, h, p.q_stride_h), D, g, qf);
+    asked_together<R::KSD>(qf);   // (and waited for: in the loop the compiler, which does not count the loads into LDS, would wait for the next stage's with them)
     const int seen = s.seen(qrow, p.causal);
     // of the wave's queries: the fewest keys and the most
     const int wave_least = active ? s.seen(q0, p.causal) : 0, wave_most = active ? s.seen(min(q0 + 31, s.q1 - 1), p.causal) : 0;
@@ -279,7 +280,11 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
         }
     }
     dl += __shfl_xor(dl, 32);
-    const float c = p.scale * kLog2e, lse = p.lse[(int64_t)h * p.Tq + qrow];
+    const float c = p.scale * kLog2e;
+    float lse[1] = {p.lse[(int64_t)h * p.Tq + qrow]};
+    asked_together<R::KSD>(qf);   // (see packed_fwd)
+    asked_together<R::KSD>(df);
+    asked_together<1>(lse);
     const int seen = s.seen(qrow, p.causal);
     const int wave_least = active ? s.seen(q0, p.causal) : 0, wave_most = active ? s.seen(min(q0 + 31, s.q1 - 1), p.causal) : 0;
     f32x16 dq[R::DT];
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float e = fast_exp2(fmaf(a[r], c, -lse));
+            const float e = fast_exp2(fmaf(a[r], c, -lse[0]));
             sum[r & 1] += e;
             d[r] *= e;
             rest[r & 1] += d[r];
@@ -373,7 +378,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
         return;
     }
     const float inv = seen ? 1.0f / sum[0] : 0.0f;
-    if (mine && g == 0) save_row(out_rows, (int64_t)h * p.Tq + qrow, lse, dl, sum[0], rest[0], c);
+    if (mine && g == 0) save_row(out_rows, (int64_t)h * p.Tq + qrow, lse[0], dl, sum[0], rest[0], c);
     bool nan = false;
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt)
