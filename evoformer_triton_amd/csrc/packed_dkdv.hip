@@ -2,7 +2,7 @@
 //
 // A wave has 32 keys, a column of the products' each, and walks over the queries of all heads that share the key head: S = Q K^T and dP = dO V^T begin with what is subtracted from them (-lse in units of
 // q . k, -delta; staged in LDS beside the rows), P and dS as they lie are operands of dV^T = dO^T P and dK^T = Q^T dS.  Four products for each pair of rows, their other operands from LDS: for head dims
-// above 64 V's too, since with K's, dK and dV in registers (2 waves to a SIMD) there is no room for them.  4 x 4096 causal rows, 32 heads (8) of 128: 1.19 ms, 0.93 Pflop/s; what is left of the rate of
+// above 64 V's too, since with K's, dK and dV in registers (2 waves to a SIMD) there is no room for them.  4 x 4096 causal rows, 32 heads (8) of 128: 1.09 ms, 1.0 Pflop/s; what is left of the rate of
 // a large product goes into LDS's reads, of which each product needs two, and into exponentials.
 #include "packed_tiles.h"
 
@@ -87,16 +87,17 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
         const unsigned at = Staged::base(buf), vat = Staged::base(vlds) + own * 32 * G::ROW;
         // (the products begin with what is subtracted from them)
         const float *sub = reinterpret_cast<const float *>(buf + 2 * K::ARRAY + (qb >> 6) * 512) + (qb & 63) + 4 * g;
-        f32x16 a, d;
+        auto begin_with = [&](const float *from) __attribute__((always_inline)) {
+            f32x16 t;
 #pragma unroll
-        for (int rr = 0; rr < 4; ++rr) {
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(sub + 8 * rr), y = *reinterpret_cast<const f32x4 *>(sub + 64 + 8 * rr);
+            for (int rr = 0; rr < 4; ++rr) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(from + 8 * rr);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[4 * rr + i] = x[i];
-                d[4 * rr + i] = y[i];
+                for (int i = 0; i < 4; ++i) t[4 * rr + i] = x[i];
             }
-        }
+            return t;
+        };
+        f32x16 a = begin_with(sub);
         const unsigned qat = at + (unsigned)(qb * G::ROW), dat = qat + K::ARRAY;
         v8 x[R::KSD];
 #pragma unroll
@@ -104,6 +105,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) a = Mfma<T>::mma(x[ks], kf[ks], a);
+        f32x16 d = begin_with(sub + 64);
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) d = Mfma<T>::mma(staged.rows<T>(dat, 0, ks), K::VLDS ? staged.rows<T>(vat, 0, ks) : vf[K::VLDS ? 0 : ks], d);
 #pragma unroll
@@ -126,6 +128,8 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
         for (int ts = 0; ts < 2; ++ts)
 #pragma unroll
             for (int dt = 0; dt < R::DT; ++dt) dv[dt] = Mfma<T>::mma(staged.cols<T>(dat, 0, ts, dt), pf[ts], dv[dt]);
+        // (without this head dim 128 keeps one of K's operands in memory, whose way back is waited for with all that is on its way into LDS: 1.16 ms instead of 1.09 for the size above)
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ts = 0; ts < 2; ++ts)
 #pragma unroll
