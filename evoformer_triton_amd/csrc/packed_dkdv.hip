@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
             wait_lds_barrier();
         }
     }
+    wait_loads();
     if constexpr (KG == 2) {
         float *const x = reinterpret_cast<float *>(lds) + own * R::DT * 16 * 64;
         wait_lds_barrier();
