@@ -13,7 +13,7 @@
 // 0.0017; without any of this 0.0035 and 0.0033.
 //
 // What bounds them: the matrix instructions and, at the same time on the same SIMD, exponentials (a quarter of the rate of other instructions) and additions.  Forward, one causal prompt of 16384 rows,
-// 32 heads (8 for keys) of 128: 1.98 ms, 1.1 Pflop/s of the 1.2 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.64 ms, dQ 1.06 (its product of K twice), dK and dV 1.19.
+// 32 heads (8 for keys) of 128: 1.98 ms, 1.1 Pflop/s of the 1.2 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.58 ms, dQ 1.06 (its product of K twice), dK and dV 1.09.
 // Inputs of zeros take a quarter less time than random ones: the power that the products take has its part in it.
 //
 // Which rows: tile t of the launch belongs to the last segment j (packed_common.h) with begin(j) / 128 + j <= t; begin(j + 1) / 128 + j + 1 leaves room for all of j's tiles, so that every workgroup finds
@@ -28,8 +28,9 @@ namespace evo {
 
 namespace EVO_CAT(packed_d, EVO_D) {
 
-// Stages in LDS: one that is computed on and the others under way
-template <int KG> constexpr int kStageBuffers = KG == 2 ? (EVO_D > 64 ? 2 : 3) : EVO_D == 32 ? 4 : EVO_D == 64 ? 3 : 2;
+// Stages in LDS: one that is computed on and the others under way.  (Head dim 64, seven prompts of 90 to 2011: 35.0 us with two, 36.1 with three; head dim 32, chains of 51 to 768, forward and dQ: 49.4 with
+// four, or three of twice as many keys, and 51.8 with three and two.)
+template <int KG> constexpr int kStageBuffers = EVO_D > 32 ? 2 : KG == 2 ? 3 : 4;
 
 // ------------------------------------------------------------------ forward
 

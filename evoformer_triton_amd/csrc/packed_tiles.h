@@ -101,9 +101,9 @@ __device__ __forceinline__ Place place_of(const EvoPacked &p, int rank, int tile
     int j;
     // Under a causal mask of few long sequences those with the longest walks begin first: a tile of queries i before a sequence's own first one sees i + 1 tiles of keys, one of keys is seen from
     // as many tiles as are behind it and its own.  Of c_j tiles of sequence j max(0, c_j - w) have walks longer than w; the rank is that of walks of w where the sum of these reaches it.  4 x 4096 rows,
-    // 32 heads (8) of 128: dK and dV 1.19 ms (1.34 with one sequence after the other), forward 0.635 (0.66), dQ 1.08 (1.06: more sequences' keys at once in an L2).  Sequences of 7 tiles on average:
-    // forward 40.8 us (43.9); of 5: 38.1 (37.4), the search costs what it gains.
-    if (p.causal && p.n + 3 <= 64 && (KEYS ? p.Tk : p.Tq) >= (int64_t)6 * kPackedRows * p.n) {
+    // 32 heads (8) of 128: dK and dV 1.19 ms (1.34 with one sequence after the other), forward 0.635 (0.66), dQ 1.08 (1.06: more sequences' keys at once in an L2).  Seven sequences of 5 tiles on average:
+    // forward 34.0 us (35.1); 16 of 3: with gradients 88 (99); 40 of one: 9 (7), the search takes longer than it gains.
+    if (p.causal && p.n + 3 <= 64 && (KEYS ? p.Tk : p.Tq) >= (int64_t)2 * kPackedRows * p.n) {
         const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x), b = KEYS ? k : q;
         const int rows = max(0, __shfl_down(b, 1) - b), own = lane < p.n + 2 ? (rows + kPackedRows - 1) / kPackedRows : 0;
         auto longer = [&](int w) {
