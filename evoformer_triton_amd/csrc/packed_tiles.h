@@ -99,28 +99,43 @@ template <bool KEYS>
 __device__ __forceinline__ Place place_of(const EvoPacked &p, int rank, int tiles) {
     Place r;
     int j;
-    // Under a causal mask of few long sequences those with the longest walks begin first: a tile of queries i before a sequence's own first one sees i + 1 tiles of keys, one of keys is seen from
-    // as many tiles as are behind it and its own.  Of c_j tiles of sequence j max(0, c_j - w) have walks longer than w; the rank is that of walks of w where the sum of these reaches it.  4 x 4096 rows,
-    // 32 heads (8) of 128: dK and dV 1.19 ms (1.34 with one sequence after the other), forward 0.635 (0.66), dQ 1.08 (1.06: more sequences' keys at once in an L2).  Seven sequences of 5 tiles on average:
-    // forward 34.0 us (35.1); 16 of 3: with gradients 88 (99); 40 of one: 9 (7), the search takes longer than it gains.
-    if (p.causal && p.n + 3 <= 64 && (KEYS ? p.Tk : p.Tq) >= (int64_t)2 * kPackedRows * p.n) {
-        const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x), b = KEYS ? k : q;
-        const int rows = max(0, __shfl_down(b, 1) - b), own = lane < p.n + 2 ? (rows + kPackedRows - 1) / kPackedRows : 0;
-        auto longer = [&](int w) {
-            int sum = 0;
-            for (int y = 0; y < p.n + 2; ++y) sum += max(0, __builtin_amdgcn_readlane(own, y) - w);
-            return sum;
-        };
-        int lo = -1, hi = tiles, at = 0;   // longer(hi) <= rank, and not of lo
-        while (hi - lo > 1) {
-            const int step = (hi - lo + 63) / 64, w = min(hi, lo + (lane + 1) * step), n = longer(w);
-            const int f = __builtin_ctzll(__ballot(n <= rank));   // (the last lane's w is hi)
-            hi = __builtin_amdgcn_readlane(w, f);
-            at = __builtin_amdgcn_readlane(n, f);
-            lo = hi - step;
+    // Of few sequences the tiles with the longest walks begin first.  Under a causal mask a tile of queries i before a sequence's own first one sees i + 1 tiles of keys, one of keys is seen from as many
+    // tiles as are behind it and its own: of c_j tiles of sequence j max(0, c_j - w) have walks longer than w, and the rank is that of walks of w where the sum of these reaches it.  Without a mask all of a
+    // sequence's tiles have the same walk.  4 x 4096 causal rows, 32 heads (8) of 128: dK and dV 1.19 ms (1.34 with one sequence after the other), forward 0.635 (0.66), dQ 1.08 (1.06: more sequences' keys
+    // at once in an L2).  Seven causal sequences of 5 tiles on average: forward 34.0 us (35.1); 16 of 3: with gradients 88 (99); 40 of one: 9 (7), the search takes longer than it
+    // gains.  24 chains of 51 to 768 rows without a mask, 8 heads of 32: forward 16.1 us (19.2), dQ 24.7 (31.1), of 64: 17 (22); 60 of 100 to 1000 with 32 heads: 218 (177), hence not for so many.
+    if (p.n < 30 && (KEYS ? p.Tk : p.Tq) >= (int64_t)2 * kPackedRows * p.n) {
+        const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x);
+        const int nq = max(0, __shfl_down(q, 1) - q), nk = max(0, __shfl_down(k, 1) - k), own = lane < p.n + 2 ? ((KEYS ? nk : nq) + kPackedRows - 1) / kPackedRows : 0;
+        int into = 0;         // the tile's place in its sequence, as far as lane j knows
+        bool chosen = false;
+        if (p.causal) {
+            auto longer = [&](int w) {
+                int sum = 0;
+                for (int y = 0; y < p.n + 2; ++y) sum += max(0, __builtin_amdgcn_readlane(own, y) - w);
+                return sum;
+            };
+            int lo = -1, hi = tiles, at = 0;   // longer(hi) <= rank, and not of lo
+            while (hi - lo > 1) {
+                const int step = (hi - lo + 63) / 64, w = min(hi, lo + (lane + 1) * step), n = longer(w);
+                const int f = __builtin_ctzll(__ballot(n <= rank));   // (the last lane's w is hi)
+                hi = __builtin_amdgcn_readlane(w, f);
+                at = __builtin_amdgcn_readlane(n, f);
+                lo = hi - step;
+            }
+            const uint64_t those = __ballot(own >= hi && own > 0);
+            chosen = hi > 0 && (those >> lane & 1) && __popcll(those & ((1ull << lane) - 1)) == rank - at;
+            into = KEYS ? own - hi : hi - 1;
+        } else {
+            const int walk = lane == 0 || lane > p.n ? -1 : KEYS ? nq : nk;   // (rows of no sequence: last)
+            int before = 0;
+            for (int y = 0; y < p.n + 2; ++y) {
+                const int other = __builtin_amdgcn_readlane(walk, y);
+                before += other > walk || (other == walk && y < lane) ? __builtin_amdgcn_readlane(own, y) : 0;
+            }
+            into = rank - before;
+            chosen = into >= 0 && into < own;
         }
-        const uint64_t those = __ballot(own >= hi && own > 0);
-        const bool chosen = hi > 0 && (those >> lane & 1) && __popcll(those & ((1ull << lane) - 1)) == rank - at;
         const uint64_t found = __ballot(chosen);
         if (!found) {   // (past the last)
             r.s = Segment{0, 0, 0, 0, true};
@@ -129,7 +144,7 @@ __device__ __forceinline__ Place place_of(const EvoPacked &p, int rank, int tile
         }
         j = __builtin_ctzll(found);
         r.s = segment_of_lanes(p, q, k, j);
-        r.first = KEYS ? r.s.k0 + (__builtin_amdgcn_readlane(own, j) - hi) * kPackedRows : r.s.q0 + (hi - 1) * kPackedRows;
+        r.first = (KEYS ? r.s.k0 : r.s.q0) + __builtin_amdgcn_readlane(into, j) * kPackedRows;
         return r;
     }
     const int t = KEYS ? rank : tiles - 1 - rank;
