@@ -400,7 +400,7 @@ int evoattn_rotary(const EvoRotary *p, void *hip_stream);
  *   o_low  16 bits: what rounding o to its type left of it, in its type and laid out like it, for the backward's sums of dout o (which end in every gradient of a row); may be NULL
  *   dk, dv  both may be NULL (not wanted)
  * D at most 128; scale 2^-64 to 2^64.  16-bit: D and all strides multiples of 8, pointers on 16-byte boundaries, row strides from D to 2^23 (EVO_EALIGN
- * otherwise).  `workspace` of evoattn_packed_fwd_workspace_bytes() (0: none needed) and evoattn_packed_bwd_workspace_bytes().  The backward is
+ * otherwise).  `workspace` of evoattn_packed_fwd_workspace_bytes() (0: none needed) and evoattn_packed_bwd_workspace_bytes(), on a 16-byte boundary.  The backward is
  * deterministic.  Nothing is allocated or synchronised. */
 typedef struct EvoPacked {
     int32_t n, H, Hk, D;

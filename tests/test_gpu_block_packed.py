@@ -279,3 +279,14 @@ def test_a_slots_gradient_that_somebody_else_has_stays(gpu_device):
     rotary.rotate_slots(y, shape, at)
     with pytest.raises(RuntimeError, match="inplace"):
         z.sum().backward()
+
+
+def test_no_rows_and_one(gpu_device):
+    for dt in (BF16, F32):
+        block = _block(gpu_device, dt, rotary={})
+        for T in (0, 1):
+            m = torch.randn(T, 96, device=gpu_device).to(dt).requires_grad_()
+            y = block.packed(m, torch.tensor([0, T], device=gpu_device))
+            g, = torch.autograd.grad(y, m, torch.ones_like(y))
+            assert y.shape == g.shape == (T, 96) and torch.isfinite(y).all() and torch.isfinite(g).all()
+        assert torch.equal(y, block.packed(m, torch.tensor([0, T], device=gpu_device), torch.tensor([-7], device=gpu_device)))      # (a token alone sees itself, wherever it is)

@@ -88,3 +88,39 @@ def test_the_oracle_is_the_formula():
         got, _ = packed(q, k, v, a, b, causal, 0.3, dout)
         for x, y in zip(got, want):
             assert torch.allclose(x, y, rtol=1e-12, atol=1e-12)
+
+
+def test_the_c_entry_points_refuse_what_is_not_aligned():
+    """16 bits: pieces of 16 bytes, rows that lie apart; and a workspace that is not there or begins between two of them."""
+    lib = _lib.load()
+    for change, code, ways in (({"q": 0x10008}, _lib.EVO_EALIGN, "fb"), ({"v": 0x10002}, _lib.EVO_EALIGN, "fb"), ({"o_low": 0x10008}, _lib.EVO_EALIGN, "fb"),
+                               ({"k_stride_t": 132}, _lib.EVO_EALIGN, "fb"), ({"k_stride_t": 56}, _lib.EVO_EALIGN, "fb"), ({"q_stride_t": 0}, _lib.EVO_EALIGN, "fb"),
+                               ({"v_stride_t": 1 << 23}, _lib.EVO_EALIGN, "fb"), ({"q_stride_h": 60}, _lib.EVO_EALIGN, "fb"), ({"D": 60}, _lib.EVO_EALIGN, "fb"),
+                               ({"dout": 0x10008}, _lib.EVO_EALIGN, "b"), ({"dout_stride_t": 0}, _lib.EVO_EALIGN, "b"), ({"dk": 0x10004}, _lib.EVO_EALIGN, "b"),
+                               ({"workspace": 0x10008}, _lib.EVO_EALIGN, "b"), ({"workspace": None}, _lib.EVO_EWORKSPACE, "b"), ({"lse": None}, _lib.EVO_EINVAL, "b"),
+                               ({"dk": None}, _lib.EVO_EINVAL, "b"), ({"H": 1 << 21, "Hk": 1}, _lib.EVO_EOVERFLOW, "fb"), ({"n": 1 << 30}, _lib.EVO_EOVERFLOW, "fb")):
+        p = _block()
+        for name, value in change.items():
+            setattr(p, name, value)
+        for way in ways:
+            call = lib.evoattn_packed_fwd if way == "f" else lib.evoattn_packed_bwd
+            assert call(ctypes.byref(p), None) == code, (change, way)
+    # parts of a long walk, in both types
+    for dtype in (_lib.EVO_BF16, _lib.EVO_F32):
+        p = _block()
+        p.dtype, p.Tk = dtype, 1 << 20
+        need = lib.evoattn_packed_fwd_workspace_bytes(ctypes.byref(p))
+        assert need > 0
+        for name, value, code in (("workspace_bytes", need - 1, _lib.EVO_EWORKSPACE), ("workspace", None, _lib.EVO_EWORKSPACE), ("workspace", 0x10004, _lib.EVO_EALIGN)):
+            p = _block()
+            p.dtype, p.Tk = dtype, 1 << 20
+            setattr(p, name, value)
+            assert lib.evoattn_packed_fwd(ctypes.byref(p), None) == code, (dtype, name)
+    # nothing at all
+    for dtype in (_lib.EVO_BF16, _lib.EVO_F32):
+        for n, Tq, Tk in ((0, 0, 0), (0, 0, 50), (0, 50, 0), (1, 0, 0), (5, 0, 50)):
+            p = _block()
+            p.dtype, p.n, p.Tq, p.Tk = dtype, n, Tq, Tk
+            assert lib.evoattn_packed_fwd_workspace_bytes(ctypes.byref(p)) >= 0 and lib.evoattn_packed_bwd_workspace_bytes(ctypes.byref(p)) >= 0
+            if Tq == 0:
+                assert lib.evoattn_packed_fwd(ctypes.byref(p), None) == 0
