@@ -30,7 +30,10 @@ EVO_PACKED(128)
 // Whether the kernels that split the keys of few queries serve the forward: by the average of a sequence's queries times the query heads that share a key head, which are columns there.
 //   16 sequences of 4096 keys, 32 heads (8), D = 128, bf16: 72 us with 32 columns (here the other kernel: 137), 195 with 128 (164); 16 of 1024, 8 heads (8), D = 64: 15 with 16 (16), 21 with 32 (17), 38
 //   with 64 (17); one of 4096, 16 heads (4), D = 128: 16 with 32 (19), 26 with 64 (19).  fp32: 286 with 64 (698) and 528 with 128 (790); 50 with 64 (55) and 90 with 128 (73); 36 (54) and 61 (56).
-static bool few_queries(const EvoPacked &p) { return p.n && p.Tq * (p.H / p.Hk) <= (int64_t)(p.dtype == EVO_F32 ? 64 : 32) * p.n; }
+// (In fp32 a launch with a wave to a row joins their parts, one of them too.)
+static bool few_queries(const EvoPacked &p) {
+    return p.n && p.Tq * (p.H / p.Hk) <= (int64_t)(p.dtype == EVO_F32 ? 64 : 32) * p.n && (p.dtype != EVO_F32 || row_waves_fit(p.Tq * p.H));
+}
 
 static int64_t align_rows(int64_t n) { return (n + 63) / 64 * 64; }   // (16-byte pieces behind them)
 

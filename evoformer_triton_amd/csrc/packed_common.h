@@ -6,6 +6,9 @@
 
 namespace evo {
 
+// Whether a launch with a wave to a row, four of them to a workgroup, holds so many rows.
+static inline bool row_waves_fit(int64_t rows) { return grid_fits((rows + 3) / 4, 256); }
+
 // Rows of a sequence: queries q0 .. q1 - 1, keys k0 .. k1 - 1.  gap: rows of no sequence, before the first and behind the last.
 struct Segment {
     int q0, q1, k0, k1;

@@ -204,7 +204,7 @@ int EVO_CAT(launch_packed_dkdv_d, EVO_D)(const EvoPacked &p, const BackwardRows 
     using namespace EVO_CAT(packed_d, EVO_D);
     const Plan plan = key_plan(p);
     const int64_t tiles = packed_tiles(p.Tk, p.n), grid = Unit::grid(tiles, p.Hk, plan.parts), rows = p.Tk * p.Hk;
-    if (!grid_fits(grid, 256 * plan.groups) || (plan.parts > 1 && (rows > INT32_MAX || !grid_fits(rows, 64)))) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 256 * plan.groups) || (plan.parts > 1 && !row_waves_fit(rows))) return EVO_EOVERFLOW;
     return by_half(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         return plan.run([&](auto groups, auto part) {

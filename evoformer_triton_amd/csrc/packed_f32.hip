@@ -560,7 +560,7 @@ int EVO_CAT(launch_packed_f32_few_d, EVO_D)(const EvoPacked &p, hipStream_t st) 
     using namespace EVO_CAT(packed_d, EVO_D);
     const int parts = few_f32_plan(p).parts;
     const int64_t grid = (int64_t)p.n * p.Hk * parts, rows = p.Tq * p.H;
-    if (!grid_fits(grid, 64) || rows > INT32_MAX) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 64) || !row_waves_fit(rows)) return EVO_EOVERFLOW;
     const Parts to = {(float *)p.workspace, (float2 *)((float *)p.workspace + parts * rows * EVO_D), 0, parts};
     const int rc = by_flag(vectors(p, false), [&](auto vec) {
         constexpr auto kern = packed_f32_few<decltype(vec)::value>;
@@ -577,7 +577,7 @@ int EVO_CAT(launch_packed_f32_fwd_d, EVO_D)(const EvoPacked &p, hipStream_t st) 
     using namespace EVO_CAT(packed_d, EVO_D);
     const int parts = f32_queries(p).parts;
     const int64_t tiles = packed_tiles(p.Tq, p.n), grid = Unit::grid(tiles, p.Hk, p.H / p.Hk * (int64_t)parts), rows = p.Tq * p.H;
-    if (!grid_fits(grid, 256) || (parts > 1 && rows > INT32_MAX)) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 256) || (parts > 1 && !row_waves_fit(rows))) return EVO_EOVERFLOW;
     auto go = [&](auto vec, auto part) {
         constexpr auto kern = packed_f32_fwd<decltype(vec)::value, decltype(part)::value>;
         static PerDevice done;
@@ -597,7 +597,7 @@ int EVO_CAT(launch_packed_f32_bwd_d, EVO_D)(const EvoPacked &p, const BackwardRo
     const Parts qparts = {sums, nullptr, 0, f32_queries(p).parts}, kparts = {sums, nullptr, 0, f32_keys(p).parts};
     const int64_t tiles = packed_tiles(p.Tq, p.n), grid = Unit::grid(tiles, p.Hk, p.H / p.Hk * (int64_t)qparts.chunks), rows = p.Tq * p.H;
     const int64_t key_tiles = packed_tiles(p.Tk, p.n), key_grid = Unit::grid(key_tiles, p.Hk, kparts.chunks), keys = p.Tk * p.Hk;
-    if (!grid_fits(grid, 256) || !grid_fits(key_grid, 256) || (qparts.chunks > 1 && rows > INT32_MAX) || (kparts.chunks > 1 && keys > INT32_MAX)) return EVO_EOVERFLOW;
+    if (!grid_fits(grid, 256) || !grid_fits(key_grid, 256) || (qparts.chunks > 1 && !row_waves_fit(rows)) || (kparts.chunks > 1 && !row_waves_fit(keys))) return EVO_EOVERFLOW;
     auto dq = [&](auto vec, auto part) {
         constexpr auto kern = packed_f32_dq<decltype(vec)::value, decltype(part)::value>;
         static PerDevice done;
