@@ -336,13 +336,14 @@ int EVO_CAT(launch_packed_few_d, EVO_D)(const EvoPacked &p, hipStream_t st) {
     const FewPlan plan = few_plan(p, p.workspace);
     const Parts &parts = plan.parts;
     const int64_t grid = (p.Tk / parts.chunk + p.n + 2) * p.Hk, rows = p.Tq * p.H;
-    if (rows > INT32_MAX || !grid_fits(grid, kFewWaves * 64) || !grid_fits(rows, 1024)) return EVO_EOVERFLOW;
+    if (parts.chunks > 1 && !grid_fits(rows, 1024)) return EVO_EOVERFLOW;   // (the join's)
     return by_half(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         auto go = [&](auto part, auto waves, auto tiles) {
             constexpr int NW = decltype(waves)::value, CT = decltype(tiles)::value, LDS = FewGeo<NW, CT>::LDS;
             constexpr auto kern = packed_few<T, decltype(part)::value, NW, CT>;
             static PerDevice done;
+            if (!grid_fits(grid, NW * 64)) return (int)EVO_EOVERFLOW;
             if (const int rc = ensure_dynamic_lds((const void *)kern, LDS, done, nullptr)) return rc;
             kern<<<(unsigned)grid, NW * 64, LDS, st>>>(p, parts);
             const int rc = hip_rc();
