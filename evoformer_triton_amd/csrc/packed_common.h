@@ -9,6 +9,15 @@ namespace evo {
 // Whether a launch with a wave to a row, four of them to a workgroup, holds so many rows.
 static inline bool row_waves_fit(int64_t rows) { return grid_fits((rows + 3) / 4, 256); }
 
+// A kernel's first argument, loaded anew: what its end alone needs is then not kept in registers over its loop.
+__device__ __forceinline__ EvoPacked parameters_again() {
+    auto *at = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(at));
+    EvoPacked p;
+    __builtin_memcpy(&p, (const void *)at, sizeof p);
+    return p;
+}
+
 // Rows of a sequence: queries q0 .. q1 - 1, keys k0 .. k1 - 1.  gap: rows of no sequence, before the first and behind the last.
 struct Segment {
     int q0, q1, k0, k1;

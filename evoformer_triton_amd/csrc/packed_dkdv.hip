@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
     f32x16 dk[R::DT], dv[R::DT];
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt) dk[dt] = dv[dt] = filled(0.0f);
+    float up = kShiftKey;   // (kShifts: P, and with it dS, dK and dV, times 2^up)
 
     const Staged staged(lane);
     auto step = [&](const unsigned char *buf, int qb, int row0) __attribute__((always_inline)) {
@@ -109,7 +110,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) d = Mfma<T>::mma(staged.rows<T>(dat, 0, ks), K::VLDS ? staged.rows<T>(vat, 0, ks) : vf[K::VLDS ? 0 : ks], d);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) a[r] = fast_exp2(a[r] * c);
+        for (int r = 0; r < 16; ++r) a[r] = fast_exp2(kShifts<T> ? fmaf(a[r], c, up) : a[r] * c);
         if (row0 < wave_to) {   // (uniform)
             asm volatile("");
 #pragma unroll
@@ -117,6 +118,19 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
                 const bool sees = row0 + crow(r, g) >= key_from;
                 a[r] = sees ? a[r] : 0.0f;
                 d[r] = sees ? d[r] : 0.0f;
+            }
+        }
+        if constexpr (kShifts<T>) {
+            d *= a;
+            bool any;
+            const int down = shift_down(d, any);
+            if (__builtin_expect(any, 0)) {
+                const float by = ldexpf(1.0f, -down);
+                up -= (float)down;
+                a *= by;
+                d *= by;
+                shift_by(dk, by);
+                shift_by(dv, by);
             }
         }
         v8 pf[2], sf[2];
@@ -133,7 +147,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
 #pragma unroll
         for (int ts = 0; ts < 2; ++ts)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sf[ts][i] = (T)(a[8 * ts + i] * d[8 * ts + i]);
+            for (int i = 0; i < 8; ++i) sf[ts][i] = (T)(kShifts<T> ? d[8 * ts + i] : a[8 * ts + i] * d[8 * ts + i]);
 #pragma unroll
         for (int ts = 0; ts < 2; ++ts)
 #pragma unroll
@@ -159,6 +173,11 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
         }
     }
     wait_loads();
+    if constexpr (kShifts<T>) {
+        const float by = ldexpf(1.0f, -(int)up);
+        shift_by(dk, by);
+        shift_by(dv, by);
+    }
     if constexpr (KG == 2) {
         float *const x = reinterpret_cast<float *>(lds) + own * R::DT * 16 * 64;
         wait_lds_barrier();
@@ -194,7 +213,9 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
         store_row_tile<T>((T *)p.dk + row * D, dt * 32, whole ? D : 0, dk[dt], p.scale, g);
         store_row_tile<T>((T *)p.dv + row * D, dt * 32, whole ? D : 0, dv[dt], 1.0f, g);
     }
-    for (; again; again &= again - 1) row_dkdv<T>(p, s, k0 + __builtin_ctz(again), hk, saved.delta);
+    if (!again) return;
+    const EvoPacked late = parameters_again();
+    for (; again; again &= again - 1) row_dkdv<T>(late, s, k0 + __builtin_ctz(again), hk, saved.delta);
 }
 
 }  // namespace

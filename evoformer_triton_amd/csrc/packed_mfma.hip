@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
     const int wave_least = active ? s.seen(q0, p.causal) : 0, wave_most = active ? s.seen(min(q0 + 31, s.q1 - 1), p.causal) : 0;
     f32x16 dq[R::DT];
     float sum[2] = {0.0f, 0.0f}, rest[2] = {0.0f, 0.0f};   // of the probabilities, which should be 1, and of ds, which should be 0
+    float less = lse[0] - (kShifts<T> ? kShiftQuery : 0);  // (and, with dQ, times what this takes off)
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt) dq[dt] = filled(0.0f);
 
@@ -316,10 +317,24 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float e = fast_exp2(fmaf(a[r], c, -lse[0]));
+            const float e = fast_exp2(fmaf(a[r], c, -less));
             sum[r & 1] += e;
             d[r] *= e;
             rest[r & 1] += d[r];
+        }
+        if constexpr (kShifts<T>) {
+            bool any;
+            const int down = shift_down(d, any);
+            if (__builtin_expect(any, 0)) {
+                const float by = ldexpf(1.0f, -down);
+                less += (float)down;
+                sum[0] *= by;
+                sum[1] *= by;
+                rest[0] *= by;
+                rest[1] *= by;
+                d *= by;
+                shift_by(dq, by);
+            }
         }
 #pragma unroll
         for (int ts = 0; ts < 2; ++ts) {
@@ -351,6 +366,12 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
     wait_loads();
     sum[0] += sum[1];
     rest[0] += rest[1];
+    if constexpr (kShifts<T>) {   // (of a row that sees nothing there are no sums; the difference is a whole number, but for its rounding)
+        const float by = ldexpf(1.0f, seen ? (int)rintf(less - lse[0]) : 0);
+        sum[0] *= by;
+        rest[0] *= by;
+        shift_by(dq, by);
+    }
     if constexpr (KG == 2) {
         float *const x = reinterpret_cast<float *>(lds) + own * (R::DT * 16 + 2) * 64, *const more = x + R::DT * 16 * 64;
         wait_lds_barrier();
