@@ -207,15 +207,20 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
 #pragma unroll
         for (int r = 0; r < 16; ++r) nan |= !(dk[dt][r] == dk[dt][r]) || !(dv[dt][r] == dv[dt][r]);
     unsigned again = rows_without_number(nan && mine);
-    const bool whole = mine && !(again >> li & 1);
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt) {
-        store_row_tile<T>((T *)p.dk + row * D, dt * 32, whole ? D : 0, dk[dt], p.scale, g);
-        store_row_tile<T>((T *)p.dv + row * D, dt * 32, whole ? D : 0, dv[dt], 1.0f, g);
+        store_row_tile<T>((T *)p.dk + row * D, dt * 32, mine ? D : 0, dk[dt], p.scale, g);
+        store_row_tile<T>((T *)p.dv + row * D, dt * 32, mine ? D : 0, dv[dt], 1.0f, g);
     }
     if (!again) return;
     const EvoPacked late = parameters_again();
-    for (; again; again &= again - 1) row_dkdv<T>(late, s, k0 + __builtin_ctz(again), hk, saved.delta);
+    const int least = max(begin, wave_from - 31);   // (of the queries that a step of the wave's has)
+    if (!spoilt_dkdv<T>(late, s, hk, k0, min(k0 + 32, s.k1), least, wave_to, saved.delta)) return;
+    wait_loads();   // (see packed_fwd)
+    for (; again; again &= again - 1) {
+        const int j = k0 + __builtin_ctz(again);
+        if (spoilt_dkdv<T>(late, s, hk, j, j + 1, least, s.first_query(j, late.causal), saved.delta)) row_dkdv<T>(late, s, j, hk, saved.delta);
+    }
 }
 
 }  // namespace

@@ -208,11 +208,19 @@ __global__ void __launch_bounds__(256, 2) packed_f32_fwd(EvoPacked p, Parts part
     for (int dt = 0; dt < F::DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[dt][r] = seen ? o[dt][r] * inv : 0.0f;
-    unsigned again = rows_without_number(no_number(o) && mine);
-    const bool whole = mine && !(again >> li & 1);
-    if (p.lse && whole && g == 0) p.lse[(int64_t)h * p.Tq + qrow] = seen ? m + __log2f(l) : INFINITY;
-    if (whole) store_values((float *)p.o + ((int64_t)qrow * p.H + h) * D, g, D, vec_out, o, 1.0f);
-    for (; again; again &= again - 1) row_forward<float>(p, s, q0 + __builtin_ctz(again), h);
+    unsigned again = rows_without_number(no_number(o) && mine && l == l);   // (see packed_fwd)
+    const unsigned none = rows_without_number(mine && seen && l == 0.0f);
+    if (p.lse && mine && g == 0) p.lse[(int64_t)h * p.Tq + qrow] = seen ? m + __log2f(l) : INFINITY;
+    if (mine) store_values((float *)p.o + ((int64_t)qrow * p.H + h) * D, g, D, vec_out, o, 1.0f);
+    if (!again) return;
+    const EvoPacked late = parameters_again();
+    const int end = min(s.nk(), (wave_most + F::STAGE - 1) / F::STAGE * F::STAGE);
+    if (!spoilt_forward<float>(late, s, hk, active ? s.seen(q0, late.causal) : 0, end)) again = none;
+    wait_loads();
+    for (; again; again &= again - 1) {
+        const int b = __builtin_ctz(again), i = q0 + b;
+        if ((none >> b & 1) || !all_finite<float>(late.v, late.v_stride_t, hk, late.v_stride_h, s.k0 + s.seen(i, late.causal), s.k0 + end, late.D)) row_forward<float>(late, s, i, h);
+    }
 }
 
 // A sequence's few queries: one wave takes a part of its keys, and the queries of all heads that share a key head are the columns (32 after 32 of them).  A wave has the LDS and the registers of its
@@ -285,9 +293,13 @@ __global__ void __launch_bounds__(256) packed_f32_join(EvoPacked p, Parts parts,
     const float inv = sees ? 1.0f / L : 0.0f;
     o.a *= inv;
     o.b *= inv;
-    if (__any(!(o.a == o.a) || !(o.b == o.b))) {
-        row_forward<float>(p, s, i, h);
-        return;
+    if (__any(!(o.a == o.a) || !(o.b == o.b)) && L == L) {
+        const EvoPacked late = parameters_again();
+        const int seen = s.seen(i, late.causal);
+        if (L == 0.0f || spoilt_forward<float>(late, s, h / (late.H / late.Hk), seen, min(s.nk(), seen + 62))) {   // (what other rows of a wave see, and the end of a stage)
+            row_forward<float, 4>(late, s, i, h);
+            return;
+        }
     }
     store_row((float *)p.o + ((int64_t)i * p.H + h) * p.D, o, p.D);
     if (p.lse && lane == 0) p.lse[(int64_t)h * p.Tq + i] = sees ? M + __log2f(L) : INFINITY;
@@ -377,11 +389,16 @@ __global__ void __launch_bounds__(256, EVO_D <= 64 ? 2 : 1) packed_f32_dq(EvoPac
         if (mine) store_values(parts.o + (((int64_t)part * p.Tq + qrow) * p.H + h) * EVO_D, g, EVO_D, true, dq, 1.0f);
         return;
     }
-    unsigned again = rows_without_number(no_number(dq) && mine);
-    if (mine && !(again >> li & 1)) store_values((float *)p.dq + ((int64_t)qrow * p.H + h) * D, g, D, vec_out, dq, p.scale);
+    unsigned again = rows_without_number(no_number(dq) && mine && lse == lse && delta == delta);   // (of a NaN among them every dS is one)
+    if (mine) store_values((float *)p.dq + ((int64_t)qrow * p.H + h) * D, g, D, vec_out, dq, p.scale);
+    if (!again) return;
+    const EvoPacked late = parameters_again();
+    const int end = min(s.nk(), (wave_most + F::STAGE - 1) / F::STAGE * F::STAGE);
+    if (!spoilt_dq<float>(late, s, hk, wave_least, end)) return;
+    wait_loads();
     for (; again; again &= again - 1) {
-        const int b = __builtin_ctz(again);
-        row_dq<float>(p, s, q0 + b, h, lane_value(delta, b));
+        const int b = __builtin_ctz(again), i = q0 + b;
+        if (spoilt_dq<float>(late, s, hk, s.seen(i, late.causal), end)) row_dq<float>(late, s, i, h, lane_value(delta, b));
     }
 }
 
@@ -487,12 +504,20 @@ __global__ void __launch_bounds__(256, EVO_D <= 64 ? 2 : 1) packed_f32_dkdv(EvoP
         return;
     }
     unsigned again = rows_without_number((no_number(dk) || no_number(dv)) && mine);
-    if (mine && !(again >> li & 1)) {
+    if (mine) {
         const int64_t row = ((int64_t)krow * p.Hk + hk) * D;
         store_values((float *)p.dk + row, g, D, vec_out, dk, p.scale);
         store_values((float *)p.dv + row, g, D, vec_out, dv, 1.0f);
     }
-    for (; again; again &= again - 1) row_dkdv<float>(p, s, k0 + __builtin_ctz(again), hk, saved.delta);
+    if (!again) return;
+    const EvoPacked late = parameters_again();
+    const int least = max(begin, wave_from - 31);
+    if (!spoilt_dkdv<float>(late, s, hk, k0, min(k0 + 32, s.k1), least, wave_to, saved.delta)) return;
+    wait_loads();
+    for (; again; again &= again - 1) {
+        const int j = k0 + __builtin_ctz(again);
+        if (spoilt_dkdv<float>(late, s, hk, j, j + 1, least, s.first_query(j, late.causal), saved.delta)) row_dkdv<float>(late, s, j, hk, saved.delta);
+    }
 }
 
 // The parts of a row of dQ (KEYS: dK and dV) added up, in their order, by a wave.
@@ -512,8 +537,20 @@ __global__ void __launch_bounds__(256) packed_f32_sum(EvoPacked p, BackwardRows 
         store_row((float *)(y ? p.dv : KEYS ? p.dk : p.dq) + (int64_t)row * p.D, y ? sum[y] : Row{sum[y].a * p.scale, sum[y].b * p.scale}, p.D);
     }
     if (!__any(nan)) return;
-    if constexpr (KEYS) row_dkdv<float>(p, s, i, h, saved.delta);
-    else row_dq<float>(p, s, i, h, -saved.delta[(int64_t)h * p.Tq + i]);
+    const EvoPacked late = parameters_again();
+    // (what other rows of a wave see, and the end of a stage)
+    if constexpr (KEYS) {
+        const int from = s.first_query(i, late.causal);
+        if (!spoilt_dkdv<float>(late, s, h, i, i + 1, max(s.q0, from - 62), from, saved.delta)) return;
+        wait_loads();   // (for what has been stored, too: it is overwritten)
+        row_dkdv<float, 4>(late, s, i, h, saved.delta);
+    } else {
+        const int64_t at = (int64_t)h * late.Tq + i;
+        const int seen = s.seen(i, late.causal);
+        if (!(late.lse[at] == late.lse[at]) || !(saved.delta[at] == saved.delta[at]) || !spoilt_dq<float>(late, s, h / (late.H / late.Hk), seen, min(s.nk(), seen + 62))) return;
+        wait_loads();
+        row_dq<float, 4>(late, s, i, h, -saved.delta[at]);
+    }
 }
 
 // Parts of the keys of few queries: as many as make 16 waves to a CU, which has room for four at once (sequences differ in length), of two stages of an average sequence at least.

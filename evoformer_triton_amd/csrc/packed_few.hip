@@ -73,6 +73,7 @@ __global__ void __launch_bounds__(NW * 64) packed_few(EvoPacked p, Parts parts) 
     for (int i = 0; i < 8; ++i) one[i] = (T)1.0f;
     const float c = p.scale * kLog2e;
 
+    bool nan = false, none = false;   // (this thread has met): what is no number beside a sum of probabilities that is one; a sum of zero: every score lies below what the maximum begins with
     for (int64_t r0 = 0; r0 < rows; r0 += Few::ROWS) {
         // this lane's columns: a query and a head each
         int seen[CT];
@@ -184,7 +185,6 @@ __global__ void __launch_bounds__(NW * 64) packed_few(EvoPacked p, Parts parts) 
             }
         }
         __syncthreads();
-        bool nan = false;
         for (int jr = threadIdx.x / (EVO_D / 4), d = threadIdx.x % (EVO_D / 4) * 4; jr < Few::ROWS && r0 + jr < rows; jr += NW * 64 / (EVO_D / 4)) {
             float M = kMaskFloor, L = 0.0f;
 #pragma unroll 4
@@ -211,17 +211,26 @@ __global__ void __launch_bounds__(NW * 64) packed_few(EvoPacked p, Parts parts) 
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     sum[y] = sees ? sum[y] * inv : 0.0f;
-                    nan |= d < D && !(sum[y] == sum[y]);
+                    nan |= d < D && !(sum[y] == sum[y]) && L == L;
                 }
+                none |= sees && L == 0.0f;
                 if (d < D) store4<T>((T *)p.o + row * D + d, sum[0], sum[1], sum[2], sum[3]);
                 if (d < D && p.o_low) store4<T>((T *)p.o_low + row * D + d, left<T>(sum[0]), left<T>(sum[1]), left<T>(sum[2]), left<T>(sum[3]));
                 if (d == 0 && p.lse) p.lse[(int64_t)oh * p.Tq + oi] = sees ? M + __log2f(L) : INFINITY;
             }
         }
-        const bool again = __syncthreads_or(!PART && nan);
-        if (again) {   // some row holds something that is no number: all of them once more, with the rows that are seen alone
-            for (int x = wave; x < Few::ROWS && r0 + x < rows; x += Few::WAVES)
-                row_forward<T>(p, s, s.q0 + (int)((r0 + x) / group), hk * group + (int)((r0 + x) % group));
+        __syncthreads();
+    }
+    if constexpr (!PART) {
+        if (!__syncthreads_or(nan || none)) return;
+        // Some row holds something that is no number, perhaps because of keys that it does not see
+        const bool below = __syncthreads_or(none);
+        wait_loads();
+        const EvoPacked late = parameters_again();
+        for (int64_t x = wave; x < rows; x += Few::WAVES) {
+            const int i = s.q0 + (int)(x / group), h = hk * group + (int)(x % group), seen = s.seen(i, late.causal);
+            if (seen == 0 || all_finite<T>(late.o, (int64_t)late.H * late.D, h, late.D, i, i + 1, late.D)) continue;
+            if (below || spoilt_forward<T>(late, s, hk, seen, nk)) row_forward<T>(late, s, i, h);
         }
     }
 }
@@ -271,9 +280,14 @@ __global__ void __launch_bounds__(PER > 4 ? PER * 64 : 256) packed_join(EvoPacke
     a = sees ? a * inv : 0.0f;
     b = sees ? b * inv : 0.0f;
     const bool used = lane * 2 < D;
-    if (__any(used && (!(a == a) || !(b == b)))) {
-        row_forward<T>(p, s, i, h);
-        return;
+    if (__any(used && (!(a == a) || !(b == b))) && L == L) {
+        // (keys that are not seen: of a chunk all of them, else what other rows of a wave see, and the end of a stage)
+        const EvoPacked late = parameters_again();
+        const int seen = s.seen(i, late.causal), end = parts.chunk ? s.nk() : min(s.nk(), seen + 31 + 63);
+        if (L == 0.0f || spoilt_forward<T>(late, s, h / (late.H / late.Hk), seen, end)) {
+            row_forward<T, 4>(late, s, i, h);
+            return;
+        }
     }
     if (used) {
         T *out = (T *)p.o + ((int64_t)i * p.H + h) * D + lane * 2;

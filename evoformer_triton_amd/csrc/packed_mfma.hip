@@ -21,7 +21,7 @@
 // causal mask have the longest walks, begin first; of few long sequences all of them by their walks (place_of).
 //
 // A row of V beyond the sequence's end is read as zeros (the load is out of range).  One that causal queries do not see may hold an infinity or a NaN, which a probability of
-// zero does not keep out of the sums: results that are no numbers are formed anew, row by row (row_forward and its like), with the rows that are seen alone.
+// zero does not keep out of the sums: results that may be no numbers because of such a row are formed anew, row by row (packed_common.h).
 #include "packed_tiles.h"
 
 namespace evo {
@@ -206,21 +206,30 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D == 32 ? 4 : EVO_
             o[dt][r] = seen ? o[dt][r] * inv : 0.0f;
             nan |= !(o[dt][r] == o[dt][r]);
         }
-    unsigned again = rows_without_number(nan && mine);
-    const bool whole = mine && !(again >> li & 1);
-    if (p.lse && whole && g == 0) p.lse[(int64_t)h * p.Tq + qrow] = seen ? m + __log2f(l) : INFINITY;
+    // (a sum of zero: every score lies below what the maximum begins with)
+    unsigned again = rows_without_number(nan && mine && l == l);
+    const unsigned none = rows_without_number(mine && seen && l == 0.0f);
+    if (p.lse && mine && g == 0) p.lse[(int64_t)h * p.Tq + qrow] = seen ? m + __log2f(l) : INFINITY;
     const int64_t row = ((int64_t)qrow * p.H + h) * D;
 #pragma unroll
-    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>((T *)p.o + row, dt * 32, whole ? D : 0, o[dt], 1.0f, g);
+    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>((T *)p.o + row, dt * 32, mine ? D : 0, o[dt], 1.0f, g);
     if (p.o_low) {
 #pragma unroll
         for (int dt = 0; dt < R::DT; ++dt) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[dt][r] = left<T>(o[dt][r]);
-            store_row_tile<T>((T *)p.o_low + row, dt * 32, whole ? D : 0, o[dt], 1.0f, g);
+            store_row_tile<T>((T *)p.o_low + row, dt * 32, mine ? D : 0, o[dt], 1.0f, g);
         }
     }
-    for (; again; again &= again - 1) row_forward<T>(p, s, q0 + __builtin_ctz(again), h);
+    if (!again) return;
+    const EvoPacked late = parameters_again();
+    const int end = min(s.nk(), (wave_most + R::STAGE - 1) / R::STAGE * R::STAGE);
+    if (!spoilt_forward<T>(late, s, hk, wave_least, end)) again = none;
+    wait_loads();   // (and for what has been stored, of which some is overwritten)
+    for (; again; again &= again - 1) {
+        const int b = __builtin_ctz(again), i = q0 + b;
+        if ((none >> b & 1) || !all_finite<T>(late.v, late.v_stride_t, hk, late.v_stride_h, s.k0 + s.seen(i, late.causal), s.k0 + end, late.D)) row_forward<T>(late, s, i, h);
+    }
 }
 
 // ------------------------------------------------------------------ dQ
@@ -406,14 +415,20 @@ __global__ void __launch_bounds__(KG * 256, KG == 2 ? 2 : EVO_D <= 64 ? 3 : 2) p
     for (int dt = 0; dt < R::DT; ++dt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) nan |= !(dq[dt][r] == dq[dt][r]);
-    unsigned again = rows_without_number(nan && mine);
-    const bool whole = mine && !(again >> li & 1);
+    // (an infinite dS has no second value)
+    unsigned again = rows_without_number(nan && mine && rest[0] == rest[0]);
+    const unsigned infinite = rows_without_number(mine && fabsf(rest[0]) == INFINITY) & again;
     T *out = (T *)p.dq + ((int64_t)qrow * p.H + h) * D;
 #pragma unroll
-    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>(out, dt * 32, whole ? D : 0, dq[dt], p.scale * inv, g);
+    for (int dt = 0; dt < R::DT; ++dt) store_row_tile<T>(out, dt * 32, mine ? D : 0, dq[dt], p.scale * inv, g);
+    if (!again) return;
+    const EvoPacked late = parameters_again();
+    const int end = min(s.nk(), (wave_most + 31) / 32 * 32);
+    if (!spoilt_dq<T>(late, s, hk, wave_least, end)) again = infinite;
+    wait_loads();   // (see packed_fwd)
     for (; again; again &= again - 1) {
-        const int b = __builtin_ctz(again);
-        row_dq<T>(p, s, q0 + b, h, lane_value(dl, b));
+        const int b = __builtin_ctz(again), i = q0 + b;
+        if ((infinite >> b & 1) || spoilt_dq<T>(late, s, hk, s.seen(i, late.causal), end)) row_dq<T>(late, s, i, h, lane_value(dl, b));
     }
 }
 

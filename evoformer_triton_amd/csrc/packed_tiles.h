@@ -300,14 +300,24 @@ __global__ void __launch_bounds__(256) packed_sum(EvoPacked p, BackwardRows save
         }
         if (lane == 0 && any) save_row(saved, at, p.lse[at], delta, total, rest, c);
         scale = any ? scale / total : 0.0f;
-        if (__any(nan)) {
-            row_dq<T>(p, s, i, h, delta);
-            return;
+        if (__any(nan) && rest == rest) {
+            const EvoPacked late = parameters_again();
+            const int seen = s.seen(i, late.causal);
+            if (!finite(rest) || spoilt_dq<T>(late, s, h / (late.H / late.Hk), seen, min(s.nk(), seen + 62))) {   // (what other rows of a wave see, and the end of a step)
+                row_dq<T, 4>(late, s, i, h, delta);
+                return;
+            }
         }
     }
-    if (__any(nan)) {
-        if constexpr (KEYS) row_dkdv<T>(p, s, i, h, saved.delta);
-        return;
+    if constexpr (KEYS) {
+        if (__any(nan)) {
+            const EvoPacked late = parameters_again();
+            const int from = s.first_query(i, late.causal);
+            if (spoilt_dkdv<T>(late, s, h, i, i + 1, max(s.q0, from - 62), from, saved.delta)) {
+                row_dkdv<T, 4>(late, s, i, h, saved.delta);
+                return;
+            }
+        }
     }
     if (lane * 2 >= D) return;
 #pragma unroll
