@@ -1,8 +1,9 @@
 """Oracle of attention within packed sequences: TEST INFRASTRUCTURE, not product code.
 
 The formula in 64 bits, sequence by sequence and head by head, its gradients, and for each result how far it may lie from that when it is formed as the kernels say:
-scores, exponentials and sums in fp32, probabilities and the scores' gradients rounded to the inputs' type where they multiply values, keys and queries,
-delta = sum of dout times the rounded output, results rounded once.
+scores, exponentials and sums in fp32, probabilities and the scores' gradients rounded to the inputs' type where they multiply values, keys and queries, results rounded once.
+Worst cases, added up: delta is allowed the output's whole bound, though the kernels form it of the output and of what rounding left of it, and dQ one rounding of the scores' gradients, which multiply
+keys as two values.  How much nearer these bring the gradients is held by norms (tests/test_gpu_packed_gradients.py).
 """
 from __future__ import annotations
 

@@ -77,3 +77,33 @@ def test_small_and_large_gradients_keep_their_bits(gpu_device, dtype, size, shap
         a, want = a[fits], want[fits]
         off, rounded = (a.double() - want).norm(), (want.to(dtype).double() - want).norm()
         assert off <= most * rounded, f"{name}: {float(off / rounded):.3f} times the error of the exact gradient rounded"
+
+
+def _near(got, want, most, dtype, name):
+    off, rounded = (got.double() - want).norm(), (want.to(dtype).double() - want).norm()
+    assert off <= most * rounded, f"{name}: {float(off / rounded):.3f} times the error of the exact result rounded"
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "-".join(str(x).replace(" ", "") for x in (len(s[0]), s[0][0], *s[1:])))
+def test_sharp_scores_keep_theirs(gpu_device, dtype, shape):
+    """Where few keys have most of the probability, what rounding leaves of the output, dS as two values and the sums' corrections decide: without one of them dQ or dK is beyond these bounds (test_packed_precision.py)."""
+    from evoformer_triton_amd import packed_attention
+    lengths, H, Hk, D, causal = shape
+    q, k, v, dout = _inputs(dtype, lengths, H, Hk, D, 1.0, sharp=6.0)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    got = torch.autograd.grad(packed_attention(*leaves, _off(lengths), causal=causal), leaves, dout)
+    for name, a, want, most in zip(("dq", "dk", "dv"), got, _exact(*(t.detach() for t in leaves), dout, lengths, causal)[1:], (1.3, 1.65, 1.65)):
+        _near(a, want, most, dtype, name)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("shape", SHAPES + [([5] * 40, 8, 2, 64, True)], ids=lambda s: "-".join(str(x).replace(" ", "") for x in (len(s[0]), s[0][0], *s[1:])))
+def test_what_rounding_left_of_the_output(gpu_device, dtype, shape):
+    """It is at most half a step, and with it the output is off by what the rounded probabilities leave alone: as much as one rounding (their errors are as large as the output's, value by value), where without it there are
+    two, sqrt(2) times that.  15 in a hundred for how values lie between two powers of two."""
+    lengths, H, Hk, D, causal = shape
+    q, k, v, dout = _inputs(dtype, lengths, H, Hk, D, 1.0)
+    o, _, left = torch.ops.evoattn.packed(q, k, v, _off(lengths), None, causal, None)
+    assert (left.double().abs() <= torch.finfo(dtype).eps / 2 * o.double().abs() + torch.finfo(dtype).tiny * torch.finfo(dtype).eps).all()
+    _near(o.double() + left.double(), _exact(q, k, v, dout, lengths, causal)[0], 1.15, dtype, "o and what is left")
