@@ -7,6 +7,7 @@ here, for any head dim and without an N x N array.  The reference takes its quer
 from __future__ import annotations
 
 import math
+from decimal import Decimal, localcontext
 from typing import Optional, Tuple, Union
 
 import torch
@@ -14,6 +15,18 @@ from torch import nn
 
 from . import _lib
 from ._transforms import refuse_tangents
+
+
+def _pi() -> Decimal:
+    """To the current context's digits: 16 atan(1/5) - 4 atan(1/239) by their series."""
+    def atan_of_one_over(n):
+        total, term, k = Decimal(0), Decimal(1) / n, 1
+        while total + term / k != total:
+            total += term / k if k % 4 == 1 else -term / k
+            term, k = term / (n * n), k + 2
+        return total
+
+    return 16 * atan_of_one_over(5) - 4 * atan_of_one_over(239)
 
 
 def rotary_turns(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[str] = None, factor: float = 1.0, original_length: Optional[int] = None,
@@ -24,7 +37,8 @@ def rotary_turns(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[st
       "linear"  every frequency divided by the factor
       "base"    the base times factor^(rotary_dim / (rotary_dim - 2)): the slowest pair's frequency divided by the factor, the fastest's kept
       "parts"   by the turns r that a pair makes over `original_length` positions: kept from r = fast on, divided by the factor up to r = slow,
-                in between blended by (r - slow) / (fast - slow)"""
+                in between blended by (r - slow) / (fast - slow)
+    Formed with as many digits as the whole numbers have (in doubles the fastest pairs would be off by 2^-56 of a turn per position)."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and at least 2, got {rotary_dim}")
     if not (math.isfinite(base) and base > 0.0):
@@ -35,22 +49,28 @@ def rotary_turns(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[st
         raise ValueError(f'scaling must be "linear", "base" or "parts", got {scaling!r}')
     if scaling is None and factor != 1.0:
         raise ValueError("a factor needs a scaling")
-    if scaling == "base":
-        if rotary_dim == 2:
-            raise ValueError('scaling "base" needs more than one pair')
-        base *= factor ** (rotary_dim / (rotary_dim - 2))
-    radians = [base ** (-2.0 * i / rotary_dim) for i in range(rotary_dim // 2)]
-    if scaling == "linear":
-        radians = [x / factor for x in radians]
-    elif scaling == "parts":
+    if scaling == "base" and rotary_dim == 2:
+        raise ValueError('scaling "base" needs more than one pair')
+    if scaling == "parts":
         if original_length is None or original_length < 1:
             raise ValueError('scaling "parts" needs original_length, the positions that the frequencies were trained on')
-        if not fast > slow:
-            raise ValueError(f"fast must be above slow, got {fast} and {slow}")
-        kept = [min(1.0, max(0.0, (original_length * x / (2.0 * math.pi) - slow) / (fast - slow))) for x in radians]
-        radians = [x * (w + (1.0 - w) / factor) for x, w in zip(radians, kept)]
-    # (modulo a turn, which positions in whole numbers do not notice; as a signed number of the same 64 bits)
-    whole = [round(math.fmod(x / (2.0 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for x in radians]
+        if not (fast > slow and math.isfinite(slow)):
+            raise ValueError(f"fast must be above slow, a number, got {fast} and {slow}")
+    with localcontext() as context:
+        # (64 bits behind the point, as many digits before it as bases and factors below one make, and some for what is lost on the way)
+        context.prec = 50 + math.ceil(max(0.0, -math.log10(base)) + 3.0 * max(0.0, -math.log10(factor)))
+        turn, factor, slow, fast = 2 * _pi(), Decimal(float(factor)), Decimal(float(slow)), Decimal(float(fast))
+        log_base = Decimal(float(base)).ln()
+        if scaling == "base":
+            log_base += factor.ln() * rotary_dim / (rotary_dim - 2)
+        turns = [(log_base * (-2 * i) / rotary_dim).exp() / turn for i in range(rotary_dim // 2)]
+        if scaling == "linear":
+            turns = [x / factor for x in turns]
+        elif scaling == "parts":
+            kept = [min(Decimal(1), max(Decimal(0), (Decimal(float(original_length)) * x - slow) / (fast - slow))) for x in turns]
+            turns = [x * (w + (1 - w) / factor) for x, w in zip(turns, kept)]
+        whole = [int((x * 2 ** 64).to_integral_value()) % 2 ** 64 for x in turns]
+    # (modulo a turn, which positions in whole numbers do not notice; as signed numbers of the same 64 bits)
     return torch.tensor([w - (1 << 64) if w >> 63 else w for w in whole], dtype=torch.int64, device=device)
 
 
