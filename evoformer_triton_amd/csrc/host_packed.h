@@ -5,16 +5,24 @@ struct Packed {
     Tensor q, k, v, offsets, key_offsets;   // as the kernels read them
     int64_t D = 0;                          // the head dim; p.D in 16 bits: with the zeros behind it
 
+    static constexpr int64_t most_apart = 1 << 23;   // values from one row to the next, in 16 bits
     // [T, heads, D] with the strides, the alignment and the columns that the kernels take
     static Tensor ready(const Tensor &t, int64_t Dp) {
         const bool wide = t.scalar_type() == at::kFloat;
-        if (t.size(2) != Dp) return at::constant_pad_nd(t, {0, Dp - t.size(2)});
+        // (a copy: row by row, or head by head where rows of all heads would lie too far apart)
+        const bool by_heads = !wide && t.size(1) * Dp >= most_apart;
+        if (t.size(2) != Dp) return by_heads ? at::constant_pad_nd(t.transpose(0, 1).contiguous(), {0, Dp - t.size(2)}).transpose(0, 1) : at::constant_pad_nd(t, {0, Dp - t.size(2)});
         if (!t.numel()) return t;
         int64_t st, sh;
         stride(t, st, sh);
         // (rows of 16 bits lie apart, so that what is beyond a sequence is out of range)
-        const bool taken = (t.stride(2) == 1 || t.size(2) == 1) && (wide || (st >= Dp && st % 8 == 0 && sh % 8 == 0 && st < 1 << 23 && (uintptr_t)t.data_ptr() % 16 == 0));
-        return taken ? t : t.clone(at::MemoryFormat::Contiguous);
+        const bool taken = (t.stride(2) == 1 || t.size(2) == 1) && (wide || (st >= Dp && st % 8 == 0 && sh % 8 == 0 && st < most_apart && (uintptr_t)t.data_ptr() % 16 == 0));
+        return taken ? t : by_heads ? t.transpose(0, 1).clone(at::MemoryFormat::Contiguous).transpose(0, 1) : t.clone(at::MemoryFormat::Contiguous);
+    }
+    // [T, heads, Dp], dense, whatever there is between two rows
+    static Tensor dense(const Tensor &t, int64_t Dp) {
+        if (t.size(2) != Dp) return at::constant_pad_nd(t.contiguous(), {0, Dp - t.size(2)});
+        return t.is_contiguous() && (uintptr_t)ptr_or_null(t) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
     }
     static void stride(const Tensor &t, int64_t &st, int64_t &sh) {
         st = t.size(0) > 1 ? t.stride(0) : t.size(2);
@@ -103,8 +111,7 @@ struct Packed {
         c10::DeviceGuard on(q.device());
         point();
         const Tensor dout = ready(dout_, p.D), lse = lse_.contiguous(), low = low_.contiguous();
-        Tensor o = ready(o_, p.D);
-        if (!o.is_contiguous()) o = o.contiguous();
+        const Tensor o = dense(o_, p.D);
         dq = at::empty({p.Tq, p.H, p.D}, q.options());
         if (need_kv) {
             dk = at::empty({p.Tk, p.Hk, p.D}, q.options());

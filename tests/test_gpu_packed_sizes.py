@@ -38,3 +38,25 @@ def test_as_many_workgroups_as_their_waves_allow(gpu_device):
     q = torch.zeros(n, H, D, device=gpu_device, dtype=torch.float16)
     v = torch.randn(n, H, D, device=gpu_device).half()
     assert torch.equal(packed_attention(q, q, v, torch.arange(n + 1, device=gpu_device)), v)
+
+
+@pytest.mark.parametrize("T,H,Hk,D,far", [(3, 2 ** 16, 2 ** 16, 128, False), (40, 2 ** 16, 2 ** 15, 128, False), (6, 2 ** 17, 2 ** 17, 61, True)])
+def test_more_heads_than_rows_lie_apart(gpu_device, T, H, Hk, D, far):
+    """Rows of 2^23 values in 16 bits and more, which the kernels take head by head; the first heads, the last and some between against the formula, with their gradients."""
+    from evoformer_triton_amd import packed_attention
+    from oracle.packed import packed
+    g = torch.Generator(device=gpu_device).manual_seed(8)
+    q, k, v, dout = (torch.randn(T, h, D, device=gpu_device, generator=g).to(torch.bfloat16) for h in (H, Hk, Hk, H))
+    if far:
+        q = torch.cat([q, q], 1)[:, :H]                 # (a slice: rows twice as far apart)
+    at = [0, T // 2, T]
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = packed_attention(*leaves, torch.tensor(at, device=gpu_device))
+    got = [out, *torch.autograd.grad(out, leaves, dout)]
+    G = H // Hk
+    for hk in (0, Hk // 2, Hk - 1):
+        heads = slice(hk * G, (hk + 1) * G), slice(hk, hk + 1)
+        parts = [t.detach()[:, heads[i]] for t, i in ((q, 0), (k, 1), (v, 1))]
+        want, bound = packed(*parts, at, at, True, D ** -0.5, dout[:, heads[0]])
+        for name, a, w, b, i in zip(("o", "dq", "dk", "dv"), got, want, bound, (0, 0, 1, 1)):
+            assert a.shape[1] == (H, Hk)[i] and ((a[:, heads[i]].double() - w).abs() <= b).all(), name
