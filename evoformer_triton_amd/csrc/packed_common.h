@@ -287,7 +287,7 @@ __device__ __forceinline__ void row_forward(const EvoPacked &p, const Segment &s
     o.a *= inv;
     o.b *= inv;
     store_row((T *)p.o + ((int64_t)i * p.H + h) * p.D, o, p.D);
-    if (p.o_low) store_row((T *)p.o_low + ((int64_t)i * p.H + h) * p.D, Row{o.a - (float)(T)o.a, o.b - (float)(T)o.b}, p.D);
+    if (sizeof(T) == 2 && p.o_low) store_row((T *)p.o_low + ((int64_t)i * p.H + h) * p.D, Row{o.a - (float)(T)o.a, o.b - (float)(T)o.b}, p.D);
     if (p.lse && lane == 0) p.lse[(int64_t)h * p.Tq + i] = seen ? m + __log2f(l) : INFINITY;
 }
 

@@ -397,7 +397,7 @@ int evoattn_rotary(const EvoRotary *p, void *hip_stream);
  * offsets, key_offsets [n + 1], signed integers of offset_bytes (4 or 8): sequence s has queries offsets[s] .. offsets[s + 1] - 1 and keys likewise; ascending, within
  * [0, T] (others are brought there: no access is out of bounds, what such rows hold is not specified).  Rows of no sequence and rows that see no key get zeros, in o and in the gradients.
  *   lse  [H][Tq] fp32: log2 of the row's sum of 2^(scale log2(e) q . k), for the backward (+inf: no key); may be NULL in the forward
- *   o_low  16 bits: what rounding o to its type left of it, in its type and laid out like it, for the backward's sums of dout o (which end in every gradient of a row); may be NULL
+ *   o_low  16 bits: what rounding o to its type left of it, in its type and laid out like it, for the backward's sums of dout o (which end in every gradient of a row); may be NULL (fp32: not written)
  *   dk, dv  both may be NULL (not wanted)
  * D at most 128; scale 2^-64 to 2^64.  16-bit: D and all strides multiples of 8, pointers on 16-byte boundaries, row strides from D to 2^23 (EVO_EALIGN
  * otherwise).  `workspace` of evoattn_packed_fwd_workspace_bytes() (0: none needed) and evoattn_packed_bwd_workspace_bytes(), on a 16-byte boundary.  The backward is
