@@ -27,12 +27,21 @@ EVO_PACKED(128)
 #define EVO_BY_HEAD_DIM(name, p, ...) \
     ((p).D <= 32 ? name##_d32(__VA_ARGS__) : (p).D <= 64 ? name##_d64(__VA_ARGS__) : (p).D <= 96 ? name##_d96(__VA_ARGS__) : name##_d128(__VA_ARGS__))
 
-// Whether the kernels that split the keys of few queries serve the forward: by the average of a sequence's queries times the query heads that share a key head, which are columns there.
-//   16 sequences of 4096 keys, 32 heads (8), D = 128, bf16: 72 us with 32 columns (here the other kernel: 137), 195 with 128 (164); 16 of 1024, 8 heads (8), D = 64: 15 with 16 (16), 21 with 32 (17), 38
-//   with 64 (17); one of 4096, 16 heads (4), D = 128: 16 with 32 (19), 26 with 64 (19).  fp32: 286 with 64 (698) and 528 with 128 (790); 50 with 64 (55) and 90 with 128 (73); 36 (54) and 61 (56).
-// (In fp32 a launch with a wave to a row joins their parts, one of them too.)
+// Whether the kernels that split the keys of few queries serve the forward: by what an average sequence has of queries times the query heads that share a key head (`columns` there), of keys, and by sequences times key
+// heads (`units`).  Measured with 1, 4, 16 and 256 sequences of 32 to 65536 keys (us; the tiled kernel in brackets):
+//   16 bits.  Up to 16 columns: 32 heads (8) of 64, one query, 256 sequences of 128 keys 18 (55), of 1024 164 (298), 16 of 1024 14 (28); 8 heads (8): 16 of 1024 keys 14 (16), of 256 keys 14.6 (12.6); least favourable, one sequence of 32 keys 8.1 (6.3).  17 to 32, which are
+//   multiplied in two halves: with shared heads, which a tile reads again for each, 256 of 128 keys 21 (55) and 16 of 4096 41 (75), but 16 of 512 27 (19); with heads of their own one of 1024 keys 13.3 (15.1), 16 of
+//   1024 22 (16), 1000 of 32 282 (226; of D = 128).
+//   fp32.  A second launch makes the results, a wave to each row.  8 heads (8) of 64, 8 queries: 1000 sequences of 8 keys 69 (84), 256 of 64 34 (39), of 1024 246 (365); 32 queries: 60 (44) and 287 (374); 64 queries: 100 (56) and 562 (538).  One sequence of 64 keys
+//   14.3 (10.9), of 1024 14.7 (18.9).  32 heads (8) of 128, 16 queries: one of 1024 keys 34 (28), of 4096 43 (59), 4 of 1024 42 (65).
 static bool few_queries(const EvoPacked &p) {
-    return p.n && p.Tq * (p.H / p.Hk) <= (int64_t)(p.dtype == EVO_F32 ? 64 : 32) * p.n && (p.dtype != EVO_F32 || row_waves_fit(p.Tq * p.H));
+    const int64_t n = p.n, group = p.H / p.Hk, columns = p.Tq * group, units = n * p.Hk;   // (columns, and keys, of all sequences)
+    if (!n) return false;
+    if (p.dtype != EVO_F32) return columns <= 16 * n || (columns <= 32 * n && p.Tk >= 1024 * n && (group > 1 || units < 128)) || (columns <= 32 * n && group > 1 && units >= 512);
+    if (columns > 64 * n || 512 * p.Tq > (p.Tk > 64 * n ? p.Tk : 64 * n) * group * p.D) return false;   // (each row's way through memory, beside what its keys take)
+    if (units < 512 && p.Tk < 128 * n) return false;
+    if (units < 32 && columns > 32 * n && p.Tk < 4096 * n) return false;
+    return row_waves_fit(p.Tq * p.H);
 }
 
 static int64_t align_rows(int64_t n) { return (n + 63) / 64 * 64; }   // (16-byte pieces behind them)

@@ -103,7 +103,9 @@ __device__ __forceinline__ Place place_of(const EvoPacked &p, int rank, int tile
     // tiles as are behind it and its own: of c_j tiles of sequence j max(0, c_j - w) have walks longer than w, and the rank is that of walks of w where the sum of these reaches it.  Without a mask all of a
     // sequence's tiles have the same walk.  4 x 4096 causal rows, 32 heads (8) of 128: dK and dV 1.19 ms (1.34 with one sequence after the other), forward 0.635 (0.66), dQ 1.08 (1.06: more sequences' keys
     // at once in an L2).  Seven causal sequences of 5 tiles on average: forward 34.0 us (35.1); 16 of 3: with gradients 88 (99); 40 of one: 9 (7), the search takes longer than it
-    // gains.  24 chains of 51 to 768 rows without a mask, 8 heads of 32: forward 16.1 us (19.2), dQ 24.7 (31.1), of 64: 17 (22); 60 of 100 to 1000 with 32 heads: 218 (177), hence not for so many.
+    // gains.  24 chains of 51 to 768 rows without a mask, 8 heads of 32: forward 16.1 us (19.2), dQ 24.7 (31.1), of 64: 17 (22); 60 of 100 to 1000 with 32 heads: 218 (177), hence not for so many.  Where it turns, by sequences of
+    // 100 to 1400 rows, with gradients, causal: 8 heads of 32: 16 87 us (109), 29 103 (116), 45 141 (149), 60 188 (174); 32 heads (8) of 64: 8 178 (209), 29 409 (434), 36 508 (513), 45 629 (622); 16 heads of 128: 16 238 (264),
+    // 24 354 (357), 29 430 (425), 36 532 (513).  Without a mask the same within 3 in a hundred.
     if (p.n < 30 && (KEYS ? p.Tk : p.Tq) >= (int64_t)2 * kPackedRows * p.n) {
         const int lane = threadIdx.x & 63, x = min(lane, p.n + 2), q = queries_begin(p, x), k = keys_begin(p, x);
         const int nq = max(0, __shfl_down(q, 1) - q), nk = max(0, __shfl_down(k, 1) - k), own = lane < p.n + 2 ? ((KEYS ? nk : nq) + kPackedRows - 1) / kPackedRows : 0;

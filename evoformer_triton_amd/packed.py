@@ -30,7 +30,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     as two values); for the backward the call keeps, beside its inputs, the output, what rounding left of it, and a number for each row and head.  Gradients: q, k and v, the same bits with every call.
 
     Room that a cache leaves between its sequences is a sequence without queries: offsets [0, 1, 1, 2, 2], key_offsets [0, n0, room, room + n1, 2 room].  Calls whose sequences have few queries each
-    (by the average of queries times H / Hk) and others are served by different kernels: prompts and single tokens are best in calls of their own.
+    (by the averages of queries times H / Hk and of keys) and others are served by different kernels: prompts and single tokens are best in calls of their own.
 
     The offsets' values are not looked at on the host (no synchronisation): where they are not ascending, results are not specified.  Runs on the current stream of the tensors' device; GPU only."""
     for name, t in (("q", q), ("k", k), ("v", v), ("offsets", offsets), ("key_offsets", key_offsets)):

@@ -17,11 +17,12 @@ def test_more_rows_in_fp32_than_a_join_holds(gpu_device):
     assert (packed_attention(q, k, v, off, koff, causal=False).view(n, each, H, D) == v[:, None]).all()
 
 
-def test_many_short_sequences_in_16_bits(gpu_device):
+@pytest.mark.parametrize("n,each", [(10000, 20), (10000, 16), (140000, 1)])
+def test_many_short_sequences_in_16_bits(gpu_device, n, each):
     """2^22 rows times heads and more, which no launch has a wave to: no parts are joined.  The sequences at both ends and in the middle against the formula."""
     from evoformer_triton_amd import packed_attention
     from oracle.packed import packed
-    n, each, H, D = 10000, 20, 32, 64
+    H, D = 32, 64
     g = torch.Generator(device=gpu_device).manual_seed(8)
     q, k, v = (torch.randn(n * each, H, D, device=gpu_device, generator=g).to(torch.bfloat16) for _ in range(3))
     out = packed_attention(q, k, v, torch.arange(0, n * each + 1, each, device=gpu_device))
