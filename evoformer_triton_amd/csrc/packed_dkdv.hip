@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
     f32x16 dk[R::DT], dv[R::DT];
 #pragma unroll
     for (int dt = 0; dt < R::DT; ++dt) dk[dt] = dv[dt] = filled(0.0f);
-    float up = kShiftKey;   // (kShifts: P, and with it dS, dK and dV, times 2^up)
+    float by = 0x1p17f;   // (kShifts: P, and with it dV, are times 2^kShiftKey, dS and dK times this too)
 
     const Staged staged(lane);
     auto step = [&](const unsigned char *buf, int qb, int row0) __attribute__((always_inline)) {
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
 #pragma unroll
         for (int ks = 0; ks < R::KSD; ++ks) d = Mfma<T>::mma(staged.rows<T>(dat, 0, ks), K::VLDS ? staged.rows<T>(vat, 0, ks) : vf[K::VLDS ? 0 : ks], d);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) a[r] = fast_exp2(kShifts<T> ? fmaf(a[r], c, up) : a[r] * c);
+        for (int r = 0; r < 16; ++r) a[r] = fast_exp2(kShifts<T> ? fmaf(a[r], c, (float)kShiftKey) : a[r] * c);
         if (row0 < wave_to) {   // (uniform)
             asm volatile("");
 #pragma unroll
@@ -122,15 +122,14 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
         }
         if constexpr (kShifts<T>) {
             d *= a;
+            d *= by;
             bool any;
             const int down = shift_down(d, any);
             if (__builtin_expect(any, 0)) {
-                const float by = ldexpf(1.0f, -down);
-                up -= (float)down;
-                a *= by;
-                d *= by;
-                shift_by(dk, by);
-                shift_by(dv, by);
+                const float more = ldexpf(1.0f, -down);
+                by *= more;
+                d *= more;
+                shift_by(dk, more);
             }
         }
         v8 pf[2], sf[2];
@@ -174,9 +173,9 @@ __global__ void __launch_bounds__(KG * 256, KG == 1 && EVO_D == 32 ? 3 : 2) pack
     }
     wait_loads();
     if constexpr (kShifts<T>) {
-        const float by = ldexpf(1.0f, -(int)up);
-        shift_by(dk, by);
-        shift_by(dv, by);
+        const float back = ldexpf(1.0f, -kShiftKey);
+        shift_by(dk, back / by);
+        shift_by(dv, back);
     }
     if constexpr (KG == 2) {
         float *const x = reinterpret_cast<float *>(lds) + own * R::DT * 16 * 64;

@@ -173,11 +173,11 @@ template <typename T>
 __device__ __forceinline__ float left(float v) { return v - (float)(T)v; }
 
 // fp16 in the backward.  Below 2^-14 it has fewer bits, below 2^-25 none, and above 65504 it is infinite, while dS = P (dP - delta) has gradients of any size in it and P as small a number as there are keys.  So a lane
-// forms P, and with it dS and its sums, times a power of two, which comes down, as the running maximum of a softmax goes up, where dS would pass kShiftTop, and is taken out of the sums at the end.  dQ's P is in fp32 and
-// begins at 2^kShiftQuery (an incoming gradient's smallest step, 2^-24, times 2^-17 is a dS of 2^-1 then); dV's is an operand, at most 2^kShiftKey (a score of up to 2^24, which fp32 leaves off by 2, still
-// has no infinite one), and so is dS's shift: a gradient of 2^-14 spread over 2^13 keys has all of its bits.  Errors of dQ, dK and dV next to the exact result rounded, 4096 rows of D = 64 without a mask, incoming gradients of
+// forms dS and its sums times a power of two, which comes down, as the running maximum of a softmax goes up, where dS would pass kShiftTop, and is taken out of the sums at the end.  For dQ, whose P stays in fp32, P has it, and
+// it begins at 2^kShiftQuery: an incoming gradient's smallest step, 2^-24, spread over 2^17 keys is a dS of 2^-1 then.  For dV P is an operand, times 2^kShiftKey always (a score of up to 2^24, which fp32 leaves off by
+// 2, still has no infinite one; of 2^27 keys alike each has bits), and dS's power is one beside it, 2^17 at first.  Errors of dQ, dK and dV next to the exact result rounded, 4096 rows of D = 64 without a mask, incoming gradients of
 // 1e-4: 8.0, 8.0 and 1.0 times without it, 1.0 for all three with it (tests/test_gpu_packed_gradients.py).  What it costs is looking for the largest of 16 values in each tile: 4 x 4096 causal rows, 32 heads (8) of 128,
-// forward and backward 2.88 ms instead of 2.79; twelve of 200 to 1500, 16 heads (4) of 64, 192 us instead of 184.  bf16 has fp32's exponents.
+// forward and backward 2.84 ms instead of 2.74; twelve of 200 to 1500, 16 heads (4) of 64, 194 us instead of 184.  bf16 has fp32's exponents.
 template <typename T> constexpr bool kShifts = std::is_same<T, f16_t>::value;
 constexpr int kShiftQuery = 40, kShiftKey = 13;
 constexpr float kShiftTop = 32768.0f;
