@@ -6,6 +6,7 @@ here, for any head dim and without an N x N array.  The reference takes its quer
 """
 from __future__ import annotations
 
+import functools
 import math
 from decimal import Decimal, localcontext
 from typing import Optional, Tuple, Union
@@ -17,8 +18,9 @@ from . import _lib
 from ._transforms import refuse_tangents
 
 
-def _pi() -> Decimal:
-    """To the current context's digits: 16 atan(1/5) - 4 atan(1/239) by their series."""
+@functools.lru_cache(maxsize=4)
+def _pi(digits: int) -> Decimal:
+    """16 atan(1/5) - 4 atan(1/239) by their series, in a context of so many digits."""
     def atan_of_one_over(n):
         total, term, k = Decimal(0), Decimal(1) / n, 1
         while total + term / k != total:
@@ -59,11 +61,13 @@ def rotary_turns(rotary_dim: int, base: float = 10000.0, *, scaling: Optional[st
     with localcontext() as context:
         # (64 bits behind the point, as many digits before it as bases and factors below one make, and some for what is lost on the way)
         context.prec = 50 + math.ceil(max(0.0, -math.log10(base)) + 3.0 * max(0.0, -math.log10(factor)))
-        turn, factor, slow, fast = 2 * _pi(), Decimal(float(factor)), Decimal(float(slow)), Decimal(float(fast))
+        turn, factor, slow, fast = 2 * _pi(context.prec), Decimal(float(factor)), Decimal(float(slow)), Decimal(float(fast))
         log_base = Decimal(float(base)).ln()
         if scaling == "base":
             log_base += factor.ln() * rotary_dim / (rotary_dim - 2)
-        turns = [(log_base * (-2 * i) / rotary_dim).exp() / turn for i in range(rotary_dim // 2)]
+        ratio, turns = (log_base * -2 / rotary_dim).exp(), [1 / turn]
+        while len(turns) < rotary_dim // 2:
+            turns.append(turns[-1] * ratio)
         if scaling == "linear":
             turns = [x / factor for x in turns]
         elif scaling == "parts":
