@@ -13,7 +13,7 @@
 // 0.0017; without any of this 0.0035 and 0.0033.
 //
 // What bounds them: the matrix instructions and, at the same time on the same SIMD, exponentials (a quarter of the rate of other instructions) and additions.  Forward, one causal prompt of 16384 rows,
-// 32 heads (8 for keys) of 128: 1.98 ms, 1.1 Pflop/s of the 1.2 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.58 ms, dQ 1.06 (its product of K twice), dK and dV 1.09.
+// 32 heads (8 for keys) of 128: 1.95 ms, 1.1 Pflop/s of the 1.30 that a large library product reaches.  Training, 4 x 4096 rows: forward 0.58 ms, dQ 1.06 (its product of K twice), dK and dV 1.09.
 // Inputs of zeros take a quarter less time than random ones: the power that the products take has its part in it.
 //
 // Which rows: tile t of the launch belongs to the last segment j (packed_common.h) with begin(j) / 128 + j <= t; begin(j + 1) / 128 + j + 1 leaves room for all of j's tiles, so that every workgroup finds
