@@ -27,7 +27,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     Rows of no sequence (behind the last) and rows without a key get zeros, as do their gradients; what lies in rows that a query does not see, infinities and NaN among
     it, does not reach its result.  Sums are in fp32.  In 16 bits probabilities are rounded to the inputs' type to multiply values, and scores' gradients to multiply queries (to multiply keys:
-    as two values); for the backward the call keeps, beside its inputs, the output, what rounding left of it, and a number for each row and head.  Gradients: q, k and v, the same bits with every call.
+    as two values; in fp16 both times powers of two, so that gradients of any size keep their bits); for the backward the call keeps, beside its inputs, the output, what rounding left of it, and a number for each row and head.  Gradients: q, k and v, the same bits with every call.
 
     Room that a cache leaves between its sequences is a sequence without queries: offsets [0, 1, 1, 2, 2], key_offsets [0, n0, room, room + n1, 2 room].  Calls whose sequences have few queries each
     (by the averages of queries times H / Hk and of keys) and others are served by different kernels: prompts and single tokens are best in calls of their own.
