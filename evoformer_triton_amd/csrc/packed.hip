@@ -29,15 +29,22 @@ EVO_PACKED(128)
 
 // Whether the kernels that split the keys of few queries serve the forward: by what an average sequence has of queries times the query heads that share a key head (`columns` there), of keys, and by sequences times key
 // heads (`units`).  Measured with 1, 4, 16 and 256 sequences of 32 to 65536 keys (us; the tiled kernel in brackets):
-//   16 bits.  Up to 16 columns: 32 heads (8) of 64, one query, 256 sequences of 128 keys 18 (55), of 1024 164 (298), 16 of 1024 14 (28); 8 heads (8): 16 of 1024 keys 14 (16), of 256 keys 14.6 (12.6); least favourable, one sequence of 32 keys 8.1 (6.3).  17 to 32, which are
-//   multiplied in two halves: with shared heads, which a tile reads again for each, 256 of 128 keys 21 (55) and 16 of 4096 41 (75), but 16 of 512 27 (19); with heads of their own one of 1024 keys 13.3 (15.1), 16 of
-//   1024 22 (16), 1000 of 32 282 (226; of D = 128).
+//   16 bits, up to 32 columns; 17 to 32 are multiplied in two halves.  Fewer than 128 units, where tiles would leave most of the chip idle: 8 heads (8) of 64, 4 sequences of 1024 keys, 8 queries 13 (15), 32 queries 16 (16), of 256 keys 10.5 (9.1); 32 heads (8): one query, 16 of
+//   1024 14 (28); least favourable, one sequence of 32 keys 8.1 (6.3).  Keys in one chunk: heads of their own cost the same both ways but for 17 to 32 columns of D = 128 (1000 of 32 keys 282 (226)); shared heads, which a tile reads again for each, 32 heads (8), 8 queries, 256 of 128
+//   26 (66), 16 of 128 8.6 (8.5).  Keys in parts, whose results go to memory and back for every row: 32 heads (8) of 64, 32 sequences of 512 keys, 1 query 14 (20), 4 20 (21), 8 28 (21); 8 queries, of 1024 keys 34 (32), of 4096 82 (102); 8 heads (8): 1 query 13.6 (12.4), 8 16 (13), 16
+//   19 (13); with 128 units 16 of 1024 keys, 1 query 14 (17), 8 14.5 (16), 16 17 (16), 32 22 (16.5).
 //   fp32.  A second launch makes the results, a wave to each row.  8 heads (8) of 64, 8 queries: 1000 sequences of 8 keys 69 (84), 256 of 64 34 (39), of 1024 246 (365); 32 queries: 60 (44) and 287 (374); 64 queries: 100 (56) and 562 (538).  One sequence of 64 keys
 //   14.3 (10.9), of 1024 14.7 (18.9).  32 heads (8) of 128, 16 queries: one of 1024 keys 34 (28), of 4096 43 (59), 4 of 1024 42 (65).
 static bool few_queries(const EvoPacked &p) {
     const int64_t n = p.n, group = p.H / p.Hk, columns = p.Tq * group, units = n * p.Hk;   // (columns, and keys, of all sequences)
     if (!n) return false;
-    if (p.dtype != EVO_F32) return columns <= 16 * n || (columns <= 32 * n && p.Tk >= 1024 * n && (group > 1 || units < 128)) || (columns <= 32 * n && group > 1 && units >= 512);
+    if (p.dtype != EVO_F32) {
+        if (columns > 32 * n) return false;
+        const bool wide = columns > 16 * n;
+        if (units < 128 && (!wide || p.Tk >= 1024 * n)) return true;
+        if (!EVO_BY_HEAD_DIM(packed_few_bytes, p, p)) return !wide || (group > 1 && n * p.H >= 768);
+        return (units < 256 && !wide ? 8192 : 24576) * p.Tq <= p.Tk * group * (p.D > 64 ? p.D : 64);
+    }
     if (columns > 64 * n || 512 * p.Tq > (p.Tk > 64 * n ? p.Tk : 64 * n) * group * p.D) return false;   // (each row's way through memory, beside what its keys take)
     if (units < 512 && p.Tk < 128 * n) return false;
     if (units < 32 && columns > 32 * n && p.Tk < 4096 * n) return false;
